@@ -1,0 +1,519 @@
+// Single-token attention over the FP8 cache with a power-of-two scale per (page of 16 tokens, head), see kv_scaled.cu.
+//
+// With K^ and V^ the cache's numbers, s_j = a q . k^_j the score in the exp2 domain (a = softmax scale * log2(e) * the key page's scale) and
+// 2^ev the value page's scale:
+//
+//   o = sum_j 2^(s_j) 2^ev v^_j / sum_j 2^(s_j) = sum_j p_j v^_j / sum_j p_j 2^-ev,     p_j = 2^(s_j + ev - M)
+//
+// so both scales ride in the exponent's multiply-add and the codes go to the tensor cores as they are.  M is the running maximum of
+// s_j + ev, that is of what a token can add to the output: p in f16 keeps its 11 bits wherever they matter, however far the pages'
+// scales are apart.  q is brought to 2^14 by a power of two and is exact in f16; the sums are fp32.
+//
+// scaled_decode_kernel: bound by the cache's bytes (2 D a token and key head).  The pages of all (sequence, key head) pairs form one list, cut
+// into equal runs, a run per warp: ragged batches and single long sequences fill the GPU alike.  A warp is on its own: it copies its pages
+// into its ring of shared memory (cp.async.bulk, a page of K and one of V per slot), reads them as mma.sync fragments (tokens along M for
+// the scores, channels along M for the outputs, heads along N) and leaves (M, l, O) of every pair it touched.  A piece's number is pair +
+// warp, which no two pieces share.
+// scaled_merge_kernel joins the pieces of a pair.  scaled_weigh_kernel adds 2^(s - M) / l over the pair's heads to the running sums.
+#include "common.cuh"
+#include "host_api.h"
+#include "tc_util.cuh"
+
+namespace atlas {
+
+constexpr int kSdPage = 16;
+constexpr int kSdWarps = 8;
+constexpr int kSdRing = 24 * 1024;        // bytes of pages in flight per warp
+constexpr int kSdLeast = 2;               // pages that make a run worth a warp of its own
+
+struct ScaledDecodeParams {
+  const __nv_bfloat16* q; long long ldq;
+  __nv_bfloat16* out; long long ldo;
+  const uint8_t* k_cache; const uint8_t* v_cache;
+  const float* k_scale; const float* v_scale; long long ks_ld, vs_ld; int ks_h, vs_h;
+  const int* block_tables; int bt_ld, bt_cols;
+  const int* seq_lens; const int* query_start_loc;
+  int nd, Hkv, G, tiles;                  // tiles: groups of at most 8 * NT query heads of a key head
+  int window, num_pages;
+  int warps;                              // of the whole grid
+  float scale_log2;
+  float* part_o; float* part_ml;          // piece: [D][cols], [cols] x (M, l)
+  int cols;
+  float* scores; long long width; int score_cols;      // [nd * Hkv][width][score_cols] or null
+  float* ml;                              // [nd][Hq] x (M, 1 / l) or null
+  status_t* status;
+};
+
+ATLAS_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+ATLAS_DEVICE uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+ATLAS_DEVICE uint32_t e4m3x2_to_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(r) : "h"((uint16_t)v));
+  return r;
+}
+ATLAS_DEVICE uint32_t f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+ATLAS_DEVICE void bulk_page(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Pages that the newest token of a sequence of `len` sees, and the first of them.
+ATLAS_DEVICE int seen_pages(int len, int window, int& first) {
+  const int lo = window > 0 ? max(len - window, 0) : 0;
+  first = lo / kSdPage;
+  return len > 0 ? (len + kSdPage - 1) / kSdPage - first : 0;
+}
+ATLAS_DEVICE int decode_len(const ScaledDecodeParams& p, int b) { return min(max(p.seq_lens[b], 0), p.bt_cols * kSdPage); }
+
+// Pages of sequences [0, n), the whole warp.
+ATLAS_DEVICE int total_pages(const ScaledDecodeParams& p, int n, int lane) {
+  int sum = 0, first;
+  for (int b = lane; b < n; b += 32) sum += seen_pages(decode_len(p, b), p.window, first);
+  return __reduce_add_sync(0xffffffffu, sum);
+}
+ATLAS_DEVICE int run_length(int pages, int warps) { return max((pages + warps - 1) / warps, kSdLeast); }
+
+// One entry of the page list.
+struct PageRef {
+  int item;            // (sequence * Hkv + key head) * tiles + tile
+  int tok0;            // first token of the page
+  int block;           // -1: an entry outside of the pool, skipped
+  float sk, ev;        // key scale, value exponent
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kSdWarps * 32, 1)
+scaled_decode_kernel(const ScaledDecodeParams p) {
+  constexpr int kPageBytes = kSdPage * D;
+  constexpr int kStages = kSdRing / (2 * kPageBytes);
+  constexpr int KS = D / 16;                      // k steps of a score
+  constexpr int QB = D / 4;                       // channels of a lane's share of a row
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kSdWarps][kStages];
+  __shared__ uint32_t abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * kSdRing;
+  volatile uint32_t* abort_flag = &abort_word;
+  if (threadIdx.x == 0) abort_word = 0;
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&bars[warp][s], 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
+  chain_trigger();
+  chain_wait();
+  const int w = warp * gridDim.x + blockIdx.x;    // neighbours in the list on different SMs
+  const int hn = p.Hkv * p.tiles;
+  const int all = total_pages(p, p.nd, lane) * hn;
+  const int run = run_length(all, p.warps);
+  const long long lo64 = (long long)w * run;
+  if (lo64 >= all) return;
+  const int n0 = (int)lo64, n1 = min(n0 + run, all);
+  const int n = n1 - n0;
+
+  // the sequence that entry n0 belongs to, and the entries before it
+  int b0 = 0, base0 = 0;
+  for (int c = 0; c < p.nd; c += 32) {
+    int first;
+    const int mine = c + lane < p.nd ? seen_pages(decode_len(p, c + lane), p.window, first) * hn : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, base0 + incl > n0);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      b0 = c + l;
+      base0 += __shfl_sync(0xffffffffu, incl - mine, l);
+      break;
+    }
+    base0 += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  // entries n0 + 32 c + lane
+  auto fetch = [&](int c) -> PageRef {
+    PageRef r{-1, 0, -1, 0.f, 0.f};
+    const int i = 32 * c + lane;
+    if (i >= n) return r;
+    int at = n0 + i - base0, b = b0, first, np;
+    for (;; ++b) {
+      if (b >= p.nd) return r;
+      np = seen_pages(decode_len(p, b), p.window, first);
+      if (at < np * hn) break;
+      at -= np * hn;
+    }
+    const int pair = at / np, pg = first + at % np;
+    r.item = b * hn + pair;
+    r.tok0 = pg * kSdPage;
+    const int block = p.block_tables[(long long)b * p.bt_ld + pg];
+    if (block >= 0 && block < p.num_pages) {
+      const int h = pair / p.tiles;
+      r.block = block;
+      r.sk = p.k_scale[block * p.ks_ld + h * p.ks_h];
+      r.ev = (float)((int)((__float_as_uint(p.v_scale[block * p.vs_ld + h * p.vs_h]) >> 23) & 255u) - 127);
+    }
+    return r;
+  };
+  PageRef cur = fetch(0), nxt = fetch(1);
+  int cur_chunk = 0;
+  auto issue = [&](int i) {                         // entry i of this run into its slot; chunk cur_chunk or the next one
+    const PageRef& r = (i >> 5) == cur_chunk ? cur : nxt;
+    const int block = __shfl_sync(0xffffffffu, r.block, i & 31);
+    const int item = __shfl_sync(0xffffffffu, r.item, i & 31);
+    if (lane == 0) {
+      const int s = i % kStages;
+      uint64_t* bar = &bars[warp][s];
+      uint8_t* dst = ring + s * 2 * kPageBytes;
+      if (block >= 0) {
+        const int h = (item / p.tiles) % p.Hkv;
+        const long long at = ((long long)block * p.Hkv + h) * kPageBytes;
+        mbar_expect_tx(bar, 2 * kPageBytes);
+        bulk_page(dst, p.k_cache + at, kPageBytes, bar);
+        bulk_page(dst + kPageBytes, p.v_cache + at, kPageBytes, bar);
+      } else {
+        mbar_arrive(bar);
+      }
+    }
+  };
+  for (int i = 0; i < min(n, kStages); ++i) issue(i);
+
+  uint32_t qf[NT][KS][2];                           // queries as B fragments: head g of n-tile, channels t * QB + 4 step + 0 .. 3
+  float a0[NT], a1[NT];                             // score factors of heads 2t, 2t + 1
+  float m0[NT], m1[NT], l0[NT], l1[NT];
+  float acc[NT][KS][4];                             // channels 16 i + g, + 8; heads 2t, 2t + 1
+  int item = -1, len = 0, lo_tok = 0;
+
+  auto flush = [&]() {
+    const long long piece = (long long)item + w;
+    float* o = p.part_o + piece * D * p.cols;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = nt * 8 + 2 * t;
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], x);
+        l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], x);
+      }
+      if (c < p.cols) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          *reinterpret_cast<float2*>(o + (16 * i + g) * p.cols + c) = make_float2(acc[nt][i][0], acc[nt][i][1]);
+          *reinterpret_cast<float2*>(o + (16 * i + g + 8) * p.cols + c) = make_float2(acc[nt][i][2], acc[nt][i][3]);
+        }
+        if (g == 0) *reinterpret_cast<float4*>(p.part_ml + (piece * p.cols + c) * 2) = make_float4(m0[nt], l0[nt], m1[nt], l1[nt]);
+      }
+    }
+  };
+  auto begin = [&](int it) {
+    item = it;
+    const int tile = it % p.tiles, h = (it / p.tiles) % p.Hkv, b = it / hn;
+    len = decode_len(p, b);
+    lo_tok = p.window > 0 ? max(len - p.window, 0) : 0;
+    const __nv_bfloat16* row = p.q + (long long)p.query_start_loc[b] * p.ldq;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int hg = tile * 8 * NT + nt * 8 + g;    // head of the group
+      uint32_t raw[QB / 2];
+#pragma unroll
+      for (int i = 0; i < QB / 8; ++i) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (hg < p.G) v = *reinterpret_cast<const uint4*>(row + (h * p.G + hg) * D + t * QB + i * 8);
+        raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w;
+      }
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < QB / 2; ++i) {
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i]));
+        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // largest magnitude to [2^13, 2^14): bf16 numbers are exact in f16 then, down to 2^-37 of it
+      const int e = min(max(13 - ((int)(__float_as_uint(amax) >> 23) - 127), -100), 100);
+      const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[2 * i + j]));
+          qf[nt][i][j] = f16x2(f.x * up, f.y * up);
+        }
+      const float a = p.scale_log2 * down;
+      a0[nt] = __shfl_sync(0xffffffffu, a, 8 * t);            // head 2t is the row g = 2t, lanes 8t ..
+      a1[nt] = __shfl_sync(0xffffffffu, a, 8 * t + 4);
+      m0[nt] = m1[nt] = -INFINITY;
+      l0[nt] = l1[nt] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.f;
+    }
+  };
+
+  const int tok_r = 4 * (g >> 1) + (g & 1);         // token of score row g; row g + 8 holds token tok_r + 2
+  bool ok = true;
+  for (int i = 0; i < n; ++i) {
+    if ((i >> 5) != cur_chunk) {
+      cur = nxt;
+      ++cur_chunk;
+      nxt = fetch(cur_chunk + 1);
+    }
+    const int it = __shfl_sync(0xffffffffu, cur.item, i & 31), tok0 = __shfl_sync(0xffffffffu, cur.tok0, i & 31);
+    const int block = __shfl_sync(0xffffffffu, cur.block, i & 31);
+    const float sk = __shfl_sync(0xffffffffu, cur.sk, i & 31), ev = __shfl_sync(0xffffffffu, cur.ev, i & 31);
+    if (it != item) {
+      if (item >= 0) flush();
+      begin(it);
+    }
+    const int s = i % kStages;
+    ok = mbar_wait(&bars[warp][s], (i / kStages) & 1, abort_flag, p.status, 0x900);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    if (block >= 0) {
+      const uint8_t* kp = ring + s * 2 * kPageBytes;
+      const uint8_t* vp = kp + kPageBytes;
+      // ---- scores: rows g, g + 8 are tokens tok_r, tok_r + 2; a lane takes QB neighbouring channels of each
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[nt][j] = 0.f;
+      const uint8_t* kr = kp + tok_r * D + t * QB;
+#pragma unroll
+      for (int c0 = 0; c0 < QB / 16; ++c0) {
+        const uint4 x = *reinterpret_cast<const uint4*>(kr + c0 * 16), y = *reinterpret_cast<const uint4*>(kr + 2 * D + c0 * 16);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t f0 = e4m3x2_to_f16x2(xs[k] & 0xffffu), f1 = e4m3x2_to_f16x2(ys[k] & 0xffffu);
+          const uint32_t f2 = e4m3x2_to_f16x2(xs[k] >> 16), f3 = e4m3x2_to_f16x2(ys[k] >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt], f0, f1, f2, f3, qf[nt][c0 * 4 + k][0], qf[nt][c0 * 4 + k][1]);
+        }
+      }
+      // ---- softmax weights
+      const bool whole = tok0 >= lo_tok && tok0 + kSdPage <= len;
+      const bool see0 = whole || (tok0 + tok_r >= lo_tok && tok0 + tok_r < len);
+      const bool see1 = whole || (tok0 + tok_r + 2 >= lo_tok && tok0 + tok_r + 2 < len);
+      uint32_t vmask = 0xffffffffu;
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = tok0 + 4 * t + j;
+          if (tok < lo_tok || tok >= len) vmask &= ~(0xffu << (8 * j));
+        }
+      }
+      uint32_t pb[NT][2];
+      const float undo = __uint_as_float((uint32_t)(127 - (int)ev) << 23);     // 2^-ev
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float f0 = a0[nt] * sk, f1 = a1[nt] * sk;
+        if (p.scores) {
+          const int c = (it % p.tiles) * 8 * NT + nt * 8 + 2 * t;
+          if (c < p.score_cols) {
+            float* to = p.scores + ((long long)(it / p.tiles) * p.width + tok0 + tok_r) * p.score_cols + c;
+            if (see0 && tok0 + tok_r < p.width) *reinterpret_cast<float2*>(to) = make_float2(sc[nt][0] * f0, sc[nt][1] * f1);
+            if (see1 && tok0 + tok_r + 2 < p.width) *reinterpret_cast<float2*>(to + 2 * p.score_cols) = make_float2(sc[nt][2] * f0, sc[nt][3] * f1);
+          }
+        }
+        const float s00 = see0 ? fmaf(sc[nt][0], f0, ev) : -INFINITY, s01 = see0 ? fmaf(sc[nt][1], f1, ev) : -INFINITY;
+        const float s10 = see1 ? fmaf(sc[nt][2], f0, ev) : -INFINITY, s11 = see1 ? fmaf(sc[nt][3], f1, ev) : -INFINITY;
+        float x0 = fmaxf(s00, s10), x1 = fmaxf(s01, s11);
+        // The reference moves only when a score passes it by 2^8 (p stays inside f16): rarely after the first pages.
+        if (__any_sync(0xffffffffu, x0 > m0[nt] + 8.f || x1 > m1[nt] + 8.f)) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+          }
+          const float n0m = fmaxf(m0[nt], x0), n1m = fmaxf(m1[nt], x1);
+          const float r0 = m0[nt] == -INFINITY ? 0.f : fast_exp2(m0[nt] - n0m), r1 = m1[nt] == -INFINITY ? 0.f : fast_exp2(m1[nt] - n1m);
+          m0[nt] = n0m; m1[nt] = n1m;
+          l0[nt] *= r0; l1[nt] *= r1;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) { acc[nt][k][0] *= r0; acc[nt][k][1] *= r1; acc[nt][k][2] *= r0; acc[nt][k][3] *= r1; }
+        }
+        const float r0 = m0[nt] == -INFINITY ? 0.f : m0[nt], r1 = m1[nt] == -INFINITY ? 0.f : m1[nt];
+        const float p00 = fast_exp2(s00 - r0), p01 = fast_exp2(s01 - r1), p10 = fast_exp2(s10 - r0), p11 = fast_exp2(s11 - r1);
+        l0[nt] += (p00 + p10) * undo;
+        l1[nt] += (p01 + p11) * undo;
+        pb[nt][0] = transpose8x8(f16x2(p00, p01));
+        pb[nt][1] = transpose8x8(f16x2(p10, p11));
+      }
+      // ---- outputs: rows are channels, a lane takes tokens 4t .. 4t + 3 of channels 16 k + g and + 8
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(vp + (16 * k + g) * kSdPage + 4 * t) & vmask;
+        const uint32_t y = *reinterpret_cast<const uint32_t*>(vp + (16 * k + g + 8) * kSdPage + 4 * t) & vmask;
+        const uint32_t f0 = e4m3x2_to_f16x2(x & 0xffffu), f1 = e4m3x2_to_f16x2(y & 0xffffu);
+        const uint32_t f2 = e4m3x2_to_f16x2(x >> 16), f3 = e4m3x2_to_f16x2(y >> 16);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][k], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
+      }
+    }
+    __syncwarp();
+    if (i + kStages < n) {
+      fence_proxy_async();                          // this slot's reads before the copy that refills it
+      issue(i + kStages);
+    }
+  }
+  if (ok) flush();
+  else
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);       // copies in flight land before the shared memory goes
+}
+
+// Pieces of a pair: warps [first page / run, last page / run] of the list; piece = pair + warp.  A thread owns one output number.
+template <int D>
+__global__ void __launch_bounds__(256)
+scaled_merge_kernel(const ScaledDecodeParams p) {
+  __shared__ float tile[256];
+  chain_trigger();
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const int item = blockIdx.x, hn = p.Hkv * p.tiles, b = item / hn, pair = item % hn;
+  const int all = total_pages(p, p.nd, lane) * hn, run = run_length(all, p.warps);
+  int first;
+  const int np = seen_pages(decode_len(p, b), p.window, first);
+  const int start = total_pages(p, b, lane) * hn + pair * np;
+  const int w0 = start / run, w1 = np > 0 ? (start + np - 1) / run : w0 - 1;
+  const int per = 256 / p.cols * p.cols;               // whole channels of a block
+  const int e = blockIdx.y * per + threadIdx.x;
+  const int c = e % p.cols, d = e / p.cols;
+  const int head = (pair % p.tiles) * p.cols + c, h = pair / p.tiles;
+  const bool live = (int)threadIdx.x < per && d < D;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + c;
+  float m = -INFINITY;
+  if (live) {
+#pragma unroll 8
+    for (int w = w0; w <= w1; ++w) m = fmaxf(m, ml[((long long)item + w) * p.cols].x);
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o = 0.f;
+  if (live) {
+#pragma unroll 8
+    for (int w = w0; w <= w1; ++w) {
+      const long long piece = (long long)item + w;
+      const float2 x = ml[piece * p.cols];
+      const float f = fast_exp2(x.x - ref);             // a piece without a visible token: 2^-inf
+      l += x.y * f;
+      o += p.part_o[piece * D * p.cols + d * p.cols + c] * f;
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const bool nan = l != l;
+  if (live && p.ml && d == 0 && head < p.G)
+    reinterpret_cast<float2*>(p.ml)[(long long)b * p.Hkv * p.G + h * p.G + head] = make_float2(ref, nan ? l : inv);
+  if (live) tile[threadIdx.x] = nan ? l : o * inv;
+  __syncthreads();
+  // rows of a head's channels
+  const int chans = per / p.cols;
+  const int cc = threadIdx.x / chans, dd = threadIdx.x % chans;
+  const int hh = (pair % p.tiles) * p.cols + cc, dg = blockIdx.y * chans + dd;
+  if (cc < p.cols && hh < p.G && dg < D)
+    p.out[(long long)p.query_start_loc[b] * p.ldo + (h * p.G + hh) * D + dg] = __float2bfloat16_rn(tile[dd * p.cols + cc]);
+}
+
+// weights[b, h, j] += sum over the pair's heads of 2^(s - M) / l, a thread per token.
+__global__ void __launch_bounds__(256)
+scaled_weigh_kernel(const ScaledDecodeParams p, float* weights, long long w_ld_b, long long w_ld_h) {
+  extern __shared__ float2 sh_ml[];
+  chain_trigger();
+  chain_wait();
+  const int pair = blockIdx.x, b = pair / p.Hkv, h = pair % p.Hkv;
+  const int len = decode_len(p, b), lo = p.window > 0 ? max(len - p.window, 0) : 0, end = (int)min((long long)len, p.width);
+  for (int g = threadIdx.x; g < p.G; g += 256) sh_ml[g] = reinterpret_cast<const float2*>(p.ml)[(long long)b * p.Hkv * p.G + h * p.G + g];
+  __syncthreads();
+  for (int j = lo + blockIdx.y * 256 + threadIdx.x; j < end; j += gridDim.y * 256) {
+    const float2* s = reinterpret_cast<const float2*>(p.scores + ((long long)pair * p.width + j) * p.score_cols);
+    float sum = 0.f;
+    for (int g = 0; g < p.G; g += 2) {
+      const float2 x = s[g >> 1];
+      sum += fast_exp2(x.x - sh_ml[g].x) * sh_ml[g].y;
+      if (g + 1 < p.G) sum += fast_exp2(x.y - sh_ml[g + 1].x) * sh_ml[g + 1].y;
+    }
+    weights[b * w_ld_b + h * w_ld_h + j] += sum;
+  }
+}
+
+}  // namespace atlas
+
+using namespace atlas;
+
+namespace {
+
+template <int D, int NT>
+int decode_launch(const ScaledDecodeParams& p, int blocks, int items, cudaStream_t st) {
+  constexpr int smem = kSdWarps * kSdRing;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(scaled_decode_kernel<D, NT>), smem) != cudaSuccess) return -20;
+  if (launch_chain(scaled_decode_kernel<D, NT>, dim3(blocks), dim3(kSdWarps * 32), smem, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
+  const int per = 256 / p.cols;
+  if (launch_chain(scaled_merge_kernel<D>, dim3(items, (D + per - 1) / per), dim3(256), 0, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
+  return 0;
+}
+
+}  // namespace
+
+// Sizes of the workspaces: numbers [pieces * D * cols], [pieces * cols * 2].  A piece is a pair's share of a warp's run.
+extern "C" int atlas_attn_scaled_decode_plan(int nd, int Hq, int Hkv, int max_seq_len, int num_sms, int* blocks, int* cols, long long* pieces) {
+  if (nd <= 0 || Hkv <= 0 || Hq % Hkv) return -1;
+  const int G = Hq / Hkv, tiles = (G + 15) / 16;
+  *cols = G <= 16 ? (G + 1) / 2 * 2 : 16;
+  const long long items = (long long)nd * Hkv * tiles, pages = items * ((max_seq_len + kSdPage - 1) / kSdPage);
+  if (pages > 0x3fffffffll) return -1;
+  const long long want = (pages + kSdLeast - 1) / kSdLeast;
+  *blocks = (int)(want < num_sms ? (want > 0 ? want : 1) : num_sms);
+  *pieces = items + (long long)*blocks * kSdWarps;
+  return 0;
+}
+
+// Decode rows of a step: sequence b's row is query_start_loc[b].  `scores`, `ml` and `weights` come together: [nd * Hkv][width][cols of G
+// rounded up to two], [nd][Hq][2] and the sums [b][h][token].  -1: sizes or alignment outside of what the kernels take.
+extern "C" int atlas_attn_scaled_decode(const void* q, long long ldq, void* out, long long ldo, const void* k_cache, const void* v_cache,
+                                        const float* k_scale, long long ks_ld, int ks_h, const float* v_scale, long long vs_ld, int vs_h,
+                                        const int* block_tables, int bt_ld, int bt_cols, const int* seq_lens, const int* query_start_loc, int nd, float scale,
+                                        int Hq, int Hkv, int D, int window, int num_pages, int max_seq_len, int num_sms, float* part_o,
+                                        float* part_ml, float* scores, long long width, float* ml, float* weights, long long w_ld_b,
+                                        long long w_ld_h, unsigned long long* status, void* stream) {
+  if (nd <= 0) return 0;
+  if ((D != 64 && D != 128 && D != 256) || Hkv <= 0 || Hq % Hkv || ldq % 8 || (reinterpret_cast<uintptr_t>(q) & 15)) return -1;
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return -1;
+  ScaledDecodeParams p;
+  int blocks;
+  long long pieces;
+  if (atlas_attn_scaled_decode_plan(nd, Hq, Hkv, max_seq_len, num_sms, &blocks, &p.cols, &pieces)) return -1;
+  p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.out = (__nv_bfloat16*)out; p.ldo = ldo;
+  p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache;
+  p.k_scale = k_scale; p.v_scale = v_scale; p.ks_ld = ks_ld; p.vs_ld = vs_ld; p.ks_h = ks_h; p.vs_h = vs_h;
+  p.block_tables = block_tables; p.bt_ld = bt_ld; p.bt_cols = bt_cols; p.seq_lens = seq_lens; p.query_start_loc = query_start_loc;
+  p.nd = nd; p.Hkv = Hkv; p.G = Hq / Hkv; p.tiles = (p.G + 15) / 16;
+  p.window = window; p.num_pages = num_pages; p.warps = blocks * kSdWarps;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part_o = part_o; p.part_ml = part_ml;
+  p.scores = weights ? scores : nullptr; p.width = width; p.score_cols = (p.G + 1) / 2 * 2; p.ml = weights ? ml : nullptr;
+  p.status = status;
+  cudaStream_t st = (cudaStream_t)stream;
+  const int items = nd * Hkv * p.tiles;
+  int rc;
+  if (p.G <= 8) rc = D == 64 ? decode_launch<64, 1>(p, blocks, items, st) : D == 128 ? decode_launch<128, 1>(p, blocks, items, st) : decode_launch<256, 1>(p, blocks, items, st);
+  else rc = D == 64 ? decode_launch<64, 2>(p, blocks, items, st) : D == 128 ? decode_launch<128, 2>(p, blocks, items, st) : decode_launch<256, 2>(p, blocks, items, st);
+  if (rc || !weights) return rc;
+  const int chunks = (max_seq_len + 1023) / 1024;
+  if (launch_chain(scaled_weigh_kernel, dim3(nd * Hkv, chunks < 64 ? chunks : 64), dim3(256), (size_t)p.G * sizeof(float2), st, p, weights, w_ld_b,
+                   w_ld_h) != cudaSuccess) { cudaGetLastError(); return -20; }
+  return 0;
+}

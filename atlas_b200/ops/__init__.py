@@ -14,6 +14,7 @@ import torch
 
 from .. import quant as Q
 from . import reference as ref
+from . import reference_scaled as ref_scaled
 
 _cuda = None
 FORCE_REFERENCE = False     # run the plain-PyTorch restatement even for GPU tensors (oracle for end-to-end tests)
@@ -32,6 +33,13 @@ def cuda_ops():
         _c.load()
         _cuda = _c
     return _cuda
+
+
+def scaled_ops():
+    """The bindings of the block-scaled cache."""
+    cuda_ops()
+    from . import cuda_scaled as CS
+    return CS
 
 
 # ----------------------------------------------------------------------------- weights / activations
@@ -403,7 +411,18 @@ def qk_norm_rope_kv_write(q, k, v, positions, rope_cache, rotary_dim, k_cache, v
                           k_scale=1.0, v_scale=1.0, q_norm_w=None, k_norm_w=None, eps=1e-6, norm_plus_one=False, rotate=False, norm_dim=0):
     """``rotate``: every q / k / v head goes through the orthonormal Walsh-Hadamard transform after RoPE, so the cache
     holds rotated keys and values (the "turbo8" cache: rotation + FP8) and the attention output comes out rotated too
-    (``head_rotate`` takes it back).  ``norm_dim``: channels of a head that its norm counts (0 = all; the rest is zero padding)."""
+    (``head_rotate`` takes it back).  ``norm_dim``: channels of a head that its norm counts (0 = all; the rest is zero padding).
+
+    ``k_scale`` and ``v_scale`` may be the tensors of :func:`alloc_kv_scales`: the FP8 cache then has a power of two per (16-token block,
+    head), which this call sets or raises (a raise moves the codes that the block holds).  Norm and rotation are in fp32 up to the one
+    rounding to e4m3, the queries come back in a new tensor, heads are 64, 128 or 256 wide, and there is no ``rotate``.  The rows of one
+    block stand next to each other in slot order; a block whose first token is written starts anew."""
+    if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor):
+        if rotate:
+            raise ValueError("a block-scaled cache holds no rotated heads")
+        put = scaled_ops().qk_norm_rope_kv_write if on_gpu(q) else ref_scaled.qk_norm_rope_kv_write
+        return put(q, k, v, positions, rope_cache, rotary_dim, k_cache, v_cache, slot_mapping, k_scale, v_scale, q_norm_w, k_norm_w, eps,
+                   norm_plus_one, norm_dim)
     if on_gpu(q):
         return cuda_ops().qk_norm_rope_kv_write(q, k, v, positions, rope_cache, rotary_dim, k_cache, v_cache,
                                                 slot_mapping, k_scale, v_scale, q_norm_w, k_norm_w, eps, norm_plus_one, rotate, norm_dim)
@@ -456,11 +475,24 @@ def head_rotate(x: torch.Tensor) -> torch.Tensor:
 
 
 def paged_attention(q, k_cache, v_cache, batch, scale, k_scale=1.0, v_scale=1.0, sliding_window=None, chunk=0,
-                    sinks=None, softcap=0.0, distance=None) -> torch.Tensor:
+                    sinks=None, softcap=0.0, distance=None, weights=None) -> torch.Tensor:
     """Attention of the step's query rows over the paged cache. ``batch`` is a ``ForwardBatch``.  ``chunk`` > 0: a token sees
     only keys of its own ``chunk``-token block of the sequence; ``sinks [Hq]``: ``exp(sink)`` joins the softmax denominator;
     ``softcap`` > 0: scores become ``softcap * tanh(score / softcap)``; ``distance [Hq, n]`` (fp32): column ``min(i - j, n - 1)``
-    joins the scaled score of query ``i`` and key ``j``."""
+    joins the scaled score of query ``i`` and key ``j``.
+
+    With the tensors of :func:`alloc_kv_scales` as ``k_scale`` and ``v_scale`` the cache is FP8 with a scale per (block, head): plain or
+    windowed attention.  ``weights [sequences, Hkv, tokens]`` (fp32, such a cache only): every cached token's softmax weight, summed over
+    the sequence's rows of this step and the query heads of a key head, is added to it."""
+    if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor):
+        if chunk or sinks is not None or softcap or distance is not None:
+            raise ValueError("a block-scaled cache: no chunked attention, softmax sinks, bounded scores or distance biases")
+        if on_gpu(q):
+            return scaled_ops().paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding_window, weights)
+        return ref_scaled.paged_attention(q, k_cache, v_cache, batch.block_tables, batch.seq_lens, batch.query_start_loc, scale, k_scale, v_scale,
+                                          sliding_window, weights)
+    if weights is not None:
+        raise ValueError("attention weights are summed over a block-scaled cache (alloc_kv_scales)")
     if on_gpu(q):
         return cuda_ops().paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding_window, chunk, sinks, softcap, distance)
     return ref.paged_attention(q, k_cache, v_cache, batch.block_tables, batch.seq_lens, batch.query_start_loc,
@@ -474,6 +506,34 @@ def paged_attention_fp8_out(q, k_cache, v_cache, batch, scale, k_scale=1.0, v_sc
         return None
     r = cuda_ops().paged_attention_q8(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding_window)
     return None if r is None else Act(q=r[0], s=r[1], dtype=q.dtype)
+
+
+def alloc_kv_scales(num_blocks: int, hkv: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 ``[num_blocks, hkv]`` scales of keys and of values for an FP8 cache with 16-token blocks; powers of two, ones at first.  They take
+    the places of the cache's ``k_scale`` and ``v_scale``."""
+    from . import cuda_scaled as CS
+    return CS.alloc_kv_scales(num_blocks, hkv, device)
+
+
+def kv_read(k_cache, v_cache, block_tables, seq_lens, max_len: int, k_scale, v_scale) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of the first ``min(seq_lens[b], max_len)`` tokens of every sequence out of a block-scaled cache: bf16 ``[sequences,
+    max_len, Hkv, D]`` each, zeros behind them.  Exact: an e4m3 number times a power of two is a bf16 number."""
+    read = scaled_ops().kv_read if on_gpu(k_cache) else ref_scaled.kv_read
+    return read(k_cache, v_cache, block_tables, seq_lens, max_len, k_scale, v_scale)
+
+
+def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep: int, new_tables, sink: int = 0, recent: int = 0):
+    """Keep ``keep`` tokens of every sequence and key head of a block-scaled cache: the first ``sink``, the last ``recent`` and, of those
+    between, the ones with the largest ``weights [sequences, Hkv, tokens]`` (ties: the earlier; NaN below everything).  They move, in their
+    order, into the blocks of ``new_tables [sequences, >= keep / 16]``, which no other table holds, and get scales of their own; the old
+    blocks stay as they are.  Sequences of at most ``keep`` tokens move whole.
+
+    Returns the new lengths (int32), the kept positions ``[sequences, Hkv, keep]`` (int32, -1 behind the last) and their weights."""
+    if on_gpu(k_cache):
+        return scaled_ops().kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep, new_tables, sink, recent)
+    if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError(f"keeping {keep} tokens of which the first {sink} and the last {recent} are fixed")
+    return ref_scaled.kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep, new_tables, sink, recent)
 
 
 # ----------------------------------------------------------------------------- MoE

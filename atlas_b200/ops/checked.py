@@ -57,6 +57,33 @@ def paged_read(block_tables: torch.Tensor, seq_lens: torch.Tensor, num_blocks: i
     index_range("block_tables (entries covered by seq_lens)", used, 0, num_blocks)
 
 
+def block_runs(slot_mapping: torch.Tensor, block_size: int) -> None:
+    """The rows of one step that fall into one block stand next to each other, in slot order."""
+    s = slot_mapping.tolist()
+    done, last = set(), -1
+    for i, x in enumerate(s):
+        blk = x // block_size if x >= 0 else -1
+        if blk != last and blk in done:
+            _fail("slot_mapping", f"row {i} comes back to block {blk}")
+        if blk >= 0 and blk == last and x != s[i - 1] + 1:
+            _fail("slot_mapping", f"row {i} writes slot {x} of block {blk} behind slot {s[i - 1]}")
+        if blk >= 0:
+            done.add(blk)
+        last = blk
+
+
+def evict(block_tables: torch.Tensor, seq_lens: torch.Tensor, new_tables: torch.Tensor, num_blocks: int, block_size: int, keep: int,
+          width: int) -> None:
+    """Tables inside the pool, lengths inside weights and tables, and new blocks that no table of the call holds already."""
+    paged_read(block_tables, seq_lens, num_blocks, block_size)
+    index_range("seq_lens", seq_lens, 0, width + 1)
+    paged_read(new_tables, seq_lens.clamp(max=keep), num_blocks, block_size)
+    cols = lambda t, n: t[:n.shape[0]][torch.arange(t.shape[1], device=t.device)[None] < ((n.long() + block_size - 1) // block_size)[:, None]]
+    old, new = cols(block_tables, seq_lens), cols(new_tables, seq_lens.clamp(max=keep))
+    if torch.unique(new).numel() != new.numel() or bool(torch.isin(new, old).any()):
+        _fail("new_tables", "a new block appears twice or holds tokens that are being read")
+
+
 def finite(what: str, t: torch.Tensor) -> None:
     if t.is_floating_point() and t.numel() and not bool(torch.isfinite(t.float()).all()):
         _fail(what, "contains inf or nan")
