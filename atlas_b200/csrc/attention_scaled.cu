@@ -377,55 +377,99 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);       // copies in flight land before the shared memory goes
 }
 
-// Pieces of a pair: warps [first page / run, last page / run] of the list; piece = pair + warp.  A thread owns one output number.
+// Pieces of a pair: warps [first page / run, last page / run] of the list; piece = pair + warp.  A block joins up to 256 output numbers,
+// four neighbouring ones a thread and every fourth piece: a single long sequence has hundreds of pieces, and their loads overlap.
+constexpr int kSmChunk = 128;                            // pieces whose factors are in shared memory at a time
+
 template <int D>
 __global__ void __launch_bounds__(256)
 scaled_merge_kernel(const ScaledDecodeParams p) {
-  __shared__ float tile[256];
+  __shared__ float factor[kSmChunk][16];
+  __shared__ float part[16][17];
+  __shared__ float top[16], sum[16];
+  __shared__ float4 quad[4][64];
   chain_trigger();
   chain_wait();
-  const int lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int item = blockIdx.x, hn = p.Hkv * p.tiles, b = item / hn, pair = item % hn;
   const int all = total_pages(p, p.nd, lane) * hn, run = run_length(all, p.warps);
   int first;
   const int np = seen_pages(decode_len(p, b), p.window, first);
   const int start = total_pages(p, b, lane) * hn + pair * np;
-  const int w0 = start / run, w1 = np > 0 ? (start + np - 1) / run : w0 - 1;
-  const int per = 256 / p.cols * p.cols;               // whole channels of a block
-  const int e = blockIdx.y * per + threadIdx.x;
-  const int c = e % p.cols, d = e / p.cols;
-  const int head = (pair % p.tiles) * p.cols + c, h = pair / p.tiles;
-  const bool live = (int)threadIdx.x < per && d < D;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + c;
+  const int w0 = start / run, pieces = np > 0 ? (start + np - 1) / run - w0 + 1 : 0;
+  const long long piece0 = (long long)item + w0;
+  // ---- references and sums of the heads: thread (piece lane, head)
+  const int pl = tid >> 4, hc = tid & 15;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + piece0 * p.cols + hc;
   float m = -INFINITY;
-  if (live) {
-#pragma unroll 8
-    for (int w = w0; w <= w1; ++w) m = fmaxf(m, ml[((long long)item + w) * p.cols].x);
-  }
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
-  if (live) {
-#pragma unroll 8
-    for (int w = w0; w <= w1; ++w) {
-      const long long piece = (long long)item + w;
-      const float2 x = ml[piece * p.cols];
-      const float f = fast_exp2(x.x - ref);             // a piece without a visible token: 2^-inf
-      l += x.y * f;
-      o += p.part_o[piece * D * p.cols + d * p.cols + c] * f;
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const bool nan = l != l;
-  if (live && p.ml && d == 0 && head < p.G)
-    reinterpret_cast<float2*>(p.ml)[(long long)b * p.Hkv * p.G + h * p.G + head] = make_float2(ref, nan ? l : inv);
-  if (live) tile[threadIdx.x] = nan ? l : o * inv;
+  if (hc < p.cols)
+#pragma unroll 4
+    for (int i = pl; i < pieces; i += 16) m = fmaxf(m, ml[(long long)i * p.cols].x);
+  part[pl][hc] = m;
   __syncthreads();
-  // rows of a head's channels
-  const int chans = per / p.cols;
-  const int cc = threadIdx.x / chans, dd = threadIdx.x % chans;
+  if (tid < 16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, part[i][tid]);
+    top[tid] = m == -INFINITY ? 0.f : m;
+  }
+  __syncthreads();
+  // ---- outputs [channel][head], numbers 4 * quad .. of this block
+  const int per = 256 / (2 * p.cols) * (2 * p.cols);     // whole channels, whole quads
+  const int e0 = (int)blockIdx.y * per + 4 * (tid & 63), g4 = tid >> 6;
+  const bool live = 4 * (tid & 63) < per && e0 < D * p.cols;
+  int c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = (e0 + j) % p.cols;
+  const float* src = p.part_o + piece0 * D * p.cols + e0;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int i0 = 0; i0 < pieces; i0 += kSmChunk) {
+    const int n = min(pieces - i0, kSmChunk);
+    if (hc < p.cols) {
+      const float ref = top[hc];
+#pragma unroll 4
+      for (int i = pl; i < n; i += 16) {
+        const float2 x = ml[(long long)(i0 + i) * p.cols];
+        const float f = fast_exp2(x.x - ref);            // a piece without a visible token: 2^-inf
+        factor[i][hc] = f;
+        l += x.y * f;
+      }
+    }
+    __syncthreads();
+    if (live)
+#pragma unroll 8
+      for (int i = g4; i < n; i += 4) {
+        const float4 o = *reinterpret_cast<const float4*>(src + (long long)(i0 + i) * D * p.cols);
+        acc.x = fmaf(o.x, factor[i][c[0]], acc.x);
+        acc.y = fmaf(o.y, factor[i][c[1]], acc.y);
+        acc.z = fmaf(o.z, factor[i][c[2]], acc.z);
+        acc.w = fmaf(o.w, factor[i][c[3]], acc.w);
+      }
+    __syncthreads();
+  }
+  part[pl][hc] = l;
+  quad[g4][tid & 63] = acc;
+  __syncthreads();
+  if (tid < 16) {
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) l += part[i][tid];
+    const float inv = l == 0.f ? 0.f : 1.f / l;          // no token: zeros
+    sum[tid] = inv;
+    const int head = (pair % p.tiles) * p.cols + tid;
+    if (p.ml && blockIdx.y == 0 && tid < p.cols && head < p.G)
+      reinterpret_cast<float2*>(p.ml)[((long long)b * p.Hkv + pair / p.tiles) * p.G + head] = make_float2(top[tid], inv);
+  }
+  __syncthreads();
+  // ---- rows of a head's channels
+  const int chans = per / p.cols, cc = tid / chans, dd = tid % chans;
   const int hh = (pair % p.tiles) * p.cols + cc, dg = blockIdx.y * chans + dd;
-  if (cc < p.cols && hh < p.G && dg < D)
-    p.out[(long long)p.query_start_loc[b] * p.ldo + (h * p.G + hh) * D + dg] = __float2bfloat16_rn(tile[dd * p.cols + cc]);
+  if (cc < p.cols && hh < p.G && dg < D) {
+    const int e = dd * p.cols + cc;
+    const float* q = reinterpret_cast<const float*>(quad);
+    const float o = (q[e] + q[256 + e]) + (q[512 + e] + q[768 + e]);
+    p.out[(long long)p.query_start_loc[b] * p.ldo + ((pair / p.tiles) * p.G + hh) * D + dg] = __float2bfloat16_rn(o * sum[cc]);
+  }
 }
 
 // weights[b, h, j] += sum over the pair's heads of 2^(s - M) / l, a thread per token.
@@ -461,59 +505,53 @@ int decode_launch(const ScaledDecodeParams& p, int blocks, int items, cudaStream
   constexpr int smem = kSdWarps * kSdRing;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(scaled_decode_kernel<D, NT>), smem) != cudaSuccess) return -20;
   if (launch_chain(scaled_decode_kernel<D, NT>, dim3(blocks), dim3(kSdWarps * 32), smem, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
-  const int per = 256 / p.cols;
-  if (launch_chain(scaled_merge_kernel<D>, dim3(items, (D + per - 1) / per), dim3(256), 0, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
+  const int chans = 256 / (2 * p.cols) * 2;
+  if (launch_chain(scaled_merge_kernel<D>, dim3(items, (D + chans - 1) / chans), dim3(256), 0, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
   return 0;
 }
 
 }  // namespace
 
-// Sizes of the workspaces: numbers [pieces * D * cols], [pieces * cols * 2].  A piece is a pair's share of a warp's run.
-extern "C" int atlas_attn_scaled_decode_plan(int nd, int Hq, int Hkv, int max_seq_len, int num_sms, int* blocks, int* cols, long long* pieces) {
-  if (nd <= 0 || Hkv <= 0 || Hq % Hkv) return -1;
-  const int G = Hq / Hkv, tiles = (G + 15) / 16;
-  *cols = G <= 16 ? (G + 1) / 2 * 2 : 16;
-  const long long items = (long long)nd * Hkv * tiles, pages = items * ((max_seq_len + kSdPage - 1) / kSdPage);
-  if (pages > 0x3fffffffll) return -1;
-  const long long want = (pages + kSdLeast - 1) / kSdLeast;
-  *blocks = (int)(want < num_sms ? (want > 0 ? want : 1) : num_sms);
-  *pieces = items + (long long)*blocks * kSdWarps;
-  return 0;
-}
-
-// Decode rows of a step: sequence b's row is query_start_loc[b].  `scores`, `ml` and `weights` come together: [nd * Hkv][width][cols of G
-// rounded up to two], [nd][Hq][2] and the sums [b][h][token].  -1: sizes or alignment outside of what the kernels take.
-extern "C" int atlas_attn_scaled_decode(const void* q, long long ldq, void* out, long long ldo, const void* k_cache, const void* v_cache,
-                                        const float* k_scale, long long ks_ld, int ks_h, const float* v_scale, long long vs_ld, int vs_h,
-                                        const int* block_tables, int bt_ld, int bt_cols, const int* seq_lens, const int* query_start_loc, int nd, float scale,
-                                        int Hq, int Hkv, int D, int window, int num_pages, int max_seq_len, int num_sms, float* part_o,
-                                        float* part_ml, float* scores, long long width, float* ml, float* weights, long long w_ld_b,
-                                        long long w_ld_h, unsigned long long* status, void* stream) {
-  if (nd <= 0) return 0;
-  if ((D != 64 && D != 128 && D != 256) || Hkv <= 0 || Hq % Hkv || ldq % 8 || (reinterpret_cast<uintptr_t>(q) & 15)) return -1;
-  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return -1;
+// Decode rows of a step: sequence b's row is query_start_loc[b].  Arguments as one record (see kv_scaled.cu).  Workspaces: part_o [pieces][D]
+// [cols] and part_ml [pieces][cols][2] with cols = min(G rounded up to two, 16) and pieces = pairs + warps, a pair being (sequence, key head,
+// group of 16 query heads).  With `weights`: scores [nd * Hkv][width][G rounded up to two], ml [nd][Hq][2] and the sums
+// [sequence][head][token], `width` tokens each.  -1: sizes or alignment outside of what the kernels take.
+struct DecodeRecord {
+  const void* q; long long ldq; void* out; long long ldo; const void* k_cache; const void* v_cache;
+  const float* ks; long long ks_ld, ks_h; const float* vs; long long vs_ld, vs_h;
+  const int* tables; long long bt_ld, bt_cols; const int* seq_lens; const int* starts;
+  long long nd, Hq, Hkv, D, window, num_pages, max_len, blocks; float* part_o; float* part_ml;
+  float* scores; long long width; float* ml; float* weights; long long w_ld_b, w_ld_h; double scale; void* status; void* stream;
+};
+extern "C" int atlas_attn_scaled_decode(const void* record) {
+  const DecodeRecord& r = *static_cast<const DecodeRecord*>(record);
+  const int D = (int)r.D;
+  if (r.nd <= 0) return 0;
+  if ((D != 64 && D != 128 && D != 256) || r.Hkv <= 0 || r.Hq % r.Hkv || r.ldq % 8 || (reinterpret_cast<uintptr_t>(r.q) & 15)) return -1;
+  if ((reinterpret_cast<uintptr_t>(r.k_cache) | reinterpret_cast<uintptr_t>(r.v_cache)) & 15) return -1;
   ScaledDecodeParams p;
-  int blocks;
-  long long pieces;
-  if (atlas_attn_scaled_decode_plan(nd, Hq, Hkv, max_seq_len, num_sms, &blocks, &p.cols, &pieces)) return -1;
-  p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.out = (__nv_bfloat16*)out; p.ldo = ldo;
-  p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache;
-  p.k_scale = k_scale; p.v_scale = v_scale; p.ks_ld = ks_ld; p.vs_ld = vs_ld; p.ks_h = ks_h; p.vs_h = vs_h;
-  p.block_tables = block_tables; p.bt_ld = bt_ld; p.bt_cols = bt_cols; p.seq_lens = seq_lens; p.query_start_loc = query_start_loc;
-  p.nd = nd; p.Hkv = Hkv; p.G = Hq / Hkv; p.tiles = (p.G + 15) / 16;
-  p.window = window; p.num_pages = num_pages; p.warps = blocks * kSdWarps;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.part_o = part_o; p.part_ml = part_ml;
-  p.scores = weights ? scores : nullptr; p.width = width; p.score_cols = (p.G + 1) / 2 * 2; p.ml = weights ? ml : nullptr;
-  p.status = status;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int items = nd * Hkv * p.tiles;
+  p.q = (const __nv_bfloat16*)r.q; p.ldq = r.ldq; p.out = (__nv_bfloat16*)r.out; p.ldo = r.ldo;
+  p.k_cache = (const uint8_t*)r.k_cache; p.v_cache = (const uint8_t*)r.v_cache;
+  p.k_scale = r.ks; p.v_scale = r.vs; p.ks_ld = r.ks_ld; p.vs_ld = r.vs_ld; p.ks_h = (int)r.ks_h; p.vs_h = (int)r.vs_h;
+  p.block_tables = r.tables; p.bt_ld = (int)r.bt_ld; p.bt_cols = (int)r.bt_cols; p.seq_lens = r.seq_lens; p.query_start_loc = r.starts;
+  p.nd = (int)r.nd; p.Hkv = (int)r.Hkv; p.G = (int)(r.Hq / r.Hkv); p.tiles = (p.G + 15) / 16;
+  p.cols = p.G <= 16 ? (p.G + 1) / 2 * 2 : 16;
+  // the list's entries and the runs' bounds are 32-bit numbers
+  const long long items = r.nd * r.Hkv * p.tiles;
+  if (items * r.bt_cols > 0x3fffffffll || items > 0x7fffffffll || r.bt_cols > (1 << 26) || r.blocks <= 0 || r.blocks > 65535) return -1;
+  p.window = (int)r.window; p.num_pages = (int)r.num_pages; p.warps = (int)r.blocks * kSdWarps;
+  p.scale_log2 = (float)(r.scale * 1.4426950408889634);
+  p.part_o = r.part_o; p.part_ml = r.part_ml;
+  p.scores = r.weights ? r.scores : nullptr; p.width = r.width; p.score_cols = (p.G + 1) / 2 * 2; p.ml = r.weights ? r.ml : nullptr;
+  p.status = (status_t*)r.status;
+  cudaStream_t st = (cudaStream_t)r.stream;
+  const int blocks = (int)r.blocks, n = (int)items;
   int rc;
-  if (p.G <= 8) rc = D == 64 ? decode_launch<64, 1>(p, blocks, items, st) : D == 128 ? decode_launch<128, 1>(p, blocks, items, st) : decode_launch<256, 1>(p, blocks, items, st);
-  else rc = D == 64 ? decode_launch<64, 2>(p, blocks, items, st) : D == 128 ? decode_launch<128, 2>(p, blocks, items, st) : decode_launch<256, 2>(p, blocks, items, st);
-  if (rc || !weights) return rc;
-  const int chunks = (max_seq_len + 1023) / 1024;
-  if (launch_chain(scaled_weigh_kernel, dim3(nd * Hkv, chunks < 64 ? chunks : 64), dim3(256), (size_t)p.G * sizeof(float2), st, p, weights, w_ld_b,
-                   w_ld_h) != cudaSuccess) { cudaGetLastError(); return -20; }
+  if (p.G <= 8) rc = D == 64 ? decode_launch<64, 1>(p, blocks, n, st) : D == 128 ? decode_launch<128, 1>(p, blocks, n, st) : decode_launch<256, 1>(p, blocks, n, st);
+  else rc = D == 64 ? decode_launch<64, 2>(p, blocks, n, st) : D == 128 ? decode_launch<128, 2>(p, blocks, n, st) : decode_launch<256, 2>(p, blocks, n, st);
+  if (rc || !r.weights) return rc;
+  const long long chunks = (r.max_len + 1023) / 1024;
+  if (launch_chain(scaled_weigh_kernel, dim3((unsigned)(r.nd * r.Hkv), (unsigned)(chunks < 1 ? 1 : chunks < 64 ? chunks : 64)), dim3(256),
+                   (size_t)p.G * sizeof(float2), st, p, r.weights, r.w_ld_b, r.w_ld_h) != cudaSuccess) { cudaGetLastError(); return -20; }
   return 0;
 }

@@ -715,48 +715,45 @@ int launch_tiles(Kern kern, int smem, dim3 grid, int threads, const CUtensorMap&
 
 }  // namespace
 
-// Rows of chunk sequences: `num_tiles` query tiles of 128 / G tokens, each (sequence, first token of the tile in its chunk).  `ml` (or null)
-// gets every row's reference and 1 / l for atlas_attn_scaled_chunk_weigh.  -1: sizes or alignment outside of what the kernel takes.
-extern "C" int atlas_attn_scaled_chunk(const void* q, long long ldq, void* out, long long ldo, const void* k_cache, const void* v_cache,
-                                       const float* k_scale, long long ks_ld, int ks_h, const float* v_scale, long long vs_ld, int vs_h,
-                                       const int* block_tables, int bt_ld, int bt_cols, const int* seq_lens, const int* query_start_loc, const int* tile_seq,
-                                       const int* tile_q0, int num_tiles, int total_tokens, float scale, int Hq, int Hkv, int D, int window,
-                                       int num_pages, float* ml, unsigned long long* status, void* stream) {
-  if (num_tiles <= 0) return 0;
-  if ((D != 64 && D != 128 && D != 256) || Hkv <= 0 || Hq % Hkv || Hq / Hkv > kScRows) return -1;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || ldq % 8 || ldo % 8 || (reinterpret_cast<uintptr_t>(out) & 15)) return -1;
-  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return -1;
-  const int G = Hq / Hkv;
+// Rows of chunk sequences: `tiles` query tiles of 128 / G tokens, each (sequence, first token of the tile in its chunk); `ml` (or null) gets
+// every row's reference and 1 / l.  With `weights`, tiles of 128 cached tokens follow, each (sequence, first token), whose sums grow by the
+// rows' softmax weights.  Arguments as one record (see kv_scaled.cu).  -1: sizes or alignment outside of what the kernels take.
+struct ChunkRecord {
+  const void* q; long long ldq; void* out; long long ldo; const void* k_cache; const void* v_cache;
+  const float* ks; long long ks_ld, ks_h; const float* vs; long long vs_ld, vs_h;
+  const int* tables; long long bt_ld, bt_cols; const int* seq_lens; const int* starts;
+  const int* tile_seq; const int* tile_q0; long long tiles, total_tokens, Hq, Hkv, D, window, num_pages; float* ml;
+  const int* key_seq; const int* key_k0; long long key_tiles; float* weights; long long w_ld_b, w_ld_h, width; double scale; void* status;
+  void* stream;
+};
+extern "C" int atlas_attn_scaled_chunk(const void* record) {
+  const ChunkRecord& r = *static_cast<const ChunkRecord*>(record);
+  const int D = (int)r.D;
+  if (r.tiles <= 0) return 0;
+  if ((D != 64 && D != 128 && D != 256) || r.Hkv <= 0 || r.Hkv > 65535 || r.Hq % r.Hkv || r.Hq / r.Hkv > kScRows) return -1;
+  if ((reinterpret_cast<uintptr_t>(r.q) & 15) || r.ldq % 8 || r.ldo % 8 || (reinterpret_cast<uintptr_t>(r.out) & 15)) return -1;
+  if ((reinterpret_cast<uintptr_t>(r.k_cache) | reinterpret_cast<uintptr_t>(r.v_cache)) & 15) return -1;
+  if (r.bt_cols > (1 << 26) || r.tiles > 0x7fffffffll || r.total_tokens > 0x7fffffffll || (r.weights && !r.ml)) return -1;
+  const int Hq = (int)r.Hq, Hkv = (int)r.Hkv, G = Hq / Hkv;
   CUtensorMap tq;
-  if (int rc = query_map(&tq, q, ldq, total_tokens, Hq, G, D)) return rc;
-  ScChunkParams p{(__nv_bfloat16*)out, ldo, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, ks_ld, vs_ld, ks_h, vs_h,
-                  block_tables, bt_ld, bt_cols, seq_lens, query_start_loc, tile_seq, tile_q0, scale * 1.4426950408889634f, Hq, Hkv, G, window, num_pages,
-                  reinterpret_cast<float2*>(ml), status};
-  const dim3 grid(num_tiles, Hkv);
-  cudaStream_t st = (cudaStream_t)stream;
-  if (D == 64) return launch_tiles(scaled_chunk_kernel<64>, ScTile<64>::kSmem, grid, kScThreads, tq, p, st);
-  if (D == 128) return launch_tiles(scaled_chunk_kernel<128>, ScTile<128>::kSmem, grid, kScThreads, tq, p, st);
-  return launch_tiles(scaled_chunk_kernel<256>, ScTile<256>::kSmem, grid, kScThreads, tq, p, st);
-}
-
-// weights[b, h, token] += the chunk's rows' softmax weights; tiles of 128 cached tokens, each (sequence, first token).
-extern "C" int atlas_attn_scaled_chunk_weigh(const void* q, long long ldq, const void* k_cache, const float* k_scale, long long ks_ld, int ks_h,
-                                             const int* block_tables, int bt_ld, int bt_cols, const int* seq_lens, const int* query_start_loc,
-                                             const int* tile_seq, const int* tile_k0, int num_tiles, int total_tokens, float scale, int Hq, int Hkv,
-                                             int D, int window, int num_pages, const float* ml, float* weights, long long w_ld_b, long long w_ld_h,
-                                             int width, unsigned long long* status, void* stream) {
-  if (num_tiles <= 0) return 0;
-  if ((D != 64 && D != 128 && D != 256) || Hkv <= 0 || Hq % Hkv || Hq / Hkv > kScRows) return -1;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || ldq % 8 || (reinterpret_cast<uintptr_t>(k_cache) & 15)) return -1;
-  const int G = Hq / Hkv;
-  CUtensorMap tq;
-  if (int rc = query_map(&tq, q, ldq, total_tokens, Hq, G, D)) return rc;
-  ScWeighParams p{(const uint8_t*)k_cache, k_scale, ks_ld, ks_h, block_tables, bt_ld, bt_cols, seq_lens, query_start_loc, tile_seq, tile_k0,
-                  scale * 1.4426950408889634f, Hq, Hkv, G, window, num_pages, reinterpret_cast<const float2*>(ml), weights, w_ld_b, w_ld_h, width,
-                  status};
-  const dim3 grid(num_tiles, Hkv);
-  cudaStream_t st = (cudaStream_t)stream;
-  if (D == 64) return launch_tiles(scaled_chunk_weigh_kernel<64>, SwTile<64>::kSmem, grid, kSwThreads, tq, p, st);
-  if (D == 128) return launch_tiles(scaled_chunk_weigh_kernel<128>, SwTile<128>::kSmem, grid, kSwThreads, tq, p, st);
-  return launch_tiles(scaled_chunk_weigh_kernel<256>, SwTile<256>::kSmem, grid, kSwThreads, tq, p, st);
+  if (int rc = query_map(&tq, r.q, r.ldq, (int)r.total_tokens, Hq, G, D)) return rc;
+  const float scale_log2 = (float)(r.scale * 1.4426950408889634);
+  status_t* status = (status_t*)r.status;
+  cudaStream_t st = (cudaStream_t)r.stream;
+  ScChunkParams p{(__nv_bfloat16*)r.out, r.ldo, (const uint8_t*)r.k_cache, (const uint8_t*)r.v_cache, r.ks, r.vs, r.ks_ld, r.vs_ld, (int)r.ks_h,
+                  (int)r.vs_h, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.seq_lens, r.starts, r.tile_seq, r.tile_q0, scale_log2, Hq, Hkv, G,
+                  (int)r.window, (int)r.num_pages, reinterpret_cast<float2*>(r.ml), status};
+  const dim3 grid((unsigned)r.tiles, Hkv);
+  int rc;
+  if (D == 64) rc = launch_tiles(scaled_chunk_kernel<64>, ScTile<64>::kSmem, grid, kScThreads, tq, p, st);
+  else if (D == 128) rc = launch_tiles(scaled_chunk_kernel<128>, ScTile<128>::kSmem, grid, kScThreads, tq, p, st);
+  else rc = launch_tiles(scaled_chunk_kernel<256>, ScTile<256>::kSmem, grid, kScThreads, tq, p, st);
+  if (rc || !r.weights || r.key_tiles <= 0) return rc;
+  ScWeighParams w{(const uint8_t*)r.k_cache, r.ks, r.ks_ld, (int)r.ks_h, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.seq_lens, r.starts, r.key_seq,
+                  r.key_k0, scale_log2, Hq, Hkv, G, (int)r.window, (int)r.num_pages, reinterpret_cast<const float2*>(r.ml), r.weights, r.w_ld_b,
+                  r.w_ld_h, (int)r.width, status};
+  const dim3 keys((unsigned)r.key_tiles, Hkv);
+  if (D == 64) return launch_tiles(scaled_chunk_weigh_kernel<64>, SwTile<64>::kSmem, keys, kSwThreads, tq, w, st);
+  if (D == 128) return launch_tiles(scaled_chunk_weigh_kernel<128>, SwTile<128>::kSmem, keys, kSwThreads, tq, w, st);
+  return launch_tiles(scaled_chunk_weigh_kernel<256>, SwTile<256>::kSmem, keys, kSwThreads, tq, w, st);
 }

@@ -11,9 +11,9 @@
 //   kv_evict_select_kernel   per sequence and head: the heaviest tokens' positions, in order
 //   kv_evict_move_kernel     those tokens into new pages, rescaled
 //
-// Layout as in elementwise.cu: K [pages, Hkv, 16, D], V [pages, Hkv, D, 16].  All four are bound by memory: a warp owns the 16 tokens of
-// one page and head, a lane D / 32 neighbouring channels of every token, so that K rows, V rows (16 bytes) and bf16 rows are all moved in
-// whole sectors without a transposition.
+// Layout as in elementwise.cu: K [pages, Hkv, 16, D], V [pages, Hkv, D, 16].  All four are bound by memory: warps own the tokens of one page
+// and head, a lane D / 32 neighbouring channels of every token, so that K rows, V rows (16 bytes) and bf16 rows are all moved in whole
+// sectors without a transposition.
 #include "common.cuh"
 #include "host_api.h"
 
@@ -70,25 +70,22 @@ ATLAS_DEVICE Codes<V> narrow(const float (&f)[V], float by) {
   for (int i = 0; i < V; i += 2) c.w[i >> 2] |= f32_to_codes2(f[i] * by, f[i + 1] * by) << (8 * (i & 3));
   return c;
 }
-// sixteen codes (one channel of a page's values) times a power of two
-ATLAS_DEVICE uint4 rescale16(uint4 v, float by) {
-  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 a = codes2_to_f32(w[i] & 0xFFFFu), b = codes2_to_f32(w[i] >> 16);
-    w[i] = f32_to_codes2(a.x * by, a.y * by) | (f32_to_codes2(b.x * by, b.y * by) << 16);
-  }
-  return v;
+template <int V>
+struct Raw { uint32_t w[V / 2]; };                    // V consecutive bf16 numbers
+
+template <int V>
+ATLAS_DEVICE Raw<V> load_raw(const __nv_bfloat16* p) {
+  Raw<V> r;
+  if constexpr (V == 2) r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  else if constexpr (V == 4) { const uint2 t = *reinterpret_cast<const uint2*>(p); r.w[0] = t.x; r.w[1] = t.y; }
+  else { const uint4 t = *reinterpret_cast<const uint4*>(p); r.w[0] = t.x; r.w[1] = t.y; r.w[2] = t.z; r.w[3] = t.w; }
+  return r;
 }
 template <int V>
-ATLAS_DEVICE void load_row(const __nv_bfloat16* p, float (&f)[V]) {
-  uint32_t w[V / 2];
-  if constexpr (V == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
-  else if constexpr (V == 4) { const uint2 t = *reinterpret_cast<const uint2*>(p); w[0] = t.x; w[1] = t.y; }
-  else { const uint4 t = *reinterpret_cast<const uint4*>(p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
+ATLAS_DEVICE void unpack(const Raw<V>& r, float (&f)[V]) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
-    const float2 t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    const float2 t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.w[i]));
     f[2 * i] = t.x; f[2 * i + 1] = t.y;
   }
 }
@@ -124,14 +121,23 @@ struct Turn {
   float c[V], s[V];      // of this lane's channels; the partner's share comes with its sign
   int hl;                // lanes between partners; lanes from 2 * hl on are not rotated
   ATLAS_DEVICE void angles(const float* rope_row, int rotary, int lane) {
-    hl = rotary / (2 * V);
     if (lane >= 2 * hl) return;
-    const int d = (lane < hl ? lane : lane - hl) * V;
+    const float* at = rope_row + (lane < hl ? lane : lane - hl) * V;
+    load_floats(at, c);
+    load_floats(at + rotary / 2, s);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      c[i] = __ldg(rope_row + d + i);
-      const float t = __ldg(rope_row + rotary / 2 + d + i);
-      s[i] = lane < hl ? -t : t;
+    for (int i = 0; i < V; ++i) s[i] = lane < hl ? -s[i] : s[i];
+  }
+  static ATLAS_DEVICE void load_floats(const float* at, float (&f)[V]) {      // rows of the table start on 16 bytes, or 8 for V = 2
+    if constexpr (V == 2) {
+      const float2 t = __ldg(reinterpret_cast<const float2*>(at));
+      f[0] = t.x; f[1] = t.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const float4 t = __ldg(reinterpret_cast<const float4*>(at + i));
+        f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
+      }
     }
   }
   ATLAS_DEVICE void operator()(float (&x)[V], const float (&w)[V], bool normed, int norm_dim, float eps, int lane) const {
@@ -156,47 +162,56 @@ struct Turn {
 template <int V>
 ATLAS_DEVICE void norm_weights(const __nv_bfloat16* w, int plus_one, int lane, float (&out)[V]) {
   if (!w) return;
-  load_row<V>(w + lane * V, out);
+  unpack<V>(load_raw<V>(w + lane * V), out);
 #pragma unroll
   for (int i = 0; i < V; ++i) out[i] += plus_one ? 1.f : 0.f;
 }
 
 constexpr int kWriteHeads = 8;      // query heads of a token that one warp turns with the same angles
 
-// Cache blocks: a warp takes the rows of one step that fall into one page, for one head's keys or values.  A run of such rows starts where
-// the slot is not the one behind the row before.  Two passes over its rows (the second one hits L1): the largest magnitude, then codes.
-template <int D>
-__global__ void __launch_bounds__(256)
+// Cache blocks: `W` warps take the rows of one step that fall into one page, for one head's keys or values, in groups of four slots; a run of
+// such rows starts where the slot is not the one behind the row before.  Prompts: four warps, a group each, every row loaded and turned once
+// and waiting in registers for the page's largest magnitude.  (A warp per page took 30 us for 517 rows of 256-wide heads, sixteen rows' angles
+// one after the other; four take 9.)  Decode steps: one warp, since most runs are one row, and 128 rows of 8 heads fit the GPU at once (7 us; with
+// four warps 11); a longer run is loaded and turned twice.
+template <int D, int W>
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 4)
 kv_scaled_write_kernel(const ScaledWriteParams p) {
   constexpr int V = D / 32;
+  __shared__ float sh_amax[8];
+  __shared__ uint32_t sh_v[W > 1 ? 8 / W : 1][W > 1 ? D * 4 : 1];      // the tasks' value pages: [channel] 16 tokens
   chain_trigger();
   chain_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kv_blocks = p.kv_blocks_x * p.kv_blocks_y;
   float w[V];
   Turn<V> turn;
-  turn.hl = 0;
+  turn.hl = p.rotary / (2 * V);
   if ((int)blockIdx.x >= kv_blocks) {
     const int groups = (p.Hq + kWriteHeads - 1) / kWriteHeads;
-    const long long unit = (long long)(blockIdx.x - kv_blocks) * 8 + warp;
-    if (unit >= (long long)p.T * groups) return;
-    const int t = (int)(unit / groups), h0 = (int)(unit % groups) * kWriteHeads;
-    if (p.rotary) turn.angles(p.rope + (long long)p.positions[t] * p.rotary, p.rotary, lane);
-    norm_weights<V>(p.q_norm, p.plus_one, lane, w);
-    float x[kWriteHeads][V];
+    const unsigned unit = (blockIdx.x - kv_blocks) * 8 + warp, at = unit / groups;
+    if (at >= (unsigned)p.T) return;
+    const int t = (int)at, h0 = (int)(unit % groups) * kWriteHeads;
+    Raw<V> raw[kWriteHeads];
 #pragma unroll
     for (int i = 0; i < kWriteHeads; ++i)
-      if (h0 + i < p.Hq) load_row<V>(p.q + t * p.ldq + (h0 + i) * D + lane * V, x[i]);
+      if (h0 + i < p.Hq) raw[i] = load_raw<V>(p.q + t * p.ldq + (h0 + i) * D + lane * V);
+    if (p.rotary) turn.angles(p.rope + (long long)p.positions[t] * p.rotary, p.rotary, lane);
+    norm_weights<V>(p.q_norm, p.plus_one, lane, w);
 #pragma unroll
     for (int i = 0; i < kWriteHeads; ++i) {
       if (h0 + i >= p.Hq) return;
-      turn(x[i], w, p.q_norm != nullptr, p.norm_dim, p.eps, lane);
-      store_row<V>(p.q_out + t * p.ldqo + (h0 + i) * D + lane * V, x[i]);
+      float x[V];
+      unpack<V>(raw[i], x);
+      turn(x, w, p.q_norm != nullptr, p.norm_dim, p.eps, lane);
+      store_row<V>(p.q_out + t * p.ldqo + (h0 + i) * D + lane * V, x);
     }
     return;
   }
-  const int task = (blockIdx.x / p.kv_blocks_x) * 8 + warp;           // (K heads, then V heads)
-  if (task >= 2 * p.Hkv) return;
+  const int local = warp / W;
+  const int task = (blockIdx.x / p.kv_blocks_x) * (8 / W) + local;     // K heads, then V heads
+  const bool on = task < 2 * p.Hkv;
+  if (W == 1 && !on) return;
   const bool is_k = task < p.Hkv;
   const int h = is_k ? task : task - p.Hkv;
   const __nv_bfloat16* src = (is_k ? p.k : p.v) + h * D + lane * V;
@@ -204,88 +219,125 @@ kv_scaled_write_kernel(const ScaledWriteParams p) {
   if (is_k) norm_weights<V>(p.k_norm, p.plus_one, lane, w);
   const bool normed = is_k && p.k_norm != nullptr;
   const int row0 = (blockIdx.x % p.kv_blocks_x) * p.rows_per_block;
-  for (int t0 = row0; t0 < min(row0 + p.rows_per_block, p.T); ++t0) {
+  for (int t0 = row0; t0 < min(row0 + p.rows_per_block, p.T); ++t0) {   // the same for the whole block
     const int slot = p.slots[t0];
     if (slot < 0 || slot >= p.num_pages * kScPage) continue;
     const int page = slot / kScPage, off = slot % kScPage;
     if (off > 0 && t0 > 0 && p.slots[t0 - 1] == slot - 1) continue;    // the row before began this run
     // rows t0 .. t0 + n - 1 fill slots off .. off + n - 1 of the page
-    const bool mine = lane < kScPage - off && t0 + lane < p.T && p.slots[min(t0 + lane, p.T - 1)] == slot + lane;
+    const int mine_t = min(t0 + lane, p.T - 1);
+    const bool mine = lane < kScPage - off && t0 + lane < p.T && p.slots[mine_t] == slot + lane;
+    const int my_pos = is_k && p.rotary ? p.positions[mine_t] : 0;
     const int n = __ffs(~__ballot_sync(0xffffffffu, mine)) - 1;
     const long long base = ((long long)page * p.Hkv + h) * (kScPage * D);
     float* scale_at = is_k ? p.k_scale + page * p.ks_ld + h * p.ks_h : p.v_scale + page * p.vs_ld + h * p.vs_h;
-    const float before = off > 0 ? *scale_at : 0.f;
-    auto row = [&](int r, float (&x)[V]) {
-      load_row<V>(src + (long long)(t0 + r) * ld, x);
-      if (is_k) {
-        if (p.rotary) turn.angles(p.rope + (long long)p.positions[t0 + r] * p.rotary, p.rotary, lane);
-        turn(x, w, normed, p.norm_dim, p.eps, lane);
+    float before = 0.f;
+    if (on && off > 0) before = *scale_at;
+    const int g_lo = W == 1 ? off / 4 : (warp & 3), g_hi = W == 1 ? (off + n - 1) / 4 : (warp & 3);      // groups with rows of the run
+    float x[4][V];
+    auto load_group = [&](int g, float amax) {
+      Raw<V> raw[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * g + j - off;
+        if (r >= 0 && r < n) raw[j] = load_raw<V>(src + (long long)(t0 + r) * ld);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * g + j - off;
+        if (r < 0 || r >= n) continue;
+        unpack<V>(raw[j], x[j]);
+        if (is_k) {
+          if (p.rotary) turn.angles(p.rope + (long long)__shfl_sync(0xffffffffu, my_pos, r) * p.rotary, p.rotary, lane);
+          turn(x[j], w, normed, p.norm_dim, p.eps, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) amax = fmaxf(amax, fabsf(x[j][i]));
+      }
+      return amax;
     };
     float amax = 0.f;
-#pragma unroll 4
-    for (int r = 0; r < n; ++r) {
-      float x[V];
-      row(r, x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    }
+    if (on)
+      for (int g = g_lo; g <= g_hi; ++g) amax = load_group(g, amax);
     amax = warp_max(amax);
+    if constexpr (W > 1) {
+      if (lane == 0) sh_amax[warp] = amax;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < W; ++i) amax = fmaxf(amax, sh_amax[local * W + i]);
+    }
     int e = block_exponent(amax);
     const int e_old = exponent_of(before);
     if (off > 0) e = max(e, e_old);
     const float inv = pow2i(-e);
     const bool raised = off > 0 && e != e_old;
     const float shift = raised ? pow2i(max(e_old - e, -126)) : 1.f;
-    if (is_k) {
-      uint8_t* page_k = p.k_cache + base + lane * V;
-      if (raised)
-        for (int r = 0; r < off; ++r) {
-          float x[V];
-          widen<V>(load_codes<V>(page_k + r * D), x);
-          store_codes<V>(page_k + r * D, narrow<V>(x, shift));
+    // a group's tokens: rows of the run, tokens before them (to the new scale, if it rose), tokens behind them (as they were)
+    auto store_group = [&](int g) {
+      if (is_k) {
+        uint8_t* page_k = p.k_cache + base + lane * V;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int s = 4 * g + j, r = s - off;
+          if (r >= 0 && r < n) {
+            store_codes<V>(page_k + s * D, narrow<V>(x[j], inv));
+          } else if (r < 0 && raised) {
+            float y[V];
+            widen<V>(load_codes<V>(page_k + s * D), y);
+            store_codes<V>(page_k + s * D, narrow<V>(y, shift));
+          }
         }
-#pragma unroll 4
-      for (int r = 0; r < n; ++r) {
-        float x[V];
-        row(r, x);
-        store_codes<V>(page_k + (off + r) * D, narrow<V>(x, inv));
+        return;
       }
-    } else {
-      uint4* page_v = reinterpret_cast<uint4*>(p.v_cache + base) + lane * V;       // [channel] 16 tokens
-      uint32_t out[V][4];
-      const bool whole = n == kScPage;
+      uint32_t word[V];                                                // four tokens of each channel: a word of the channel's sixteen
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        uint4 was = make_uint4(0, 0, 0, 0);
-        if (!whole) was = page_v[i];
-        const uint4 moved = raised ? rescale16(was, shift) : was;
-        const uint32_t* a = reinterpret_cast<const uint32_t*>(&was);
-        const uint32_t* b = reinterpret_cast<const uint32_t*>(&moved);
+      for (int i = 0; i < V; ++i) word[i] = 0;
+      uint32_t fresh = 0, old = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {                                  // tokens before `off` moved, those behind the run as they were
-          const int lo = min(max(off - 4 * j, 0), 4);
-          const uint32_t m = lo == 4 ? 0xffffffffu : ((1u << (8 * lo)) - 1u);
-          out[i][j] = (b[j] & m) | (a[j] & ~m);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * g + j - off;
+        if (r < 0) old |= 0xFFu << (8 * j);
+        if (r < 0 || r >= n) continue;
+        fresh |= 0xFFu << (8 * j);
+        const Codes<V> c = narrow<V>(x[j], inv);
+#pragma unroll
+        for (int i = 0; i < V; ++i) word[i] |= ((c.w[i >> 2] >> (8 * (i & 3))) & 0xFFu) << (8 * j);
       }
-#pragma unroll
-      for (int tok = 0; tok < kScPage; ++tok) {
-        if (tok < off || tok >= off + n) continue;                     // the same for all lanes
-        float x[V];
-        load_row<V>(src + (long long)(t0 + tok - off) * ld, x);
-        const Codes<V> c = narrow<V>(x, inv);
+      uint32_t* at = reinterpret_cast<uint32_t*>(p.v_cache + base) + lane * V * 4 + g;
+      if (fresh != 0xffffffffu) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const uint32_t code = (c.w[i >> 2] >> (8 * (i & 3))) & 0xFFu;
-          out[i][tok >> 2] = (out[i][tok >> 2] & ~(0xFFu << (8 * (tok & 3)))) | (code << (8 * (tok & 3)));
+          const uint32_t was = at[4 * i];
+          uint32_t moved = was;
+          if (raised && old) {
+            const float2 lo = codes2_to_f32(was & 0xFFFFu), hi = codes2_to_f32(was >> 16);
+            moved = f32_to_codes2(lo.x * shift, lo.y * shift) | (f32_to_codes2(hi.x * shift, hi.y * shift) << 16);
+          }
+          word[i] = (word[i] & fresh) | (moved & old) | (was & ~(fresh | old));
         }
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) page_v[i] = make_uint4(out[i][0], out[i][1], out[i][2], out[i][3]);
+      for (int i = 0; i < V; ++i) {
+        if constexpr (W > 1) sh_v[local][(lane * V + i) * 4 + g] = word[i];
+        else at[4 * i] = word[i];
+      }
+    };
+    if constexpr (W == 1) {
+      for (int g = raised ? 0 : g_lo; g <= g_hi; ++g) {
+        if (g >= g_lo && g_lo != g_hi) load_group(g, 0.f);
+        store_group(g);
+      }
+      __syncwarp();
+      if (lane == 0 && (off == 0 || raised)) *scale_at = pow2i(e);
+    } else {
+      if (on) store_group(warp & 3);
+      __syncthreads();
+      if (on && !is_k) {                                               // whole channels, 16 bytes each
+        uint4* page_v = reinterpret_cast<uint4*>(p.v_cache + base);
+        for (int c = (warp & 3) * 32 + lane; c < D; c += 128) page_v[c] = reinterpret_cast<const uint4*>(sh_v[local])[c];
+      }
+      if (on && lane == 0 && (warp & 3) == 0 && (off == 0 || raised)) *scale_at = pow2i(e);
     }
-    __syncwarp();
-    if (lane == 0 && (off == 0 || raised)) *scale_at = pow2i(e);
   }
 }
 
@@ -299,18 +351,18 @@ struct ScaledCache {
 template <int D>
 __global__ void __launch_bounds__(256)
 kv_scaled_read_kernel(const ScaledCache c, const int* __restrict__ tables, int bt_ld, int bt_cols, const int* __restrict__ lens, int max_len, int pages,
-                      long long units, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out) {
+                      unsigned units, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out) {
   constexpr int V = D / 32;
   chain_trigger();
   chain_wait();
   const int lane = threadIdx.x & 31;
-  long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  unsigned u = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (u >= units) return;
   const bool is_k = (u & 1) == 0;
   u >>= 1;
-  const int h = (int)(u % c.Hkv);
-  const long long bp = u / c.Hkv;
-  const int b = (int)(bp / pages), pg = (int)(bp % pages);
+  const int h = (int)(u % (unsigned)c.Hkv);
+  const unsigned bp = u / (unsigned)c.Hkv;
+  const int b = (int)(bp / (unsigned)pages), pg = (int)(bp % (unsigned)pages);
   const int len = min(lens[b], min(max_len, bt_cols * kScPage));
   const int live = min(max(len - pg * kScPage, 0), kScPage), rows = min(max_len - pg * kScPage, kScPage);
   const long long step = (long long)c.Hkv * D;
@@ -377,60 +429,88 @@ struct SelectParams {
 constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048;
 
-// One block per (sequence, head).  The `room`-th largest key among the tokens between sink and recent, 11, 11 and 10 bits at a time
-// (a histogram each, weights come from L2), then the positions in order: every warp counts its span of tokens, the spans' counts are
-// summed, and each warp writes its own.
+ATLAS_DEVICE uint32_t ld_cluster_u32(const void* mine, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(cluster_map_shared(smem_u32(mine), rank)) : "memory");
+  return v;
+}
+
+// One block, or a cluster of eight, per (sequence, head); a warp has a span of neighbouring tokens.  The `room`-th largest key among the tokens
+// between sink and recent, 11, 11 and 10 bits at a time: every block counts its tokens, the cluster's counts are summed through distributed
+// shared memory.  Then the positions in order: the spans' counts are summed and each warp writes its own.  The first kHeld tokens of a lane
+// stay in registers for the five looks at them: up to 8192 tokens of a block (cluster barriers empty L1).
+constexpr int kHeld = 8;
+
+template <int kCluster>
 __global__ void __launch_bounds__(kSelThreads)
 kv_evict_select_kernel(const SelectParams p) {
   __shared__ uint32_t hist[kSelBins];
   __shared__ uint32_t warp_a[32], warp_b[32];
-  __shared__ uint32_t sh_bin, sh_above;
+  __shared__ uint32_t sh_bin, sh_above, sh_more, sh_equal;
   chain_trigger();
   chain_wait();
-  const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
+  const int rank = blockIdx.x % kCluster, at_bh = blockIdx.x / kCluster;
+  const int b = at_bh / p.Hkv, h = at_bh % p.Hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int gtid = rank * kSelThreads + tid;
+  constexpr int kAll = kCluster * kSelThreads;
   const int len = min(max(p.seq_lens[b], 0), p.width);
   const int kept = min(len, p.keep);
   const float* w = p.weights + b * p.w_ld_b + h * p.w_ld_h;
   int* out = p.kept + ((long long)b * p.Hkv + h) * p.keep;
   float* wo = p.w_out + ((long long)b * p.Hkv + h) * p.keep;
-  if (h == 0 && tid == 0) p.new_lens[b] = kept;
-  for (int i = kept + tid; i < p.keep; i += kSelThreads) { out[i] = -1; wo[i] = 0.f; }
-  if (len <= p.keep) {
-    for (int i = tid; i < len; i += kSelThreads) { out[i] = i; wo[i] = w[i]; }
+  if (h == 0 && gtid == 0) p.new_lens[b] = kept;
+  for (int i = kept + gtid; i < p.keep; i += kAll) { out[i] = -1; wo[i] = 0.f; }
+  if (len <= p.keep) {                                  // the whole cluster
+    for (int i = gtid; i < len; i += kAll) { out[i] = i; wo[i] = w[i]; }
     return;
   }
   const int lo = p.sink, hi = len - p.recent;
-  int room = p.keep - p.sink - p.recent;                // >= 0; hi - lo = len - sink - recent > room
+  for (int i = gtid; i < p.sink; i += kAll) { out[i] = i; wo[i] = w[i]; }
+  for (int i = gtid; i < p.recent; i += kAll) { out[p.keep - p.recent + i] = hi + i; wo[p.keep - p.recent + i] = w[hi + i]; }
+  const int span = (hi - lo + kAll - 1) / kAll * 32;    // tokens of a warp
+  const int s0 = min(lo + (rank * 32 + warp) * span, hi), s1 = min(s0 + span, hi);
+  int room = p.keep - p.sink - p.recent;                // hi - lo = len - sink - recent > room >= 0
+  uint32_t held[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = s0 + 32 * j + lane;
+    held[j] = i < s1 ? weight_key(w[i]) : 0u;
+  }
+  // look(first token of 32, this lane's token and key) over the span; lanes behind its end take part
+  auto span_keys = [&](auto look) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (s0 + 32 * j < s1) look(s0 + 32 * j + lane, held[j]);
+#pragma unroll 2
+    for (int i0 = s0 + 32 * kHeld; i0 < s1; i0 += 32) look(i0 + lane, i0 + lane < s1 ? weight_key(w[i0 + lane]) : 0u);
+  };
   uint32_t prefix = 0, mask = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
     for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    for (int i0 = lo; i0 < hi; i0 += kSelThreads * 4) {
-      uint32_t key[4];
-      bool in[4];
+    span_keys([&](int i, uint32_t key) {
+      const bool hit = i < s1 && (key & mask) == prefix;
+      const uint32_t bin = (key >> shift) & ((1u << bits) - 1u);
+      // tokens that nothing looked at share one bin: a warp adds equal neighbours at once
+      const uint32_t first = __shfl_sync(0xffffffffu, bin, 0);
+      const uint32_t same = __ballot_sync(0xffffffffu, hit && bin == first);
+      if (hit && bin != first) atomicAdd(&hist[bin], 1u);
+      if (lane == 0 && same) atomicAdd(&hist[first], (uint32_t)__popc(same));
+    });
+    uint32_t c0, c1;                                     // two bins a thread
+    if constexpr (kCluster > 1) {
+      cluster_sync_all();
+      c0 = c1 = 0;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * kSelThreads + tid;
-        in[u] = i < hi;
-        key[u] = in[u] ? weight_key(w[i]) : 0u;
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool hit = in[u] && (key[u] & mask) == prefix;
-        const uint32_t bin = (key[u] >> shift) & ((1u << bits) - 1u);
-        // tokens that nothing looked at share one bin: a warp adds equal neighbours at once
-        const uint32_t first = __shfl_sync(0xffffffffu, bin, 0);
-        const uint32_t same = __ballot_sync(0xffffffffu, hit && bin == first);
-        if (hit && bin != first) atomicAdd(&hist[bin], 1u);
-        if (lane == 0 && same) atomicAdd(&hist[first], (uint32_t)__popc(same));
-      }
+      for (int r = 0; r < kCluster; ++r) { c0 += ld_cluster_u32(&hist[2 * tid], r); c1 += ld_cluster_u32(&hist[2 * tid + 1], r); }
+    } else {
+      __syncthreads();
+      c0 = hist[2 * tid]; c1 = hist[2 * tid + 1];
     }
-    __syncthreads();
-    // the bin that holds the room-th largest: suffix sums over 2048 bins, two a thread
-    const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
+    // the bin that holds the room-th largest: suffix sums over the bins
     uint32_t suffix = c0 + c1;                           // inclusive sum from this thread's bins to the warp's end
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -439,9 +519,11 @@ kv_evict_select_kernel(const SelectParams p) {
     }
     if (lane == 0) warp_a[warp] = suffix;
     if (tid == 0) { sh_bin = 0; sh_above = 0; }
-    __syncthreads();
+    if constexpr (kCluster > 1) cluster_sync_all();      // and every block has read the others' counts
+    else __syncthreads();
     uint32_t above = suffix - c0 - c1;
-    for (int i = warp + 1; i < 32; ++i) above += warp_a[i];
+    const uint32_t behind = (uint32_t)__reduce_add_sync(0xffffffffu, lane > warp ? warp_a[lane] : 0u);
+    above += behind;
     // exactly one bin has above < room <= above + count (room >= 1)
     if (room > 0) {
       if (above < (uint32_t)room && (uint32_t)room <= above + c1) { sh_bin = 2 * tid + 1; sh_above = above; }
@@ -455,41 +537,37 @@ kv_evict_select_kernel(const SelectParams p) {
   }
   // keys above `prefix` stay, the first `room` that equal it too
   if (p.keep - p.sink - p.recent == 0) { prefix = 0xffffffffu; room = 0; }
-  for (int i = tid; i < p.sink; i += kSelThreads) { out[i] = i; wo[i] = w[i]; }
-  for (int i = tid; i < p.recent; i += kSelThreads) { out[p.keep - p.recent + i] = hi + i; wo[p.keep - p.recent + i] = w[hi + i]; }
-  const int span = ((hi - lo + 31) / 32 + 31) / 32 * 32;             // tokens of a warp
-  const int s0 = lo + warp * span, s1 = min(s0 + span, hi);
   uint32_t more = 0, equal = 0;
-#pragma unroll 4
-  for (int i = s0 + lane; i < s1; i += 32) {
-    const uint32_t key = weight_key(w[i]);
-    more += key > prefix;
-    equal += key == prefix;
-  }
+  span_keys([&](int i, uint32_t key) {
+    more += i < s1 && key > prefix;
+    equal += i < s1 && key == prefix;
+  });
   more = (uint32_t)__reduce_add_sync(0xffffffffu, more);
   equal = (uint32_t)__reduce_add_sync(0xffffffffu, equal);
   if (lane == 0) { warp_a[warp] = more; warp_b[warp] = equal; }
   __syncthreads();
-  int at = p.sink, ties = 0;
-  for (int i = 0; i < warp; ++i) {
-    at += (int)warp_a[i];
-    ties += (int)warp_b[i];
+  int at = p.sink + (int)__reduce_add_sync(0xffffffffu, lane < warp ? warp_a[lane] : 0u);
+  int ties = (int)__reduce_add_sync(0xffffffffu, lane < warp ? warp_b[lane] : 0u);
+  if constexpr (kCluster > 1) {
+    if (warp == 31 && lane == 0) { sh_more = (uint32_t)(at - p.sink) + more; sh_equal = (uint32_t)ties + equal; }
+    cluster_sync_all();
+    for (int r = 0; r < rank; ++r) {
+      at += (int)ld_cluster_u32(&sh_more, r);
+      ties += (int)ld_cluster_u32(&sh_equal, r);
+    }
   }
   at += min(ties, room);
-#pragma unroll 4
-  for (int i0 = s0; i0 < s1; i0 += 32) {
-    const int i = i0 + lane;
-    const float x = i < s1 ? w[i] : 0.f;
-    const uint32_t key = weight_key(x);
+  span_keys([&](int i, uint32_t key) {
     const bool eq = i < s1 && key == prefix;
     const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
     const bool take = (i < s1 && key > prefix) || (eq && ties + __popc(eqs & ((1u << lane) - 1u)) < room);
     const uint32_t takes = __ballot_sync(0xffffffffu, take);
     const int to = at + __popc(takes & ((1u << lane) - 1u));
-    if (take && to < p.keep - p.recent) { out[to] = i; wo[to] = x; }
+    if (take && to < p.keep - p.recent) { out[to] = i; wo[to] = w[i]; }
     at += __popc(takes);
     ties += __popc(eqs);
-  }
+  });
+  if constexpr (kCluster > 1) cluster_sync_all();        // no block leaves while another reads its shared memory
 }
 
 struct MoveParams {
@@ -501,104 +579,153 @@ struct MoveParams {
   int keep, pages; long long units;
 };
 
-// A warp writes one page of one head.  A kept value token's 16-byte columns hold its neighbours too: every source page is read once as a
-// whole for all tokens that come from it.
+// A warp fills two pages of one head, keys and values: one chain of loads (position, block, scales) for 32 tokens.  A kept value token's
+// 16-byte columns hold its neighbours too: every source page is read once, as a whole, for all tokens that come from it, kAhead pages at a
+// time.
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128, D == 256 ? 3 : 6)
 kv_evict_move_kernel(const MoveParams p) {
   constexpr int V = D / 32;
+  constexpr int kAhead = 2;
   chain_trigger();
   chain_wait();
   const int lane = threadIdx.x & 31;
-  long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (u >= p.units) return;
-  const bool is_k = (u & 1) == 0;
-  u >>= 1;
+  unsigned u = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (u >= (unsigned)p.units) return;
   const ScaledCache& c = p.from;
-  const int pg = (int)(u % p.pages);
-  u /= p.pages;
-  const int h = (int)(u % c.Hkv), b = (int)(u / c.Hkv);
-  const int live = min(p.new_lens[b] - pg * kScPage, kScPage);
+  const unsigned pairs = (unsigned)(p.pages + 1) / 2;
+  const int pg0 = (int)(u % pairs) * 2;
+  u /= pairs;
+  const int h = (int)(u % (unsigned)c.Hkv), b = (int)(u / (unsigned)c.Hkv);
+  const int live = p.new_lens[b] - pg0 * kScPage;        // tokens from the first page on
   if (live <= 0) return;
-  const int dst = p.to[(long long)b * p.to_ld + pg];
-  if (dst < 0 || dst >= c.num_pages) return;
-  // lane r < 16: where token r of the new page comes from
-  int page = -1, off = 0;
-  float scale = 0.f;
+  int page = -1, off = 0, dst = -1;
+  float ks = 0.f, vs = 0.f;
+  if (lane < 2 && lane * kScPage < live) dst = p.to[(long long)b * p.to_ld + pg0 + lane];
   if (lane < live) {
-    const int pos = p.kept[((long long)b * c.Hkv + h) * p.keep + pg * kScPage + lane];
+    const int pos = p.kept[((long long)b * c.Hkv + h) * p.keep + pg0 * kScPage + lane];
     page = p.tables[(long long)b * p.bt_ld + pos / kScPage];
     off = pos % kScPage;
     if (page < 0 || page >= c.num_pages) page = -1;
-    else scale = is_k ? c.ks[page * c.ks_ld + h * c.ks_h] : c.vs[page * c.vs_ld + h * c.vs_h];
-  }
-  const uint8_t* pool = (is_k ? c.k : c.v) + (long long)h * (kScPage * D);
-  const long long step = (long long)c.Hkv * (kScPage * D);
-  Codes<V> codes[kScPage];
-#pragma unroll
-  for (int r = 0; r < kScPage; ++r)
-#pragma unroll
-    for (int i = 0; i < (V + 3) / 4; ++i) codes[r].w[i] = 0;
-  if (is_k) {
-#pragma unroll
-    for (int r = 0; r < kScPage; ++r) {
-      const int pr = __shfl_sync(0xffffffffu, page, r), o = __shfl_sync(0xffffffffu, off, r);
-      if (pr >= 0) codes[r] = load_codes<V>(pool + pr * step + o * D + lane * V);
+    else {
+      ks = c.ks[page * c.ks_ld + h * c.ks_h];
+      vs = c.vs[page * c.vs_ld + h * c.vs_h];
     }
-  } else {
-    int have = -1;
-    uint4 col[V];
+  }
+  const long long head = (long long)h * (kScPage * D), step = (long long)c.Hkv * (kScPage * D);
+#pragma unroll 1
+  for (int s = 0; s < 2; ++s) {
+    const int to = __shfl_sync(0xffffffffu, dst, s);
+    if (to < 0 || to >= c.num_pages) continue;
+    const long long base = (long long)to * step + head;
+    int ke, ve;
+    {
+      Codes<V> codes[kScPage];
 #pragma unroll
-    for (int r = 0; r < kScPage; ++r) {
-      const int pr = __shfl_sync(0xffffffffu, page, r), o = __shfl_sync(0xffffffffu, off, r);
-      if (pr < 0) continue;
-      if (pr != have) {
-        have = pr;
+      for (int r = 0; r < kScPage; ++r) {
+        const int pr = __shfl_sync(0xffffffffu, page, 16 * s + r), o = __shfl_sync(0xffffffffu, off, 16 * s + r);
 #pragma unroll
-        for (int i = 0; i < V; ++i) col[i] = reinterpret_cast<const uint4*>(pool + pr * step)[lane * V + i];
+        for (int i = 0; i < (V + 3) / 4; ++i) codes[r].w[i] = 0;
+        if (pr >= 0) codes[r] = load_codes<V>(c.k + head + pr * step + o * D + lane * V);
+      }
+      float amax = 0.f;
+#pragma unroll
+      for (int r = 0; r < kScPage; ++r) {
+        float x[V], m = 0.f;
+        widen<V>(codes[r], x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = fmaxf(m, fabsf(x[i]));
+        amax = fmaxf(amax, m * __shfl_sync(0xffffffffu, ks, 16 * s + r));
+      }
+      ke = block_exponent(warp_max(amax));
+      const float by = ks * pow2i(-ke);                     // a power of two: exact
+#pragma unroll
+      for (int r = 0; r < kScPage; ++r) {
+        const float f = __shfl_sync(0xffffffffu, by, 16 * s + r);
+        if (f != 1.f) {                                     // the same for all lanes
+          float x[V];
+          widen<V>(codes[r], x);
+          codes[r] = narrow<V>(x, f);
+        }
+        store_codes<V>(p.k + base + r * D + lane * V, codes[r]);
+      }
+    }
+    // values: the distinct source pages in order, first token of each marked
+    const int before = __shfl_up_sync(0xffffffffu, page, 1);
+    const bool lead = (lane & 15) == 0 || page != before;
+    uint32_t leads = (__ballot_sync(0xffffffffu, lead) >> (16 * s)) & 0xFFFFu;
+    uint32_t word[V][4];                                    // sixteen tokens of each of the lane's channels
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) word[i][j] = 0;
+    while (leads) {
+      uint4 col[kAhead][V];
+      uint32_t mine[kAhead];                                // tokens of the new page that come from the source page
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        mine[a] = 0;
+        if (leads) {
+          const int r = __ffs(leads) - 1;
+          leads &= leads - 1;
+          const int end = leads ? __ffs(leads) - 1 : kScPage;
+          const int pr = __shfl_sync(0xffffffffu, page, 16 * s + r);
+          if (pr >= 0) {
+            mine[a] = ((1u << end) - 1u) & ~((1u << r) - 1u);
+#pragma unroll
+            for (int i = 0; i < V; ++i) col[a][i] = reinterpret_cast<const uint4*>(c.v + head + pr * step)[lane * V + i];
+          }
+        }
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const uint32_t lo = (o & 4) ? col[i].y : col[i].x, hi = (o & 4) ? col[i].w : col[i].z;
-        const uint32_t code = (((o & 8) ? hi : lo) >> (8 * (o & 3))) & 0xFFu;
-        codes[r].w[i >> 2] |= code << (8 * (i & 3));
+      for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int r = 0; r < kScPage; ++r) {
+          if (!((mine[a] >> r) & 1u)) continue;             // the same for all lanes
+          const int o = __shfl_sync(0xffffffffu, off, 16 * s + r);
+          // byte r & 3 of the word becomes byte o & 3 of the column's word o / 4
+          const uint32_t pick = (0x3210u & ~(0xFu << (4 * (r & 3)))) | ((4u + (o & 3)) << (4 * (r & 3)));
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const uint32_t lo = (o & 4) ? col[a][i].y : col[a][i].x, hi = (o & 4) ? col[a][i].w : col[a][i].z;
+            word[i][r >> 2] = __byte_perm(word[i][r >> 2], (o & 8) ? hi : lo, pick);
+          }
+        }
+    }
+    {
+      float amax = 0.f;
+#pragma unroll
+      for (int r = 0; r < kScPage; r += 2) {
+        float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float2 t = codes2_to_f32((word[i][r >> 2] >> (8 * (r & 3))) & 0xFFFFu);
+          m0 = fmaxf(m0, fabsf(t.x));
+          m1 = fmaxf(m1, fabsf(t.y));
+        }
+        amax = fmaxf(amax, fmaxf(m0 * __shfl_sync(0xffffffffu, vs, 16 * s + r), m1 * __shfl_sync(0xffffffffu, vs, 16 * s + r + 1)));
       }
+      ve = block_exponent(warp_max(amax));
+      const float by = vs * pow2i(-ve);
+#pragma unroll
+      for (int r = 0; r < kScPage; r += 2) {
+        const float f0 = __shfl_sync(0xffffffffu, by, 16 * s + r), f1 = __shfl_sync(0xffffffffu, by, 16 * s + r + 1);
+        if (f0 == 1.f && f1 == 1.f) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float2 t = codes2_to_f32((word[i][r >> 2] >> (8 * (r & 3))) & 0xFFFFu);
+          const uint32_t two = f32_to_codes2(t.x * f0, t.y * f1);
+          word[i][r >> 2] = (r & 2) ? __byte_perm(word[i][r >> 2], two, 0x5410) : __byte_perm(word[i][r >> 2], two, 0x3254);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        reinterpret_cast<uint4*>(p.v + base)[lane * V + i] = make_uint4(word[i][0], word[i][1], word[i][2], word[i][3]);
     }
-  }
-  float amax = 0.f;
-#pragma unroll
-  for (int r = 0; r < kScPage; ++r) {
-    const float s = __shfl_sync(0xffffffffu, scale, r);
-    float x[V];
-    widen<V>(codes[r], x);
-#pragma unroll
-    for (int i = 0; i < V; ++i) amax = fmaxf(amax, fabsf(x[i]) * s);
-  }
-  amax = warp_max(amax);
-  const int e = block_exponent(amax);
-#pragma unroll
-  for (int r = 0; r < kScPage; ++r) {
-    const float s = __shfl_sync(0xffffffffu, scale, r);
-    float x[V];
-    widen<V>(codes[r], x);
-    codes[r] = narrow<V>(x, s * pow2i(-e));      // a power of two: exact
-  }
-  const long long base = ((long long)dst * c.Hkv + h) * (kScPage * D);
-  if (is_k) {
-#pragma unroll
-    for (int r = 0; r < kScPage; ++r) store_codes<V>(p.k + base + r * D + lane * V, codes[r]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      uint32_t out[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int r = 0; r < kScPage; ++r) out[r >> 2] |= ((codes[r].w[i >> 2] >> (8 * (i & 3))) & 0xFFu) << (8 * (r & 3));
-      reinterpret_cast<uint4*>(p.v + base)[lane * V + i] = make_uint4(out[0], out[1], out[2], out[3]);
+    if (lane == 0) {
+      p.ks[to * c.ks_ld + h * c.ks_h] = pow2i(ke);
+      p.vs[to * c.vs_ld + h * c.vs_h] = pow2i(ve);
     }
-  }
-  if (lane == 0) {
-    if (is_k) p.ks[dst * c.ks_ld + h * c.ks_h] = pow2i(e);
-    else p.vs[dst * c.vs_ld + h * c.vs_h] = pow2i(e);
   }
 }
 
@@ -626,12 +753,13 @@ int launched(cudaError_t e) {
 template <int D>
 struct Write {
   static int launch(const ScaledWriteParams& p, unsigned blocks, cudaStream_t st) {
-    return launched(launch_chain_if(p.T <= 256, kv_scaled_write_kernel<D>, dim3(blocks), dim3(256), 0, st, p));
+    if (p.rows_per_block == 1) return launched(launch_chain(kv_scaled_write_kernel<D, 1>, dim3(blocks), dim3(256), 0, st, p));
+    return launched(launch_chain_if(false, kv_scaled_write_kernel<D, 4>, dim3(blocks), dim3(256), 0, st, p));
   }
 };
 template <int D>
 struct Read {
-  static int launch(const ScaledCache& c, const int* tables, int bt_ld, int bt_cols, const int* lens, int max_len, int pages, long long units,
+  static int launch(const ScaledCache& c, const int* tables, int bt_ld, int bt_cols, const int* lens, int max_len, int pages, unsigned units,
                     __nv_bfloat16* k, __nv_bfloat16* v, cudaStream_t st) {
     return launched(launch_chain(kv_scaled_read_kernel<D>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, st, c, tables, bt_ld, bt_cols, lens, max_len,
                                  pages, units, k, v));
@@ -640,73 +768,103 @@ struct Read {
 template <int D>
 struct Move {
   static int launch(const MoveParams& p, cudaStream_t st) {
-    return launched(launch_chain(kv_evict_move_kernel<D>, dim3((unsigned)((p.units + 7) / 8)), dim3(256), 0, st, p));
+    return launched(launch_chain(kv_evict_move_kernel<D>, dim3((unsigned)((p.units + 3) / 4)), dim3(128), 0, st, p));
   }
 };
 
 }  // namespace
 
-// -1: sizes or alignment that the kernels do not take (16-token pages, heads of 64, 128 or 256, rows on 2 * D / 32 elements, rotary widths
-// of whole lanes); -20: a launch failed.
-extern "C" int atlas_kv_scaled_write(const void* q, long long ldq, void* q_out, long long ldqo, const void* k, long long ldk, const void* v,
-                                     long long ldv, const int* positions, const float* rope, const void* q_norm, const void* k_norm,
-                                     void* k_cache, void* v_cache, float* k_scale, long long ks_ld, int ks_h, float* v_scale, long long vs_ld,
-                                     int vs_h, const int* slots, int T, int Hq, int Hkv, int D, int rotary, int num_pages, int plus_one,
-                                     int norm_dim, float eps, void* stream) {
-  if (T <= 0) return 0;
+// The entry points take their arguments as one record (all fields 8 bytes wide): a call from Python costs 0.6 us so, and 3 us as thirty
+// converted arguments.  -1: sizes or alignment that the kernels do not take (16-token pages, heads of 64, 128 or 256, rows on 2 * D / 32
+// bytes, rotary widths of whole lanes); -20: a launch failed.
+struct ScalesRecord { float* ks; long long ks_ld, ks_h; float* vs; long long vs_ld, vs_h; };
+
+struct WriteRecord {
+  const void* q; long long ldq; void* q_out; long long ldqo; const void* k; long long ldk; const void* v; long long ldv;
+  const int* positions; const float* rope; const void* q_norm; const void* k_norm;
+  void* k_cache; void* v_cache; ScalesRecord s;
+  const int* slots; long long T, Hq, Hkv, D, rotary, num_pages, plus_one, norm_dim; double eps; void* stream;
+};
+extern "C" int atlas_kv_scaled_write(const void* record) {
+  const WriteRecord& r = *static_cast<const WriteRecord*>(record);
+  const int D = (int)r.D;
+  if (r.T <= 0) return 0;
   if (D != 64 && D != 128 && D != 256) return -1;
   const int V = D / 32;
-  if (rotary < 0 || rotary > D || rotary % (2 * V) || num_pages <= 0 || num_pages > (1 << 27) || Hkv <= 0 || Hq < 0) return -1;
-  if (ldq % V || ldqo % V || ldk % V || ldv % V || !aligned(k, 2 * V) || !aligned(v, 2 * V) || !aligned(k_cache, 16) || !aligned(v_cache, 16)) return -1;
-  if (Hq > 0 && (!aligned(q, 2 * V) || !aligned(q_out, 2 * V))) return -1;
-  if ((q_norm && !aligned(q_norm, 2 * V)) || (k_norm && !aligned(k_norm, 2 * V))) return -1;
+  if (r.T > 0x7fffffff || r.rotary < 0 || r.rotary > D || r.rotary % (2 * V) || r.num_pages <= 0 || r.num_pages > (1 << 27) || r.Hkv <= 0 || r.Hq < 0)
+    return -1;
+  if (r.ldq % V || r.ldqo % V || r.ldk % V || r.ldv % V || !aligned(r.k, 2 * V) || !aligned(r.v, 2 * V) || !aligned(r.k_cache, 16) ||
+      !aligned(r.v_cache, 16) || !aligned(r.rope, 16))
+    return -1;
+  if (r.Hq > 0 && (!aligned(r.q, 2 * V) || !aligned(r.q_out, 2 * V))) return -1;
+  if (!aligned(r.q_norm, 2 * V) || !aligned(r.k_norm, 2 * V)) return -1;
   ScaledWriteParams p;
-  p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.q_out = (__nv_bfloat16*)q_out; p.ldqo = ldqo;
-  p.k = (const __nv_bfloat16*)k; p.ldk = ldk; p.v = (const __nv_bfloat16*)v; p.ldv = ldv;
-  p.positions = positions; p.rope = rope; p.q_norm = (const __nv_bfloat16*)q_norm; p.k_norm = (const __nv_bfloat16*)k_norm;
-  p.k_cache = (uint8_t*)k_cache; p.v_cache = (uint8_t*)v_cache;
-  p.k_scale = k_scale; p.v_scale = v_scale; p.ks_ld = ks_ld; p.vs_ld = vs_ld; p.ks_h = ks_h; p.vs_h = vs_h;
-  p.slots = slots; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.rotary = rotary; p.num_pages = num_pages; p.plus_one = plus_one;
-  p.norm_dim = norm_dim > 0 ? norm_dim : D; p.eps = eps;
-  // Decode steps: every row begins a run, one row a block.  Prompts: one row in 16 does, and blocks of four rows leave fewer blocks empty.
-  p.rows_per_block = T <= 512 ? 1 : 4;
-  p.kv_blocks_x = (T + p.rows_per_block - 1) / p.rows_per_block;
-  p.kv_blocks_y = (2 * Hkv + 7) / 8;
-  const long long q_units = (long long)T * ((Hq + kWriteHeads - 1) / kWriteHeads);
+  p.q = (const __nv_bfloat16*)r.q; p.ldq = r.ldq; p.q_out = (__nv_bfloat16*)r.q_out; p.ldqo = r.ldqo;
+  p.k = (const __nv_bfloat16*)r.k; p.ldk = r.ldk; p.v = (const __nv_bfloat16*)r.v; p.ldv = r.ldv;
+  p.positions = r.positions; p.rope = r.rope; p.q_norm = (const __nv_bfloat16*)r.q_norm; p.k_norm = (const __nv_bfloat16*)r.k_norm;
+  p.k_cache = (uint8_t*)r.k_cache; p.v_cache = (uint8_t*)r.v_cache;
+  p.k_scale = r.s.ks; p.v_scale = r.s.vs; p.ks_ld = r.s.ks_ld; p.vs_ld = r.s.vs_ld; p.ks_h = (int)r.s.ks_h; p.vs_h = (int)r.s.vs_h;
+  p.slots = r.slots; p.T = (int)r.T; p.Hq = (int)r.Hq; p.Hkv = (int)r.Hkv; p.rotary = (int)r.rotary; p.num_pages = (int)r.num_pages;
+  p.plus_one = (int)r.plus_one; p.norm_dim = r.norm_dim > 0 ? (int)r.norm_dim : D; p.eps = (float)r.eps;
+  // Up to 512 rows: one row a block, a warp per page.  More are prompts: a page gets four warps, and one row in 16 begins a page; blocks of
+  // four or sixteen rows leave fewer blocks empty (8192 rows: 20 us of a GPU's instructions for blocks of four), but a mixed step's decode rows
+  // go through their block one after the other, which a long prompt beside them hides.
+  p.rows_per_block = p.T <= 512 ? 1 : p.T < 2048 ? 4 : 16;
+  p.kv_blocks_x = (p.T + p.rows_per_block - 1) / p.rows_per_block;
+  p.kv_blocks_y = p.rows_per_block == 1 ? (2 * p.Hkv + 7) / 8 : p.Hkv;
+  const long long q_units = r.T * ((p.Hq + kWriteHeads - 1) / kWriteHeads);
   const long long blocks = (long long)p.kv_blocks_x * p.kv_blocks_y + (q_units + 7) / 8;
-  if (blocks > 0x7fffffffll) return -1;
-  return by_width<Write>(D, p, (unsigned)blocks, (cudaStream_t)stream);
+  if (blocks > 0x7fffffffll / 8) return -1;
+  return by_width<Write>(D, p, (unsigned)blocks, (cudaStream_t)r.stream);
 }
 
-extern "C" int atlas_kv_scaled_read(const void* k_cache, const void* v_cache, const float* k_scale, long long ks_ld, int ks_h,
-                                    const float* v_scale, long long vs_ld, int vs_h, const int* tables, int bt_ld, int bt_cols, const int* lens, int B,
-                                    int max_len, int Hkv, int D, int num_pages, void* k_out, void* v_out, void* stream) {
-  if (B <= 0 || max_len <= 0) return 0;
-  if (bt_cols > (1 << 26)) return -1;
-  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_out, 16) || !aligned(v_out, 16)) return -1;
-  const ScaledCache c{(const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, ks_ld, vs_ld, ks_h, vs_h, Hkv, num_pages};
-  const int pages = (max_len + kScPage - 1) / kScPage;
-  const long long units = 2ll * B * pages * Hkv;
-  if ((units + 7) / 8 > 0x7fffffffll) return -1;
-  return by_width<Read>(D, c, tables, bt_ld, bt_cols, lens, max_len, pages, units, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, (cudaStream_t)stream);
+struct ReadRecord {
+  const void* k_cache; const void* v_cache; ScalesRecord s;
+  const int* tables; long long bt_ld, bt_cols; const int* lens; long long B, max_len, Hkv, D, num_pages; void* k_out; void* v_out; void* stream;
+};
+extern "C" int atlas_kv_scaled_read(const void* record) {
+  const ReadRecord& r = *static_cast<const ReadRecord*>(record);
+  if (r.B <= 0 || r.max_len <= 0) return 0;
+  if (!aligned(r.k_cache, 16) || !aligned(r.v_cache, 16) || !aligned(r.k_out, 16) || !aligned(r.v_out, 16) || r.bt_cols > (1 << 26) ||
+      r.max_len > (1 << 30))
+    return -1;
+  const ScaledCache c{(const uint8_t*)r.k_cache, (const uint8_t*)r.v_cache, r.s.ks, r.s.vs, r.s.ks_ld, r.s.vs_ld, (int)r.s.ks_h, (int)r.s.vs_h,
+                      (int)r.Hkv, (int)r.num_pages};
+  const int pages = (int)((r.max_len + kScPage - 1) / kScPage);
+  const long long units = 2ll * r.B * pages * r.Hkv;
+  if (units > 0x7fffffffll) return -1;
+  return by_width<Read>((int)r.D, c, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.lens, (int)r.max_len, pages, (unsigned)units, (__nv_bfloat16*)r.k_out,
+                        (__nv_bfloat16*)r.v_out, (cudaStream_t)r.stream);
 }
 
-extern "C" int atlas_kv_evict(void* k_cache, void* v_cache, float* k_scale, long long ks_ld, int ks_h, float* v_scale, long long vs_ld, int vs_h,
-                              const int* tables, int bt_ld, const int* seq_lens, const float* weights, long long w_ld_b, long long w_ld_h, int width,
-                              int B, int Hkv, int D, int num_pages, int keep, int sink, int recent, const int* to, int to_ld, int* new_lens,
-                              int* kept, float* w_out, void* stream) {
-  if (B <= 0) return 0;
-  if (keep <= 0 || sink < 0 || recent < 0 || sink + recent > keep || !aligned(k_cache, 16) || !aligned(v_cache, 16)) return -1;
-  if (D != 64 && D != 128 && D != 256) return -1;
-  cudaStream_t st = (cudaStream_t)stream;
-  SelectParams s{weights, w_ld_b, w_ld_h, seq_lens, new_lens, kept, w_out, Hkv, keep, sink, recent, width};
-  const int rc = launched(launch_chain(kv_evict_select_kernel, dim3(B * Hkv), dim3(kSelThreads), 0, st, s));
-  if (rc) return rc;
+struct EvictRecord {
+  void* k_cache; void* v_cache; ScalesRecord s;
+  const int* tables; long long bt_ld; const int* seq_lens; const float* weights; long long w_ld_b, w_ld_h, width;
+  long long B, Hkv, D, num_pages, keep, sink, recent; const int* to; long long to_ld; int* new_lens; int* kept; float* w_out; void* stream;
+};
+extern "C" int atlas_kv_evict(const void* record) {
+  const EvictRecord& r = *static_cast<const EvictRecord*>(record);
+  if (r.B <= 0) return 0;
+  if (r.keep <= 0 || r.sink < 0 || r.recent < 0 || r.sink + r.recent > r.keep || r.keep > (1 << 30) || !aligned(r.k_cache, 16) ||
+      !aligned(r.v_cache, 16) || r.B * r.Hkv > 0x7fffffffll)
+    return -1;
+  if (r.D != 64 && r.D != 128 && r.D != 256) return -1;
+  cudaStream_t st = (cudaStream_t)r.stream;
+  const int Hkv = (int)r.Hkv, keep = (int)r.keep;
+  SelectParams s{r.weights, r.w_ld_b, r.w_ld_h, r.seq_lens, r.new_lens, r.kept, r.w_out, Hkv, keep, (int)r.sink, (int)r.recent, (int)r.width};
   MoveParams m;
-  m.from = ScaledCache{(const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, ks_ld, vs_ld, ks_h, vs_h, Hkv, num_pages};
-  m.k = (uint8_t*)k_cache; m.v = (uint8_t*)v_cache; m.ks = k_scale; m.vs = v_scale;
-  m.tables = tables; m.bt_ld = bt_ld; m.to = to; m.to_ld = to_ld; m.kept = kept; m.new_lens = new_lens; m.keep = keep;
-  m.pages = (keep + kScPage - 1) / kScPage;
-  m.units = 2ll * B * Hkv * m.pages;
-  return by_width<Move>(D, m, st);
+  m.from = ScaledCache{(const uint8_t*)r.k_cache, (const uint8_t*)r.v_cache, r.s.ks, r.s.vs, r.s.ks_ld, r.s.vs_ld, (int)r.s.ks_h, (int)r.s.vs_h, Hkv,
+                       (int)r.num_pages};
+  m.k = (uint8_t*)r.k_cache; m.v = (uint8_t*)r.v_cache; m.ks = r.s.ks; m.vs = r.s.vs;
+  m.tables = r.tables; m.bt_ld = (int)r.bt_ld; m.to = r.to; m.to_ld = (int)r.to_ld; m.kept = r.kept; m.new_lens = r.new_lens; m.keep = keep;
+  const long long longest = r.width < r.keep ? r.width : r.keep;
+  m.pages = (int)((longest + kScPage - 1) / kScPage);
+  m.units = r.B * Hkv * ((m.pages + 1) / 2);
+  if (m.units > 0x7fffffffll || r.B * Hkv > 0x7fffffffll / 8) return -1;
+  // Eight blocks a head where one would look at more than 8192 tokens.
+  const int rc = r.width > 8192
+      ? launched(launch_chain_cluster(true, 8, kv_evict_select_kernel<8>, dim3((unsigned)(r.B * Hkv * 8)), dim3(kSelThreads), 0, st, s))
+      : launched(launch_chain(kv_evict_select_kernel<1>, dim3((unsigned)(r.B * Hkv)), dim3(kSelThreads), 0, st, s));
+  if (rc || m.units == 0) return rc;
+  return by_width<Move>((int)r.D, m, st);
 }
