@@ -167,141 +167,182 @@ ATLAS_DEVICE void norm_weights(const __nv_bfloat16* w, int plus_one, int lane, f
   for (int i = 0; i < V; ++i) out[i] += plus_one ? 1.f : 0.f;
 }
 
-constexpr int kWriteHeads = 8;      // query heads of a token that one warp turns with the same angles
+// Queries: 16 bytes a lane, so that D / 8 lanes hold a head and a warp 256 / D of them; four such loads of one token are in flight and share
+// the angles.
+template <int D>
+ATLAS_DEVICE void turn_queries(const ScaledWriteParams& p, unsigned unit, int lane) {
+  constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kHeads = 4 * kAtOnce;
+  const unsigned groups = (unsigned)(p.Hq + kHeads - 1) / kHeads, t = unit / groups;
+  if (t >= (unsigned)p.T) return;
+  const int h0 = (int)(unit % groups) * kHeads + lane / kLanes, sl = lane % kLanes;
+  const __nv_bfloat16* src = p.q + (long long)t * p.ldq + h0 * D + sl * 8;
+  __nv_bfloat16* dst = p.q_out + (long long)t * p.ldqo + h0 * D + sl * 8;
+  Raw<8> raw[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (h0 + j * kAtOnce < p.Hq) raw[j] = load_raw<8>(src + j * kAtOnce * D);
+  const int hl = p.rotary / 16;                      // lanes between the channels of a rotated pair
+  float c[8], s[8], w[8];
+  if (sl < 2 * hl) {
+    const float* at = p.rope + (long long)p.positions[t] * p.rotary + (sl < hl ? sl : sl - hl) * 8;
+    Turn<8>::load_floats(at, c);
+    Turn<8>::load_floats(at + p.rotary / 2, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = sl < hl ? -s[i] : s[i];
+  }
+  norm_weights<8>(p.q_norm, p.plus_one, sl, w);
+  const int from = sl < hl ? lane + hl : (sl < 2 * hl ? lane - hl : lane);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float x[8];
+    unpack<8>(raw[j], x);
+    if (p.q_norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss / (float)p.norm_dim + p.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
+    }
+    if (hl > 0)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = __shfl_sync(0xffffffffu, x[i], from);
+        if (sl < 2 * hl) x[i] = x[i] * c[i] + y * s[i];
+      }
+    if (h0 + j * kAtOnce < p.Hq) store_row<8>(dst + j * kAtOnce * D, x);
+  }
+}
 
-// Cache blocks: `W` warps take the rows of one step that fall into one page, for one head's keys or values, in groups of four slots; a run of
+// Cache blocks: `W` warps take the rows of one step that fall into one page, for one head's keys and values, in groups of four slots; a run of
 // such rows starts where the slot is not the one behind the row before.  Prompts: four warps, a group each, every row loaded and turned once
 // and waiting in registers for the page's largest magnitude.  (A warp per page took 30 us for 517 rows of 256-wide heads, sixteen rows' angles
-// one after the other; four take 9.)  Decode steps: one warp, since most runs are one row, and 128 rows of 8 heads fit the GPU at once (7 us; with
+// one after the other; four take 9.)  Decode steps: one warp, since most runs are one row, and 128 rows of 8 heads fit the GPU at once (6 us; with
 // four warps 11); a longer run is loaded and turned twice.
 template <int D, int W>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : 4)
 kv_scaled_write_kernel(const ScaledWriteParams p) {
   constexpr int V = D / 32;
-  __shared__ float sh_amax[8];
-  __shared__ uint32_t sh_v[W > 1 ? 8 / W : 1][W > 1 ? D * 4 : 1];      // the tasks' value pages: [channel] 16 tokens
+  __shared__ float2 sh_amax[8];
+  __shared__ uint32_t sh_v[W > 1 ? 8 / W : 1][W > 1 ? D * 4 : 1];      // value pages: [channel] 16 tokens
   chain_trigger();
   chain_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kv_blocks = p.kv_blocks_x * p.kv_blocks_y;
-  float w[V];
-  Turn<V> turn;
-  turn.hl = p.rotary / (2 * V);
   if ((int)blockIdx.x >= kv_blocks) {
-    const int groups = (p.Hq + kWriteHeads - 1) / kWriteHeads;
-    const unsigned unit = (blockIdx.x - kv_blocks) * 8 + warp, at = unit / groups;
-    if (at >= (unsigned)p.T) return;
-    const int t = (int)at, h0 = (int)(unit % groups) * kWriteHeads;
-    Raw<V> raw[kWriteHeads];
-#pragma unroll
-    for (int i = 0; i < kWriteHeads; ++i)
-      if (h0 + i < p.Hq) raw[i] = load_raw<V>(p.q + t * p.ldq + (h0 + i) * D + lane * V);
-    if (p.rotary) turn.angles(p.rope + (long long)p.positions[t] * p.rotary, p.rotary, lane);
-    norm_weights<V>(p.q_norm, p.plus_one, lane, w);
-#pragma unroll
-    for (int i = 0; i < kWriteHeads; ++i) {
-      if (h0 + i >= p.Hq) return;
-      float x[V];
-      unpack<V>(raw[i], x);
-      turn(x, w, p.q_norm != nullptr, p.norm_dim, p.eps, lane);
-      store_row<V>(p.q_out + t * p.ldqo + (h0 + i) * D + lane * V, x);
-    }
+    turn_queries<D>(p, (blockIdx.x - kv_blocks) * 8 + warp, lane);
     return;
   }
   const int local = warp / W;
-  const int task = (blockIdx.x / p.kv_blocks_x) * (8 / W) + local;     // K heads, then V heads
-  const bool on = task < 2 * p.Hkv;
+  const int h = (blockIdx.x / p.kv_blocks_x) * (8 / W) + local;
+  const bool on = h < p.Hkv;
   if (W == 1 && !on) return;
-  const bool is_k = task < p.Hkv;
-  const int h = is_k ? task : task - p.Hkv;
-  const __nv_bfloat16* src = (is_k ? p.k : p.v) + h * D + lane * V;
-  const long long ld = is_k ? p.ldk : p.ldv;
-  if (is_k) norm_weights<V>(p.k_norm, p.plus_one, lane, w);
-  const bool normed = is_k && p.k_norm != nullptr;
+  float w[V];
+  Turn<V> turn;
+  turn.hl = p.rotary / (2 * V);
+  const __nv_bfloat16* k_src = p.k + h * D + lane * V;
+  const __nv_bfloat16* v_src = p.v + h * D + lane * V;
+  norm_weights<V>(p.k_norm, p.plus_one, lane, w);
+  const bool normed = p.k_norm != nullptr;
+  // the runs that start in this block's rows, all lanes looking at once
   const int row0 = (blockIdx.x % p.kv_blocks_x) * p.rows_per_block;
-  for (int t0 = row0; t0 < min(row0 + p.rows_per_block, p.T); ++t0) {   // the same for the whole block
-    const int slot = p.slots[t0];
-    if (slot < 0 || slot >= p.num_pages * kScPage) continue;
-    const int page = slot / kScPage, off = slot % kScPage;
-    if (off > 0 && t0 > 0 && p.slots[t0 - 1] == slot - 1) continue;    // the row before began this run
+  bool starts = false;
+  if (lane < p.rows_per_block && row0 + lane < p.T) {
+    const int slot = p.slots[row0 + lane];
+    starts = slot >= 0 && slot < p.num_pages * kScPage && !(slot % kScPage > 0 && row0 + lane > 0 && p.slots[row0 + lane - 1] == slot - 1);
+  }
+  uint32_t runs = __ballot_sync(0xffffffffu, starts);                  // the same for the whole block
+  while (runs) {
+    const int t0 = row0 + __ffs(runs) - 1;
+    runs &= runs - 1;
+    const int slot = p.slots[t0], page = slot / kScPage, off = slot % kScPage;
     // rows t0 .. t0 + n - 1 fill slots off .. off + n - 1 of the page
     const int mine_t = min(t0 + lane, p.T - 1);
     const bool mine = lane < kScPage - off && t0 + lane < p.T && p.slots[mine_t] == slot + lane;
-    const int my_pos = is_k && p.rotary ? p.positions[mine_t] : 0;
+    const int my_pos = p.rotary ? p.positions[mine_t] : 0;
     const int n = __ffs(~__ballot_sync(0xffffffffu, mine)) - 1;
     const long long base = ((long long)page * p.Hkv + h) * (kScPage * D);
-    float* scale_at = is_k ? p.k_scale + page * p.ks_ld + h * p.ks_h : p.v_scale + page * p.vs_ld + h * p.vs_h;
-    float before = 0.f;
-    if (on && off > 0) before = *scale_at;
+    float* ks_at = p.k_scale + page * p.ks_ld + h * p.ks_h;
+    float* vs_at = p.v_scale + page * p.vs_ld + h * p.vs_h;
+    float k_before = 0.f, v_before = 0.f;
+    if (on && off > 0) { k_before = *ks_at; v_before = *vs_at; }
     const int g_lo = W == 1 ? off / 4 : (warp & 3), g_hi = W == 1 ? (off + n - 1) / 4 : (warp & 3);      // groups with rows of the run
     float x[4][V];
-    auto load_group = [&](int g, float amax) {
-      Raw<V> raw[4];
+    Raw<V> v_raw[4];
+    auto load_group = [&](int g, float2 amax) {
+      Raw<V> k_raw[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * g + j - off;
-        if (r >= 0 && r < n) raw[j] = load_raw<V>(src + (long long)(t0 + r) * ld);
+        if (r >= 0 && r < n) {
+          k_raw[j] = load_raw<V>(k_src + (long long)(t0 + r) * p.ldk);
+          v_raw[j] = load_raw<V>(v_src + (long long)(t0 + r) * p.ldv);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * g + j - off;
         if (r < 0 || r >= n) continue;
-        unpack<V>(raw[j], x[j]);
-        if (is_k) {
-          if (p.rotary) turn.angles(p.rope + (long long)__shfl_sync(0xffffffffu, my_pos, r) * p.rotary, p.rotary, lane);
-          turn(x[j], w, normed, p.norm_dim, p.eps, lane);
-        }
+        float y[V];
+        unpack<V>(v_raw[j], y);
 #pragma unroll
-        for (int i = 0; i < V; ++i) amax = fmaxf(amax, fabsf(x[j][i]));
+        for (int i = 0; i < V; ++i) amax.y = fmaxf(amax.y, fabsf(y[i]));
+        unpack<V>(k_raw[j], x[j]);
+        if (p.rotary) turn.angles(p.rope + (long long)__shfl_sync(0xffffffffu, my_pos, r) * p.rotary, p.rotary, lane);
+        turn(x[j], w, normed, p.norm_dim, p.eps, lane);
+#pragma unroll
+        for (int i = 0; i < V; ++i) amax.x = fmaxf(amax.x, fabsf(x[j][i]));
       }
       return amax;
     };
-    float amax = 0.f;
+    float2 amax = make_float2(0.f, 0.f);
     if (on)
       for (int g = g_lo; g <= g_hi; ++g) amax = load_group(g, amax);
-    amax = warp_max(amax);
+    amax.x = warp_max(amax.x);
+    amax.y = warp_max(amax.y);
     if constexpr (W > 1) {
       if (lane == 0) sh_amax[warp] = amax;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < W; ++i) amax = fmaxf(amax, sh_amax[local * W + i]);
+      for (int i = 0; i < W; ++i) {
+        const float2 o = sh_amax[local * W + i];
+        amax.x = fmaxf(amax.x, o.x);
+        amax.y = fmaxf(amax.y, o.y);
+      }
     }
-    int e = block_exponent(amax);
-    const int e_old = exponent_of(before);
-    if (off > 0) e = max(e, e_old);
-    const float inv = pow2i(-e);
-    const bool raised = off > 0 && e != e_old;
-    const float shift = raised ? pow2i(max(e_old - e, -126)) : 1.f;
+    int ke = block_exponent(amax.x), ve = block_exponent(amax.y);
+    const int ke_old = exponent_of(k_before), ve_old = exponent_of(v_before);
+    if (off > 0) { ke = max(ke, ke_old); ve = max(ve, ve_old); }
+    const bool k_raised = off > 0 && ke != ke_old, v_raised = off > 0 && ve != ve_old;
+    const float k_shift = pow2i(max(ke_old - ke, -126)), v_shift = pow2i(max(ve_old - ve, -126));      // used where the scale rose
     // a group's tokens: rows of the run, tokens before them (to the new scale, if it rose), tokens behind them (as they were)
     auto store_group = [&](int g) {
-      if (is_k) {
-        uint8_t* page_k = p.k_cache + base + lane * V;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int s = 4 * g + j, r = s - off;
-          if (r >= 0 && r < n) {
-            store_codes<V>(page_k + s * D, narrow<V>(x[j], inv));
-          } else if (r < 0 && raised) {
-            float y[V];
-            widen<V>(load_codes<V>(page_k + s * D), y);
-            store_codes<V>(page_k + s * D, narrow<V>(y, shift));
-          }
-        }
-        return;
-      }
+      uint8_t* page_k = p.k_cache + base + lane * V;
       uint32_t word[V];                                                // four tokens of each channel: a word of the channel's sixteen
 #pragma unroll
       for (int i = 0; i < V; ++i) word[i] = 0;
       uint32_t fresh = 0, old = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int r = 4 * g + j - off;
-        if (r < 0) old |= 0xFFu << (8 * j);
-        if (r < 0 || r >= n) continue;
-        fresh |= 0xFFu << (8 * j);
-        const Codes<V> c = narrow<V>(x[j], inv);
+        const int s = 4 * g + j, r = s - off;
+        if (r >= 0 && r < n) {
+          store_codes<V>(page_k + s * D, narrow<V>(x[j], pow2i(-ke)));
+          fresh |= 0xFFu << (8 * j);
+          float y[V];
+          unpack<V>(v_raw[j], y);
+          const Codes<V> c = narrow<V>(y, pow2i(-ve));
 #pragma unroll
-        for (int i = 0; i < V; ++i) word[i] |= ((c.w[i >> 2] >> (8 * (i & 3))) & 0xFFu) << (8 * j);
+          for (int i = 0; i < V; ++i) word[i] |= ((c.w[i >> 2] >> (8 * (i & 3))) & 0xFFu) << (8 * j);
+        } else if (r < 0) {
+          old |= 0xFFu << (8 * j);
+          if (k_raised) {
+            float y[V];
+            widen<V>(load_codes<V>(page_k + s * D), y);
+            store_codes<V>(page_k + s * D, narrow<V>(y, k_shift));
+          }
+        }
       }
       uint32_t* at = reinterpret_cast<uint32_t*>(p.v_cache + base) + lane * V * 4 + g;
       if (fresh != 0xffffffffu) {
@@ -309,9 +350,9 @@ kv_scaled_write_kernel(const ScaledWriteParams p) {
         for (int i = 0; i < V; ++i) {
           const uint32_t was = at[4 * i];
           uint32_t moved = was;
-          if (raised && old) {
+          if (v_raised && old) {
             const float2 lo = codes2_to_f32(was & 0xFFFFu), hi = codes2_to_f32(was >> 16);
-            moved = f32_to_codes2(lo.x * shift, lo.y * shift) | (f32_to_codes2(hi.x * shift, hi.y * shift) << 16);
+            moved = f32_to_codes2(lo.x * v_shift, lo.y * v_shift) | (f32_to_codes2(hi.x * v_shift, hi.y * v_shift) << 16);
           }
           word[i] = (word[i] & fresh) | (moved & old) | (was & ~(fresh | old));
         }
@@ -323,20 +364,22 @@ kv_scaled_write_kernel(const ScaledWriteParams p) {
       }
     };
     if constexpr (W == 1) {
-      for (int g = raised ? 0 : g_lo; g <= g_hi; ++g) {
-        if (g >= g_lo && g_lo != g_hi) load_group(g, 0.f);
+      for (int g = k_raised || v_raised ? 0 : g_lo; g <= g_hi; ++g) {
+        if (g >= g_lo && g_lo != g_hi) load_group(g, amax);
         store_group(g);
       }
       __syncwarp();
-      if (lane == 0 && (off == 0 || raised)) *scale_at = pow2i(e);
     } else {
       if (on) store_group(warp & 3);
       __syncthreads();
-      if (on && !is_k) {                                               // whole channels, 16 bytes each
+      if (on) {                                                        // whole channels, 16 bytes each
         uint4* page_v = reinterpret_cast<uint4*>(p.v_cache + base);
         for (int c = (warp & 3) * 32 + lane; c < D; c += 128) page_v[c] = reinterpret_cast<const uint4*>(sh_v[local])[c];
       }
-      if (on && lane == 0 && (warp & 3) == 0 && (off == 0 || raised)) *scale_at = pow2i(e);
+    }
+    if (on && lane == 0 && (W == 1 || (warp & 3) == 0)) {
+      if (off == 0 || k_raised) *ks_at = pow2i(ke);
+      if (off == 0 || v_raised) *vs_at = pow2i(ve);
     }
   }
 }
@@ -775,8 +818,8 @@ struct Move {
 }  // namespace
 
 // The entry points take their arguments as one record (all fields 8 bytes wide): a call from Python costs 0.6 us so, and 3 us as thirty
-// converted arguments.  -1: sizes or alignment that the kernels do not take (16-token pages, heads of 64, 128 or 256, rows on 2 * D / 32
-// bytes, rotary widths of whole lanes); -20: a launch failed.
+// converted arguments.  -1: sizes or alignment that the kernels do not take (16-token pages, heads of 64, 128 or 256, queries and norm
+// weights on 16 bytes, keys and values on 2 * D / 32, rotary widths in sixteens); -20: a launch failed.
 struct ScalesRecord { float* ks; long long ks_ld, ks_h; float* vs; long long vs_ld, vs_h; };
 
 struct WriteRecord {
@@ -791,13 +834,13 @@ extern "C" int atlas_kv_scaled_write(const void* record) {
   if (r.T <= 0) return 0;
   if (D != 64 && D != 128 && D != 256) return -1;
   const int V = D / 32;
-  if (r.T > 0x7fffffff || r.rotary < 0 || r.rotary > D || r.rotary % (2 * V) || r.num_pages <= 0 || r.num_pages > (1 << 27) || r.Hkv <= 0 || r.Hq < 0)
+  if (r.T > 0x7fffffff || r.rotary < 0 || r.rotary > D || r.rotary % 16 || r.num_pages <= 0 || r.num_pages > (1 << 27) || r.Hkv <= 0 || r.Hq < 0)
     return -1;
-  if (r.ldq % V || r.ldqo % V || r.ldk % V || r.ldv % V || !aligned(r.k, 2 * V) || !aligned(r.v, 2 * V) || !aligned(r.k_cache, 16) ||
+  if (r.ldk % V || r.ldv % V || !aligned(r.k, 2 * V) || !aligned(r.v, 2 * V) || !aligned(r.k_cache, 16) ||
       !aligned(r.v_cache, 16) || !aligned(r.rope, 16))
     return -1;
-  if (r.Hq > 0 && (!aligned(r.q, 2 * V) || !aligned(r.q_out, 2 * V))) return -1;
-  if (!aligned(r.q_norm, 2 * V) || !aligned(r.k_norm, 2 * V)) return -1;
+  if (r.Hq > 0 && (!aligned(r.q, 16) || !aligned(r.q_out, 16) || r.ldq % 8 || r.ldqo % 8)) return -1;
+  if (!aligned(r.q_norm, 16) || !aligned(r.k_norm, 2 * V)) return -1;
   ScaledWriteParams p;
   p.q = (const __nv_bfloat16*)r.q; p.ldq = r.ldq; p.q_out = (__nv_bfloat16*)r.q_out; p.ldqo = r.ldqo;
   p.k = (const __nv_bfloat16*)r.k; p.ldk = r.ldk; p.v = (const __nv_bfloat16*)r.v; p.ldv = r.ldv;
@@ -807,12 +850,13 @@ extern "C" int atlas_kv_scaled_write(const void* record) {
   p.slots = r.slots; p.T = (int)r.T; p.Hq = (int)r.Hq; p.Hkv = (int)r.Hkv; p.rotary = (int)r.rotary; p.num_pages = (int)r.num_pages;
   p.plus_one = (int)r.plus_one; p.norm_dim = r.norm_dim > 0 ? (int)r.norm_dim : D; p.eps = (float)r.eps;
   // Up to 512 rows: one row a block, a warp per page.  More are prompts: a page gets four warps, and one row in 16 begins a page; blocks of
-  // four or sixteen rows leave fewer blocks empty (8192 rows: 20 us of a GPU's instructions for blocks of four), but a mixed step's decode rows
-  // go through their block one after the other, which a long prompt beside them hides.
+  // four or sixteen rows leave fewer blocks empty, but a mixed step's decode rows go through their block one after the other, which a long
+  // prompt beside them hides.
   p.rows_per_block = p.T <= 512 ? 1 : p.T < 2048 ? 4 : 16;
   p.kv_blocks_x = (p.T + p.rows_per_block - 1) / p.rows_per_block;
-  p.kv_blocks_y = p.rows_per_block == 1 ? (2 * p.Hkv + 7) / 8 : p.Hkv;
-  const long long q_units = r.T * ((p.Hq + kWriteHeads - 1) / kWriteHeads);
+  p.kv_blocks_y = p.rows_per_block == 1 ? (p.Hkv + 7) / 8 : (p.Hkv + 1) / 2;
+  const int heads = 4 * 256 / D;                   // queries of a warp
+  const long long q_units = r.T * ((p.Hq + heads - 1) / heads);
   const long long blocks = (long long)p.kv_blocks_x * p.kv_blocks_y + (q_units + 7) / 8;
   if (blocks > 0x7fffffffll / 8) return -1;
   return by_width<Write>(D, p, (unsigned)blocks, (cudaStream_t)r.stream);

@@ -112,8 +112,8 @@ def qk_norm_rope_kv_write(q, k, v, positions, rope_cache, rotary_dim, k_cache, v
     pos = rope = 0
     if rotary_dim:
         _ints(positions, "positions", dev, 1)
-        if rotary_dim < 0 or rotary_dim > d or rotary_dim % (d // 16):
-            raise K.KernelError(f"the rotated width of {d}-wide heads is a multiple of {d // 16}, at most {d}, not {rotary_dim}")
+        if rotary_dim < 0 or rotary_dim > d or rotary_dim % 16:
+            raise K.KernelError(f"the rotated width of {d}-wide heads is a multiple of 16, at most {d}, not {rotary_dim}")
         if positions.shape[0] != T or rope_cache.dtype != _F32 or rope_cache.dim() != 2 or rope_cache.shape[1] != rotary_dim \
                 or not rope_cache.is_contiguous() or rope_cache.get_device() != dev:
             raise K.KernelError("rotation: a position per row and an fp32 [positions, rotary_dim] table beside the cache")
