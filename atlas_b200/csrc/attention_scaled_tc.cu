@@ -485,6 +485,532 @@ scaled_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPar
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- two tiles at a time
+// Heads of 64 and 128: two query tiles share every widened key tile, so that one tile's products run under the other one's softmax, and P
+// stays in TMEM.  Persistent, one CTA per SM; items (pair of query tiles, key head) with the most keys first.
+//   warps 0..3, 4..7   softmax of tile A and of tile B, a thread a row
+//   warp 15            pages by bulk copies, their scales
+//   warps 8..11        keys to bf16, values to f16 (two buffers of each)
+//   warps 12, 14       products of tile A and of tile B; QK_{j+1} behind PV_j, whose P lies where the scores go
+//   warp 13            query tiles by TMA, as they are (bf16: keys are exact in it)
+// Per pair of tiles and 128 keys: products 2048 clocks of the tensor cores, exponentials 2048 of the special-function units, shared memory
+// 1536 for operands and 512 for the widened tiles.
+constexpr int kC2Threads = 512;
+constexpr int kC2Kv = 128, kC2Pages = 8, kC2Ring = 8;
+
+template <int D>
+struct C2Tile {
+  static constexpr int kQ = (D / 64) * kScSub;                    // a query tile
+  static constexpr int kK = (D / 64) * kScSub;                    // 128 keys
+  static constexpr int kV = 2 * D * 128;                          // D channels x 128 tokens
+  static constexpr int kStage = kC2Kv * D;                        // the pages of a key tile
+  static constexpr int kSmem = 2 * (kQ + kK + kV) + 2 * kStage + kC2Ring * 64 + 256 + 1024;      // at most 227 KB
+};
+
+// The low word of a descriptor (make_smem_desc_sw128) carries the address, which steps along K; the high word is the same for all tiles.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+ATLAS_DEVICE uint32_t desc_low(const void* p) { return ((smem_u32(p) & 0x3FFFFu) >> 4) | (1u << 16); }
+ATLAS_DEVICE void umma_f16_lo(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+// A from TMEM: a row a lane, two 16-bit numbers a column
+ATLAS_DEVICE void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+ATLAS_DEVICE void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// pairs of fp32 numbers in one instruction
+ATLAS_DEVICE uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+ATLAS_DEVICE float2 unpair2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+ATLAS_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+ATLAS_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+ATLAS_DEVICE uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+ATLAS_DEVICE float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+struct C2Item {
+  int b, kvh, L, q_row0, q_len, q0, ctx0, page0;
+  int n[2], n_kv;                                                 // key tiles of tile A, of tile B, of both
+};
+ATLAS_DEVICE C2Item c2_item(const ScChunkParams& p, int it) {
+  C2Item r;
+  const int tile = it / p.Hkv, toks = kScRows / p.G;
+  r.kvh = it % p.Hkv;
+  r.b = p.tile_seq[tile];
+  r.q0 = p.tile_q0[tile];
+  r.L = min(p.seq_lens[r.b], p.bt_cols * kScPg);
+  r.q_row0 = p.query_start_loc[r.b];
+  r.q_len = p.query_start_loc[r.b + 1] - r.q_row0;
+  r.ctx0 = r.L - r.q_len;
+  r.page0 = p.window > 0 ? max(r.ctx0 + r.q0 - p.window + 1, 0) / kScPg : 0;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int first = r.q0 + x * toks, last = min(first + toks, r.q_len);
+    r.n[x] = first < r.q_len ? max((min(r.L, r.ctx0 + last) - r.page0 * kScPg + kC2Kv - 1) / kC2Kv, 0) : 0;
+  }
+  r.n_kv = max(r.n[0], r.n[1]);
+  return r;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kC2Threads, 1)
+scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkParams p, int items) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using Tile = C2Tile<D>;
+  uint8_t* sQ = smem;                                             // tile A, tile B: D / 64 sub-tiles [128 rows][64 channels]
+  uint8_t* sK = sQ + 2 * Tile::kQ;                                // two buffers: D / 64 sub-tiles [128 tokens][64 channels]
+  uint8_t* sV = sK + 2 * Tile::kK;                                // two buffers: 2 sub-tiles [D channels][64 tokens]
+  uint8_t* sStK = sV + 2 * Tile::kV;                              // the pages as they come, keys and values
+  uint8_t* sStV = sStK + Tile::kStage;
+  float2* sScale = reinterpret_cast<float2*>(sStV + Tile::kStage);  // [kC2Ring][8] (score factor, value exponent) of a page
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + kC2Ring * 8);
+  uint64_t* q_full = bars;
+  uint64_t* q_free = bars + 1;                                    // the item's last QK
+  uint64_t* k_full = bars + 2;                                    // [2] 4 warps
+  uint64_t* k_free = bars + 4;                                    // [2] QK of both tiles
+  uint64_t* v_full = bars + 6;                                    // [2] 4 warps
+  uint64_t* v_free = bars + 8;                                    // [2] PV of both tiles
+  uint64_t* s_full = bars + 10;                                   // [tile]
+  uint64_t* p_ready = bars + 22;                                  // [tile][half] 4 warps
+  uint64_t* pv_done = bars + 14;                                  // [tile]
+  uint64_t* o_free = bars + 16;                                   // [tile] 4 warps have read the item's output
+  uint64_t* ks_full = bars + 18;                                  // [keys, values] pages have come
+  uint64_t* ks_free = bars + 20;                                  // [keys, values] 4 warps
+  uint64_t* pv_half = bars + 26;                                  // [tile] the first half's product
+  uint64_t* stagger = bars + 28;                                  // 4 warps of tile A, once an item
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.G, toks = kScRows / G;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) { mbar_init(&ks_full[s], 1); mbar_init(&ks_free[s], 4); }
+    mbar_init(q_full, 1); mbar_init(q_free, 2); mbar_init(stagger, 4);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 4); mbar_init(&k_free[s], 2); mbar_init(&v_full[s], 4); mbar_init(&v_free[s], 2);
+      mbar_init(&s_full[s], 1); mbar_init(&pv_done[s], 1); mbar_init(&pv_half[s], 1); mbar_init(&o_free[s], 4);
+    }
+    for (int s = 0; s < 4; ++s) mbar_init(&p_ready[s], 4);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 12) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 13 && lane == 0) tma_prefetch_desc(&tmap_q);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;                               // scores of A, of B (128 columns each, P over them), outputs of A, of B
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ softmax: tile x, a thread a row
+    const int x = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + x * 128 + t_lane, tO = tmem + 256 + x * D + t_lane;
+    int n_s = 0, ring = 0;                                        // score tiles of this tile so far, key tiles of both
+    bool ok = true;
+    C2Item nxt = c2_item(p, blockIdx.x);
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+      const C2Item m_ = nxt;
+      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
+      const int n = m_.n[x];
+      const int tok = m_.q0 + x * toks + row / G, head = m_.kvh * G + row % G;
+      const bool live = row < toks * G && tok < m_.q_len;
+      const int pos = m_.ctx0 + tok;
+      // keys [start, end) are visible; rows that are not there see all, so that their warp need not mask, and are not stored
+      const int end = live ? min(pos + 1, m_.L) : 1 << 30;
+      const int start = live && p.window > 0 ? pos - p.window + 1 : 0;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j) {
+        ok = mbar_wait(&s_full[x], n_s & 1, abort_flag, p.status, 0xC00 + x);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        ++n_s;
+        tc_fence_after();
+        const int kv0 = (m_.page0 + j * kC2Pages) * kScPg;
+        const int hi = end - kv0, lo = start - kv0;
+        const bool whole = __all_sync(0xffffffffu, hi >= kC2Kv && lo <= 0);
+        const float2* sc = sScale + ((ring + j) % kC2Ring) * 8;
+        // ---- 64 columns at a time: their largest s + ev, then p = 2^(s + ev - m).  The reference m moves only when a score passes it by 2^8 (p
+        // stays inside f16), which is rare after a row's first columns; the output then moves with it (its last product was done before these scores
+        // began, and the second half waits for the first half's).  P takes half of the columns that its scores had.
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {                               // no further unrolled: the roles' code shares one instruction cache
+          uint32_t v[2][32];
+          tmem_ld_32x32b_x32(tS + c * 64, v[0]);
+          tmem_ld_32x32b_x32(tS + c * 64 + 32, v[1]);
+          float2 f[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) f[q] = sc[c * 4 + q];
+          tmem_ld_wait();
+          if (!whole) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t seen = bits_below(hi - c * 64 - k * 32) & ~bits_below(lo - c * 64 - k * 32);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[k][i] = (seen >> i) & 1u ? v[k][i] : 0xff800000u;
+            }
+          }
+          float mx[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t* u = &v[q >> 1][(q & 1) * 16];
+            float a = __uint_as_float(u[0]), z = __uint_as_float(u[1]);
+#pragma unroll
+            for (int i = 2; i < 14; i += 4) {
+              a = max3_nan(a, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+              z = max3_nan(z, __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
+            }
+            a = max3_nan(a, __uint_as_float(u[14]), __uint_as_float(u[15]));
+            mx[q] = fmaf(max3_nan(a, z, z), f[q].x, f[q].y);
+          }
+          const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+          if (__any_sync(0xffffffffu, !(top <= m + 8.f))) {         // NaN too: the row is NaN from here on
+            float alpha = 1.f;
+            if (!(top <= m + 8.f)) {
+              alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - top);
+              m = top;
+            }
+            l *= alpha;
+            if (c == 1) {                                           // the first half's product is under way
+              ok = mbar_wait(&pv_half[x], (n_s - 1) & 1, abort_flag, p.status, 0xC04 + x);
+              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+              tc_fence_after();
+            }
+            if (j > 0 || c == 1)
+#pragma unroll 1
+              for (int k = 0; k < D / 16; ++k) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(tO + k * 16, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_32x32b_x16(tO + k * 16, o);
+              }
+            tmem_st_wait();
+          }
+          const float ref = (m == -INFINITY) ? 0.f : m;
+          uint32_t w[2][16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t* u = &v[q >> 1][(q & 1) * 16];
+            const float add = f[q].y - ref;
+            const uint64_t f2 = pair2(f[q].x, f[q].x), a2 = pair2(add, add);
+            uint64_t s2 = 0;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const uint64_t x2 = fma2(pair2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), f2, a2);
+              float2 e = unpair2(x2);
+              e.x = fast_exp2(e.x);
+              e.y = fast_exp2(e.y);
+              s2 = add2(s2, pair2(e.x, e.y));
+              w[q >> 1][(q & 1) * 8 + i / 2] = sc_h2(e.x, e.y);
+            }
+            const float2 s = unpair2(s2);
+            l = fmaf(s.x + s.y, exact_pow2(-(int)f[q].y), l);
+          }
+          tmem_st_32x32b_x16(tS + c * 32, w[0]);
+          tmem_st_32x32b_x16(tS + c * 32 + 16, w[1]);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&p_ready[2 * x + c]);                       // the first half's product runs under the second half
+            if (x == 0 && c == 0 && j == 0) mbar_arrive(stagger);
+          }
+        }
+        if (!ok) break;
+      }
+      ring += m_.n_kv;
+      if (!ok) break;
+      // ---- o / l
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      __nv_bfloat16* out = p.out + (long long)(m_.q_row0 + tok) * p.ldo + head * D;
+      if (n > 0) {
+        ok = mbar_wait(&pv_done[x], (n_s - 1) & 1, abort_flag, p.status, 0xC02 + x);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(tO, r[0]);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          tmem_ld_wait();
+          if (c + 1 < D / 32) tmem_ld_32x32b_x32(tO + (c + 1) * 32, r[(c + 1) & 1]);
+          else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[x]);
+          }
+          if (live) {
+            uint32_t (&v)[32] = r[c & 1];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4 o;
+              o.x = pack_bf16x2(__uint_as_float(v[q * 8 + 0]) * inv, __uint_as_float(v[q * 8 + 1]) * inv);
+              o.y = pack_bf16x2(__uint_as_float(v[q * 8 + 2]) * inv, __uint_as_float(v[q * 8 + 3]) * inv);
+              o.z = pack_bf16x2(__uint_as_float(v[q * 8 + 4]) * inv, __uint_as_float(v[q * 8 + 5]) * inv);
+              o.w = pack_bf16x2(__uint_as_float(v[q * 8 + 6]) * inv, __uint_as_float(v[q * 8 + 7]) * inv);
+              *reinterpret_cast<uint4*>(out + c * 32 + q * 8) = o;
+            }
+          }
+        }
+      } else if (live) {
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+      }
+      if (p.ml && live) p.ml[(long long)(m_.q_row0 + tok) * p.Hq + head] = make_float2(m == -INFINITY ? 0.f : m, inv);
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ converters
+    const int r = threadIdx.x - 256;
+    constexpr int kPer = D / 16;                                  // 16-byte pieces of a thread and tile: piece i of page i / D
+    uint32_t n_t = 0;                                             // key tiles so far
+    bool ok = true;
+    C2Item nxt = c2_item(p, blockIdx.x);
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+      const int L = nxt.L, page0 = nxt.page0, n_kv = nxt.n_kv;
+      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
+      for (int j = 0; j < n_kv; ++j, ++n_t) {
+        const int s = n_t & 1;
+        // ---- keys
+        ok = mbar_wait(&ks_full[0], n_t & 1, abort_flag, p.status, 0xC10) &&
+             mbar_wait(&k_free[s], ((n_t >> 1) & 1) ^ 1u, abort_flag, p.status, 0xC11);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll 4
+        for (int k = 0; k < kPer; ++k) {
+          const int i = k * 128 + r, in = i % D, trow = (i / D) * kScPg + in / (D / 16), c = in % (D / 16), tsw = trow & 7;
+          uint4 lo, hi;
+          sc_widen16(reinterpret_cast<const uint4*>(sStK)[i], lo, hi);
+          uint8_t* rowp = sK + s * Tile::kK + (c >> 2) * kScSub + (trow >> 3) * 1024 + tsw * 128;
+          const int ch = (c & 3) * 2;
+          *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = make_uint4(h2_to_bf2(lo.x), h2_to_bf2(lo.y), h2_to_bf2(lo.z), h2_to_bf2(lo.w));
+          *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ tsw) << 4)) = make_uint4(h2_to_bf2(hi.x), h2_to_bf2(hi.y), h2_to_bf2(hi.z), h2_to_bf2(hi.w));
+        }
+        fence_proxy_async();                                      // the tile for the products, and the pages read before they are copied over
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(&k_full[s]); mbar_arrive(&ks_free[0]); }
+        // ---- values
+        ok = mbar_wait(&ks_full[1], n_t & 1, abort_flag, p.status, 0xC12) &&
+             mbar_wait(&v_free[s], ((n_t >> 1) & 1) ^ 1u, abort_flag, p.status, 0xC13);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll 4
+        for (int k = 0; k < kPer; ++k) {
+          const int i = k * 128 + r, pg = i / D, dim = i % D, sw = dim & 7;
+          const int left = L - (page0 + j * kC2Pages + pg) * kScPg;      // tokens of the page; the others are cleared
+          uint4 v = reinterpret_cast<const uint4*>(sStV)[i];
+          if (left < kScPg) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int there = min(max(left - 4 * q, 0), 4);
+              w[q] = there == 4 ? w[q] : (w[q] & ((1u << (8 * there)) - 1u));
+            }
+          }
+          uint4 lo, hi;
+          sc_widen16(v, lo, hi);
+          uint8_t* rowp = sV + s * Tile::kV + (pg >> 2) * (D * 128) + (dim >> 3) * 1024 + sw * 128;
+          const int ch = (pg & 3) * 2;
+          *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
+          *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(&v_full[s]); mbar_arrive(&ks_free[1]); }
+      }
+    }
+  } else if (warp == 15) {
+    // ------------------------------------------------------------------ pages: lanes 0..7 keys, 8..15 values, entries and scales two tiles ahead
+    const bool is_v = (lane & 8) != 0;
+    uint32_t n_t = 0;
+    bool ok = true;
+    C2Item nxt = c2_item(p, blockIdx.x);
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+      const C2Item m_ = nxt;
+      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
+      const int n_pages = (m_.L + kScPg - 1) / kScPg;
+      const int* bt = p.block_tables + (long long)m_.b * p.bt_ld;
+      auto entry = [&](int j) {                                   // -1: behind the end or outside of the pool
+        const int pg = m_.page0 + j * kC2Pages + (lane & 7);
+        return lane < 16 && j < m_.n_kv && pg < n_pages ? bt[pg] : -1;
+      };
+      auto scale_of = [&](int blk) {
+        if ((unsigned)blk >= (unsigned)p.num_pages) return 1.f;
+        return is_v ? p.v_scale[blk * p.vs_ld + m_.kvh * p.vs_h] : p.k_scale[blk * p.ks_ld + m_.kvh * p.ks_h];
+      };
+      int blk = entry(0), blk1 = entry(1);
+      float sc = scale_of(blk);
+      for (int j = 0; j < m_.n_kv; ++j, ++n_t) {
+        const int blk2 = entry(j + 2);
+        const float sc1 = scale_of(blk1);
+        const bool live = (unsigned)blk < (unsigned)p.num_pages;
+        const uint32_t pages = __ballot_sync(0xffffffffu, live);
+        const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
+        if (lane < 8) sScale[(n_t % kC2Ring) * 8 + lane] = make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
+        __syncwarp();
+        const long long at = ((long long)blk * p.Hkv + m_.kvh) * (kScPg * D);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          ok = mbar_wait(&ks_free[w], (n_t & 1) ^ 1u, abort_flag, p.status, 0xC30 + w);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          if (lane == 0) mbar_expect_tx(&ks_full[w], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
+          __syncwarp();
+          if (live && is_v == (w == 1)) sc_bulk((w ? sStV : sStK) + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &ks_full[w]);
+        }
+        if (!ok) break;
+        blk = blk1; blk1 = blk2;
+        sc = sc1;
+      }
+    }
+    if (!ok)
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  } else if (warp == 12 || warp == 14) {
+    // ------------------------------------------------------------------ products of tile x, each tile at its own pace.  The whole warp walks the
+    // list and one elected lane issues: descriptors stay in uniform registers so (under a lane's branch an MMA took 110 clocks to issue).
+    constexpr uint32_t kIdescS = make_idesc(kScRows, kC2Kv, 1u), kIdescO = make_idesc(kScRows, D, 0u);      // bf16 scores, f16 outputs
+    const int x = (warp - 12) >> 1;
+    const uint32_t dQ = desc_low(sQ + x * Tile::kQ), dK = desc_low(sK), dV = desc_low(sV);
+    const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * D;
+    uint32_t n_t = 0, n_i = 0, pvs = 0, outs = 0, staggers = 0;   // key tiles, items, PV products, items with output, items of tile A
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, site + x)); };
+    auto full = [&](uint64_t* bar, uint32_t t, uint32_t site) { return wait(bar + (t & 1), (t >> 1) & 1, site); };
+    // scores with key tile t; the PV product that read P out of the same columns is done
+    auto score = [&](uint32_t t, bool last) -> bool {
+      if (pvs > 0 && !wait(&pv_done[x], (pvs - 1) & 1, 0xC20)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t bd = dK + (t & 1) * (Tile::kK >> 4);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t at = (ks >> 2) * (kScSub >> 4) + 2 * (ks & 3);
+          umma_f16_lo(tS, dQ + at, bd + at, kIdescS, ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[x]);
+        umma_commit(&k_free[t & 1]);
+        if (last) umma_commit(q_free);
+      }
+      __syncwarp();
+      return true;
+    };
+    // a tile that has no use for a buffer hands it on, once it is full (its last use is counted then)
+    auto skip = [&](uint64_t* bar_free, uint32_t t) {
+      if (lane == 0) mbar_arrive(bar_free + (t & 1));
+    };
+    C2Item nxt = c2_item(p, blockIdx.x);
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++n_i) {
+      const int n = __shfl_sync(0xffffffffu, nxt.n[x], 0), n_kv = __shfl_sync(0xffffffffu, nxt.n_kv, 0), n_of_a = nxt.n[0];
+      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
+      ok = wait(q_full, n_i & 1, 0xC22);
+      if (!ok) break;
+      if (n == 0 && lane == 0) mbar_arrive(q_free);
+      if (n_kv == 0) continue;
+      ok = full(k_full, n_t, 0xC24);
+      // tile B begins when tile A has half of its first P: the two then take turns at products and exponentials (in step, both waited for the
+      // products and the special-function units idled for a third of the time)
+      const int n_a = __shfl_sync(0xffffffffu, n_of_a, 0);
+      if (x == 1 && n > 0 && n_a > 0) ok = ok && wait(stagger, staggers & 1, 0xC2E);
+      if (n_a > 0) ++staggers;
+      if (ok && n > 0) ok = score(n_t, n == 1);
+      else if (ok) skip(k_free, n_t);
+      for (int j = 0; j < n_kv && ok; ++j, ++n_t) {
+        // what the next products need besides P, before P is waited for
+        ok = full(v_full, n_t, 0xC26) && (j + 1 >= n_kv || full(k_full, n_t + 1, 0xC2C));
+        if (!ok) break;
+        if (j < n) {
+          if (j == 0 && outs > 0) ok = wait(&o_free[x], (outs - 1) & 1, 0xC28);
+          for (int half = 0; half < 2 && ok; ++half) {
+            ok = wait(&p_ready[2 * x + half], pvs & 1, 0xC2A);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t bd = dV + (n_t & 1) * (Tile::kV >> 4) + half * (D * 128 >> 4);
+#pragma unroll
+              for (int ks = 0; ks < kC2Kv / 32; ++ks) umma_f16_ta(tO, tS + half * 32 + ks * 8, bd + 2 * ks, kIdescO, (j > 0 || half > 0 || ks > 0) ? 1u : 0u);
+              if (half == 0) {
+                umma_commit(&pv_half[x]);
+              } else {
+                umma_commit(&pv_done[x]);
+                umma_commit(&v_free[n_t & 1]);
+              }
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          ++pvs;
+          if (j + 1 == n) ++outs;
+        } else {
+          skip(v_free, n_t);
+        }
+        if (j + 1 < n_kv) {
+          if (j + 1 < n) ok = score(n_t + 1, j + 2 == n);
+          else skip(k_free, n_t + 1);
+        }
+      }
+    }
+  } else if (warp == 13) {
+    // ------------------------------------------------------------------ query tiles
+    if (lane == 0) {
+      uint32_t n_i = 0;
+      bool ok = true;
+      for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++n_i) {
+        const int tile = it / p.Hkv, kvh = it % p.Hkv, row = p.query_start_loc[p.tile_seq[tile]] + p.tile_q0[tile];
+        ok = mbar_wait(q_free, (n_i & 1) ^ 1u, abort_flag, p.status, 0xC30);
+        if (!ok) break;
+        mbar_expect_tx(q_full, 2u * (uint32_t)(D / 64) * 128u * (uint32_t)(toks * G));
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) tma_load_3d(sQ + x * Tile::kQ + c * kScSub, &tmap_q, q_full, c * 64, kvh * G, row + x * toks);
+      }
+      if (!ok)
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------- weights
 constexpr int kSwThreads = 320;        // producer, issuer, eight warps that add
 constexpr int kSwStages = 2;           // query tiles in shared memory, score buffers in TMEM
@@ -706,6 +1232,13 @@ int query_map(CUtensorMap* m, const void* q, long long ldq, int total_tokens, in
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -11;
 }
 
+template <typename Kern>
+int launch_pairs(Kern kern, int smem, int blocks, const CUtensorMap& tq, const ScChunkParams& p, int items, cudaStream_t st) {
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem) != cudaSuccess) return -20;
+  kern<<<blocks, kC2Threads, smem, st>>>(tq, p, items);
+  return cudaGetLastError() == cudaSuccess ? 0 : -20;
+}
+
 template <typename Kern, typename P>
 int launch_tiles(Kern kern, int smem, dim3 grid, int threads, const CUtensorMap& tq, const P& p, cudaStream_t st) {
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem) != cudaSuccess) return -20;
@@ -715,7 +1248,8 @@ int launch_tiles(Kern kern, int smem, dim3 grid, int threads, const CUtensorMap&
 
 }  // namespace
 
-// Rows of chunk sequences: `tiles` query tiles of 128 / G tokens, each (sequence, first token of the tile in its chunk); `ml` (or null) gets
+// Rows of chunk sequences: `tiles` query tiles of 128 / G tokens (heads of 64 and 128: pairs of tiles), each (sequence, first token in its
+// chunk); `ml` (or null) gets
 // every row's reference and 1 / l.  With `weights`, tiles of 128 cached tokens follow, each (sequence, first token), whose sums grow by the
 // rows' softmax weights.  Arguments as one record (see kv_scaled.cu).  -1: sizes or alignment outside of what the kernels take.
 struct ChunkRecord {
@@ -723,7 +1257,7 @@ struct ChunkRecord {
   const float* ks; long long ks_ld, ks_h; const float* vs; long long vs_ld, vs_h;
   const int* tables; long long bt_ld, bt_cols; const int* seq_lens; const int* starts;
   const int* tile_seq; const int* tile_q0; long long tiles, total_tokens, Hq, Hkv, D, window, num_pages; float* ml;
-  const int* key_seq; const int* key_k0; long long key_tiles; float* weights; long long w_ld_b, w_ld_h, width; double scale; void* status;
+  const int* key_seq; const int* key_k0; long long key_tiles; float* weights; long long w_ld_b, w_ld_h, width, sms; double scale; void* status;
   void* stream;
 };
 extern "C" int atlas_attn_scaled_chunk(const void* record) {
@@ -745,9 +1279,13 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
                   (int)r.window, (int)r.num_pages, reinterpret_cast<float2*>(r.ml), status};
   const dim3 grid((unsigned)r.tiles, Hkv);
   int rc;
-  if (D == 64) rc = launch_tiles(scaled_chunk_kernel<64>, ScTile<64>::kSmem, grid, kScThreads, tq, p, st);
-  else if (D == 128) rc = launch_tiles(scaled_chunk_kernel<128>, ScTile<128>::kSmem, grid, kScThreads, tq, p, st);
-  else rc = launch_tiles(scaled_chunk_kernel<256>, ScTile<256>::kSmem, grid, kScThreads, tq, p, st);
+  if (D <= 128) {
+    const long long items = r.tiles * Hkv;
+    if (items > 0x3fffffffll) return -1;
+    const int blocks = (int)(items < r.sms ? items : r.sms);
+    if (D == 64) rc = launch_pairs(scaled_chunk2_kernel<64>, C2Tile<64>::kSmem, blocks, tq, p, (int)items, st);
+    else rc = launch_pairs(scaled_chunk2_kernel<128>, C2Tile<128>::kSmem, blocks, tq, p, (int)items, st);
+  } else rc = launch_tiles(scaled_chunk_kernel<256>, ScTile<256>::kSmem, grid, kScThreads, tq, p, st);
   if (rc || !r.weights || r.key_tiles <= 0) return rc;
   ScWeighParams w{(const uint8_t*)r.k_cache, r.ks, r.ks_ld, (int)r.ks_h, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.seq_lens, r.starts, r.key_seq,
                   r.key_k0, scale_log2, Hq, Hkv, G, (int)r.window, (int)r.num_pages, reinterpret_cast<const float2*>(r.ml), r.weights, r.w_ld_b,

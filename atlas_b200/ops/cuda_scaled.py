@@ -25,7 +25,7 @@ _WRITE = struct.Struct("=29qdq")
 _READ = struct.Struct("=20q")
 _EVICT = struct.Struct("=28q")
 _DECODE = struct.Struct("=33qd2q")
-_CHUNK = struct.Struct("=34qd2q")
+_CHUNK = struct.Struct("=35qd2q")
 _calls: dict = {}
 
 
@@ -259,7 +259,7 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
                 at_q, ldq, at_out, hq * d, *cache, nd, hq, hkv, d, window, nb, longest, blocks, at, at + 4 * n_o, at_s if n_s else 0, width,
                 at_s + 4 * n_s if n_r else 0, *sums, scale, status, stream), "attn_scaled_decode")
         if B > nd:
-            tiles, n, _ = K._tc_tiles(q, batch, nd, 128 // g)
+            tiles, n, _ = K._tc_tiles(q, batch, nd, 128 // g * (2 if d <= 128 else 1))
             ml = key_tiles = None
             at_keys = n_keys = 0
             if weights is not None:
@@ -269,5 +269,5 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
             at = tiles.data_ptr()
             _call("atlas_attn_scaled_chunk", _CHUNK.pack(
                 at_q, ldq, at_out, hq * d, *cache, at, at + 4 * n, n, T, hq, hkv, d, window, nb, 0 if ml is None else ml.data_ptr(), at_keys,
-                at_keys + 4 * n_keys, n_keys, *sums, width, scale, status, stream), "attn_scaled_chunk")
+                at_keys + 4 * n_keys, n_keys, *sums, width, K._num_sms[index], scale, status, stream), "attn_scaled_chunk")
     return out
