@@ -569,25 +569,55 @@ struct C2Item {
   int b, kvh, L, q_row0, q_len, q0, ctx0, page0;
   int n[2], n_kv;                                                 // key tiles of tile A, of tile B, of both
 };
-ATLAS_DEVICE C2Item c2_item(const ScChunkParams& p, int it) {
-  C2Item r;
-  const int tile = it / p.Hkv, toks = kScRows / p.G;
-  r.kvh = it % p.Hkv;
-  r.b = p.tile_seq[tile];
-  r.q0 = p.tile_q0[tile];
-  r.L = min(p.seq_lens[r.b], p.bt_cols * kScPg);
-  r.q_row0 = p.query_start_loc[r.b];
-  r.q_len = p.query_start_loc[r.b + 1] - r.q_row0;
-  r.ctx0 = r.L - r.q_len;
-  r.page0 = p.window > 0 ? max(r.ctx0 + r.q0 - p.window + 1, 0) / kScPg : 0;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int first = r.q0 + x * toks, last = min(first + toks, r.q_len);
-    r.n[x] = first < r.q_len ? max((min(r.L, r.ctx0 + last) - r.page0 * kScPg + kC2Kv - 1) / kC2Kv, 0) : 0;
+// Item of a CTA in round `rd`: the rounds go to and fro over the CTAs, so that the ones with the longest item of a round get the shortest of
+// the next (2 x 3001 ragged rows: 47 key tiles on the busiest CTA of 44 on average, 56 with rounds all one way).
+ATLAS_DEVICE int c2_turn(int rd) { return rd * (int)gridDim.x + ((rd & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); }
+
+// Every role walks the CTA's items by itself.  An item's two dependent loads (its sequence, the sequence's lengths) are issued two items and
+// one item ahead, so that no role waits for them.
+struct C2Walk {
+  const ScChunkParams& p;
+  int items, rd, b1, q1, len1, s1, e1, b2, q2;
+  ATLAS_DEVICE C2Walk(const ScChunkParams& params, int n) : p(params), items(n), rd(0) {
+    tile(0, b1, q1);
+    tile(1, b2, q2);
+    lengths();
   }
-  r.n_kv = max(r.n[0], r.n[1]);
-  return r;
-}
+  ATLAS_DEVICE void tile(int round, int& b, int& q) const {
+    const int it = min(c2_turn(round), items - 1) / p.Hkv;
+    b = p.tile_seq[it];
+    q = p.tile_q0[it];
+  }
+  ATLAS_DEVICE void lengths() {
+    len1 = p.seq_lens[b1];
+    s1 = p.query_start_loc[b1];
+    e1 = p.query_start_loc[b1 + 1];
+  }
+  ATLAS_DEVICE bool more() const { return c2_turn(rd) < items; }
+  ATLAS_DEVICE C2Item next() {
+    C2Item r;
+    const int toks = kScRows / p.G;
+    r.kvh = c2_turn(rd) % p.Hkv;
+    r.b = b1;
+    r.q0 = q1;
+    r.L = min(len1, p.bt_cols * kScPg);
+    r.q_row0 = s1;
+    r.q_len = e1 - s1;
+    r.ctx0 = r.L - r.q_len;
+    r.page0 = p.window > 0 ? max(r.ctx0 + r.q0 - p.window + 1, 0) / kScPg : 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int first = r.q0 + x * toks, last = min(first + toks, r.q_len);
+      r.n[x] = first < r.q_len ? max((min(r.L, r.ctx0 + last) - r.page0 * kScPg + kC2Kv - 1) / kC2Kv, 0) : 0;
+    }
+    r.n_kv = max(r.n[0], r.n[1]);
+    b1 = b2;
+    q1 = q2;
+    lengths();
+    tile(++rd + 1, b2, q2);
+    return r;
+  }
+};
 
 template <int D>
 __global__ void __launch_bounds__(kC2Threads, 1)
@@ -648,10 +678,9 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     const uint32_t tS = tmem + x * 128 + t_lane, tO = tmem + 256 + x * D + t_lane;
     int n_s = 0, ring = 0;                                        // score tiles of this tile so far, key tiles of both
     bool ok = true;
-    C2Item nxt = c2_item(p, blockIdx.x);
-    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
-      const C2Item m_ = nxt;
-      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
+    C2Walk walk(p, items);
+    while (walk.more() && ok) {
+      const C2Item m_ = walk.next();
       const int n = m_.n[x];
       const int tok = m_.q0 + x * toks + row / G, head = m_.kvh * G + row % G;
       const bool live = row < toks * G && tok < m_.q_len;
@@ -803,10 +832,10 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     constexpr int kPer = D / 16;                                  // 16-byte pieces of a thread and tile: piece i of page i / D
     uint32_t n_t = 0;                                             // key tiles so far
     bool ok = true;
-    C2Item nxt = c2_item(p, blockIdx.x);
-    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+    C2Walk walk(p, items);
+    while (walk.more() && ok) {
+      const C2Item nxt = walk.next();
       const int L = nxt.L, page0 = nxt.page0, n_kv = nxt.n_kv;
-      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
       for (int j = 0; j < n_kv; ++j, ++n_t) {
         const int s = n_t & 1;
         // ---- keys
@@ -860,10 +889,9 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     const bool is_v = (lane & 8) != 0;
     uint32_t n_t = 0;
     bool ok = true;
-    C2Item nxt = c2_item(p, blockIdx.x);
-    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
-      const C2Item m_ = nxt;
-      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
+    C2Walk walk(p, items);
+    while (walk.more() && ok) {
+      const C2Item m_ = walk.next();
       const int n_pages = (m_.L + kScPg - 1) / kScPg;
       const int* bt = p.block_tables + (long long)m_.b * p.bt_ld;
       auto entry = [&](int j) {                                   // -1: behind the end or outside of the pool
@@ -933,10 +961,10 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     auto skip = [&](uint64_t* bar_free, uint32_t t) {
       if (lane == 0) mbar_arrive(bar_free + (t & 1));
     };
-    C2Item nxt = c2_item(p, blockIdx.x);
-    for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++n_i) {
+    C2Walk walk(p, items);
+    for (; walk.more() && ok; ++n_i) {
+      const C2Item nxt = walk.next();
       const int n = __shfl_sync(0xffffffffu, nxt.n[x], 0), n_kv = __shfl_sync(0xffffffffu, nxt.n_kv, 0), n_of_a = nxt.n[0];
-      if (it + (int)gridDim.x < items) nxt = c2_item(p, it + gridDim.x);
       ok = wait(q_full, n_i & 1, 0xC22);
       if (!ok) break;
       if (n == 0 && lane == 0) mbar_arrive(q_free);
@@ -989,8 +1017,10 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     if (lane == 0) {
       uint32_t n_i = 0;
       bool ok = true;
-      for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++n_i) {
-        const int tile = it / p.Hkv, kvh = it % p.Hkv, row = p.query_start_loc[p.tile_seq[tile]] + p.tile_q0[tile];
+      C2Walk walk(p, items);
+      for (; walk.more() && ok; ++n_i) {
+        const C2Item m_ = walk.next();
+        const int row = m_.q_row0 + m_.q0, kvh = m_.kvh;
         ok = mbar_wait(q_free, (n_i & 1) ^ 1u, abort_flag, p.status, 0xC30);
         if (!ok) break;
         mbar_expect_tx(q_full, 2u * (uint32_t)(D / 64) * 128u * (uint32_t)(toks * G));
