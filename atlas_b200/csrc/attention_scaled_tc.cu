@@ -12,8 +12,9 @@
 //   warps 2..5   e4m3 -> f16, into the 128-byte-swizzled K-major layout (values are stored with tokens along rows already)
 //   warps 6..13  softmax, two threads a row; O is rescaled in TMEM only when a row's maximum has passed its reference by 2^8
 //
-// scaled_chunk_weigh_kernel: one CTA per (128 cached tokens, key head), rows of the chunk go by.  S^T = K Q^T in bf16 (an e4m3 number is one
-// exactly, and Q stays as it is): a TMEM lane is a token, so that the sum over rows and heads is a register's sum, with no atomics.
+// scaled_chunk_weigh_kernel: a cluster of two CTAs per (128 cached tokens, key head); tiles of the chunk's rows go by, every other one to each.
+// S^T = K Q^T in bf16 (an e4m3 number is one exactly, and Q stays as it is): a TMEM lane is a token, so that the sum over rows and heads is a
+// register's sum, and the two CTAs' sums are added in their order, with no atomics.
 #include "common.cuh"
 #include "host_api.h"
 #include "tc_util.cuh"
@@ -1045,6 +1046,8 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
 constexpr int kSwThreads = 320;        // producer, issuer, eight warps that add
 constexpr int kSwStages = 2;           // query tiles in shared memory, score buffers in TMEM
 
+ATLAS_DEVICE void st_cluster_f32(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(addr), "f"(v) : "memory"); }
+
 struct ScWeighParams {
   const uint8_t* k_cache; const float* k_scale; long long ks_ld; int ks_h;
   const int* block_tables; int bt_ld, bt_cols;
@@ -1060,20 +1063,22 @@ struct ScWeighParams {
 template <int D>
 struct SwTile {
   static constexpr int kQ = (D / 64) * kScSub;                    // a query tile
-  static constexpr int kSmem = (1 + kSwStages) * kQ + kSwStages * kScRows * 8 + kScRows * 4 + 512 + 1024;
+  static constexpr int kSmem = (1 + kSwStages) * kQ + kSwStages * kScRows * 8 + 3 * kScRows * 4 + 128 + 1024;      // 101 KB for heads of 128: two CTAs
 };
 
 template <int D>
-__global__ void __launch_bounds__(kSwThreads, 1)
+__global__ void __launch_bounds__(kSwThreads, D == 256 ? 1 : 2)
 scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWeighParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int kQ = SwTile<D>::kQ;
   uint8_t* sK = smem;                                              // D / 64 sub-tiles [128 tokens][64 channels], bf16
   uint8_t* sQ = sK + kQ;                                           // kSwStages x the same of query rows
-  float2* sMl = reinterpret_cast<float2*>(sQ + kSwStages * kQ);    // [stages][128] (M, 1 / l) of a row
-  float* sSum = reinterpret_cast<float*>(sMl + kSwStages * kScRows);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sSum + kScRows);
+  float* sM = reinterpret_cast<float*>(sQ + kSwStages * kQ);       // [stages][-M of 128 rows, 1 / l of 128 rows]
+  float* sSum = sM + kSwStages * 2 * kScRows;
+  float* sOwn = sSum + kScRows;                                    // [128] this CTA's sums
+  float* sOther = sOwn + kScRows;                                  // [128] the other CTA's, in the first one
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sOther + kScRows);
   uint64_t* q_full = bars;                                         // [stages] one arrival + the tile's bytes
   uint64_t* q_empty = q_full + kSwStages;                          // [stages] QK done
   uint64_t* s_full = q_empty + kSwStages;                          // [stages]
@@ -1083,14 +1088,15 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.G, toks = kScRows / G;
-  const int b = p.tile_seq[blockIdx.x], k0 = p.tile_k0[blockIdx.x], kvh = blockIdx.y;
+  const int part = blockIdx.x & 1, at = blockIdx.x >> 1;          // of a cluster of two: every other tile of rows
+  const int b = p.tile_seq[at / p.Hkv], k0 = p.tile_k0[at / p.Hkv], kvh = at % p.Hkv;
   const int L = min(p.seq_lens[b], p.bt_cols * kScPg);
   const int q_row0 = p.query_start_loc[b], q_len = p.query_start_loc[b + 1] - q_row0;
   const int ctx0 = L - q_len;
   // rows that see some of the tokens [k0, k0 + 128): positions [k0, k0 + 127 + window)
-  const int r_lo = max(k0 - ctx0, 0) / toks * toks;
+  const int r_lo = max(k0 - ctx0, 0) / toks * toks + part * toks;
   const int r_hi = p.window > 0 ? min(q_len, k0 + kScRows - 1 + p.window - ctx0) : q_len;
-  const int n_q = r_hi > r_lo ? (r_hi - r_lo + toks - 1) / toks : 0;
+  const int n_q = r_hi > r_lo ? (r_hi - r_lo + 2 * toks - 1) / (2 * toks) : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSwStages; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); }
@@ -1136,7 +1142,7 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
     // ------------------------------------------------------------------ producer: query rows, their M and 1 / l
     bool ok = true;
     for (int j = 0; j < n_q && ok; ++j) {
-      const int s = j % kSwStages, q0 = r_lo + j * toks;
+      const int s = j % kSwStages, q0 = r_lo + j * 2 * toks;
       if (lane == 0) ok = mbar_wait(&q_empty[s], ((j / kSwStages) & 1) ^ 1u, abort_flag, p.status, 0xB00) &&
                           mbar_wait(&s_free[s], ((j / kSwStages) & 1) ^ 1u, abort_flag, p.status, 0xB01);
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -1146,7 +1152,8 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
         const int r = i + lane, tok = q0 + r / G;
         float2 x = make_float2(INFINITY, 0.f);                     // a row that is not there adds 2^-inf * 0
         if (r < toks * G && tok < q_len) x = p.ml[(long long)(q_row0 + tok) * p.Hq + kvh * G + r % G];
-        sMl[s * kScRows + r] = x;
+        sM[s * 2 * kScRows + r] = -x.x;
+        sM[s * 2 * kScRows + kScRows + r] = x.y;
       }
       __syncwarp();
       if (lane == 0) {
@@ -1158,23 +1165,23 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
     if (!ok)
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer: S^T = K Q^T
-    if (lane == 0) {
-      constexpr uint32_t kIdesc = make_idesc(kScRows, kScRows, 1u);      // bf16 x bf16 -> f32
-      const uint32_t aK = smem_u32(sK), aQ = smem_u32(sQ);
-      for (int j = 0; j < n_q; ++j) {
-        const int s = j % kSwStages;
-        if (!mbar_wait(&q_full[s], (j / kSwStages) & 1, abort_flag, p.status, 0xB10)) break;
-        tc_fence_after();
+    // ------------------------------------------------------------------ products: S^T = K Q^T (the whole warp, one elected lane issues)
+    constexpr uint32_t kIdesc = make_idesc(kScRows, kScRows, 1u);        // bf16 x bf16 -> f32
+    const uint32_t dK = desc_low(sK), dQ = desc_low(sQ);
+    for (int j = 0; j < n_q; ++j) {
+      const int s = j % kSwStages;
+      if (!__all_sync(0xffffffffu, mbar_wait(&q_full[s], (j / kSwStages) & 1, abort_flag, p.status, 0xB10))) break;
+      tc_fence_after();
+      if (elect_one()) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint64_t ad = make_smem_desc_sw128(aK + (ks >> 2) * kScSub) + 2 * (ks & 3);
-          const uint64_t bd = make_smem_desc_sw128(aQ + s * kQ + (ks >> 2) * kScSub) + 2 * (ks & 3);
-          umma_f16(tS + s * kScRows, ad, bd, kIdesc, ks > 0 ? 1u : 0u);
+          const uint32_t at = (ks >> 2) * (kScSub >> 4) + 2 * (ks & 3);
+          umma_f16_lo(tS + s * kScRows, dK + at, dQ + s * (kQ >> 4) + at, kIdesc, ks > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[s]);
         umma_commit(&q_empty[s]);
       }
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------------ two threads a token, 64 rows each
@@ -1189,55 +1196,62 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
     float total = 0.f;
     bool ok = true;
     for (int j = 0; j < n_q && ok; ++j) {
-      const int s = j % kSwStages, q0 = r_lo + j * toks;
+      const int s = j % kSwStages, q0 = r_lo + j * 2 * toks;
       ok = mbar_wait(&s_full[s], (j / kSwStages) & 1, abort_flag, p.status, 0xB20);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
-      uint32_t r[2][32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(tS + s * kScRows + t_lane + half * 64 + c * 32, r[c]);
-      tmem_ld_wait();
-      const float4* ml = reinterpret_cast<const float4*>(sMl + s * kScRows + half * 64);
       // row r of the tile stands at position first + r / G: seen by tokens in (position - window, position]
       const int first = ctx0 + q0;
       const int there = min(toks, q_len - q0);             // rows behind them are another sequence's
       const bool all_seen = there == toks && k0 + kScRows - 1 <= first && (p.window == 0 || first + toks - 1 - p.window < k0);
-      float a[4] = {0.f, 0.f, 0.f, 0.f};
-      if (all_seen) {
+      // columns of rows that see this lane's token
+      const int c_lo = max(tok - first, 0) * G, c_hi = (p.window > 0 ? min(tok + p.window - first, there) : there) * G;
+      const uint64_t f2 = pair2(f, f);
+      uint64_t sum2 = 0;
+#pragma unroll 1
+      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tS + s * kScRows + t_lane + c, r);
+        const float4* m4 = reinterpret_cast<const float4*>(sM + s * 2 * kScRows + c);
+        const float4* l4 = reinterpret_cast<const float4*>(sM + s * 2 * kScRows + kScRows + c);
+        const uint32_t seen = all_seen ? 0xffffffffu : bits_below(c_hi - c) & ~bits_below(c_lo - c);
+        tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float4 x = ml[c * 16 + i / 2];
-            a[i & 3] = fmaf(fast_exp2(fmaf(__uint_as_float(r[c][i]), f, -x.x)), x.y, a[i & 3]);
-            a[(i & 3) + 1] = fmaf(fast_exp2(fmaf(__uint_as_float(r[c][i + 1]), f, -x.z)), x.w, a[(i & 3) + 1]);
+        for (int i = 0; i < 32; i += 4) {
+          const float4 m = m4[i / 4], l = l4[i / 4];
+          float2 a = unpair2(fma2(pair2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2, pair2(m.x, m.y)));
+          float2 b2 = unpair2(fma2(pair2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), f2, pair2(m.z, m.w)));
+          a.x = fast_exp2(a.x); a.y = fast_exp2(a.y); b2.x = fast_exp2(b2.x); b2.y = fast_exp2(b2.y);
+          if (!all_seen) {                                  // the same for all lanes
+            a.x = (seen >> i) & 1u ? a.x : 0.f;
+            a.y = (seen >> (i + 1)) & 1u ? a.y : 0.f;
+            b2.x = (seen >> (i + 2)) & 1u ? b2.x : 0.f;
+            b2.y = (seen >> (i + 3)) & 1u ? b2.y : 0.f;
           }
-      } else {
-        // columns of tokens [lo, hi) of the chunk see this lane's token
-        const int c_lo = max(tok - first, 0) * G, c_hi = (p.window > 0 ? min(tok + p.window - first, there) : there) * G;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float4 x = ml[c * 16 + i / 2];
-            const int col = half * 64 + c * 32 + i;
-            const float e0 = fast_exp2(fmaf(__uint_as_float(r[c][i]), f, -x.x)) * x.y;
-            const float e1 = fast_exp2(fmaf(__uint_as_float(r[c][i + 1]), f, -x.z)) * x.w;
-            a[i & 3] += col >= c_lo && col < c_hi ? e0 : 0.f;
-            a[(i & 3) + 1] += col + 1 >= c_lo && col + 1 < c_hi ? e1 : 0.f;
-          }
+          sum2 = fma2(pair2(a.x, a.y), pair2(l.x, l.y), sum2);
+          sum2 = fma2(pair2(b2.x, b2.y), pair2(l.z, l.w), sum2);
+        }
       }
-      total += (a[0] + a[1]) + (a[2] + a[3]);
+      const float2 sums = unpair2(sum2);
+      total += sums.x + sums.y;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_free[s]);
     }
     if (half == 1) sSum[trow] = total;
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
-    if (half == 0 && ok && tok < L && tok < p.width) p.weights[b * p.w_ld_b + kvh * p.w_ld_h + tok] += total + sSum[trow];
+    if (half == 0) {
+      total += sSum[trow];
+      if (part == 0) sOwn[trow] = total;
+      else st_cluster_f32(cluster_map_shared(smem_u32(sOther + trow), 0), total);
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();
+  if (part == 0 && threadIdx.x < kScRows && !*abort_flag) {
+    const int tok = k0 + (int)threadIdx.x;
+    if (tok < L && tok < p.width) p.weights[b * p.w_ld_b + kvh * p.w_ld_h + tok] += sOwn[threadIdx.x] + sOther[threadIdx.x];
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tS, 256);
@@ -1267,6 +1281,12 @@ int launch_pairs(Kern kern, int smem, int blocks, const CUtensorMap& tq, const S
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem) != cudaSuccess) return -20;
   kern<<<blocks, kC2Threads, smem, st>>>(tq, p, items);
   return cudaGetLastError() == cudaSuccess ? 0 : -20;
+}
+
+int launch_weigh(void (*kern)(CUtensorMap, ScWeighParams), int smem, unsigned blocks, const CUtensorMap& tq, const ScWeighParams& p, cudaStream_t st) {
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem) != cudaSuccess) return -20;
+  if (launch_chain_cluster(false, 2, kern, dim3(blocks), dim3(kSwThreads), smem, st, tq, p) != cudaSuccess) { cudaGetLastError(); return -20; }
+  return 0;
 }
 
 template <typename Kern, typename P>
@@ -1320,8 +1340,9 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
   ScWeighParams w{(const uint8_t*)r.k_cache, r.ks, r.ks_ld, (int)r.ks_h, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.seq_lens, r.starts, r.key_seq,
                   r.key_k0, scale_log2, Hq, Hkv, G, (int)r.window, (int)r.num_pages, reinterpret_cast<const float2*>(r.ml), r.weights, r.w_ld_b,
                   r.w_ld_h, (int)r.width, status};
-  const dim3 keys((unsigned)r.key_tiles, Hkv);
-  if (D == 64) return launch_tiles(scaled_chunk_weigh_kernel<64>, SwTile<64>::kSmem, keys, kSwThreads, tq, w, st);
-  if (D == 128) return launch_tiles(scaled_chunk_weigh_kernel<128>, SwTile<128>::kSmem, keys, kSwThreads, tq, w, st);
-  return launch_tiles(scaled_chunk_weigh_kernel<256>, SwTile<256>::kSmem, keys, kSwThreads, tq, w, st);
+  const long long keys = 2 * r.key_tiles * Hkv;
+  if (keys > 0x7fffffffll) return -1;
+  if (D == 64) return launch_weigh(scaled_chunk_weigh_kernel<64>, SwTile<64>::kSmem, (unsigned)keys, tq, w, st);
+  if (D == 128) return launch_weigh(scaled_chunk_weigh_kernel<128>, SwTile<128>::kSmem, (unsigned)keys, tq, w, st);
+  return launch_weigh(scaled_chunk_weigh_kernel<256>, SwTile<256>::kSmem, (unsigned)keys, tq, w, st);
 }
