@@ -22,8 +22,11 @@
 namespace atlas {
 
 constexpr int kSdPage = 16;
-constexpr int kSdWarps = 8;
-constexpr int kSdRing = 24 * 1024;        // bytes of pages in flight per warp
+constexpr int kSdRings = 192 * 1024;      // bytes of pages in flight per SM
+// Warps of a block: sixteen where 128 registers a thread are enough for the output numbers (a page costs a warp 300 instructions, and with two
+// warps a scheduler half of its time was waiting: 128 x 1152 tokens of 8 heads of 128 took 77 us), eight for wider heads or groups.
+template <int D, int NT>
+constexpr int kSdWarps = D * NT <= 128 ? 16 : 8;
 constexpr int kSdLeast = 2;               // pages that make a run worth a warp of its own
 
 struct ScaledDecodeParams {
@@ -95,14 +98,15 @@ struct PageRef {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kSdWarps * 32, 1)
+__global__ void __launch_bounds__(kSdWarps<D, NT> * 32, 1)
 scaled_decode_kernel(const ScaledDecodeParams p) {
+  constexpr int kWarps = kSdWarps<D, NT>, kSdRing = kSdRings / kWarps;
   constexpr int kPageBytes = kSdPage * D;
   constexpr int kStages = kSdRing / (2 * kPageBytes);
   constexpr int KS = D / 16;                      // k steps of a score
   constexpr int QB = D / 4;                       // channels of a lane's share of a row
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t bars[kSdWarps][kStages];
+  __shared__ uint64_t bars[kWarps][kStages];
   __shared__ uint32_t abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -501,10 +505,11 @@ using namespace atlas;
 namespace {
 
 template <int D, int NT>
-int decode_launch(const ScaledDecodeParams& p, int blocks, int items, cudaStream_t st) {
-  constexpr int smem = kSdWarps * kSdRing;
+int decode_launch(ScaledDecodeParams p, int blocks, int items, cudaStream_t st) {
+  constexpr int smem = kSdRings;
+  p.warps = blocks * kSdWarps<D, NT>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(scaled_decode_kernel<D, NT>), smem) != cudaSuccess) return -20;
-  if (launch_chain(scaled_decode_kernel<D, NT>, dim3(blocks), dim3(kSdWarps * 32), smem, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
+  if (launch_chain(scaled_decode_kernel<D, NT>, dim3(blocks), dim3(kSdWarps<D, NT> * 32), smem, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
   const int chans = 256 / (2 * p.cols) * 2;
   if (launch_chain(scaled_merge_kernel<D>, dim3(items, (D + chans - 1) / chans), dim3(256), 0, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
   return 0;
@@ -513,7 +518,7 @@ int decode_launch(const ScaledDecodeParams& p, int blocks, int items, cudaStream
 }  // namespace
 
 // Decode rows of a step: sequence b's row is query_start_loc[b].  Arguments as one record (see kv_scaled.cu).  Workspaces: part_o [pieces][D]
-// [cols] and part_ml [pieces][cols][2] with cols = min(G rounded up to two, 16) and pieces = pairs + warps, a pair being (sequence, key head,
+// [cols] and part_ml [pieces][cols][2] with cols = min(G rounded up to two, 16) and pieces = pairs + 16 blocks, a pair being (sequence, key head,
 // group of 16 query heads).  With `weights`: scores [nd * Hkv][width][G rounded up to two], ml [nd][Hq][2] and the sums
 // [sequence][head][token], `width` tokens each.  -1: sizes or alignment outside of what the kernels take.
 struct DecodeRecord {
@@ -539,7 +544,7 @@ extern "C" int atlas_attn_scaled_decode(const void* record) {
   // the list's entries and the runs' bounds are 32-bit numbers
   const long long items = r.nd * r.Hkv * p.tiles;
   if (items * r.bt_cols > 0x3fffffffll || items > 0x7fffffffll || r.bt_cols > (1 << 26) || r.blocks <= 0 || r.blocks > 65535) return -1;
-  p.window = (int)r.window; p.num_pages = (int)r.num_pages; p.warps = (int)r.blocks * kSdWarps;
+  p.window = (int)r.window; p.num_pages = (int)r.num_pages;
   p.scale_log2 = (float)(r.scale * 1.4426950408889634);
   p.part_o = r.part_o; p.part_ml = r.part_ml;
   p.scores = r.weights ? r.scores : nullptr; p.width = r.width; p.score_cols = (p.G + 1) / 2 * 2; p.ml = r.weights ? r.ml : nullptr;

@@ -17,7 +17,7 @@ from . import checked, cuda as K
 
 BLOCK = 16
 HEAD_DIMS = (64, 128, 256)
-WARPS, LEAST = 8, 2                # of scaled_decode_kernel: warps of a block, pages worth a warp
+WARPS, LEAST = 16, 2               # of scaled_decode_kernel: most warps of a block, pages worth a warp
 _F32, _BF16, _I32, _FP8 = torch.float32, torch.bfloat16, torch.int32, torch.float8_e4m3fn
 
 # records of the entry points, in the order of their C structs: integers and pointers, one double
