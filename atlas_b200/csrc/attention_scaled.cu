@@ -14,7 +14,7 @@
 // into its ring of shared memory (cp.async.bulk, a page of K and one of V per slot), reads them as mma.sync fragments (tokens along M for
 // the scores, channels along M for the outputs, heads along N) and leaves (M, l, O) of every pair it touched.  A piece's number is pair +
 // warp, which no two pieces share.
-// scaled_merge_kernel joins the pieces of a pair.  scaled_weigh_kernel adds 2^(s - M) / l over the pair's heads to the running sums.
+// scaled_join_kernel and scaled_merge_kernel join the pieces of a pair.  scaled_weigh_kernel adds 2^(s - M) / l over the pair's heads to the running sums.
 #include "common.cuh"
 #include "host_api.h"
 #include "tc_util.cuh"
@@ -81,11 +81,20 @@ ATLAS_DEVICE int seen_pages(int len, int window, int& first) {
 }
 ATLAS_DEVICE int decode_len(const ScaledDecodeParams& p, int b) { return min(max(p.seq_lens[b], 0), p.bt_cols * kSdPage); }
 
-// Pages of sequences [0, n), the whole warp.
-ATLAS_DEVICE int total_pages(const ScaledDecodeParams& p, int n, int lane) {
-  int sum = 0, first;
-  for (int b = lane; b < n; b += 32) sum += seen_pages(decode_len(p, b), p.window, first);
-  return __reduce_add_sync(0xffffffffu, sum);
+// Pages of all sequences and of those before sequence `b`, the whole warp; up to 128 sequences in one round of loads.
+ATLAS_DEVICE void count_pages(const ScaledDecodeParams& p, int b, int lane, int& all, int& before) {
+  int sum = 0, pre = 0, first;
+  for (int c = 0; c < p.nd; c += 128) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = c + 4 * lane + k;
+      const int n = i < p.nd ? seen_pages(decode_len(p, i), p.window, first) : 0;
+      sum += n;
+      pre += i < b ? n : 0;
+    }
+  }
+  all = __reduce_add_sync(0xffffffffu, sum);
+  before = __reduce_add_sync(0xffffffffu, pre);
 }
 ATLAS_DEVICE int run_length(int pages, int warps) { return max((pages + warps - 1) / warps, kSdLeast); }
 
@@ -122,7 +131,24 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
   chain_wait();
   const int w = warp * gridDim.x + blockIdx.x;    // neighbours in the list on different SMs
   const int hn = p.Hkv * p.tiles;
-  const int all = total_pages(p, p.nd, lane) * hn;
+  int seen[4];                                    // pages of the first 128 sequences, four neighbours a lane: one round of loads
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    int first;
+    const int b = 4 * lane + k;
+    seen[k] = b < p.nd ? seen_pages(decode_len(p, b), p.window, first) : 0;
+  }
+  const int mine4 = seen[0] + seen[1] + seen[2] + seen[3];
+  int incl = mine4;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  const int some = __shfl_sync(0xffffffffu, incl, 31);          // of those 128
+  int all = some, before;
+  if (p.nd > 128) count_pages(p, 0, lane, all, before);
+  all *= hn;
   const int run = run_length(all, p.warps);
   const long long lo64 = (long long)w * run;
   if (lo64 >= all) return;
@@ -131,23 +157,34 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
 
   // the sequence that entry n0 belongs to, and the entries before it
   int b0 = 0, base0 = 0;
-  for (int c = 0; c < p.nd; c += 32) {
-    int first;
-    const int mine = c + lane < p.nd ? seen_pages(decode_len(p, c + lane), p.window, first) * hn : 0;
-    int incl = mine;
+  if (n0 < some * hn) {
+    const int l = __ffs(__ballot_sync(0xffffffffu, incl * hn > n0)) - 1;
+    int at = incl - mine4, b = 4 * lane;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
+    for (int k = 0; k < 3; ++k)
+      if (b == 4 * lane + k && (at + seen[k]) * hn <= n0) { at += seen[k]; ++b; }
+    b0 = __shfl_sync(0xffffffffu, b, l);
+    base0 = __shfl_sync(0xffffffffu, at, l) * hn;
+  } else {
+    base0 = some * hn;
+    for (int c = 128; c < p.nd; c += 32) {
+      int first;
+      const int mine = c + lane < p.nd ? seen_pages(decode_len(p, c + lane), p.window, first) * hn : 0;
+      int in = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += x;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, base0 + in > n0);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b0 = c + l;
+        base0 += __shfl_sync(0xffffffffu, in - mine, l);
+        break;
+      }
+      base0 += __shfl_sync(0xffffffffu, in, 31);
     }
-    const unsigned past = __ballot_sync(0xffffffffu, base0 + incl > n0);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      b0 = c + l;
-      base0 += __shfl_sync(0xffffffffu, incl - mine, l);
-      break;
-    }
-    base0 += __shfl_sync(0xffffffffu, incl, 31);
   }
   // entries n0 + 32 c + lane
   auto fetch = [&](int c) -> PageRef {
@@ -381,34 +418,100 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);       // copies in flight land before the shared memory goes
 }
 
-// Pieces of a pair: warps [first page / run, last page / run] of the list; piece = pair + warp.  A block joins up to 256 output numbers,
-// four neighbouring ones a thread and every fourth piece: a single long sequence has hundreds of pieces, and their loads overlap.
-constexpr int kSmChunk = 128;                            // pieces whose factors are in shared memory at a time
+// Pieces of a pair: warps [first page / run, last page / run] of the list; piece = pair + warp.
+struct Pieces {
+  long long first; int n;
+};
+ATLAS_DEVICE Pieces pieces_of(const ScaledDecodeParams& p, int item, int lane) {
+  const int hn = p.Hkv * p.tiles, b = item / hn;
+  int all, before, first;
+  count_pages(p, b, lane, all, before);
+  const int np = seen_pages(decode_len(p, b), p.window, first);
+  const int run = run_length(all * hn, p.warps), start = before * hn + item % hn * np, w0 = start / run;
+  return Pieces{(long long)item + w0, np > 0 ? (start + np - 1) / run - w0 + 1 : 0};
+}
+
+// A few pieces a pair: a thread joins four neighbouring output numbers by itself, two global loads deep and without a barrier.  (Blocks that
+// share the factors, four barriers: 20 us for 128 sequences of 8 heads.)
+template <int D>
+__global__ void __launch_bounds__(128)
+scaled_join_kernel(const ScaledDecodeParams p) {
+  chain_trigger();
+  chain_wait();
+  const int item = blockIdx.x, hn = p.Hkv * p.tiles, b = item / hn, pair = item % hn;
+  const Pieces pc = pieces_of(p, item, threadIdx.x & 31);
+  const int e0 = 4 * (blockIdx.y * 128 + threadIdx.x);
+  if (e0 >= D * p.cols) return;
+  int c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = (e0 + j) % p.cols;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + pc.first * p.cols;
+  const float* src = p.part_o + pc.first * D * p.cols + e0;
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 4
+  for (int i = 0; i < pc.n; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], ml[i * p.cols + c[j]].x);
+  float l[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m[j] = m[j] == -INFINITY ? 0.f : m[j];
+#pragma unroll 4
+  for (int i = 0; i < pc.n; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(src + (long long)i * D * p.cols);
+    const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 y = ml[i * p.cols + c[j]];
+      const float f = fast_exp2(y.x - m[j]);             // a piece without a visible token: 2^-inf
+      l[j] += y.y * f;
+      o[j] = fmaf(xs[j], f, o[j]);
+    }
+  }
+  const long long row = (long long)p.query_start_loc[b] * p.ldo + (long long)(pair / p.tiles) * p.G * D;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int head = (pair % p.tiles) * p.cols + c[j], d = (e0 + j) / p.cols;
+    if (head >= p.G) continue;
+    const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];    // no token: zeros
+    p.out[row + head * D + d] = __float2bfloat16_rn(o[j] * inv);
+    if (p.ml && d == 0) reinterpret_cast<float2*>(p.ml)[((long long)b * p.Hkv + pair / p.tiles) * p.G + head] = make_float2(m[j], inv);
+  }
+}
+
+// Hundreds of pieces a pair (long sequences, few pairs): a thread owns four neighbouring output numbers and every sixteenth piece, so that
+// their loads overlap (3 x 65531 tokens of 2 heads: 13 us, with four groups of pieces 26 us).
+constexpr int kSmChunk = 256;                            // pieces whose factors are in shared memory at a time
 
 template <int D>
 __global__ void __launch_bounds__(256)
 scaled_merge_kernel(const ScaledDecodeParams p) {
+  constexpr int kGroups = 16, kQuads = 256 / kGroups;
   __shared__ float factor[kSmChunk][16];
   __shared__ float part[16][17];
   __shared__ float top[16], sum[16];
-  __shared__ float4 quad[4][64];
+  __shared__ float4 quad[256];
   chain_trigger();
   chain_wait();
   const int tid = threadIdx.x, lane = tid & 31;
   const int item = blockIdx.x, hn = p.Hkv * p.tiles, b = item / hn, pair = item % hn;
-  const int all = total_pages(p, p.nd, lane) * hn, run = run_length(all, p.warps);
-  int first;
-  const int np = seen_pages(decode_len(p, b), p.window, first);
-  const int start = total_pages(p, b, lane) * hn + pair * np;
-  const int w0 = start / run, pieces = np > 0 ? (start + np - 1) / run - w0 + 1 : 0;
-  const long long piece0 = (long long)item + w0;
+  const Pieces pc = pieces_of(p, item, lane);
+  const int pieces = pc.n;
+  const long long piece0 = pc.first;
   // ---- references and sums of the heads: thread (piece lane, head)
   const int pl = tid >> 4, hc = tid & 15;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + piece0 * p.cols + hc;
+  float2 x[kSmChunk / 16];
   float m = -INFINITY;
-  if (hc < p.cols)
-#pragma unroll 4
-    for (int i = pl; i < pieces; i += 16) m = fmaxf(m, ml[(long long)i * p.cols].x);
+  for (int i0 = 0; i0 < pieces; i0 += kSmChunk) {
+    const int n = min(pieces - i0, kSmChunk);
+#pragma unroll
+    for (int k = 0; k < kSmChunk / 16; ++k) {
+      x[k] = make_float2(-INFINITY, 0.f);
+      if (hc < p.cols && pl + 16 * k < n) x[k] = ml[(long long)(i0 + pl + 16 * k) * p.cols];
+    }
+#pragma unroll
+    for (int k = 0; k < kSmChunk / 16; ++k) m = fmaxf(m, x[k].x);
+  }
   part[pl][hc] = m;
   __syncthreads();
   if (tid < 16) {
@@ -418,31 +521,31 @@ scaled_merge_kernel(const ScaledDecodeParams p) {
   }
   __syncthreads();
   // ---- outputs [channel][head], numbers 4 * quad .. of this block
-  const int per = 256 / (2 * p.cols) * (2 * p.cols);     // whole channels, whole quads
-  const int e0 = (int)blockIdx.y * per + 4 * (tid & 63), g4 = tid >> 6;
-  const bool live = 4 * (tid & 63) < per && e0 < D * p.cols;
+  const int per = 4 * kQuads / (2 * p.cols) * (2 * p.cols);     // whole channels, whole quads
+  const int qd = tid % kQuads, grp = tid / kQuads;
+  const int e0 = (int)blockIdx.y * per + 4 * qd;
+  const bool live = 4 * qd < per && e0 < D * p.cols;
   int c[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) c[j] = (e0 + j) % p.cols;
   const float* src = p.part_o + piece0 * D * p.cols + e0;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
+  const float ref = top[hc];
   for (int i0 = 0; i0 < pieces; i0 += kSmChunk) {
     const int n = min(pieces - i0, kSmChunk);
-    if (hc < p.cols) {
-      const float ref = top[hc];
-#pragma unroll 4
-      for (int i = pl; i < n; i += 16) {
-        const float2 x = ml[(long long)(i0 + i) * p.cols];
-        const float f = fast_exp2(x.x - ref);            // a piece without a visible token: 2^-inf
-        factor[i][hc] = f;
-        l += x.y * f;
-      }
+#pragma unroll
+    for (int k = 0; k < kSmChunk / 16; ++k) {
+      if (pl + 16 * k >= n) break;
+      if (pieces > kSmChunk && hc < p.cols) x[k] = ml[(long long)(i0 + pl + 16 * k) * p.cols];
+      const float f = fast_exp2(x[k].x - ref);           // a piece without a visible token: 2^-inf
+      factor[pl + 16 * k][hc] = f;
+      l += x[k].y * f;
     }
     __syncthreads();
     if (live)
 #pragma unroll 8
-      for (int i = g4; i < n; i += 4) {
+      for (int i = grp; i < n; i += kGroups) {
         const float4 o = *reinterpret_cast<const float4*>(src + (long long)(i0 + i) * D * p.cols);
         acc.x = fmaf(o.x, factor[i][c[0]], acc.x);
         acc.y = fmaf(o.y, factor[i][c[1]], acc.y);
@@ -452,7 +555,7 @@ scaled_merge_kernel(const ScaledDecodeParams p) {
     __syncthreads();
   }
   part[pl][hc] = l;
-  quad[g4][tid & 63] = acc;
+  quad[tid] = acc;
   __syncthreads();
   if (tid < 16) {
     l = 0.f;
@@ -466,13 +569,19 @@ scaled_merge_kernel(const ScaledDecodeParams p) {
   }
   __syncthreads();
   // ---- rows of a head's channels
-  const int chans = per / p.cols, cc = tid / chans, dd = tid % chans;
-  const int hh = (pair % p.tiles) * p.cols + cc, dg = blockIdx.y * chans + dd;
-  if (cc < p.cols && hh < p.G && dg < D) {
-    const int e = dd * p.cols + cc;
-    const float* q = reinterpret_cast<const float*>(quad);
-    const float o = (q[e] + q[256 + e]) + (q[512 + e] + q[768 + e]);
-    p.out[(long long)p.query_start_loc[b] * p.ldo + ((pair / p.tiles) * p.G + hh) * D + dg] = __float2bfloat16_rn(o * sum[cc]);
+  const int chans = per / p.cols;
+  const long long row = (long long)p.query_start_loc[b] * p.ldo;
+  for (int i = tid; i < per; i += 256) {
+    const int cc = i / chans, dd = i % chans;
+    const int hh = (pair % p.tiles) * p.cols + cc, dg = blockIdx.y * chans + dd;
+    if (hh < p.G && dg < D) {
+      const int e = dd * p.cols + cc;
+      const float* q = reinterpret_cast<const float*>(quad);
+      float o = 0.f;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) o += q[4 * kQuads * k + e];
+      p.out[row + ((pair / p.tiles) * p.G + hh) * D + dg] = __float2bfloat16_rn(o * sum[cc]);
+    }
   }
 }
 
@@ -510,8 +619,12 @@ int decode_launch(ScaledDecodeParams p, int blocks, int items, cudaStream_t st) 
   p.warps = blocks * kSdWarps<D, NT>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(scaled_decode_kernel<D, NT>), smem) != cudaSuccess) return -20;
   if (launch_chain(scaled_decode_kernel<D, NT>, dim3(blocks), dim3(kSdWarps<D, NT> * 32), smem, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
-  const int chans = 256 / (2 * p.cols) * 2;
-  if (launch_chain(scaled_merge_kernel<D>, dim3(items, (D + chans - 1) / chans), dim3(256), 0, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
+  // Up to sixteen pieces a pair on average are joined by single threads.
+  const bool few = 16ll * items >= p.warps;
+  const int chans = 64 / (2 * p.cols) * 2;
+  const cudaError_t e = few ? launch_chain(scaled_join_kernel<D>, dim3(items, (D * p.cols / 4 + 127) / 128), dim3(128), 0, st, p)
+                            : launch_chain(scaled_merge_kernel<D>, dim3(items, (D + chans - 1) / chans), dim3(256), 0, st, p);
+  if (e != cudaSuccess) { cudaGetLastError(); return -20; }
   return 0;
 }
 

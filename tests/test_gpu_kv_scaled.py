@@ -167,6 +167,8 @@ ATTEND = [
     (64, 1, 40, [70, 16], [1] * 2, 0),
     (128, 4, 5, [400, 16, 50], [1] * 3, 33),
     (64, 3, 2, [257] * 40, [1] * 40, 1),
+    (64, 1, 2, [1 + (7 * i) % 50 for i in range(300)], [1] * 300, 0),
+    (64, 1, 4, [30000, 20], [1] * 2, 0),
     # chunks
     (128, 8, 4, [300, 129], [300, 129], 0),
     (128, 2, 8, [40, 700], [2, 100], 0),
