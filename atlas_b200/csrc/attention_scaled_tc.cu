@@ -49,6 +49,9 @@ struct ScChunkParams {
   float scale_log2;
   int Hq, Hkv, G, window, num_pages;
   float2* ml;                                     // [rows of the step][Hq] (M, 1 / l) or null
+  // Few rows behind many keys: the keys of a query tile go to `splits` CTAs in equal shares, whose parts are joined by scaled_chunk_join_kernel
+  int splits, first_row, rows;
+  float* part_o; float2* part_ml;                 // [split][rows][Hq][D] and [split][rows][Hq] (M, l), rows from first_row on
   status_t* status;
 };
 
@@ -56,6 +59,19 @@ ATLAS_DEVICE void sc_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* 
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dst)),
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
+}
+// The low word of a descriptor (make_smem_desc_sw128) carries the address, which steps along K; the high word is the same for all tiles.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+ATLAS_DEVICE uint32_t desc_low(const void* p) { return ((smem_u32(p) & 0x3FFFFu) >> 4) | (1u << 16); }
+ATLAS_DEVICE void umma_f16_lo(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
 }
 ATLAS_DEVICE uint32_t sc_e4m3x2(uint32_t v) {
   uint32_t r;
@@ -76,6 +92,59 @@ ATLAS_DEVICE uint32_t h2_to_bf2(uint32_t v) {      // e4m3 numbers: exact in bot
 }
 ATLAS_DEVICE int scale_exponent(float s) { return (int)((__float_as_uint(s) >> 23) & 255u) - 127; }
 ATLAS_DEVICE float exact_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// 32 output numbers of a row: times 1 / l to bf16, or as they are to a part of the row
+ATLAS_DEVICE void store_outputs(const uint32_t (&v)[32], float inv, __nv_bfloat16* out, float* part) {
+  if (part) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(part + 4 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint4 o;
+    o.x = pack_bf16x2(__uint_as_float(v[q * 8 + 0]) * inv, __uint_as_float(v[q * 8 + 1]) * inv);
+    o.y = pack_bf16x2(__uint_as_float(v[q * 8 + 2]) * inv, __uint_as_float(v[q * 8 + 3]) * inv);
+    o.z = pack_bf16x2(__uint_as_float(v[q * 8 + 4]) * inv, __uint_as_float(v[q * 8 + 5]) * inv);
+    o.w = pack_bf16x2(__uint_as_float(v[q * 8 + 6]) * inv, __uint_as_float(v[q * 8 + 7]) * inv);
+    *reinterpret_cast<uint4*>(out + q * 8) = o;
+  }
+}
+
+// The shares of a row: o = sum_s o_s 2^(M_s - M) / sum_s l_s 2^(M_s - M); a warp a (row, head).
+template <int D>
+__global__ void __launch_bounds__(256)
+scaled_chunk_join_kernel(const ScChunkParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const long long step = (long long)p.rows * p.Hq;
+  if (u >= step) return;
+  const long long row = p.first_row + u / p.Hq;
+  const int head = (int)(u % p.Hq);
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[s * step + u].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 x = p.part_ml[s * step + u];
+    const float f = fast_exp2(x.x - ref);                        // a share that the row sees nothing of: 2^-inf
+    l += x.y * f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const float2 y = *reinterpret_cast<const float2*>(p.part_o + (s * step + u) * D + i * 64 + lane * 2);
+      o[2 * i] = fmaf(y.x, f, o[2 * i]);
+      o[2 * i + 1] = fmaf(y.y, f, o[2 * i + 1]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+    *reinterpret_cast<uint32_t*>(p.out + row * p.ldo + head * D + i * 64 + lane * 2) = pack_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
+  if (p.ml && lane == 0) p.ml[row * p.Hq + head] = make_float2(ref, inv);
+}
 
 template <int D>
 __global__ void __launch_bounds__(kScThreads, 1)
@@ -116,9 +185,11 @@ scaled_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPar
   const int ctx0 = L - q_len;                                   // position of the chunk's first row
   const int last_tok = min(q0 + tok_per_tile, q_len) - 1;
   const int kv_hi = min(L, ctx0 + last_tok + 1);                // keys [.., kv_hi)
-  const int page0 = p.window > 0 ? max(ctx0 + q0 - p.window + 1, 0) / kScPg : 0;
-  const int base = page0 * kScPg;                               // first key of tile 0
-  const int n_kv = max((kv_hi - base + kKv - 1) / kKv, 0);
+  const int first_page = p.window > 0 ? max(ctx0 + q0 - p.window + 1, 0) / kScPg : 0;
+  const int all_kv = max((kv_hi - first_page * kScPg + kKv - 1) / kKv, 0), share = (all_kv + p.splits - 1) / p.splits;
+  const int page0 = first_page + blockIdx.z * share * kPages;
+  const int base = page0 * kScPg;                               // first key of tile 0 of this share
+  const int n_kv = min(max(all_kv - (int)blockIdx.z * share, 0), share);
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -185,41 +256,39 @@ scaled_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPar
     if (!ok)
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t kIdescS = make_idesc(kScRows, kKv, 0u), kIdescO = make_idesc(kScRows, D, 0u);     // f16 x f16 -> f32
-      const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK), aV = smem_u32(sV), aP = smem_u32(sP);
-      bool ok = mbar_wait(q_conv, 0, abort_flag, p.status, 0xA10);
-      auto issue_pv = [&](int i) -> bool {
-        if (!mbar_wait(p_ready, i & 1, abort_flag, p.status, 0xA12)) return false;
-        if (!mbar_wait(v_ready, i & 1, abort_flag, p.status, 0xA13)) return false;
-        tc_fence_after();
+    // ------------------------------------------------------------------ products (the whole warp, one elected lane issues)
+    constexpr uint32_t kIdescS = make_idesc(kScRows, kKv, 0u), kIdescO = make_idesc(kScRows, D, 0u);     // f16 x f16 -> f32
+    const uint32_t dQ = desc_low(sQ), dK = desc_low(sK), dV = desc_low(sV), dP = desc_low(sP);
+    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, site)); };
+    bool ok = wait(q_conv, 0, 0xA10);
+    auto issue_pv = [&](int i) -> bool {
+      if (!wait(v_ready, i & 1, 0xA13) || !wait(p_ready, i & 1, 0xA12)) return false;
+      tc_fence_after();
+      if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < kKv / 16; ++ks) {
-          const uint64_t ad = make_smem_desc_sw128(aP + (ks >> 2) * kScSub) + 2 * (ks & 3);
-          const uint64_t bd = make_smem_desc_sw128(aV + (ks >> 2) * kVSub) + 2 * (ks & 3);
-          umma_f16(tO, ad, bd, kIdescO, (i > 0 || ks > 0) ? 1u : 0u);
-        }
+        for (int ks = 0; ks < kKv / 16; ++ks)
+          umma_f16_lo(tO, dP + (ks >> 2) * (kScSub >> 4) + 2 * (ks & 3), dV + (ks >> 2) * (kVSub >> 4) + 2 * (ks & 3), kIdescO, (i > 0 || ks > 0) ? 1u : 0u);
         umma_commit(pv_done);
-        return true;
-      };
-      for (int j = 0; j < n_kv && ok; ++j) {
-        const int sb = j & 1;
-        if (!mbar_wait(k_ready, j & 1, abort_flag, p.status, 0xA14)) { ok = false; break; }
-        if (!mbar_wait(&s_free[sb], ((j >> 1) & 1) ^ 1u, abort_flag, p.status, 0xA15)) { ok = false; break; }
-        tc_fence_after();
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int j = 0; j < n_kv && ok; ++j) {
+      const int sb = j & 1;
+      ok = wait(k_ready, j & 1, 0xA14) && wait(&s_free[sb], ((j >> 1) & 1) ^ 1u, 0xA15);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint64_t ad = make_smem_desc_sw128(aQ + (ks >> 2) * kScSub) + 2 * (ks & 3);
-          const uint64_t bd = make_smem_desc_sw128(aK + (ks >> 2) * kKSub) + 2 * (ks & 3);
-          umma_f16(tS + sb * kKv, ad, bd, kIdescS, ks > 0 ? 1u : 0u);
-        }
+        for (int ks = 0; ks < D / 16; ++ks)
+          umma_f16_lo(tS + sb * kKv, dQ + (ks >> 2) * (kScSub >> 4) + 2 * (ks & 3), dK + (ks >> 2) * (kKSub >> 4) + 2 * (ks & 3), kIdescS, ks > 0 ? 1u : 0u);
         umma_commit(&s_full[sb]);
         umma_commit(k_free);
-        if (j > 0) ok = issue_pv(j - 1);
       }
-      if (ok && n_kv > 0) issue_pv(n_kv - 1);
+      __syncwarp();
+      if (j > 0) ok = issue_pv(j - 1);
     }
+    if (ok && n_kv > 0) issue_pv(n_kv - 1);
   } else if (warp < 6) {
     // ------------------------------------------------------------------ converters
     const int r = threadIdx.x - 64;
@@ -454,27 +523,28 @@ scaled_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPar
     if (ok && n_kv > 0) ok = exchange(l, l_other);
     l += l_other;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (ok && n_kv > 0 && mbar_wait(pv_done, (n_kv - 1) & 1, abort_flag, p.status, 0xA32)) {
+    const long long at = (long long)(q_row0 + tok) * p.Hq + head, at_part = ((long long)blockIdx.z * p.rows - p.first_row) * p.Hq + at;
+    if (ok && n_kv > 0) ok = mbar_wait(pv_done, (n_kv - 1) & 1, abort_flag, p.status, 0xA32);
+    if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       __nv_bfloat16* orow = p.out + (long long)(q_row0 + tok) * p.ldo + head * D + ocol0;
+      float* part = p.splits > 1 ? p.part_o + at_part * D + ocol0 : nullptr;
 #pragma unroll
       for (int c = 0; c < HO / 32; ++c) {
         uint32_t r[32];
-        tmem_ld_32x32b_x32(tO + t_lane + ocol0 + c * 32, r);
-        tmem_ld_wait();
-        if (row_live) {
+        if (n_kv > 0) {
+          tmem_ld_32x32b_x32(tO + t_lane + ocol0 + c * 32, r);
+          tmem_ld_wait();
+        } else {                                                 // no keys: zeros
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 o;
-            o.x = pack_bf16x2(__uint_as_float(r[q * 8 + 0]) * inv, __uint_as_float(r[q * 8 + 1]) * inv);
-            o.y = pack_bf16x2(__uint_as_float(r[q * 8 + 2]) * inv, __uint_as_float(r[q * 8 + 3]) * inv);
-            o.z = pack_bf16x2(__uint_as_float(r[q * 8 + 4]) * inv, __uint_as_float(r[q * 8 + 5]) * inv);
-            o.w = pack_bf16x2(__uint_as_float(r[q * 8 + 6]) * inv, __uint_as_float(r[q * 8 + 7]) * inv);
-            *reinterpret_cast<uint4*>(orow + c * 32 + q * 8) = o;
-          }
+          for (int i = 0; i < 32; ++i) r[i] = 0;
         }
+        if (row_live) store_outputs(r, inv, orow + c * 32, part ? part + c * 32 : nullptr);
       }
-      if (p.ml && row_live && half == 0) p.ml[(long long)(q_row0 + tok) * p.Hq + head] = make_float2(m == -INFINITY ? 0.f : m, inv);
+      if (row_live && half == 0) {
+        if (part) p.part_ml[at_part] = make_float2(m, l);
+        else if (p.ml) p.ml[at] = make_float2(m == -INFINITY ? 0.f : m, inv);
+      }
     }
   }
 
@@ -508,19 +578,6 @@ struct C2Tile {
   static constexpr int kSmem = 2 * (kQ + kK + kV) + 2 * kStage + kC2Ring * 64 + 256 + 1024;      // at most 227 KB
 };
 
-// The low word of a descriptor (make_smem_desc_sw128) carries the address, which steps along K; the high word is the same for all tiles.
-constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
-ATLAS_DEVICE uint32_t desc_low(const void* p) { return ((smem_u32(p) & 0x3FFFFu) >> 4) | (1u << 16); }
-ATLAS_DEVICE void umma_f16_lo(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "mov.b64 a, {%1, %5};\n\t"
-      "mov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
-      : "memory");
-}
 // A from TMEM: a row a lane, two 16-bit numbers a column
 ATLAS_DEVICE void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -567,7 +624,7 @@ ATLAS_DEVICE float max3_nan(float a, float b, float c) {
   return r;
 }
 struct C2Item {
-  int b, kvh, L, q_row0, q_len, q0, ctx0, page0;
+  int b, kvh, split, L, q_row0, q_len, q0, ctx0, page0;           // page0: the first of this share of the keys
   int n[2], n_kv;                                                 // key tiles of tile A, of tile B, of both
 };
 // Item of a CTA in round `rd`: the rounds go to and fro over the CTAs, so that the ones with the longest item of a round get the shortest of
@@ -585,7 +642,7 @@ struct C2Walk {
     lengths();
   }
   ATLAS_DEVICE void tile(int round, int& b, int& q) const {
-    const int it = min(c2_turn(round), items - 1) / p.Hkv;
+    const int it = min(c2_turn(round), items - 1) / (p.Hkv * p.splits);
     b = p.tile_seq[it];
     q = p.tile_q0[it];
   }
@@ -599,6 +656,7 @@ struct C2Walk {
     C2Item r;
     const int toks = kScRows / p.G;
     r.kvh = c2_turn(rd) % p.Hkv;
+    r.split = c2_turn(rd) / p.Hkv % p.splits;
     r.b = b1;
     r.q0 = q1;
     r.L = min(len1, p.bt_cols * kScPg);
@@ -612,6 +670,13 @@ struct C2Walk {
       r.n[x] = first < r.q_len ? max((min(r.L, r.ctx0 + last) - r.page0 * kScPg + kC2Kv - 1) / kC2Kv, 0) : 0;
     }
     r.n_kv = max(r.n[0], r.n[1]);
+    if (p.splits > 1) {
+      const int share = (r.n_kv + p.splits - 1) / p.splits;
+      r.page0 += r.split * share * kC2Pages;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) r.n[x] = min(max(r.n[x] - r.split * share, 0), share);
+      r.n_kv = max(r.n[0], r.n[1]);
+    }
     b1 = b2;
     q1 = q2;
     lengths();
@@ -791,14 +856,16 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
       }
       ring += m_.n_kv;
       if (!ok) break;
-      // ---- o / l
+      // ---- o / l, or this share's o and l
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      const long long at = (long long)(m_.q_row0 + tok) * p.Hq + head, at_part = ((long long)m_.split * p.rows - p.first_row) * p.Hq + at;
       __nv_bfloat16* out = p.out + (long long)(m_.q_row0 + tok) * p.ldo + head * D;
+      float* part = p.splits > 1 ? p.part_o + at_part * D : nullptr;
+      uint32_t r[2][32];
       if (n > 0) {
         ok = mbar_wait(&pv_done[x], (n_s - 1) & 1, abort_flag, p.status, 0xC02 + x);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
-        uint32_t r[2][32];
         tmem_ld_32x32b_x32(tO, r[0]);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -809,23 +876,17 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_free[x]);
           }
-          if (live) {
-            uint32_t (&v)[32] = r[c & 1];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4 o;
-              o.x = pack_bf16x2(__uint_as_float(v[q * 8 + 0]) * inv, __uint_as_float(v[q * 8 + 1]) * inv);
-              o.y = pack_bf16x2(__uint_as_float(v[q * 8 + 2]) * inv, __uint_as_float(v[q * 8 + 3]) * inv);
-              o.z = pack_bf16x2(__uint_as_float(v[q * 8 + 4]) * inv, __uint_as_float(v[q * 8 + 5]) * inv);
-              o.w = pack_bf16x2(__uint_as_float(v[q * 8 + 6]) * inv, __uint_as_float(v[q * 8 + 7]) * inv);
-              *reinterpret_cast<uint4*>(out + c * 32 + q * 8) = o;
-            }
-          }
+          if (live) store_outputs(r[c & 1], inv, out + c * 32, part ? part + c * 32 : nullptr);
         }
-      } else if (live) {
-        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+      } else if (live) {                                          // no keys: zeros
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[0][i] = 0;
+        for (int c = 0; c < D; c += 32) store_outputs(r[0], inv, out + c, part ? part + c : nullptr);
       }
-      if (p.ml && live) p.ml[(long long)(m_.q_row0 + tok) * p.Hq + head] = make_float2(m == -INFINITY ? 0.f : m, inv);
+      if (live) {
+        if (part) p.part_ml[at_part] = make_float2(m, l);
+        else if (p.ml) p.ml[at] = make_float2(m == -INFINITY ? 0.f : m, inv);
+      }
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------------ converters
@@ -1300,13 +1361,14 @@ int launch_tiles(Kern kern, int smem, dim3 grid, int threads, const CUtensorMap&
 
 // Rows of chunk sequences: `tiles` query tiles of 128 / G tokens (heads of 64 and 128: pairs of tiles), each (sequence, first token in its
 // chunk); `ml` (or null) gets
-// every row's reference and 1 / l.  With `weights`, tiles of 128 cached tokens follow, each (sequence, first token), whose sums grow by the
+// every row's reference and 1 / l.  `splits` > 1: part_o [splits][rows][Hq][D] and part_ml
+// [splits][rows][Hq][2] for the rows from first_row on, the chunks'.  With `weights`, tiles of 128 cached tokens follow, each (sequence, first token), whose sums grow by the
 // rows' softmax weights.  Arguments as one record (see kv_scaled.cu).  -1: sizes or alignment outside of what the kernels take.
 struct ChunkRecord {
   const void* q; long long ldq; void* out; long long ldo; const void* k_cache; const void* v_cache;
   const float* ks; long long ks_ld, ks_h; const float* vs; long long vs_ld, vs_h;
   const int* tables; long long bt_ld, bt_cols; const int* seq_lens; const int* starts;
-  const int* tile_seq; const int* tile_q0; long long tiles, total_tokens, Hq, Hkv, D, window, num_pages; float* ml;
+  const int* tile_seq; const int* tile_q0; long long tiles, total_tokens, Hq, Hkv, D, window, num_pages; float* ml; long long splits, first_row; float* part_o; float* part_ml;
   const int* key_seq; const int* key_k0; long long key_tiles; float* weights; long long w_ld_b, w_ld_h, width, sms; double scale; void* status;
   void* stream;
 };
@@ -1318,6 +1380,7 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
   if ((reinterpret_cast<uintptr_t>(r.q) & 15) || r.ldq % 8 || r.ldo % 8 || (reinterpret_cast<uintptr_t>(r.out) & 15)) return -1;
   if ((reinterpret_cast<uintptr_t>(r.k_cache) | reinterpret_cast<uintptr_t>(r.v_cache)) & 15) return -1;
   if (r.bt_cols > (1 << 26) || r.tiles > 0x7fffffffll || r.total_tokens > 0x7fffffffll || (r.weights && !r.ml)) return -1;
+  if (r.splits < 1 || r.splits > 65535 || (r.splits > 1 && (!r.part_o || !r.part_ml)) || r.first_row < 0 || r.first_row >= r.total_tokens) return -1;
   const int Hq = (int)r.Hq, Hkv = (int)r.Hkv, G = Hq / Hkv;
   CUtensorMap tq;
   if (int rc = query_map(&tq, r.q, r.ldq, (int)r.total_tokens, Hq, G, D)) return rc;
@@ -1326,17 +1389,27 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
   cudaStream_t st = (cudaStream_t)r.stream;
   ScChunkParams p{(__nv_bfloat16*)r.out, r.ldo, (const uint8_t*)r.k_cache, (const uint8_t*)r.v_cache, r.ks, r.vs, r.ks_ld, r.vs_ld, (int)r.ks_h,
                   (int)r.vs_h, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.seq_lens, r.starts, r.tile_seq, r.tile_q0, scale_log2, Hq, Hkv, G,
-                  (int)r.window, (int)r.num_pages, reinterpret_cast<float2*>(r.ml), status};
-  const dim3 grid((unsigned)r.tiles, Hkv);
+                  (int)r.window, (int)r.num_pages, reinterpret_cast<float2*>(r.ml), (int)r.splits, (int)r.first_row,
+                  (int)(r.total_tokens - r.first_row), r.part_o,
+                  reinterpret_cast<float2*>(r.part_ml), status};
+  const dim3 grid((unsigned)r.tiles, Hkv, (unsigned)r.splits);
   int rc;
   if (D <= 128) {
-    const long long items = r.tiles * Hkv;
+    const long long items = r.tiles * Hkv * r.splits;
     if (items > 0x3fffffffll) return -1;
     const int blocks = (int)(items < r.sms ? items : r.sms);
     if (D == 64) rc = launch_pairs(scaled_chunk2_kernel<64>, C2Tile<64>::kSmem, blocks, tq, p, (int)items, st);
     else rc = launch_pairs(scaled_chunk2_kernel<128>, C2Tile<128>::kSmem, blocks, tq, p, (int)items, st);
   } else rc = launch_tiles(scaled_chunk_kernel<256>, ScTile<256>::kSmem, grid, kScThreads, tq, p, st);
-  if (rc || !r.weights || r.key_tiles <= 0) return rc;
+  if (rc) return rc;
+  if (r.splits > 1) {
+    const unsigned blocks = (unsigned)(((r.total_tokens - r.first_row) * Hq + 7) / 8);
+    if (D == 64) scaled_chunk_join_kernel<64><<<blocks, 256, 0, st>>>(p);
+    else if (D == 128) scaled_chunk_join_kernel<128><<<blocks, 256, 0, st>>>(p);
+    else scaled_chunk_join_kernel<256><<<blocks, 256, 0, st>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return -20;
+  }
+  if (!r.weights || r.key_tiles <= 0) return 0;
   ScWeighParams w{(const uint8_t*)r.k_cache, r.ks, r.ks_ld, (int)r.ks_h, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.seq_lens, r.starts, r.key_seq,
                   r.key_k0, scale_log2, Hq, Hkv, G, (int)r.window, (int)r.num_pages, reinterpret_cast<const float2*>(r.ml), r.weights, r.w_ld_b,
                   r.w_ld_h, (int)r.width, status};

@@ -25,7 +25,7 @@ _WRITE = struct.Struct("=29qdq")
 _READ = struct.Struct("=20q")
 _EVICT = struct.Struct("=28q")
 _DECODE = struct.Struct("=33qd2q")
-_CHUNK = struct.Struct("=35qd2q")
+_CHUNK = struct.Struct("=39qd2q")
 _calls: dict = {}
 
 
@@ -260,14 +260,20 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
                 at_s + 4 * n_s if n_r else 0, *sums, scale, status, stream), "attn_scaled_decode")
         if B > nd:
             tiles, n, _ = K._tc_tiles(q, batch, nd, 128 // g * (2 if d <= 128 else 1))
-            ml = key_tiles = None
-            at_keys = n_keys = 0
+            ml = key_tiles = parts = None
+            at_keys = n_keys = n_o = 0
+            # few query tiles behind many keys: as many shares of the keys as fill the GPU once, at least four key tiles each
+            splits = max(1, min(K._num_sms[index] // (n * hkv), (min(longest, window + 128) if window else longest) // 512)) if n else 1
+            if splits > 1:
+                n_o = splits * (T - nd) * hq * d
+                parts = torch.empty(n_o + splits * (T - nd) * hq * 2, dtype=_F32, device=q.device)
             if weights is not None:
                 ml = torch.empty((T, hq, 2), dtype=_F32, device=q.device)
                 key_tiles, n_keys = _weigh_tiles(batch, nd, q.device)
                 at_keys = key_tiles.data_ptr()
             at = tiles.data_ptr()
             _call("atlas_attn_scaled_chunk", _CHUNK.pack(
-                at_q, ldq, at_out, hq * d, *cache, at, at + 4 * n, n, T, hq, hkv, d, window, nb, 0 if ml is None else ml.data_ptr(), at_keys,
+                at_q, ldq, at_out, hq * d, *cache, at, at + 4 * n, n, T, hq, hkv, d, window, nb, 0 if ml is None else ml.data_ptr(), splits, nd,
+                parts.data_ptr() if n_o else 0, parts.data_ptr() + 4 * n_o if n_o else 0, at_keys,
                 at_keys + 4 * n_keys, n_keys, *sums, width, K._num_sms[index], scale, status, stream), "attn_scaled_chunk")
     return out

@@ -180,6 +180,11 @@ ATTEND = [
     (128, 1, 128, [20], [9], 0),
     (128, 4, 4, [600, 250], [600, 100], 100),
     (64, 2, 1, [400], [300], 17),
+    # few rows behind many keys: shares of the keys
+    (128, 1, 4, [5000, 700], [40, 2], 0),
+    (64, 2, 8, [3000], [3], 0),
+    (256, 1, 8, [4000, 130, 2000], [1, 5, 40], 0),
+    (128, 2, 4, [9000], [300], 2500),
     # both
     (128, 4, 7, [90, 2000, 300, 65], [1, 1, 300, 3], 0),
     (256, 2, 2, [70, 200], [1, 130], 50),
