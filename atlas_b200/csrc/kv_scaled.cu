@@ -478,7 +478,7 @@ ATLAS_DEVICE uint32_t ld_cluster_u32(const void* mine, uint32_t rank) {
   return v;
 }
 
-// One block, or a cluster of eight, per (sequence, head); a warp has a span of neighbouring tokens.  The `room`-th largest key among the tokens
+// One block, or a cluster of up to eight, per (sequence, head); a warp has a span of neighbouring tokens.  The `room`-th largest key among the tokens
 // between sink and recent, 11, 11 and 10 bits at a time: every block counts its tokens, the cluster's counts are summed through distributed
 // shared memory.  Then the positions in order: the spans' counts are summed and each warp writes its own.  The first kHeld tokens of a lane
 // stay in registers for the five looks at them: up to 8192 tokens of a block (cluster barriers empty L1).
@@ -622,154 +622,145 @@ struct MoveParams {
   int keep, pages; long long units;
 };
 
-// A warp fills two pages of one head, keys and values: one chain of loads (position, block, scales) for 32 tokens.  A kept value token's
-// 16-byte columns hold its neighbours too: every source page is read once, as a whole, for all tokens that come from it, kAhead pages at a
-// time.
+// A warp fills one page of one head's keys or values.  A kept value token's 16-byte columns hold its neighbours too: every source page is read
+// once, as a whole, for all tokens that come from it, kAhead pages at a time.  (A warp for two pages, keys and values one after the other: 31
+// instead of 20 us for one sequence's 4096 tokens.)
 template <int D>
 __global__ void __launch_bounds__(128, D == 256 ? 3 : 6)
 kv_evict_move_kernel(const MoveParams p) {
   constexpr int V = D / 32;
-  constexpr int kAhead = 2;
+  constexpr int kAhead = 2;      // four pages ahead leave room for four blocks an SM in place of six: 138 us a call, not 115 (32 x 4096 tokens to 1024)
   chain_trigger();
   chain_wait();
   const int lane = threadIdx.x & 31;
   unsigned u = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (u >= (unsigned)p.units) return;
   const ScaledCache& c = p.from;
-  const unsigned pairs = (unsigned)(p.pages + 1) / 2;
-  const int pg0 = (int)(u % pairs) * 2;
-  u /= pairs;
+  const bool is_k = (u & 1) == 0;
+  u >>= 1;
+  const int pg = (int)(u % (unsigned)p.pages);
+  u /= (unsigned)p.pages;
   const int h = (int)(u % (unsigned)c.Hkv), b = (int)(u / (unsigned)c.Hkv);
-  const int live = p.new_lens[b] - pg0 * kScPage;        // tokens from the first page on
-  if (live <= 0) return;
-  int page = -1, off = 0, dst = -1;
-  float ks = 0.f, vs = 0.f;
-  if (lane < 2 && lane * kScPage < live) dst = p.to[(long long)b * p.to_ld + pg0 + lane];
-  if (lane < live) {
-    const int pos = p.kept[((long long)b * c.Hkv + h) * p.keep + pg0 * kScPage + lane];
+  // lane r < 16: where token r of the new page comes from (loads side by side; positions behind the last token are -1)
+  const long long at = ((long long)b * c.Hkv + h) * p.keep + pg * kScPage + lane;
+  const int pos = lane < kScPage && pg * kScPage + lane < p.keep ? p.kept[at] : -1;
+  const int to = p.to[(long long)b * p.to_ld + pg];
+  const int live = min(p.new_lens[b] - pg * kScPage, kScPage);
+  if (live <= 0 || to < 0 || to >= c.num_pages) return;
+  int page = -1, off = 0;
+  float scale = 0.f;
+  if (lane < live && pos >= 0) {
     page = p.tables[(long long)b * p.bt_ld + pos / kScPage];
     off = pos % kScPage;
     if (page < 0 || page >= c.num_pages) page = -1;
-    else {
-      ks = c.ks[page * c.ks_ld + h * c.ks_h];
-      vs = c.vs[page * c.vs_ld + h * c.vs_h];
-    }
+    else scale = is_k ? c.ks[page * c.ks_ld + h * c.ks_h] : c.vs[page * c.vs_ld + h * c.vs_h];
   }
   const long long head = (long long)h * (kScPage * D), step = (long long)c.Hkv * (kScPage * D);
-#pragma unroll 1
-  for (int s = 0; s < 2; ++s) {
-    const int to = __shfl_sync(0xffffffffu, dst, s);
-    if (to < 0 || to >= c.num_pages) continue;
-    const long long base = (long long)to * step + head;
-    int ke, ve;
-    {
-      Codes<V> codes[kScPage];
+  const long long base = (long long)to * step + head;
+  if (is_k) {
+    Codes<V> codes[kScPage];
 #pragma unroll
-      for (int r = 0; r < kScPage; ++r) {
-        const int pr = __shfl_sync(0xffffffffu, page, 16 * s + r), o = __shfl_sync(0xffffffffu, off, 16 * s + r);
+    for (int r = 0; r < kScPage; ++r) {
+      const int pr = __shfl_sync(0xffffffffu, page, r), o = __shfl_sync(0xffffffffu, off, r);
 #pragma unroll
-        for (int i = 0; i < (V + 3) / 4; ++i) codes[r].w[i] = 0;
-        if (pr >= 0) codes[r] = load_codes<V>(c.k + head + pr * step + o * D + lane * V);
-      }
-      float amax = 0.f;
+      for (int i = 0; i < (V + 3) / 4; ++i) codes[r].w[i] = 0;
+      if (pr >= 0) codes[r] = load_codes<V>(c.k + head + pr * step + o * D + lane * V);
+    }
+    float amax = 0.f;
 #pragma unroll
-      for (int r = 0; r < kScPage; ++r) {
-        float x[V], m = 0.f;
+    for (int r = 0; r < kScPage; ++r) {
+      float x[V], m = 0.f;
+      widen<V>(codes[r], x);
+#pragma unroll
+      for (int i = 0; i < V; ++i) m = fmaxf(m, fabsf(x[i]));
+      amax = fmaxf(amax, m * __shfl_sync(0xffffffffu, scale, r));
+    }
+    const int e = block_exponent(warp_max(amax));
+    const float by = scale * pow2i(-e);                     // a power of two: exact
+#pragma unroll
+    for (int r = 0; r < kScPage; ++r) {
+      const float f = __shfl_sync(0xffffffffu, by, r);
+      if (f != 1.f) {                                       // the same for all lanes
+        float x[V];
         widen<V>(codes[r], x);
-#pragma unroll
-        for (int i = 0; i < V; ++i) m = fmaxf(m, fabsf(x[i]));
-        amax = fmaxf(amax, m * __shfl_sync(0xffffffffu, ks, 16 * s + r));
+        codes[r] = narrow<V>(x, f);
       }
-      ke = block_exponent(warp_max(amax));
-      const float by = ks * pow2i(-ke);                     // a power of two: exact
+      store_codes<V>(p.k + base + r * D + lane * V, codes[r]);
+    }
+    if (lane == 0) p.ks[to * c.ks_ld + h * c.ks_h] = pow2i(e);
+    return;
+  }
+  // values: the distinct source pages in order, first token of each marked
+  const int before = __shfl_up_sync(0xffffffffu, page, 1);
+  uint32_t leads = __ballot_sync(0xffffffffu, lane < kScPage && (lane == 0 || page != before));
+  uint32_t word[V][4];                                      // sixteen tokens of each of the lane's channels
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) word[i][j] = 0;
+#pragma unroll 1
+  while (leads) {
+    uint4 col[kAhead][V];
+    uint32_t mine[kAhead];                                  // tokens of the new page that come from the source page
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      mine[a] = 0;
+      if (leads) {
+        const int r = __ffs(leads) - 1;
+        leads &= leads - 1;
+        const int end = leads ? __ffs(leads) - 1 : kScPage;
+        const int pr = __shfl_sync(0xffffffffu, page, r);
+        if (pr >= 0) {
+          mine[a] = ((1u << end) - 1u) & ~((1u << r) - 1u);
+#pragma unroll
+          for (int i = 0; i < V; ++i) col[a][i] = reinterpret_cast<const uint4*>(c.v + head + pr * step)[lane * V + i];
+        }
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
 #pragma unroll
       for (int r = 0; r < kScPage; ++r) {
-        const float f = __shfl_sync(0xffffffffu, by, 16 * s + r);
-        if (f != 1.f) {                                     // the same for all lanes
-          float x[V];
-          widen<V>(codes[r], x);
-          codes[r] = narrow<V>(x, f);
-        }
-        store_codes<V>(p.k + base + r * D + lane * V, codes[r]);
-      }
-    }
-    // values: the distinct source pages in order, first token of each marked
-    const int before = __shfl_up_sync(0xffffffffu, page, 1);
-    const bool lead = (lane & 15) == 0 || page != before;
-    uint32_t leads = (__ballot_sync(0xffffffffu, lead) >> (16 * s)) & 0xFFFFu;
-    uint32_t word[V][4];                                    // sixteen tokens of each of the lane's channels
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) word[i][j] = 0;
-    while (leads) {
-      uint4 col[kAhead][V];
-      uint32_t mine[kAhead];                                // tokens of the new page that come from the source page
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        mine[a] = 0;
-        if (leads) {
-          const int r = __ffs(leads) - 1;
-          leads &= leads - 1;
-          const int end = leads ? __ffs(leads) - 1 : kScPage;
-          const int pr = __shfl_sync(0xffffffffu, page, 16 * s + r);
-          if (pr >= 0) {
-            mine[a] = ((1u << end) - 1u) & ~((1u << r) - 1u);
-#pragma unroll
-            for (int i = 0; i < V; ++i) col[a][i] = reinterpret_cast<const uint4*>(c.v + head + pr * step)[lane * V + i];
-          }
-        }
-      }
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-        for (int r = 0; r < kScPage; ++r) {
-          if (!((mine[a] >> r) & 1u)) continue;             // the same for all lanes
-          const int o = __shfl_sync(0xffffffffu, off, 16 * s + r);
-          // byte r & 3 of the word becomes byte o & 3 of the column's word o / 4
-          const uint32_t pick = (0x3210u & ~(0xFu << (4 * (r & 3)))) | ((4u + (o & 3)) << (4 * (r & 3)));
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const uint32_t lo = (o & 4) ? col[a][i].y : col[a][i].x, hi = (o & 4) ? col[a][i].w : col[a][i].z;
-            word[i][r >> 2] = __byte_perm(word[i][r >> 2], (o & 8) ? hi : lo, pick);
-          }
-        }
-    }
-    {
-      float amax = 0.f;
-#pragma unroll
-      for (int r = 0; r < kScPage; r += 2) {
-        float m0 = 0.f, m1 = 0.f;
+        if (!((mine[a] >> r) & 1u)) continue;               // the same for all lanes
+        const int o = __shfl_sync(0xffffffffu, off, r);
+        // byte r & 3 of the word becomes byte o & 3 of the column's word o / 4
+        const uint32_t pick = (0x3210u & ~(0xFu << (4 * (r & 3)))) | ((4u + (o & 3)) << (4 * (r & 3)));
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float2 t = codes2_to_f32((word[i][r >> 2] >> (8 * (r & 3))) & 0xFFFFu);
-          m0 = fmaxf(m0, fabsf(t.x));
-          m1 = fmaxf(m1, fabsf(t.y));
-        }
-        amax = fmaxf(amax, fmaxf(m0 * __shfl_sync(0xffffffffu, vs, 16 * s + r), m1 * __shfl_sync(0xffffffffu, vs, 16 * s + r + 1)));
-      }
-      ve = block_exponent(warp_max(amax));
-      const float by = vs * pow2i(-ve);
-#pragma unroll
-      for (int r = 0; r < kScPage; r += 2) {
-        const float f0 = __shfl_sync(0xffffffffu, by, 16 * s + r), f1 = __shfl_sync(0xffffffffu, by, 16 * s + r + 1);
-        if (f0 == 1.f && f1 == 1.f) continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float2 t = codes2_to_f32((word[i][r >> 2] >> (8 * (r & 3))) & 0xFFFFu);
-          const uint32_t two = f32_to_codes2(t.x * f0, t.y * f1);
-          word[i][r >> 2] = (r & 2) ? __byte_perm(word[i][r >> 2], two, 0x5410) : __byte_perm(word[i][r >> 2], two, 0x3254);
+          const uint32_t lo = (o & 4) ? col[a][i].y : col[a][i].x, hi = (o & 4) ? col[a][i].w : col[a][i].z;
+          word[i][r >> 2] = __byte_perm(word[i][r >> 2], (o & 8) ? hi : lo, pick);
         }
       }
+  }
+  float amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        reinterpret_cast<uint4*>(p.v + base)[lane * V + i] = make_uint4(word[i][0], word[i][1], word[i][2], word[i][3]);
+  for (int r = 0; r < kScPage; r += 2) {
+    float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 t = codes2_to_f32((word[i][r >> 2] >> (8 * (r & 3))) & 0xFFFFu);
+      m0 = fmaxf(m0, fabsf(t.x));
+      m1 = fmaxf(m1, fabsf(t.y));
     }
-    if (lane == 0) {
-      p.ks[to * c.ks_ld + h * c.ks_h] = pow2i(ke);
-      p.vs[to * c.vs_ld + h * c.vs_h] = pow2i(ve);
+    amax = fmaxf(amax, fmaxf(m0 * __shfl_sync(0xffffffffu, scale, r), m1 * __shfl_sync(0xffffffffu, scale, r + 1)));
+  }
+  const int e = block_exponent(warp_max(amax));
+  const float by = scale * pow2i(-e);
+#pragma unroll
+  for (int r = 0; r < kScPage; r += 2) {
+    const float f0 = __shfl_sync(0xffffffffu, by, r), f1 = __shfl_sync(0xffffffffu, by, r + 1);
+    if (f0 == 1.f && f1 == 1.f) continue;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 t = codes2_to_f32((word[i][r >> 2] >> (8 * (r & 3))) & 0xFFFFu);
+      const uint32_t two = f32_to_codes2(t.x * f0, t.y * f1);
+      word[i][r >> 2] = (r & 2) ? __byte_perm(word[i][r >> 2], two, 0x5410) : __byte_perm(word[i][r >> 2], two, 0x3254);
     }
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    reinterpret_cast<uint4*>(p.v + base)[lane * V + i] = make_uint4(word[i][0], word[i][1], word[i][2], word[i][3]);
+  if (lane == 0) p.vs[to * c.vs_ld + h * c.vs_h] = pow2i(e);
 }
 
 }  // namespace atlas
@@ -884,7 +875,7 @@ extern "C" int atlas_kv_scaled_read(const void* record) {
 struct EvictRecord {
   void* k_cache; void* v_cache; ScalesRecord s;
   const int* tables; long long bt_ld; const int* seq_lens; const float* weights; long long w_ld_b, w_ld_h, width;
-  long long B, Hkv, D, num_pages, keep, sink, recent; const int* to; long long to_ld; int* new_lens; int* kept; float* w_out; void* stream;
+  long long B, Hkv, D, num_pages, keep, sink, recent; const int* to; long long to_ld; int* new_lens; int* kept; float* w_out; long long sms; void* stream;
 };
 extern "C" int atlas_kv_evict(const void* record) {
   const EvictRecord& r = *static_cast<const EvictRecord*>(record);
@@ -903,12 +894,18 @@ extern "C" int atlas_kv_evict(const void* record) {
   m.tables = r.tables; m.bt_ld = (int)r.bt_ld; m.to = r.to; m.to_ld = (int)r.to_ld; m.kept = r.kept; m.new_lens = r.new_lens; m.keep = keep;
   const long long longest = r.width < r.keep ? r.width : r.keep;
   m.pages = (int)((longest + kScPage - 1) / kScPage);
-  m.units = r.B * Hkv * ((m.pages + 1) / 2);
+  m.units = 2ll * r.B * Hkv * m.pages;
   if (m.units > 0x7fffffffll || r.B * Hkv > 0x7fffffffll / 8) return -1;
-  // Eight blocks a head where one would look at more than 8192 tokens.
-  const int rc = r.width > 8192
-      ? launched(launch_chain_cluster(true, 8, kv_evict_select_kernel<8>, dim3((unsigned)(r.B * Hkv * 8)), dim3(kSelThreads), 0, st, s))
-      : launched(launch_chain(kv_evict_select_kernel<1>, dim3((unsigned)(r.B * Hkv)), dim3(kSelThreads), 0, st, s));
+  // As many blocks a head, up to eight, as there are SMs for and 2048 tokens each: a block has an SM to itself, and a second wave of
+  // clusters doubles the time (256 heads of 4096 tokens: 19 us on a block each, 470 on clusters of eight).
+  int n = 1;
+  while (n < 8 && r.B * Hkv * n * 2 <= r.sms && r.width >= 4096ll * n) n *= 2;
+  const dim3 blocks((unsigned)(r.B * Hkv * n)), threads(kSelThreads);
+  const cudaError_t e = n == 8   ? launch_chain_cluster(true, 8, kv_evict_select_kernel<8>, blocks, threads, 0, st, s)
+                        : n == 4 ? launch_chain_cluster(true, 4, kv_evict_select_kernel<4>, blocks, threads, 0, st, s)
+                        : n == 2 ? launch_chain_cluster(true, 2, kv_evict_select_kernel<2>, blocks, threads, 0, st, s)
+                                 : launch_chain(kv_evict_select_kernel<1>, blocks, threads, 0, st, s);
+  const int rc = launched(e);
   if (rc || m.units == 0) return rc;
   return by_width<Move>((int)r.D, m, st);
 }

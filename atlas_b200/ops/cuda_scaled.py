@@ -23,7 +23,7 @@ _F32, _BF16, _I32, _FP8 = torch.float32, torch.bfloat16, torch.int32, torch.floa
 # records of the entry points, in the order of their C structs: integers and pointers, one double
 _WRITE = struct.Struct("=29qdq")
 _READ = struct.Struct("=20q")
-_EVICT = struct.Struct("=28q")
+_EVICT = struct.Struct("=29q")
 _DECODE = struct.Struct("=33qd2q")
 _CHUNK = struct.Struct("=39qd2q")
 _calls: dict = {}
@@ -183,12 +183,12 @@ def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights
         return lens, kept, out_w
     if checked.ENABLED:
         checked.evict(block_tables, seq_lens, new_tables, nb, BLOCK, keep, width)
-    guard, _, stream = _place(k_cache)
+    guard, index, stream = _place(k_cache)
     with guard:
         _call("atlas_kv_evict", _EVICT.pack(
             k_cache.data_ptr(), v_cache.data_ptr(), *_scales(k_scale, v_scale), block_tables.data_ptr(), block_tables.stride(0),
             seq_lens.data_ptr(), weights.data_ptr(), weights.stride(0), weights.stride(1), width, B, hkv, d, nb, keep, sink, recent,
-            new_tables.data_ptr(), new_tables.stride(0), lens.data_ptr(), kept.data_ptr(), out_w.data_ptr(), stream), "kv_evict")
+            new_tables.data_ptr(), new_tables.stride(0), lens.data_ptr(), kept.data_ptr(), out_w.data_ptr(), K._num_sms[index], stream), "kv_evict")
     return lens, kept, out_w
 
 

@@ -264,7 +264,7 @@ def test_empty_decode_sequences_give_zeros():
 # ----------------------------------------------------------------------------- eviction
 @pytest.mark.parametrize("d,hkv,lens,keep,sink,recent", [
     (128, 2, [100, 37, 64], 37, 4, 8), (64, 1, [1000, 3], 16, 0, 0), (256, 3, [333], 100, 0, 100), (128, 1, [5000, 40, 1], 1000, 16, 1),
-    (64, 2, [50], 1, 1, 0), (128, 2, [70], 70, 3, 3), (64, 1, [20000], 333, 1, 30)])
+    (64, 2, [50], 1, 1, 0), (128, 2, [70], 70, 3, 3), (64, 1, [20000], 333, 1, 30), (64, 1, [9000, 100], 700, 3, 9), (64, 20, [5000], 40, 0, 4)])
 @pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
 def test_evict_keeps_the_heaviest_in_order(d, hkv, lens, keep, sink, recent, kind):
     gen = torch.Generator().manual_seed(keep)
