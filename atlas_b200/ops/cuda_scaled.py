@@ -27,6 +27,7 @@ _EVICT = struct.Struct("=29q")
 _DECODE = struct.Struct("=33qd2q")
 _CHUNK = struct.Struct("=39qd2q")
 _calls: dict = {}
+_HERE = contextlib.nullcontext()
 
 
 def _call(name: str, record: bytes, what: str) -> None:
@@ -48,24 +49,24 @@ def _place(t: torch.Tensor):
         raise K.KernelError("the kernels take tensors on a GPU")
     if i not in K._status_ptr:
         K._dev(t)
-    guard = contextlib.nullcontext() if torch._C._cuda_getDevice() == i else torch.cuda.device(i)
-    return guard, i, torch._C._cuda_getCurrentRawStream(i)
+    return _HERE if torch._C._cuda_getDevice() == i else torch.cuda.device(i), i, torch._C._cuda_getCurrentRawStream(i)
 
 
 def check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale, v_scale) -> Tuple[int, int, int]:
     """(blocks, heads, head width) of a block-scaled cache, or the error of what does not fit."""
     if not (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)):
         raise K.KernelError("a block-scaled cache takes a scale tensor for the keys and one for the values")
-    if k_cache.dim() != 4:
+    shape, dev = k_cache.shape, k_cache.get_device()
+    if len(shape) != 4:
         raise K.KernelError("a cache has four dimensions: blocks, tokens, heads, channels")
-    nb, bs, hkv, d = k_cache.shape
-    if k_cache.dtype != _FP8 or v_cache.dtype != _FP8 or v_cache.shape != (nb, bs, hkv, d):
+    nb, bs, hkv, d = shape
+    if k_cache.dtype != _FP8 or v_cache.dtype != _FP8 or v_cache.shape != shape:
         raise K.KernelError("block scales belong to an FP8 (e4m3) cache of keys and values of one size")
     if bs != BLOCK or d not in HEAD_DIMS:
         raise K.KernelError(f"block scales take blocks of {BLOCK} tokens and heads of 64, 128 or 256, not {bs} and {d}")
-    if k_cache.stride() != (hkv * BLOCK * d, d, BLOCK * d, 1) or v_cache.stride() != (hkv * BLOCK * d, 1, d * BLOCK, BLOCK):
+    page = BLOCK * d
+    if k_cache.stride() != (hkv * page, d, page, 1) or v_cache.stride() != (hkv * page, 1, page, BLOCK):
         raise K.KernelError("KV cache is not in the kernel layout (allocate it with ops.cuda.alloc_kv_cache)")
-    dev = k_cache.get_device()
     if v_cache.get_device() != dev:
         raise K.KernelError("keys and values of a cache are on one device")
     for s in (k_scale, v_scale):
@@ -133,7 +134,7 @@ def qk_norm_rope_kv_write(q, k, v, positions, rope_cache, rotary_dim, k_cache, v
         checked.block_runs(slot_mapping, BLOCK)
     guard, _, stream = _place(k_cache)
     with guard:
-        out = q.new_empty((T, hq, d))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         _call("atlas_kv_scaled_write", _WRITE.pack(
             q.data_ptr(), q.stride(0), out.data_ptr(), hq * d, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), pos, rope, qw, kw,
             k_cache.data_ptr(), v_cache.data_ptr(), *_scales(k_scale, v_scale), slot_mapping.data_ptr(), T, hq, hkv, d, rotary_dim, nb,
@@ -241,7 +242,7 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
         checked.paged_read(bt, lens, nb, BLOCK)
     guard, index, stream = _place(k_cache)
     with guard:
-        out = q.new_empty((T, hq, d))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         cache = (k_cache.data_ptr(), v_cache.data_ptr(), *_scales(k_scale, v_scale), bt.data_ptr(), bt.stride(0), cols, lens.data_ptr(),
                  starts.data_ptr())
         status, at_out = K._status_ptr[index], out.data_ptr()
