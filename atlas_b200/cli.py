@@ -39,7 +39,7 @@ def build_parser() -> argparse.ArgumentParser:
                    help="end thinking early after this many consecutive tokens with top-1 probability >= 0.95 (0 = off)")
     s.add_argument("--mtp-vocab", type=int, default=0, help="draft steps score this many rows of the lm_head (0 = all)")
     s.add_argument("--mtp-vocab-rank", default="id", help="'id' (first rows) or the path of a ranked token-id table")
-    s.add_argument("--kv-cache-dtype", default="fp8", choices=["auto", "fp8", "bf16", "nvfp4", "turbo8"])
+    s.add_argument("--kv-cache-dtype", default="fp8", choices=["auto", "fp8", "bf16", "nvfp4", "turbo8", "fp8_scaled"])
     s.add_argument("--sparse-attention-blocks", type=int, default=0,
                    help="long contexts: decode attention reads at most this many KV blocks per sequence, chosen by a "
                         "block predictor (first and most recent blocks always kept); 0 = dense attention")

@@ -53,13 +53,15 @@ class LLMEngine:
         self.mcfg: ModelConfig = model.cfg
         dev = model.device
         self.hybrid = self.mcfg.family == "hybrid" and len(model.gdn_layers()) > 0
+        self.kv_block_scales = False      # FP8 cache with a scale per (block, head): "fp8_scaled"
         self.kv_dtype = self._resolve_kv_dtype()
         num_blocks = self.cfg.num_kv_blocks or self._profile_num_blocks()
         n_active = self.cfg.max_num_seqs if self.hybrid else 0
         n_snap = self.cfg.ssm_cache_slots if (self.hybrid and self.cfg.enable_prefix_caching) else 0
         self.cache: CacheStore = model.alloc_cache(num_blocks, self.cfg.block_size, self.kv_dtype,
                                                    n_active + n_snap + (1 if self.hybrid else 0),      # + padding rows of decode graphs
-                                                   high_precision_layers=self.cfg.kv_high_precision_layers)
+                                                   high_precision_layers=self.cfg.kv_high_precision_layers,
+                                                   block_scales=self.kv_block_scales)
         if os.environ.get("ATLAS_NATIVE_RUNTIME", "0") not in ("0", "", "false"):
             from .runtime_native import NativeBlockPool          # C++ pool, same interface
             self.pool = NativeBlockPool(num_blocks, self.cfg.block_size)
@@ -71,7 +73,8 @@ class LLMEngine:
         self.host_tier = None
         if self.cfg.swap_space_gb > 0:
             from .kv.host_tier import HostKVTier
-            per_block = max(1, model.kv_bytes_per_block(self.cfg.block_size, self.kv_dtype, self.cfg.kv_high_precision_layers))
+            per_block = max(1, model.kv_bytes_per_block(self.cfg.block_size, self.kv_dtype, self.cfg.kv_high_precision_layers,
+                                                        self.kv_block_scales))
             n_host = int(self.cfg.swap_space_gb * (1 << 30)) // per_block
             if n_host > 0:
                 self.host_tier = HostKVTier(self.cache, n_host, self.cfg.max_num_seqs if self.hybrid else 0,
@@ -140,6 +143,10 @@ class LLMEngine:
             # rotation does not cover keeps the plain FP8 cache
             self.model.set_kv_rotation(True)
             want = "fp8"
+        if want == "fp8_scaled":
+            # a power of two per (block, head), set from what the block holds; where that does not apply, the plain FP8 cache
+            self.kv_block_scales = self.model.takes_block_scales(self.cfg.block_size) and not self.cfg.sparse_attention_blocks
+            want = "fp8"
         if want == "bf16":
             return torch.bfloat16           # GPU: the general mma.sync attention kernel on a 16-bit cache
         if want == "fp8" or (want == "auto" and self.model.device.type == "cuda"):
@@ -147,7 +154,8 @@ class LLMEngine:
         return self.model.dtype
 
     def _profile_num_blocks(self) -> int:
-        per_block = max(1, self.model.kv_bytes_per_block(self.cfg.block_size, self.kv_dtype, self.cfg.kv_high_precision_layers))
+        per_block = max(1, self.model.kv_bytes_per_block(self.cfg.block_size, self.kv_dtype, self.cfg.kv_high_precision_layers,
+                                                         self.kv_block_scales))
         if self.model.device.type == "cuda":
             free, total = torch.cuda.mem_get_info(self.model.device)
             budget = int(total * self.cfg.gpu_memory_utilization) - (total - free)

@@ -116,7 +116,7 @@ class DiskKVTier:
 
 class HostKVTier:
     """Pinned host pool of fixed-size records: record ``hb`` holds one KV block of every layer (K then V, layer after
-    layer, the logical ``[block, head, dim]`` order of the pool views).
+    layer, the logical ``[block, head, dim]`` order of the pool views; behind them its scales, where each block has its own).
 
     Copies run on a dedicated CUDA stream and never block the host: a swap-out gathers the blocks of each layer into one
     device staging matrix (a handful of indexing kernels ordered after the compute stream by an event), then issues one
@@ -135,7 +135,8 @@ class HostKVTier:
         self.layout: List[tuple] = []
         off = 0
         for l, (k, v) in cache.kv.items():
-            for which, t in (("k", k), ("v", v)):
+            scales = [(w, s) for w, s in zip(("ks", "vs"), cache.kv_scales.get(l, ())) if isinstance(s, torch.Tensor)]
+            for which, t in [("k", k), ("v", v)] + scales:
                 n = t[0].numel() * t.element_size()
                 if n == 0:
                     continue                                  # a latent cache has one pool
@@ -205,8 +206,7 @@ class HostKVTier:
         return self._staging[:n]
 
     def _tensor(self, l: int, which: str) -> torch.Tensor:
-        k, v = self.cache.kv[l]
-        return k if which == "k" else v
+        return dict(zip(("k", "v", "ks", "vs"), self.cache.layer_kv(l)))[which]
 
     def copy_out(self, dev_blocks: List[int], host_blocks: List[int], state_slot: Optional[int] = None,
                  host_state: Optional[int] = None) -> None:

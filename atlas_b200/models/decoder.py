@@ -80,7 +80,7 @@ class CacheStore:
     """Device memory the model reads/writes across steps: paged KV per attention layer and the
     recurrent-state slot pool per GDN layer."""
     kv: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = field(default_factory=dict)
-    kv_scales: Dict[int, Tuple[float, float]] = field(default_factory=dict)
+    kv_scales: Dict[int, Tuple] = field(default_factory=dict)       # of keys and values: numbers, or tensors [blocks, heads]
     states: Dict[int, dict] = field(default_factory=dict)
     block_size: int = 16
     num_blocks: int = 0
@@ -592,6 +592,19 @@ class DecoderLM:
                 l.mixer.kv_rotate = bool(on)
         return True
 
+    def takes_block_scales(self, block_size: int) -> bool:
+        """Every attention layer's FP8 cache can have a scale per (block, head): plain attention, 16-token blocks, heads of 64, 128 or
+        256 with a rotated width that is a multiple of 16."""
+        from ..layers.attention import Attention
+        from ..ops.cuda_scaled import BLOCK, HEAD_DIMS
+        cfg = self.cfg
+        if cfg.layer_specs or cfg.kv_lora_rank > 0 or block_size != BLOCK or cfg.rotary_dim % 16:
+            return False
+        if self.device.type == "cuda" and self.dtype != torch.bfloat16:
+            return False
+        layers = [a for a in (attention_of(l) for l in self.layers) if a is not None]
+        return all(type(a) is Attention and a.plain and a.d in HEAD_DIMS and not a.kv_rotate for a in layers)
+
     def register_adapter(self, adapter) -> int:
         """Make ``adapter`` (whole, as loaded) resident on this rank, cut like the base weights; returns its slot."""
         from ..lora import localize
@@ -648,7 +661,7 @@ class DecoderLM:
             return torch.bfloat16 if self.dtype == torch.bfloat16 else self.dtype
         return kv_dtype
 
-    def kv_bytes_per_block(self, block_size: int, kv_dtype: torch.dtype, high_precision_layers=()) -> int:
+    def kv_bytes_per_block(self, block_size: int, kv_dtype: torch.dtype, high_precision_layers=(), block_scales: bool = False) -> int:
         if self.cfg.layer_specs:
             owners = [(l, attention_of(l)) for l in self.layers if attention_of(l) is not None]
             return int(sum(block_size * kv_elements_of(a) * kv_element_bytes(self._cache_dtype(l, kv_dtype, set(high_precision_layers)))
@@ -657,12 +670,14 @@ class DecoderLM:
         hkv = self.layers[self.attention_layers()[0]].mixer.hkv if n_attn else 0
         n_hi = len([i for i in self.attention_layers() if i in set(high_precision_layers)])
         per = 2 * block_size * hkv * self.cfg.head_dim
-        return int(per * ((n_attn - n_hi) * kv_element_bytes(kv_dtype) + n_hi * max(2.0, kv_element_bytes(kv_dtype))))
+        scales = 8 * hkv * (n_attn - n_hi) if block_scales else 0
+        return scales + int(per * ((n_attn - n_hi) * kv_element_bytes(kv_dtype) + n_hi * max(2.0, kv_element_bytes(kv_dtype))))
 
     def alloc_cache(self, num_blocks: int, block_size: int, kv_dtype: torch.dtype, state_slots: int = 0,
-                    high_precision_layers=()) -> CacheStore:
+                    high_precision_layers=(), block_scales: bool = False) -> CacheStore:
         """``high_precision_layers``: attention layers whose cache stays in 16 bits when ``kv_dtype`` is FP8 or NVFP4 (the
-        layers most sensitive to KV quantisation, typically the first and last ones)."""
+        layers most sensitive to KV quantisation, typically the first and last ones).  ``block_scales``: the layers' FP8 caches
+        have a power of two per (block, head) instead of one scale (the draft head's cache keeps that)."""
         store = CacheStore(block_size=block_size, num_blocks=num_blocks)
         hi = set(high_precision_layers)
         for l in self.layers:
@@ -672,7 +687,8 @@ class DecoderLM:
                 own = getattr(a, "alloc_kv", None)
                 store.kv[l.idx] = (own(num_blocks, block_size, dt, self.device) if own is not None
                                    else alloc_kv(num_blocks, block_size, a.hkv, a.d, dt, self.device))
-                store.kv_scales[l.idx] = (1.0, 1.0)
+                scaled = block_scales and kv_dtype_is_fp8(dt)
+                store.kv_scales[l.idx] = ops.alloc_kv_scales(num_blocks, a.hkv, self.device) if scaled else (1.0, 1.0)
             if recurrent_of(l) is not None:
                 store.states[l.idx] = recurrent_of(l).alloc_state(max(1, state_slots), self.device, self.dtype)
         if self.mtp is not None:

@@ -35,11 +35,17 @@ def cuda_ops():
     return _cuda
 
 
+_scaled = None
+
+
 def scaled_ops():
     """The bindings of the block-scaled cache."""
-    cuda_ops()
-    from . import cuda_scaled as CS
-    return CS
+    global _scaled
+    if _scaled is None:
+        cuda_ops()
+        from . import cuda_scaled as _s
+        _scaled = _s
+    return _scaled
 
 
 # ----------------------------------------------------------------------------- weights / activations
@@ -502,7 +508,7 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale=1.0, v_scale=1.0,
 def paged_attention_fp8_out(q, k_cache, v_cache, batch, scale, k_scale=1.0, v_scale=1.0, sliding_window=None) -> Optional[Act]:
     """Decode attention that hands its output over already group-quantised for an FP8 output projection (one kernel
     less per layer); None when the step / cache / head size is not covered and the caller takes the bf16 path."""
-    if not (FUSED_EPILOGUES and on_gpu(q)):
+    if not (FUSED_EPILOGUES and on_gpu(q)) or isinstance(k_scale, torch.Tensor):
         return None
     r = cuda_ops().paged_attention_q8(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding_window)
     return None if r is None else Act(q=r[0], s=r[1], dtype=q.dtype)
