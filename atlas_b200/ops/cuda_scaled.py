@@ -158,7 +158,7 @@ def kv_read(k_cache, v_cache, block_tables, seq_lens, max_len: int, k_scale, v_s
             _call("atlas_kv_scaled_read", _READ.pack(
                 k_cache.data_ptr(), v_cache.data_ptr(), *_scales(k_scale, v_scale), block_tables.data_ptr(), block_tables.stride(0), cols,
                 seq_lens.data_ptr(), B, max_len, hkv, d, nb, at, at + B * max_len * hkv * d * 2, stream), "kv_scaled_read")
-    return out[0], out[1]
+    return out.unbind(0)
 
 
 def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep: int, new_tables, sink: int, recent: int):
@@ -176,10 +176,9 @@ def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights
     need = (min(keep, width) + BLOCK - 1) // BLOCK
     if seq_lens.shape[0] != B or new_tables.shape[0] != B or new_tables.shape[1] < need:
         raise K.KernelError(f"{B} sequences that keep up to {min(keep, width)} tokens need their lengths and new block tables of {need} columns")
-    # lengths, positions and weights of the kept tokens share one allocation
-    n = B * hkv * keep
-    both = torch.empty(2 * n + B, dtype=_I32, device=k_cache.device)
-    kept, out_w, lens = both[:n].view(B, hkv, keep), both[n:2 * n].view(_F32).view(B, hkv, keep), both[2 * n:]
+    kept = torch.empty((B, hkv, keep), dtype=_I32, device=k_cache.device)
+    out_w = torch.empty((B, hkv, keep), dtype=_F32, device=k_cache.device)
+    lens = torch.empty(B, dtype=_I32, device=k_cache.device)
     if B == 0:
         return lens, kept, out_w
     if checked.ENABLED:
