@@ -5,12 +5,10 @@
 // 2^(row's own power) * key page's scale, p_j = 2^(s_j + ev - M) in f16, o = sum p_j v^_j / sum p_j 2^-ev.  A page covers 16 score columns, so
 // f and ev - M are constants of a multiply-add over them, and a page's largest score is found before they are applied.
 //
-// scaled_chunk_kernel: one CTA per (128 query rows, key head); the G query heads of a key head are packed into the rows (row = token * G +
-// head), so that a page is fetched and widened once for all of them.
-//   warp 0       Q tile by TMA; the pages of each key tile (cp.async.bulk) and their scales, a tile of block-table entries ahead
-//   warp 1       tcgen05.mma: S_j = Q K_j^T into one of two score buffers, O += P_j V_j; QK_{j+1} goes before PV_j
-//   warps 2..5   e4m3 -> f16, into the 128-byte-swizzled K-major layout (values are stored with tokens along rows already)
-//   warps 6..13  softmax, two threads a row; O is rescaled in TMEM only when a row's maximum has passed its reference by 2^8
+// scaled_chunk2_kernel (heads of 64 and 128), scaled_chunk_wide_kernel (256): tiles of 128 query rows of a key head; the G query heads of a key
+// head are packed into the rows (row = token * G + head), so that a page is fetched and widened once for all of them.  One warp fetches pages
+// (cp.async.bulk) and scales, others widen e4m3 to 16 bits into the 128-byte-swizzled K-major layout (values are stored with tokens along rows
+// already), softmax takes a thread a row, and P goes back to TMEM over its scores as the operand of the next product.
 //
 // scaled_chunk_weigh_kernel: a cluster of two CTAs per (128 cached tokens, key head); tiles of the chunk's rows go by, every other one to each.
 // S^T = K Q^T in bf16 (an e4m3 number is one exactly, and Q stays as it is): a TMEM lane is a token, so that the sum over rows and heads is a
@@ -23,24 +21,10 @@ namespace atlas {
 
 constexpr int kScRows = 128;
 constexpr int kScPg = 16;
-constexpr int kScThreads = 448;
 constexpr int kScSub = 16 * 1024;                 // 128 rows x 64 16-bit numbers
-constexpr int kScRingTiles = 8;                   // key tiles whose page scales are kept
-
-template <int D>
-struct ScTile {
-  static constexpr int kKv = D <= 128 ? 128 : 64;                // keys of a tile: 256-wide heads would not fit twice that
-  static constexpr int kPages = kKv / kScPg;
-  static constexpr int kKSub = kKv * 128, kVSub = D * 128;
-  static constexpr int kPageBytes = kScPg * D;
-  static constexpr int kStageBytes = 2 * kPages * kPageBytes;
-  static constexpr int kStages = D <= 128 ? 3 : 2;
-  static constexpr int kTiles = (D / 64) * (kScSub + kKSub) + (kKv / 64) * (kVSub + kScSub);
-  static constexpr int kSmem = kTiles + kStages * kStageBytes + 2048 + 1024;
-};
 
 struct ScChunkParams {
-  __nv_bfloat16* out; long long ldo;
+  const __nv_bfloat16* q; long long ldq; __nv_bfloat16* out; long long ldo;
   const uint8_t* k_cache; const uint8_t* v_cache;
   const float* k_scale; const float* v_scale; long long ks_ld, vs_ld; int ks_h, vs_h;
   const int* block_tables; int bt_ld, bt_cols;
@@ -146,416 +130,6 @@ scaled_chunk_join_kernel(const ScChunkParams p) {
   if (p.ml && lane == 0) p.ml[row * p.Hq + head] = make_float2(ref, inv);
 }
 
-template <int D>
-__global__ void __launch_bounds__(kScThreads, 1)
-scaled_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  using Tile = ScTile<D>;
-  constexpr int kKv = Tile::kKv, kPages = Tile::kPages, kStages = Tile::kStages, kStageBytes = Tile::kStageBytes;
-  constexpr int kPageBytes = Tile::kPageBytes, kKSub = Tile::kKSub, kVSub = Tile::kVSub;
-  uint8_t* sQ = smem;                              // D / 64 sub-tiles [128 rows][64 channels]
-  uint8_t* sK = sQ + (D / 64) * kScSub;            // D / 64 sub-tiles [tokens][64 channels]
-  uint8_t* sV = sK + (D / 64) * kKSub;             // kKv / 64 sub-tiles [channels][64 tokens]
-  uint8_t* sP = sV + (kKv / 64) * kVSub;           // kKv / 64 sub-tiles [128 rows][64 tokens]
-  uint8_t* sStage = smem + Tile::kTiles;           // kStages x (K pages, V pages)
-  float2* sScale = reinterpret_cast<float2*>(sStage + kStages * kStageBytes);      // [kScRingTiles][8] (key scale, value exponent)
-  float* sRow = reinterpret_cast<float*>(sScale + kScRingTiles * 8);               // [128] score factor of a row
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + kScRows);
-  uint64_t* q_full = bars;
-  uint64_t* stg_full = bars + 1;                   // [kStages]
-  uint64_t* stg_empty = stg_full + kStages;        // [kStages] 4 converter warps
-  uint64_t* k_ready = stg_empty + kStages;         // 4 converter warps
-  uint64_t* k_free = k_ready + 1;                  // QK done
-  uint64_t* v_ready = k_ready + 2;                 // 4 converter warps
-  uint64_t* pv_done = k_ready + 3;                 // V tile, P tile and O are free
-  uint64_t* s_full = k_ready + 4;                  // [2]
-  uint64_t* s_free = k_ready + 6;                  // [2] 8 softmax warps
-  uint64_t* p_ready = k_ready + 8;                 // 8 softmax warps
-  uint64_t* q_conv = k_ready + 9;                  // 8 softmax warps
-  uint64_t* x_ready = k_ready + 10;                // [2 parities][4 row groups]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(k_ready + 18);
-  volatile uint32_t* abort_flag = tmem_slot + 1;
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = p.G, tok_per_tile = kScRows / G;
-  const int b = p.tile_seq[blockIdx.x], q0 = p.tile_q0[blockIdx.x], kvh = blockIdx.y;
-  const int L = min(p.seq_lens[b], p.bt_cols * kScPg);
-  const int q_row0 = p.query_start_loc[b], q_len = p.query_start_loc[b + 1] - q_row0;
-  const int ctx0 = L - q_len;                                   // position of the chunk's first row
-  const int last_tok = min(q0 + tok_per_tile, q_len) - 1;
-  const int kv_hi = min(L, ctx0 + last_tok + 1);                // keys [.., kv_hi)
-  const int first_page = p.window > 0 ? max(ctx0 + q0 - p.window + 1, 0) / kScPg : 0;
-  const int all_kv = max((kv_hi - first_page * kScPg + kKv - 1) / kKv, 0), share = (all_kv + p.splits - 1) / p.splits;
-  const int page0 = first_page + blockIdx.z * share * kPages;
-  const int base = page0 * kScPg;                               // first key of tile 0 of this share
-  const int n_kv = min(max(all_kv - (int)blockIdx.z * share, 0), share);
-
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int s = 0; s < kStages; ++s) { mbar_init(&stg_full[s], 1); mbar_init(&stg_empty[s], 4); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); }
-    mbar_init(k_ready, 4); mbar_init(k_free, 1); mbar_init(v_ready, 4); mbar_init(pv_done, 1); mbar_init(p_ready, 8);
-    mbar_init(q_conv, 8);
-    for (int s = 0; s < 8; ++s) mbar_init(&x_ready[s], 2);
-    *abort_flag = 0;
-    mbar_fence_init();
-  }
-  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  if (warp == 0 && lane == 0) tma_prefetch_desc(&tmap_q);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  const uint32_t tS = tmem_base, tO = tmem_base + 2 * kKv, tX = tO + D;
-
-  if (warp == 0) {
-    // ------------------------------------------------------------------ producer
-    if (lane == 0) {
-      mbar_expect_tx(q_full, (uint32_t)(D / 64) * 128u * (uint32_t)(tok_per_tile * G));
-#pragma unroll
-      for (int s = 0; s < D / 64; ++s) tma_load_3d(sQ + s * kScSub, &tmap_q, q_full, s * 64, kvh * G, q_row0 + q0);
-    }
-    const int* bt = p.block_tables + (long long)b * p.bt_ld;
-    const int n_pages = (L + kScPg - 1) / kScPg;
-    const int pi = lane & 7;                           // lanes 0..7 fetch key pages, 8..15 value pages, the first kPages of each
-    const bool is_v = (lane & 8) != 0;
-    auto entry = [&](int j) {                          // block and scale of this lane's page of tile j
-      const int pg = page0 + j * kPages + pi;
-      int blk = lane < 16 && pi < kPages && pg < n_pages ? bt[pg] : -1;
-      return blk >= p.num_pages ? -1 : blk;
-    };
-    auto scale_of = [&](int blk) {
-      if (blk < 0) return 1.f;
-      return is_v ? p.v_scale[blk * p.vs_ld + kvh * p.vs_h] : p.k_scale[blk * p.ks_ld + kvh * p.ks_h];
-    };
-    int blk_next = entry(0);
-    float sc_next = scale_of(blk_next);
-    uint32_t stage = 0, phase = 0;
-    bool ok = true;
-    for (int j = 0; j < n_kv && ok; ++j) {
-      const int blk = blk_next;
-      const float sc = sc_next;
-      if (j + 1 < n_kv) { blk_next = entry(j + 1); sc_next = scale_of(blk_next); }
-      if (lane == 0) ok = mbar_wait(&stg_empty[stage], phase ^ 1u, abort_flag, p.status, 0xA00);
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      if (!ok) break;
-      const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
-      if (lane < kPages) sScale[(j % kScRingTiles) * 8 + lane] = make_float2(sc, (float)scale_exponent(vs));
-      const uint32_t live = __popc(__ballot_sync(0xffffffffu, blk >= 0));
-      __syncwarp();
-      if (lane == 0) mbar_expect_tx(&stg_full[stage], live * (uint32_t)kPageBytes);
-      __syncwarp();
-      if (blk >= 0) {
-        const long long page = (long long)blk * p.Hkv + kvh;
-        uint8_t* dst = sStage + stage * kStageBytes + ((is_v ? kPages : 0) + pi) * kPageBytes;
-        sc_bulk(dst, (is_v ? p.v_cache : p.k_cache) + page * kPageBytes, kPageBytes, &stg_full[stage]);
-      }
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
-    }
-    if (!ok)
-      for (int i = 0; i < 64; ++i) __nanosleep(1000);
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ products (the whole warp, one elected lane issues)
-    constexpr uint32_t kIdescS = make_idesc(kScRows, kKv, 0u), kIdescO = make_idesc(kScRows, D, 0u);     // f16 x f16 -> f32
-    const uint32_t dQ = desc_low(sQ), dK = desc_low(sK), dV = desc_low(sV), dP = desc_low(sP);
-    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, site)); };
-    bool ok = wait(q_conv, 0, 0xA10);
-    auto issue_pv = [&](int i) -> bool {
-      if (!wait(v_ready, i & 1, 0xA13) || !wait(p_ready, i & 1, 0xA12)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < kKv / 16; ++ks)
-          umma_f16_lo(tO, dP + (ks >> 2) * (kScSub >> 4) + 2 * (ks & 3), dV + (ks >> 2) * (kVSub >> 4) + 2 * (ks & 3), kIdescO, (i > 0 || ks > 0) ? 1u : 0u);
-        umma_commit(pv_done);
-      }
-      __syncwarp();
-      return true;
-    };
-    for (int j = 0; j < n_kv && ok; ++j) {
-      const int sb = j & 1;
-      ok = wait(k_ready, j & 1, 0xA14) && wait(&s_free[sb], ((j >> 1) & 1) ^ 1u, 0xA15);
-      if (!ok) break;
-      tc_fence_after();
-      if (elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          umma_f16_lo(tS + sb * kKv, dQ + (ks >> 2) * (kScSub >> 4) + 2 * (ks & 3), dK + (ks >> 2) * (kKSub >> 4) + 2 * (ks & 3), kIdescS, ks > 0 ? 1u : 0u);
-        umma_commit(&s_full[sb]);
-        umma_commit(k_free);
-      }
-      __syncwarp();
-      if (j > 0) ok = issue_pv(j - 1);
-    }
-    if (ok && n_kv > 0) issue_pv(n_kv - 1);
-  } else if (warp < 6) {
-    // ------------------------------------------------------------------ converters
-    const int r = threadIdx.x - 64;
-    bool ok = true;
-    auto conv_k = [&](int j) -> bool {
-      const int s = j % kStages;
-      if (!mbar_wait(&stg_full[s], (j / kStages) & 1, abort_flag, p.status, 0xA21)) return false;
-      if (j > 0 && !mbar_wait(k_free, (j - 1) & 1, abort_flag, p.status, 0xA22)) return false;
-      const int kv0 = base + j * kKv;
-      const uint4* src = reinterpret_cast<const uint4*>(sStage + s * kStageBytes);
-      // consecutive threads take consecutive 16-byte pieces: piece i = token i / (D / 16), channels (i % (D / 16)) * 16 ..
-#pragma unroll
-      for (int k8 = 0; k8 < kKv * (D / 16) / 128; ++k8) {
-        const int i = k8 * 128 + r;
-        const int trow = i / (D / 16), c = i % (D / 16), tsw = trow & 7;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (kv0 + trow < L) sc_widen16(src[i], lo, hi);
-        uint8_t* rowp = sK + (c >> 2) * kKSub + (trow >> 3) * 1024 + tsw * 128;
-        const int ch = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = lo;
-        *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ tsw) << 4)) = hi;
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(k_ready);
-      return true;
-    };
-    auto conv_v = [&](int j) -> bool {
-      const int s = j % kStages;
-      const int kv0 = base + j * kKv;
-      const uint8_t* stg = sStage + s * kStageBytes + kPages * kPageBytes;
-      if (j > 0 && !mbar_wait(pv_done, (j - 1) & 1, abort_flag, p.status, 0xA23)) return false;
-#pragma unroll
-      for (int it = 0; it < D * kPages / 128; ++it) {
-        const int i = it * 128 + r;
-        const int pg = i / D, dim = i % D, sw = dim & 7;
-        const int t0 = kv0 + pg * kScPg;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (t0 < L) {
-          uint4 v = *reinterpret_cast<const uint4*>(stg + pg * kPageBytes + dim * kScPg);
-          if (t0 + kScPg > L) {                       // the sequence ends inside this page
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int left = min(max(L - t0 - 4 * q, 0), 4);
-              w[q] = left == 4 ? w[q] : (w[q] & ((1u << (8 * left)) - 1u));
-            }
-          }
-          sc_widen16(v, lo, hi);
-        }
-        uint8_t* rowp = sV + (pg >> 2) * kVSub + (dim >> 3) * 1024 + sw * 128;
-        const int ch = (pg & 3) * 2;
-        *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
-        *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) { mbar_arrive(v_ready); mbar_arrive(&stg_empty[s]); }
-      return true;
-    };
-    if (n_kv > 0) ok = conv_k(0);
-    for (int j = 0; j < n_kv && ok; ++j) {
-      if (j + 1 < n_kv) ok = conv_k(j + 1);
-      if (ok) ok = conv_v(j);
-    }
-  } else {
-    // ------------------------------------------------------------------ softmax, two threads a row
-    const int lane_group = warp & 3;                             // TMEM lanes 32 * (warp % 4) ..
-    const int half = (warp - 6) >> 2;
-    constexpr int HC = kKv / 2, HO = D / 2, HP = HC / kScPg;     // score columns, output columns and pages of a thread
-    const int col0 = half * HC, ocol0 = half * HO;
-    const int row = lane_group * 32 + lane;
-    const uint32_t t_lane = (uint32_t)(lane_group * 32) << 16;
-    bool ok = mbar_wait(q_full, 0, abort_flag, p.status, 0xA20);
-    if (ok) {
-      // Q to f16 in place: a row's largest magnitude to [2^13, 2^14), which keeps every bf16 number of it; two neighbouring lanes a row
-      const int i = threadIdx.x - 192, r = i >> 1, part = i & 1, rsw = r & 7;
-      constexpr int CH = D / 16;                                 // 16-byte chunks of a thread
-      uint8_t* rowp = sQ + (r >> 3) * 1024 + rsw * 128;
-      auto at = [&](int c) { return reinterpret_cast<uint4*>(rowp + (c >> 3) * kScSub + (((c & 7) ^ rsw) << 4)); };
-      float amax = 0.f;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const uint4 v = *at(2 * c + part);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-      }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      const int e2 = min(max(13 - ((int)(__float_as_uint(amax) >> 23) - 127), -100), 100);
-      const float up = exact_pow2(e2);
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        uint4* q4 = at(2 * c + part);
-        uint4 v = *q4;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-          w[e] = sc_h2(f.x * up, f.y * up);
-        }
-        *q4 = v;
-      }
-      if (part == 0) sRow[r] = p.scale_log2 * exact_pow2(-e2);
-      fence_proxy_async();
-    }
-    asm volatile("bar.sync 1, 256;\n" ::: "memory");             // the row factors, all softmax warps
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_conv);
-    const float rf = sRow[row];
-    int xn = 0;
-    // one value per thread to the other thread of its row, through a TMEM column of the row's lane; slots alternate
-    auto exchange = [&](float mine, float& other) -> bool {
-      const int par = xn & 1;
-      uint64_t* xb = &x_ready[par * 4 + lane_group];
-      tmem_st_32x32b_x1(tX + t_lane + par * 2 + half, __float_as_uint(mine));
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(xb);
-      if (!mbar_wait(xb, (xn >> 1) & 1, abort_flag, p.status, 0xA33)) return false;
-      tc_fence_after();
-      uint32_t o;
-      tmem_ld_32x32b_x1(tX + t_lane + par * 2 + (half ^ 1), o);
-      tmem_ld_wait();
-      other = __uint_as_float(o);
-      ++xn;
-      return true;
-    };
-    const int tok = q0 + row / G;
-    const int head = kvh * G + row % G;
-    const bool row_live = row < tok_per_tile * G && tok < q_len;
-    const int pos = ctx0 + tok;
-    const int lo_key = p.window > 0 ? pos - p.window + 1 : 0;
-    float m = -INFINITY, l = 0.f;
-    const int sw = row & 7;
-    uint8_t* prow = sP + (col0 >> 6) * kScSub + (row >> 3) * 1024 + sw * 128;
-    const int pch = (col0 >> 3) & 7;
-    for (int j = 0; j < n_kv && ok; ++j) {
-      const int sb = j & 1, kv0 = base + j * kKv;
-      if (!mbar_wait(&s_full[sb], (j >> 1) & 1, abort_flag, p.status, 0xA30)) { ok = false; break; }
-      tc_fence_after();
-      const int vis = row_live ? min(pos + 1, L) - kv0 : 0;      // columns [lo, vis) of this tile are visible
-      const int low = lo_key - kv0;
-      uint32_t sr[HC / 32][32];
-#pragma unroll
-      for (int c = 0; c < HC / 32; ++c) tmem_ld_32x32b_x32(tS + sb * kKv + t_lane + col0 + c * 32, sr[c]);
-      float2 ps[HP];                                              // score factor and value exponent of a page
-#pragma unroll
-      for (int q = 0; q < HP; ++q) {
-        const float2 x = sScale[(j % kScRingTiles) * 8 + half * HP + q];
-        ps[q] = make_float2(rf * x.x, x.y);
-      }
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[sb]);
-      const bool full = __all_sync(0xffffffffu, vis >= col0 + HC && low <= col0);
-      if (!full) {
-#pragma unroll
-        for (int c = 0; c < HC / 32; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (col0 + c * 32 + i >= vis || col0 + c * 32 + i < low) sr[c][i] = 0xff800000u;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int q = 0; q < HP; ++q) {
-        float a = -INFINITY, z = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          a = fmaxf(a, __uint_as_float(sr[q >> 1][(q & 1) * 16 + i]));
-          z = fmaxf(z, __uint_as_float(sr[q >> 1][(q & 1) * 16 + i + 1]));
-        }
-        mx = fmaxf(mx, fmaf(fmaxf(a, z), ps[q].x, ps[q].y));
-      }
-      float mx_other;
-      if (!exchange(mx, mx_other)) { ok = false; break; }
-      mx = fmaxf(mx, mx_other);
-      float m_new = m, alpha = 1.f;
-      if (mx > m + 8.f) {
-        m_new = mx;
-        alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - mx);
-      }
-      if (j > 0) {
-        if (!mbar_wait(pv_done, (j - 1) & 1, abort_flag, p.status, 0xA31)) { ok = false; break; }
-        tc_fence_after();
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-          for (int c = 0; c < HO / 32; ++c) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(tO + t_lane + ocol0 + c * 32, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-            tmem_st_32x32b_x32(tO + t_lane + ocol0 + c * 32, r);
-          }
-          tmem_st_wait();
-        }
-      }
-      const float mref = (m_new == -INFINITY) ? 0.f : m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int q = 0; q < HP; ++q) {
-        const float f = ps[q].x, add = ps[q].y - mref;
-        float s0 = 0.f, s1 = 0.f;
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float e0 = fast_exp2(fmaf(__uint_as_float(sr[q >> 1][(q & 1) * 16 + i]), f, add));
-          const float e1 = fast_exp2(fmaf(__uint_as_float(sr[q >> 1][(q & 1) * 16 + i + 1]), f, add));
-          s0 += e0;
-          s1 += e1;
-          w[i >> 1] = sc_h2(e0, e1);
-        }
-        sum = fmaf(s0 + s1, exact_pow2(-(int)ps[q].y), sum);
-        const int ch = pch + 2 * q;
-        *reinterpret_cast<uint4*>(prow + ((ch ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4*>(prow + (((ch + 1) ^ sw) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-      l = l * alpha + sum;
-      m = m_new;
-      fence_proxy_async();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready);
-    }
-    float l_other = 0.f;
-    if (ok && n_kv > 0) ok = exchange(l, l_other);
-    l += l_other;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const long long at = (long long)(q_row0 + tok) * p.Hq + head, at_part = ((long long)blockIdx.z * p.rows - p.first_row) * p.Hq + at;
-    if (ok && n_kv > 0) ok = mbar_wait(pv_done, (n_kv - 1) & 1, abort_flag, p.status, 0xA32);
-    if (__all_sync(0xffffffffu, ok)) {
-      tc_fence_after();
-      __nv_bfloat16* orow = p.out + (long long)(q_row0 + tok) * p.ldo + head * D + ocol0;
-      float* part = p.splits > 1 ? p.part_o + at_part * D + ocol0 : nullptr;
-#pragma unroll
-      for (int c = 0; c < HO / 32; ++c) {
-        uint32_t r[32];
-        if (n_kv > 0) {
-          tmem_ld_32x32b_x32(tO + t_lane + ocol0 + c * 32, r);
-          tmem_ld_wait();
-        } else {                                                 // no keys: zeros
-#pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0;
-        }
-        if (row_live) store_outputs(r, inv, orow + c * 32, part ? part + c * 32 : nullptr);
-      }
-      if (row_live && half == 0) {
-        if (part) p.part_ml[at_part] = make_float2(m, l);
-        else if (p.ml) p.ml[at] = make_float2(m == -INFINITY ? 0.f : m, inv);
-      }
-    }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
-  }
-}
-
 // ---------------------------------------------------------------------------------------------------------------- two tiles at a time
 // Heads of 64 and 128: two query tiles share every widened key tile, so that one tile's products run under the other one's softmax, and P
 // stays in TMEM.  Persistent, one CTA per SM; items (pair of query tiles, key head) with the most keys first.
@@ -623,6 +197,86 @@ ATLAS_DEVICE float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// A row's step over 64 score columns (a thread a row): their largest s + ev, then p = 2^(s + ev - m) as f16 over the first half of the columns
+// at tP.  f: (score factor, value exponent) of the four pages; columns [lo, hi) are visible.  The reference m moves only when a score passes
+// it by 2^8 (p stays inside f16), which is rare after a row's first columns; the output, where there is one, then moves with it, after
+// wait_output() has seen the last product that goes to it.  False: that wait ran out.
+template <int D, typename Wait>
+ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const float2 (&f)[4], bool whole, int hi, int lo, bool output, float& m, float& l,
+                               Wait wait_output) {
+  uint32_t v[2][32];
+  tmem_ld_32x32b_x32(tS, v[0]);
+  tmem_ld_32x32b_x32(tS + 32, v[1]);
+  tmem_ld_wait();
+  if (!whole) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t seen = bits_below(hi - k * 32) & ~bits_below(lo - k * 32);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[k][i] = (seen >> i) & 1u ? v[k][i] : 0xff800000u;
+    }
+  }
+  float mx[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t* u = &v[q >> 1][(q & 1) * 16];
+    float a = __uint_as_float(u[0]), z = __uint_as_float(u[1]);
+#pragma unroll
+    for (int i = 2; i < 14; i += 4) {
+      a = max3_nan(a, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+      z = max3_nan(z, __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
+    }
+    a = max3_nan(a, __uint_as_float(u[14]), __uint_as_float(u[15]));
+    mx[q] = fmaf(max3_nan(a, z, z), f[q].x, f[q].y);
+  }
+  const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+  if (__any_sync(0xffffffffu, !(top <= m + 8.f))) {               // NaN too: the row is NaN from here on
+    float alpha = 1.f;
+    if (!(top <= m + 8.f)) {
+      alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - top);
+      m = top;
+    }
+    l *= alpha;
+    if (output) {
+      if (!wait_output()) return false;
+      tc_fence_after();
+#pragma unroll 1
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t o[16];
+        tmem_ld_32x32b_x16(tO + k * 16, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+        tmem_st_32x32b_x16(tO + k * 16, o);
+      }
+    }
+  }
+  const float ref = (m == -INFINITY) ? 0.f : m;
+  uint32_t w[2][16];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t* u = &v[q >> 1][(q & 1) * 16];
+    const float add = f[q].y - ref;
+    const uint64_t f2 = pair2(f[q].x, f[q].x), a2 = pair2(add, add);
+    uint64_t s2 = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const uint64_t x2 = fma2(pair2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), f2, a2);
+      float2 e = unpair2(x2);
+      e.x = fast_exp2(e.x);
+      e.y = fast_exp2(e.y);
+      s2 = add2(s2, pair2(e.x, e.y));
+      w[q >> 1][(q & 1) * 8 + i / 2] = sc_h2(e.x, e.y);
+    }
+    const float2 s = unpair2(s2);
+    l = fmaf(s.x + s.y, exact_pow2(-(int)f[q].y), l);
+  }
+  tmem_st_32x32b_x16(tP, w[0]);
+  tmem_st_32x32b_x16(tP + 16, w[1]);
+  tmem_st_wait();
+  return true;
+}
+
 struct C2Item {
   int b, kvh, split, L, q_row0, q_len, q0, ctx0, page0;           // page0: the first of this share of the keys
   int n[2], n_kv;                                                 // key tiles of tile A, of tile B, of both
@@ -764,87 +418,16 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         const int hi = end - kv0, lo = start - kv0;
         const bool whole = __all_sync(0xffffffffu, hi >= kC2Kv && lo <= 0);
         const float2* sc = sScale + ((ring + j) % kC2Ring) * 8;
-        // ---- 64 columns at a time: their largest s + ev, then p = 2^(s + ev - m).  The reference m moves only when a score passes it by 2^8 (p
-        // stays inside f16), which is rare after a row's first columns; the output then moves with it (its last product was done before these scores
-        // began, and the second half waits for the first half's).  P takes half of the columns that its scores had.
+        // ---- 64 columns at a time; P takes half of the columns that its scores had
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {                               // no further unrolled: the roles' code shares one instruction cache
-          uint32_t v[2][32];
-          tmem_ld_32x32b_x32(tS + c * 64, v[0]);
-          tmem_ld_32x32b_x32(tS + c * 64 + 32, v[1]);
           float2 f[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) f[q] = sc[c * 4 + q];
-          tmem_ld_wait();
-          if (!whole) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t seen = bits_below(hi - c * 64 - k * 32) & ~bits_below(lo - c * 64 - k * 32);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[k][i] = (seen >> i) & 1u ? v[k][i] : 0xff800000u;
-            }
-          }
-          float mx[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t* u = &v[q >> 1][(q & 1) * 16];
-            float a = __uint_as_float(u[0]), z = __uint_as_float(u[1]);
-#pragma unroll
-            for (int i = 2; i < 14; i += 4) {
-              a = max3_nan(a, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
-              z = max3_nan(z, __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
-            }
-            a = max3_nan(a, __uint_as_float(u[14]), __uint_as_float(u[15]));
-            mx[q] = fmaf(max3_nan(a, z, z), f[q].x, f[q].y);
-          }
-          const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-          if (__any_sync(0xffffffffu, !(top <= m + 8.f))) {         // NaN too: the row is NaN from here on
-            float alpha = 1.f;
-            if (!(top <= m + 8.f)) {
-              alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - top);
-              m = top;
-            }
-            l *= alpha;
-            if (c == 1) {                                           // the first half's product is under way
-              ok = mbar_wait(&pv_half[x], (n_s - 1) & 1, abort_flag, p.status, 0xC04 + x);
-              if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-              tc_fence_after();
-            }
-            if (j > 0 || c == 1)
-#pragma unroll 1
-              for (int k = 0; k < D / 16; ++k) {
-                uint32_t o[16];
-                tmem_ld_32x32b_x16(tO + k * 16, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                tmem_st_32x32b_x16(tO + k * 16, o);
-              }
-            tmem_st_wait();
-          }
-          const float ref = (m == -INFINITY) ? 0.f : m;
-          uint32_t w[2][16];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t* u = &v[q >> 1][(q & 1) * 16];
-            const float add = f[q].y - ref;
-            const uint64_t f2 = pair2(f[q].x, f[q].x), a2 = pair2(add, add);
-            uint64_t s2 = 0;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const uint64_t x2 = fma2(pair2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), f2, a2);
-              float2 e = unpair2(x2);
-              e.x = fast_exp2(e.x);
-              e.y = fast_exp2(e.y);
-              s2 = add2(s2, pair2(e.x, e.y));
-              w[q >> 1][(q & 1) * 8 + i / 2] = sc_h2(e.x, e.y);
-            }
-            const float2 s = unpair2(s2);
-            l = fmaf(s.x + s.y, exact_pow2(-(int)f[q].y), l);
-          }
-          tmem_st_32x32b_x16(tS + c * 32, w[0]);
-          tmem_st_32x32b_x16(tS + c * 32 + 16, w[1]);
-          tmem_st_wait();
+          ok = softmax_step<D>(tS + c * 64, tS + c * 32, tO, f, whole, hi - c * 64, lo - c * 64, j > 0 || c == 1, m, l, [&] {
+            return c == 0 || (bool)__all_sync(0xffffffffu, mbar_wait(&pv_half[x], (n_s - 1) & 1, abort_flag, p.status, 0xC04 + x));
+          });
+          if (!ok) break;
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -1103,6 +686,294 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- heads of 256
+// One query tile a CTA: its output takes half of TMEM, the query rows a quarter (as operands of the scores they would be read from shared
+// memory once for 64 keys), two buffers of 64 score columns the rest.
+//   warps 0..3     query rows to TMEM, softmax, a thread a row; P goes over its scores
+//   warps 4..7     keys to bf16          warps 8..11   values to f16          (two buffers of each)
+//   warp 12        products: QK_{j+2} behind PV_j, whose P lies where the scores go
+//   warp 13        pages by bulk copies, their scales
+// Per 64 keys: products 512 clocks, exponentials 512, shared memory 1536 (512 for operands, 512 for the widened tiles, 512 for the codes).
+constexpr int kWideThreads = 448, kWideKv = 64, kWidePages = 4, kWideRing = 8;
+
+struct WideTile {
+  static constexpr int D = 256;
+  static constexpr int kSub = kWideKv * 128;                      // 64 tokens x 64 channels
+  static constexpr int kK = (D / 64) * kSub, kV = D * 128;        // 64 tokens x D channels, D channels x 64 tokens
+  static constexpr int kStage = kWideKv * D;
+  static constexpr int kSmem = 2 * (kK + kV + 2 * kStage) + kWideRing * kWidePages * 8 + 256 + 1024;
+};
+
+__global__ void __launch_bounds__(kWideThreads, 1)
+scaled_chunk_wide_kernel(const ScChunkParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using Tile = WideTile;
+  constexpr int D = Tile::D;
+  uint8_t* sK = smem;                                             // two buffers: D / 64 sub-tiles [64 tokens][64 channels]
+  uint8_t* sV = sK + 2 * Tile::kK;                                // two buffers: [D channels][64 tokens]
+  uint8_t* sStK = sV + 2 * Tile::kV;                              // two stages of pages as they come, keys and values
+  uint8_t* sStV = sStK + 2 * Tile::kStage;
+  float2* sScale = reinterpret_cast<float2*>(sStV + 2 * Tile::kStage);      // [kWideRing][4] (score factor, value exponent) of a page
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + kWideRing * kWidePages);
+  uint64_t* stage_full = bars;                                    // [keys, values][2] pages have come
+  uint64_t* stage_free = bars + 4;                                // [keys, values][2] 4 warps
+  uint64_t* k_full = bars + 8;                                    // [2] 4 warps
+  uint64_t* k_free = bars + 10;                                   // [2] QK
+  uint64_t* v_full = bars + 12;                                   // [2] 4 warps
+  uint64_t* v_free = bars + 14;                                   // [2] PV
+  uint64_t* s_full = bars + 16;                                   // [2]
+  uint64_t* p_ready = bars + 18;                                  // [2] 4 warps
+  uint64_t* pv_done = bars + 20;                                  // [2]
+  uint64_t* q_ready = bars + 22;                                  // 4 warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.G, toks = kScRows / G;
+  const int b = p.tile_seq[blockIdx.x], q0 = p.tile_q0[blockIdx.x], kvh = blockIdx.y, split = blockIdx.z;
+  const int L = min(p.seq_lens[b], p.bt_cols * kScPg);
+  const int q_row0 = p.query_start_loc[b], q_len = p.query_start_loc[b + 1] - q_row0;
+  const int ctx0 = L - q_len;                                     // position of the chunk's first row
+  const int kv_hi = min(L, ctx0 + min(q0 + toks, q_len));         // keys [.., kv_hi)
+  const int first_page = p.window > 0 ? max(ctx0 + q0 - p.window + 1, 0) / kScPg : 0;
+  const int all_kv = max((kv_hi - first_page * kScPg + kWideKv - 1) / kWideKv, 0), share = (all_kv + p.splits - 1) / p.splits;
+  const int page0 = first_page + split * share * kWidePages;
+  const int n_kv = min(max(all_kv - split * share, 0), share);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 4; ++s) { mbar_init(&stage_full[s], 1); mbar_init(&stage_free[s], 4); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 4); mbar_init(&k_free[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_free[s], 1);
+      mbar_init(&s_full[s], 1); mbar_init(&p_ready[s], 4); mbar_init(&pv_done[s], 1);
+    }
+    mbar_init(q_ready, 4);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 12) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;                               // scores (two times 64 columns), query rows (128), output (256)
+
+  if (warp < 4) {
+    // ------------------------------------------------------------------ softmax
+    const int row = warp * 32 + lane;
+    const uint32_t t_lane = (uint32_t)(warp * 32) << 16;
+    const uint32_t tQ = tmem + 128 + t_lane, tO = tmem + 256 + t_lane;
+    const int tok = q0 + row / G, head = kvh * G + row % G;
+    const bool live = row < toks * G && tok < q_len;
+    const __nv_bfloat16* q = p.q + (long long)(q_row0 + tok) * p.ldq + head * D;
+#pragma unroll 2
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t v[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (live) x = *reinterpret_cast<const uint4*>(q + c * 32 + i * 8);
+        v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+      }
+      tmem_st_32x32b_x16(tQ + c * 16, v);
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_ready);
+    // keys [start, end) are visible; rows that are not there see all, so that their warp need not mask, and are not stored
+    const int pos = ctx0 + tok;
+    const int end = live ? min(pos + 1, L) : 1 << 30;
+    const int start = live && p.window > 0 ? pos - p.window + 1 : 0;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+#pragma unroll 1
+    for (int j = 0; j < n_kv; ++j) {
+      const int sb = j & 1;
+      ok = mbar_wait(&s_full[sb], (j >> 1) & 1, abort_flag, p.status, 0xA00);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc_fence_after();
+      const int kv0 = (page0 + j * kWidePages) * kScPg;
+      const int hi = end - kv0, lo = start - kv0;
+      const bool whole = __all_sync(0xffffffffu, hi >= kWideKv && lo <= 0);
+      float2 f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = sScale[(j % kWideRing) * kWidePages + i];
+      const uint32_t tS = tmem + sb * kWideKv + t_lane;
+      ok = softmax_step<D>(tS, tS, tO, f, whole, hi, lo, j > 0, m, l, [&] {
+        return (bool)__all_sync(0xffffffffu, mbar_wait(&pv_done[sb ^ 1], ((j - 1) >> 1) & 1, abort_flag, p.status, 0xA01));
+      });
+      if (!ok) break;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[sb]);
+    }
+    if (ok && n_kv > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(n_kv - 1) & 1], ((n_kv - 1) >> 1) & 1, abort_flag, p.status, 0xA02));
+    if (ok) {
+      // ---- o / l, or this share's o and l
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const long long at = (long long)(q_row0 + tok) * p.Hq + head, at_part = ((long long)split * p.rows - p.first_row) * p.Hq + at;
+      __nv_bfloat16* out = p.out + (long long)(q_row0 + tok) * p.ldo + head * D;
+      float* part = p.splits > 1 ? p.part_o + at_part * D : nullptr;
+      uint32_t r[2][32];
+      if (n_kv > 0) {
+        tc_fence_after();
+        tmem_ld_32x32b_x32(tO, r[0]);
+#pragma unroll 2
+        for (int c = 0; c < D / 32; ++c) {
+          tmem_ld_wait();
+          if (c + 1 < D / 32) tmem_ld_32x32b_x32(tO + (c + 1) * 32, r[(c + 1) & 1]);
+          if (live) store_outputs(r[c & 1], inv, out + c * 32, part ? part + c * 32 : nullptr);
+        }
+      } else if (live) {                                          // no keys: zeros
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[0][i] = 0;
+        for (int c = 0; c < D; c += 32) store_outputs(r[0], inv, out + c, part ? part + c : nullptr);
+      }
+      if (live) {
+        if (part) p.part_ml[at_part] = make_float2(m, l);
+        else if (p.ml) p.ml[at] = make_float2(m == -INFINITY ? 0.f : m, inv);
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ keys.  Eight neighbouring lanes take 64 bytes each of two rows, from
+    // different sub-tiles: no two of their loads, and none of their stores, fall into the same banks.
+    const int i8 = (threadIdx.x - 128) >> 5, sub = (lane >> 2) & 3, par = ((lane >> 2) & 1) ^ (lane >> 4), ch = (lane & 3) * 2;
+    for (int j = 0; j < n_kv; ++j) {
+      const int s = j & 1;
+      const bool ok = mbar_wait(&stage_full[s], (j >> 1) & 1, abort_flag, p.status, 0xA10) &&
+                      mbar_wait(&k_free[s], ((j >> 1) & 1) ^ 1u, abort_flag, p.status, 0xA11);
+      if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll 4
+      for (int k = 0; k < kWideKv / 8; ++k) {
+        const int trow = (k * 4 + i8) * 2 + par, tsw = trow & 7;
+        uint4 lo, hi;
+        sc_widen16(*reinterpret_cast<const uint4*>(sStK + s * Tile::kStage + trow * D + sub * 64 + (lane & 3) * 16), lo, hi);
+        uint8_t* rowp = sK + s * Tile::kK + sub * Tile::kSub + trow * 128;
+        *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = make_uint4(h2_to_bf2(lo.x), h2_to_bf2(lo.y), h2_to_bf2(lo.z), h2_to_bf2(lo.w));
+        *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ tsw) << 4)) = make_uint4(h2_to_bf2(hi.x), h2_to_bf2(hi.y), h2_to_bf2(hi.z), h2_to_bf2(hi.w));
+      }
+      fence_proxy_async();                                        // the tile for the products, and the pages read before they are copied over
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&k_full[s]); mbar_arrive(&stage_free[s]); }
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ values
+    const int r = threadIdx.x - 256;
+    for (int j = 0; j < n_kv; ++j) {
+      const int s = j & 1;
+      const bool ok = mbar_wait(&stage_full[2 + s], (j >> 1) & 1, abort_flag, p.status, 0xA12) &&
+                      mbar_wait(&v_free[s], ((j >> 1) & 1) ^ 1u, abort_flag, p.status, 0xA13);
+      if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll 4
+      for (int k = 0; k < kWidePages * D / 128; ++k) {
+        const int i = k * 128 + r, pg = i / D, dim = i % D, sw = dim & 7, ch = pg * 2;
+        const int left = L - (page0 + j * kWidePages + pg) * kScPg;       // tokens of the page; the others are cleared
+        uint4 v = reinterpret_cast<const uint4*>(sStV + s * Tile::kStage)[i];
+        if (left < kScPg) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int there = min(max(left - 4 * q, 0), 4);
+            w[q] = there == 4 ? w[q] : (w[q] & ((1u << (8 * there)) - 1u));
+          }
+        }
+        uint4 lo, hi;
+        sc_widen16(v, lo, hi);
+        uint8_t* rowp = sV + s * Tile::kV + dim * 128;
+        *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
+        *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&v_full[s]); mbar_arrive(&stage_free[2 + s]); }
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------------------ products (the whole warp, one elected lane issues)
+    constexpr uint32_t kIdescS = make_idesc(kScRows, kWideKv, 1u), kIdescO = make_idesc(kScRows, D, 0u);      // bf16 scores, f16 outputs
+    const uint32_t dK = desc_low(sK), dV = desc_low(sV), tQ = tmem + 128, tO = tmem + 256;
+    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, site)); };
+    auto score = [&](int j) -> bool {
+      if (!wait(&k_full[j & 1], (j >> 1) & 1, 0xA20)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          umma_f16_ta(tmem + (j & 1) * kWideKv, tQ + ks * 8, dK + (j & 1) * (Tile::kK >> 4) + (ks >> 2) * (Tile::kSub >> 4) + 2 * (ks & 3), kIdescS,
+                      ks > 0 ? 1u : 0u);
+        umma_commit(&s_full[j & 1]);
+        umma_commit(&k_free[j & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = wait(q_ready, 0, 0xA21);
+    for (int j = 0; j < min(n_kv, 2) && ok; ++j) ok = score(j);
+    for (int j = 0; j < n_kv && ok; ++j) {
+      ok = wait(&v_full[j & 1], (j >> 1) & 1, 0xA22) && wait(&p_ready[j & 1], (j >> 1) & 1, 0xA23);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < kWideKv / 16; ++ks)
+          umma_f16_ta(tO, tmem + (j & 1) * kWideKv + ks * 8, dV + (j & 1) * (Tile::kV >> 4) + 2 * ks, kIdescO, (j > 0 || ks > 0) ? 1u : 0u);
+        umma_commit(&pv_done[j & 1]);
+        umma_commit(&v_free[j & 1]);
+      }
+      __syncwarp();
+      if (j + 2 < n_kv) ok = wait(&pv_done[j & 1], (j >> 1) & 1, 0xA24) && score(j + 2);
+    }
+  } else {
+    // ------------------------------------------------------------------ pages: lanes 0..3 keys, 8..11 values, entries and scales two tiles ahead
+    const bool is_v = (lane & 8) != 0;
+    const int n_pages = (L + kScPg - 1) / kScPg;
+    const int* bt = p.block_tables + (long long)b * p.bt_ld;
+    auto entry = [&](int j) {                                     // -1: behind the end or outside of the pool
+      const int pg = page0 + j * kWidePages + (lane & 7);
+      return lane < 16 && (lane & 7) < kWidePages && j < n_kv && pg < n_pages ? bt[pg] : -1;
+    };
+    auto scale_of = [&](int blk) {
+      if ((unsigned)blk >= (unsigned)p.num_pages) return 1.f;
+      return is_v ? p.v_scale[blk * p.vs_ld + kvh * p.vs_h] : p.k_scale[blk * p.ks_ld + kvh * p.ks_h];
+    };
+    int blk = entry(0), blk1 = entry(1);
+    float sc = scale_of(blk);
+    bool ok = true;
+    for (int j = 0; j < n_kv; ++j) {
+      const int blk2 = entry(j + 2), s = j & 1;
+      const float sc1 = scale_of(blk1);
+      const bool live = (unsigned)blk < (unsigned)p.num_pages;
+      const uint32_t pages = __ballot_sync(0xffffffffu, live);
+      const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
+      const long long at = ((long long)blk * p.Hkv + kvh) * (kScPg * D);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        ok = mbar_wait(&stage_free[2 * w + s], ((j >> 1) & 1) ^ 1u, abort_flag, p.status, 0xA30 + w);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (w == 0) {                                             // tile j - kWideRing is done: its keys left this stage long ago
+          if (lane < kWidePages) sScale[(j % kWideRing) * kWidePages + lane] = make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
+          __syncwarp();
+        }
+        if (lane == 0) mbar_expect_tx(&stage_full[2 * w + s], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
+        __syncwarp();
+        if (live && is_v == (w == 1))
+          sc_bulk((w ? sStV : sStK) + s * Tile::kStage + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &stage_full[2 * w + s]);
+      }
+      if (!ok) break;
+      blk = blk1; blk1 = blk2;
+      sc = sc1;
+    }
+    if (!ok)
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------- weights
 constexpr int kSwThreads = 320;        // producer, issuer, eight warps that add
 constexpr int kSwStages = 2;           // query tiles in shared memory, score buffers in TMEM
@@ -1350,10 +1221,9 @@ int launch_weigh(void (*kern)(CUtensorMap, ScWeighParams), int smem, unsigned bl
   return 0;
 }
 
-template <typename Kern, typename P>
-int launch_tiles(Kern kern, int smem, dim3 grid, int threads, const CUtensorMap& tq, const P& p, cudaStream_t st) {
-  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem) != cudaSuccess) return -20;
-  kern<<<grid, threads, smem, st>>>(tq, p);
+int launch_wide(dim3 grid, const ScChunkParams& p, cudaStream_t st) {
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(scaled_chunk_wide_kernel), WideTile::kSmem) != cudaSuccess) return -20;
+  scaled_chunk_wide_kernel<<<grid, kWideThreads, WideTile::kSmem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -20;
 }
 
@@ -1387,12 +1257,11 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
   const float scale_log2 = (float)(r.scale * 1.4426950408889634);
   status_t* status = (status_t*)r.status;
   cudaStream_t st = (cudaStream_t)r.stream;
-  ScChunkParams p{(__nv_bfloat16*)r.out, r.ldo, (const uint8_t*)r.k_cache, (const uint8_t*)r.v_cache, r.ks, r.vs, r.ks_ld, r.vs_ld, (int)r.ks_h,
+  ScChunkParams p{(const __nv_bfloat16*)r.q, r.ldq, (__nv_bfloat16*)r.out, r.ldo, (const uint8_t*)r.k_cache, (const uint8_t*)r.v_cache, r.ks, r.vs, r.ks_ld, r.vs_ld, (int)r.ks_h,
                   (int)r.vs_h, r.tables, (int)r.bt_ld, (int)r.bt_cols, r.seq_lens, r.starts, r.tile_seq, r.tile_q0, scale_log2, Hq, Hkv, G,
                   (int)r.window, (int)r.num_pages, reinterpret_cast<float2*>(r.ml), (int)r.splits, (int)r.first_row,
                   (int)(r.total_tokens - r.first_row), r.part_o,
                   reinterpret_cast<float2*>(r.part_ml), status};
-  const dim3 grid((unsigned)r.tiles, Hkv, (unsigned)r.splits);
   int rc;
   if (D <= 128) {
     const long long items = r.tiles * Hkv * r.splits;
@@ -1400,7 +1269,7 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
     const int blocks = (int)(items < r.sms ? items : r.sms);
     if (D == 64) rc = launch_pairs(scaled_chunk2_kernel<64>, C2Tile<64>::kSmem, blocks, tq, p, (int)items, st);
     else rc = launch_pairs(scaled_chunk2_kernel<128>, C2Tile<128>::kSmem, blocks, tq, p, (int)items, st);
-  } else rc = launch_tiles(scaled_chunk_kernel<256>, ScTile<256>::kSmem, grid, kScThreads, tq, p, st);
+  } else rc = launch_wide(dim3((unsigned)r.tiles, Hkv, (unsigned)r.splits), p, st);
   if (rc) return rc;
   if (r.splits > 1) {
     const unsigned blocks = (unsigned)(((r.total_tokens - r.first_row) * Hq + 7) / 8);
