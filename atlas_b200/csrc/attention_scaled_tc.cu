@@ -358,15 +358,14 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   uint64_t* k_free = bars + 4;                                    // [2] QK of both tiles
   uint64_t* v_full = bars + 6;                                    // [2] 4 warps
   uint64_t* v_free = bars + 8;                                    // [2] PV of both tiles
-  uint64_t* s_full = bars + 10;                                   // [tile]
+  uint64_t* s_full = bars + 10;                                   // [tile][half]
   uint64_t* p_ready = bars + 22;                                  // [tile][half] 4 warps
   uint64_t* pv_done = bars + 14;                                  // [tile]
   uint64_t* o_free = bars + 16;                                   // [tile] 4 warps have read the item's output
   uint64_t* ks_full = bars + 18;                                  // [keys, values] pages have come
   uint64_t* ks_free = bars + 20;                                  // [keys, values] 4 warps
   uint64_t* pv_half = bars + 26;                                  // [tile] the first half's product
-  uint64_t* stagger = bars + 28;                                  // 4 warps of tile A, once an item
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -374,12 +373,12 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) { mbar_init(&ks_full[s], 1); mbar_init(&ks_free[s], 4); }
-    mbar_init(q_full, 1); mbar_init(q_free, 2); mbar_init(stagger, 4);
+    mbar_init(q_full, 1); mbar_init(q_free, 2);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 4); mbar_init(&k_free[s], 2); mbar_init(&v_full[s], 4); mbar_init(&v_free[s], 2);
-      mbar_init(&s_full[s], 1); mbar_init(&pv_done[s], 1); mbar_init(&pv_half[s], 1); mbar_init(&o_free[s], 4);
+      mbar_init(&pv_done[s], 1); mbar_init(&pv_half[s], 1); mbar_init(&o_free[s], 4);
     }
-    for (int s = 0; s < 4; ++s) mbar_init(&p_ready[s], 4);
+    for (int s = 0; s < 4; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_ready[s], 4); }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -410,10 +409,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
       const int start = live && p.window > 0 ? pos - p.window + 1 : 0;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j) {
-        ok = mbar_wait(&s_full[x], n_s & 1, abort_flag, p.status, 0xC00 + x);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         ++n_s;
-        tc_fence_after();
         const int kv0 = (m_.page0 + j * kC2Pages) * kScPg;
         const int hi = end - kv0, lo = start - kv0;
         const bool whole = __all_sync(0xffffffffu, hi >= kC2Kv && lo <= 0);
@@ -421,19 +417,19 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         // ---- 64 columns at a time; P takes half of the columns that its scores had
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {                               // no further unrolled: the roles' code shares one instruction cache
+          ok = mbar_wait(&s_full[2 * x + c], (n_s - 1) & 1, abort_flag, p.status, 0xC00 + x);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          tc_fence_after();
           float2 f[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) f[q] = sc[c * 4 + q];
-          ok = softmax_step<D>(tS + c * 64, tS + c * 32, tO, f, whole, hi - c * 64, lo - c * 64, j > 0 || c == 1, m, l, [&] {
-            return c == 0 || (bool)__all_sync(0xffffffffu, mbar_wait(&pv_half[x], (n_s - 1) & 1, abort_flag, p.status, 0xC04 + x));
+          ok = softmax_step<D>(tS + c * 64, tS + c * 64, tO, f, whole, hi - c * 64, lo - c * 64, j > 0 || c == 1, m, l, [&] {
+            return (bool)__all_sync(0xffffffffu, mbar_wait(c ? &pv_half[x] : &pv_done[x], (n_s - 2 + c) & 1, abort_flag, p.status, 0xC04 + x));
           });
           if (!ok) break;
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&p_ready[2 * x + c]);                       // the first half's product runs under the second half
-            if (x == 0 && c == 0 && j == 0) mbar_arrive(stagger);
-          }
+          if (lane == 0) mbar_arrive(&p_ready[2 * x + c]);          // the first half's product runs under the second half
         }
         if (!ok) break;
       }
@@ -489,9 +485,12 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
 #pragma unroll 4
         for (int k = 0; k < kPer; ++k) {
-          const int i = k * 128 + r, in = i % D, trow = (i / D) * kScPg + in / (D / 16), c = in % (D / 16), tsw = trow & 7;
+          // eight neighbouring lanes take 64 bytes each of two rows, with heads of 128 from different sub-tiles: no two of their loads or
+          // stores fall into the same banks
+          const int i = k * 128 + r, trow = D == 128 ? k * kScPg + (r >> 5) * 4 + (r >> 4 & 1) * 2 + ((r >> 2 ^ r >> 3) & 1) : i / 4;
+          const int c = D == 128 ? r & 7 : i % 4, tsw = trow & 7;
           uint4 lo, hi;
-          sc_widen16(reinterpret_cast<const uint4*>(sStK)[i], lo, hi);
+          sc_widen16(reinterpret_cast<const uint4*>(sStK)[trow * (D / 16) + c], lo, hi);
           uint8_t* rowp = sK + s * Tile::kK + (c >> 2) * kScSub + (trow >> 3) * 1024 + tsw * 128;
           const int ch = (c & 3) * 2;
           *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = make_uint4(h2_to_bf2(lo.x), h2_to_bf2(lo.y), h2_to_bf2(lo.z), h2_to_bf2(lo.w));
@@ -576,28 +575,30 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   } else if (warp == 12 || warp == 14) {
     // ------------------------------------------------------------------ products of tile x, each tile at its own pace.  The whole warp walks the
     // list and one elected lane issues: descriptors stay in uniform registers so (under a lane's branch an MMA took 110 clocks to issue).
-    constexpr uint32_t kIdescS = make_idesc(kScRows, kC2Kv, 1u), kIdescO = make_idesc(kScRows, D, 0u);      // bf16 scores, f16 outputs
+    constexpr uint32_t kIdescS = make_idesc(kScRows, 64, 1u), kIdescO = make_idesc(kScRows, D, 0u);      // bf16 scores, f16 outputs
     const int x = (warp - 12) >> 1;
     const uint32_t dQ = desc_low(sQ + x * Tile::kQ), dK = desc_low(sK), dV = desc_low(sV);
     const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * D;
-    uint32_t n_t = 0, n_i = 0, pvs = 0, outs = 0, staggers = 0;   // key tiles, items, PV products, items with output, items of tile A
+    uint32_t n_t = 0, n_i = 0, pvs = 0, outs = 0;   // key tiles, items, PV products, items with output
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, site + x)); };
     auto full = [&](uint64_t* bar, uint32_t t, uint32_t site) { return wait(bar + (t & 1), (t >> 1) & 1, site); };
-    // scores with key tile t; the PV product that read P out of the same columns is done
-    auto score = [&](uint32_t t, bool last) -> bool {
-      if (pvs > 0 && !wait(&pv_done[x], (pvs - 1) & 1, 0xC20)) return false;
+    // scores with half of key tile t; the PV product that read P out of the same columns is done
+    auto score = [&](uint32_t t, int half, bool last) -> bool {
+      if (pvs > 0 && !wait(half ? &pv_done[x] : &pv_half[x], (pvs - 1) & 1, 0xC20)) return false;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t bd = dK + (t & 1) * (Tile::kK >> 4);
+        const uint32_t bd = dK + (t & 1) * (Tile::kK >> 4) + half * (64 * 128 >> 4);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint32_t at = (ks >> 2) * (kScSub >> 4) + 2 * (ks & 3);
-          umma_f16_lo(tS, dQ + at, bd + at, kIdescS, ks > 0 ? 1u : 0u);
+          umma_f16_lo(tS + half * 64, dQ + at, bd + at, kIdescS, ks > 0 ? 1u : 0u);
         }
-        umma_commit(&s_full[x]);
-        umma_commit(&k_free[t & 1]);
-        if (last) umma_commit(q_free);
+        umma_commit(&s_full[2 * x + half]);
+        if (half) {
+          umma_commit(&k_free[t & 1]);
+          if (last) umma_commit(q_free);
+        }
       }
       __syncwarp();
       return true;
@@ -609,18 +610,13 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     C2Walk walk(p, items);
     for (; walk.more() && ok; ++n_i) {
       const C2Item nxt = walk.next();
-      const int n = __shfl_sync(0xffffffffu, nxt.n[x], 0), n_kv = __shfl_sync(0xffffffffu, nxt.n_kv, 0), n_of_a = nxt.n[0];
+      const int n = __shfl_sync(0xffffffffu, nxt.n[x], 0), n_kv = __shfl_sync(0xffffffffu, nxt.n_kv, 0);
       ok = wait(q_full, n_i & 1, 0xC22);
       if (!ok) break;
       if (n == 0 && lane == 0) mbar_arrive(q_free);
       if (n_kv == 0) continue;
       ok = full(k_full, n_t, 0xC24);
-      // tile B begins when tile A has half of its first P: the two then take turns at products and exponentials (in step, both waited for the
-      // products and the special-function units idled for a third of the time)
-      const int n_a = __shfl_sync(0xffffffffu, n_of_a, 0);
-      if (x == 1 && n > 0 && n_a > 0) ok = ok && wait(stagger, staggers & 1, 0xC2E);
-      if (n_a > 0) ++staggers;
-      if (ok && n > 0) ok = score(n_t, n == 1);
+      if (ok && n > 0) ok = score(n_t, 0, false) && score(n_t, 1, n == 1);
       else if (ok) skip(k_free, n_t);
       for (int j = 0; j < n_kv && ok; ++j, ++n_t) {
         // what the next products need besides P, before P is waited for
@@ -629,13 +625,13 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         if (j < n) {
           if (j == 0 && outs > 0) ok = wait(&o_free[x], (outs - 1) & 1, 0xC28);
           for (int half = 0; half < 2 && ok; ++half) {
-            ok = wait(&p_ready[2 * x + half], pvs & 1, 0xC2A);
+            ok = wait(&p_ready[2 * x + half], (pvs - half) & 1, 0xC2A);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
               const uint32_t bd = dV + (n_t & 1) * (Tile::kV >> 4) + half * (D * 128 >> 4);
 #pragma unroll
-              for (int ks = 0; ks < kC2Kv / 32; ++ks) umma_f16_ta(tO, tS + half * 32 + ks * 8, bd + 2 * ks, kIdescO, (j > 0 || half > 0 || ks > 0) ? 1u : 0u);
+              for (int ks = 0; ks < kC2Kv / 32; ++ks) umma_f16_ta(tO, tS + half * 64 + ks * 8, bd + 2 * ks, kIdescO, (j > 0 || half > 0 || ks > 0) ? 1u : 0u);
               if (half == 0) {
                 umma_commit(&pv_half[x]);
               } else {
@@ -644,17 +640,15 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
               }
             }
             __syncwarp();
+            if (half == 0) ++pvs;
+            if (j + 1 < n) ok = score(n_t + 1, half, j + 2 == n);
           }
           if (!ok) break;
-          ++pvs;
           if (j + 1 == n) ++outs;
         } else {
           skip(v_free, n_t);
         }
-        if (j + 1 < n_kv) {
-          if (j + 1 < n) ok = score(n_t + 1, j + 2 == n);
-          else skip(k_free, n_t + 1);
-        }
+        if (j + 1 < n_kv && j + 1 >= n) skip(k_free, n_t + 1);
       }
     }
   } else if (warp == 13) {
