@@ -77,21 +77,72 @@ ATLAS_DEVICE uint32_t h2_to_bf2(uint32_t v) {      // e4m3 numbers: exact in bot
 ATLAS_DEVICE int scale_exponent(float s) { return (int)((__float_as_uint(s) >> 23) & 255u) - 127; }
 ATLAS_DEVICE float exact_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// 32 output numbers of a row: times 1 / l to bf16, or as they are to a part of the row
-ATLAS_DEVICE void store_outputs(const uint32_t (&v)[32], float inv, __nv_bfloat16* out, float* part) {
-  if (part) {
+// Column of TMEM that holds channel `d` of the outputs (rows of the value tiles go there): of 32 channels 8 i + 2 k + e, column 8 k + 2 i + e.
+// A load of 16 lanes x 256 bits gives thread 4 r + i columns 8 k + 2 i and one more of rows r and r + 8: eight channels in a row.
+ATLAS_DEVICE int output_column(int d) { return (d & ~31) | (d & 6) << 2 | (d >> 2 & 6) | (d & 1); }
+// Channel of 32 for a lane that widens values: eight neighbouring lanes have channels, and output columns, that differ modulo 8 (no two of them
+// in the same banks, neither reading nor writing).
+ATLAS_DEVICE int value_piece(int r) {
+  const int i = r >> 1 & 3, k = (i + (r >> 3)) & 3;
+  return (r & ~31) | 8 * i + 2 * k | (r & 1);
+}
+ATLAS_DEVICE void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+      "%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// A warp's 32 rows of outputs, times 1 / l to bf16, or as they are to a part of the row.  at: where this lane's row begins, -1 where it is not
+// stored; done() when TMEM has been read.  A store writes 64 bytes of eight rows (a row a lane, 16 bytes of 32 rows, took 4500 clocks for two
+// tiles).
+template <int D, typename Done>
+ATLAS_DEVICE void store_outputs(uint32_t tO, bool zeros, float inv, long long at, __nv_bfloat16* out, float* part, Done done) {
+  const int lane = threadIdx.x & 31, ch = (lane & 3) * 8;
+#pragma unroll 1
+  for (int g = 0; g < 2; ++g) {
+    float f[2];
+    long long to[2];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(part + 4 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    return;
-  }
+    for (int h = 0; h < 2; ++h) {
+      f[h] = __shfl_sync(0xffffffffu, inv, g * 16 + h * 8 + (lane >> 2));
+      to[h] = __shfl_sync(0xffffffffu, at, g * 16 + h * 8 + (lane >> 2));
+    }
+#pragma unroll 1
+    for (int c = 0; c < D; c += 64) {
+      uint32_t r[32];
+      if (zeros) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint4 o;
-    o.x = pack_bf16x2(__uint_as_float(v[q * 8 + 0]) * inv, __uint_as_float(v[q * 8 + 1]) * inv);
-    o.y = pack_bf16x2(__uint_as_float(v[q * 8 + 2]) * inv, __uint_as_float(v[q * 8 + 3]) * inv);
-    o.z = pack_bf16x2(__uint_as_float(v[q * 8 + 4]) * inv, __uint_as_float(v[q * 8 + 5]) * inv);
-    o.w = pack_bf16x2(__uint_as_float(v[q * 8 + 6]) * inv, __uint_as_float(v[q * 8 + 7]) * inv);
-    *reinterpret_cast<uint4*>(out + q * 8) = o;
+        for (int i = 0; i < 32; ++i) r[i] = 0;
+      } else {
+        tmem_ld_16x256b_x8(tO + (g << 20) + c, r);
+        tmem_ld_wait();
+      }
+      if (g == 1 && c + 64 == D) done();
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (to[h] < 0) continue;
+          const uint32_t* v = r + 16 * u + 2 * h;
+          if (part) {
+            float* o = part + to[h] + c + 32 * u + ch;
+            *reinterpret_cast<uint4*>(o) = make_uint4(v[0], v[1], v[4], v[5]);
+            *reinterpret_cast<uint4*>(o + 4) = make_uint4(v[8], v[9], v[12], v[13]);
+          } else {
+            uint4 o;
+            o.x = pack_bf16x2(__uint_as_float(v[0]) * f[h], __uint_as_float(v[1]) * f[h]);
+            o.y = pack_bf16x2(__uint_as_float(v[4]) * f[h], __uint_as_float(v[5]) * f[h]);
+            o.z = pack_bf16x2(__uint_as_float(v[8]) * f[h], __uint_as_float(v[9]) * f[h]);
+            o.w = pack_bf16x2(__uint_as_float(v[12]) * f[h], __uint_as_float(v[13]) * f[h]);
+            *reinterpret_cast<uint4*>(out + to[h] + c + 32 * u + ch) = o;
+          }
+        }
+    }
   }
 }
 
@@ -149,7 +200,7 @@ struct C2Tile {
   static constexpr int kK = (D / 64) * kScSub;                    // 128 keys
   static constexpr int kV = 2 * D * 128;                          // D channels x 128 tokens
   static constexpr int kStage = kC2Kv * D;                        // the pages of a key tile
-  static constexpr int kSmem = 2 * (kQ + kK + kV) + 2 * kStage + kC2Ring * 64 + 256 + 1024;      // at most 227 KB
+  static constexpr int kSmem = 2 * (kQ + kK + kV) + 2 * kStage + kC2Ring * 64 + 512 + 1024;      // at most 227 KB
 };
 
 // A from TMEM: a row a lane, two 16-bit numbers a column
@@ -277,67 +328,41 @@ ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const floa
   return true;
 }
 
-struct C2Item {
-  int b, kvh, split, L, q_row0, q_len, q0, ctx0, page0;           // page0: the first of this share of the keys
+struct alignas(16) C2Item {
+  int b, kvh, split, L, q_row0, q_len, q0, ctx0, page0;           // b < 0: no more; page0: the first of this share of the keys
   int n[2], n_kv;                                                 // key tiles of tile A, of tile B, of both
 };
 // Item of a CTA in round `rd`: the rounds go to and fro over the CTAs, so that the ones with the longest item of a round get the shortest of
 // the next (2 x 3001 ragged rows: 47 key tiles on the busiest CTA of 44 on average, 56 with rounds all one way).
-ATLAS_DEVICE int c2_turn(int rd) { return rd * (int)gridDim.x + ((rd & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); }
-
-// Every role walks the CTA's items by itself.  An item's two dependent loads (its sequence, the sequence's lengths) are issued two items and
-// one item ahead, so that no role waits for them.
-struct C2Walk {
-  const ScChunkParams& p;
-  int items, rd, b1, q1, len1, s1, e1, b2, q2;
-  ATLAS_DEVICE C2Walk(const ScChunkParams& params, int n) : p(params), items(n), rd(0) {
-    tile(0, b1, q1);
-    tile(1, b2, q2);
-    lengths();
-  }
-  ATLAS_DEVICE void tile(int round, int& b, int& q) const {
-    const int it = min(c2_turn(round), items - 1) / (p.Hkv * p.splits);
-    b = p.tile_seq[it];
-    q = p.tile_q0[it];
-  }
-  ATLAS_DEVICE void lengths() {
-    len1 = p.seq_lens[b1];
-    s1 = p.query_start_loc[b1];
-    e1 = p.query_start_loc[b1 + 1];
-  }
-  ATLAS_DEVICE bool more() const { return c2_turn(rd) < items; }
-  ATLAS_DEVICE C2Item next() {
-    C2Item r;
-    const int toks = kScRows / p.G;
-    r.kvh = c2_turn(rd) % p.Hkv;
-    r.split = c2_turn(rd) / p.Hkv % p.splits;
-    r.b = b1;
-    r.q0 = q1;
-    r.L = min(len1, p.bt_cols * kScPg);
-    r.q_row0 = s1;
-    r.q_len = e1 - s1;
-    r.ctx0 = r.L - r.q_len;
-    r.page0 = p.window > 0 ? max(r.ctx0 + r.q0 - p.window + 1, 0) / kScPg : 0;
+ATLAS_DEVICE C2Item c2_item(const ScChunkParams& p, int rd, int items) {
+  const int it = rd * (int)gridDim.x + ((rd & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+  C2Item r;
+  r.b = -1;
+  if (it >= items) return r;
+  const int tile = it / (p.Hkv * p.splits), toks = kScRows / p.G;
+  r.b = p.tile_seq[tile];
+  r.q0 = p.tile_q0[tile];
+  r.kvh = it % p.Hkv;
+  r.split = it / p.Hkv % p.splits;
+  r.L = min(p.seq_lens[r.b], p.bt_cols * kScPg);
+  r.q_row0 = p.query_start_loc[r.b];
+  r.q_len = p.query_start_loc[r.b + 1] - r.q_row0;
+  r.ctx0 = r.L - r.q_len;
+  r.page0 = p.window > 0 ? max(r.ctx0 + r.q0 - p.window + 1, 0) / kScPg : 0;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int first = r.q0 + x * toks, last = min(first + toks, r.q_len);
-      r.n[x] = first < r.q_len ? max((min(r.L, r.ctx0 + last) - r.page0 * kScPg + kC2Kv - 1) / kC2Kv, 0) : 0;
-    }
-    r.n_kv = max(r.n[0], r.n[1]);
-    if (p.splits > 1) {
-      const int share = (r.n_kv + p.splits - 1) / p.splits;
-      r.page0 += r.split * share * kC2Pages;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) r.n[x] = min(max(r.n[x] - r.split * share, 0), share);
-      r.n_kv = max(r.n[0], r.n[1]);
-    }
-    b1 = b2;
-    q1 = q2;
-    lengths();
-    tile(++rd + 1, b2, q2);
-    return r;
+  for (int x = 0; x < 2; ++x) {
+    const int first = r.q0 + x * toks, last = min(first + toks, r.q_len);
+    r.n[x] = first < r.q_len ? max((min(r.L, r.ctx0 + last) - r.page0 * kScPg + kC2Kv - 1) / kC2Kv, 0) : 0;
   }
-};
+  if (p.splits > 1) {
+    const int share = (max(r.n[0], r.n[1]) + p.splits - 1) / p.splits;
+    r.page0 += r.split * share * kC2Pages;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) r.n[x] = min(max(r.n[x] - r.split * share, 0), share);
+  }
+  r.n_kv = max(r.n[0], r.n[1]);
+  return r;
+}
 
 template <int D>
 __global__ void __launch_bounds__(kC2Threads, 1)
@@ -365,7 +390,10 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   uint64_t* ks_full = bars + 18;                                  // [keys, values] pages have come
   uint64_t* ks_free = bars + 20;                                  // [keys, values] 4 warps
   uint64_t* pv_half = bars + 26;                                  // [tile] the first half's product
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
+  uint64_t* item_full = bars + 28;                                // [2] warp 13
+  uint64_t* item_free = bars + 30;                                // [2] the 15 other warps have read it
+  C2Item* sItem = reinterpret_cast<C2Item*>(bars + 32);           // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sItem + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -379,6 +407,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
       mbar_init(&pv_done[s], 1); mbar_init(&pv_half[s], 1); mbar_init(&o_free[s], 4);
     }
     for (int s = 0; s < 4; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_ready[s], 4); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&item_full[s], 1); mbar_init(&item_free[s], 15); }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -389,6 +418,21 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;                               // scores of A, of B (128 columns each, P over them), outputs of A, of B
 
+  // Every role but warp 13 gets the CTA's items from shared memory.  (Each role working them out for itself, in a copy of that code of its own
+  // that was cold by the next item, took 5000 clocks an item.)
+  uint32_t n_item = 0;
+  C2Item m_;
+  auto next = [&]() -> bool {
+    const uint32_t s = n_item & 1;
+    const bool got = mbar_wait(&item_full[s], (n_item >> 1) & 1, abort_flag, p.status, 0xC40);
+    if (!__all_sync(0xffffffffu, got)) return false;
+    m_ = sItem[s];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_free[s]);
+    ++n_item;
+    return m_.b >= 0;
+  };
+
   if (warp < 8) {
     // ------------------------------------------------------------------ softmax: tile x, a thread a row
     const int x = warp >> 2;
@@ -397,9 +441,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     const uint32_t tS = tmem + x * 128 + t_lane, tO = tmem + 256 + x * D + t_lane;
     int n_s = 0, ring = 0;                                        // score tiles of this tile so far, key tiles of both
     bool ok = true;
-    C2Walk walk(p, items);
-    while (walk.more() && ok) {
-      const C2Item m_ = walk.next();
+    while (ok && next()) {
       const int n = m_.n[x];
       const int tok = m_.q0 + x * toks + row / G, head = m_.kvh * G + row % G;
       const bool live = row < toks * G && tok < m_.q_len;
@@ -438,30 +480,18 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
       // ---- o / l, or this share's o and l
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long at = (long long)(m_.q_row0 + tok) * p.Hq + head, at_part = ((long long)m_.split * p.rows - p.first_row) * p.Hq + at;
-      __nv_bfloat16* out = p.out + (long long)(m_.q_row0 + tok) * p.ldo + head * D;
-      float* part = p.splits > 1 ? p.part_o + at_part * D : nullptr;
-      uint32_t r[2][32];
+      const bool part = p.splits > 1;
       if (n > 0) {
         ok = mbar_wait(&pv_done[x], (n_s - 1) & 1, abort_flag, p.status, 0xC02 + x);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
-        tmem_ld_32x32b_x32(tO, r[0]);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          tmem_ld_wait();
-          if (c + 1 < D / 32) tmem_ld_32x32b_x32(tO + (c + 1) * 32, r[(c + 1) & 1]);
-          else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free[x]);
-          }
-          if (live) store_outputs(r[c & 1], inv, out + c * 32, part ? part + c * 32 : nullptr);
-        }
-      } else if (live) {                                          // no keys: zeros
-#pragma unroll
-        for (int i = 0; i < 32; ++i) r[0][i] = 0;
-        for (int c = 0; c < D; c += 32) store_outputs(r[0], inv, out + c, part ? part + c : nullptr);
       }
+      store_outputs<D>(tO, n == 0, inv, !live ? -1 : part ? at_part * D : (long long)(m_.q_row0 + tok) * p.ldo + head * D, p.out, part ? p.part_o : nullptr, [&] {
+        if (n == 0) return;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[x]);
+      });
       if (live) {
         if (part) p.part_ml[at_part] = make_float2(m, l);
         else if (p.ml) p.ml[at] = make_float2(m == -INFINITY ? 0.f : m, inv);
@@ -473,10 +503,8 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     constexpr int kPer = D / 16;                                  // 16-byte pieces of a thread and tile: piece i of page i / D
     uint32_t n_t = 0;                                             // key tiles so far
     bool ok = true;
-    C2Walk walk(p, items);
-    while (walk.more() && ok) {
-      const C2Item nxt = walk.next();
-      const int L = nxt.L, page0 = nxt.page0, n_kv = nxt.n_kv;
+    while (ok && next()) {
+      const int L = m_.L, page0 = m_.page0, n_kv = m_.n_kv;
       for (int j = 0; j < n_kv; ++j, ++n_t) {
         const int s = n_t & 1;
         // ---- keys
@@ -505,7 +533,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
 #pragma unroll 4
         for (int k = 0; k < kPer; ++k) {
-          const int i = k * 128 + r, pg = i / D, dim = i % D, sw = dim & 7;
+          const int i = k * 128 + value_piece(r), pg = i / D, dim = i % D, col = output_column(dim), sw = col & 7;
           const int left = L - (page0 + j * kC2Pages + pg) * kScPg;      // tokens of the page; the others are cleared
           uint4 v = reinterpret_cast<const uint4*>(sStV)[i];
           if (left < kScPg) {
@@ -518,7 +546,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
           }
           uint4 lo, hi;
           sc_widen16(v, lo, hi);
-          uint8_t* rowp = sV + s * Tile::kV + (pg >> 2) * (D * 128) + (dim >> 3) * 1024 + sw * 128;
+          uint8_t* rowp = sV + s * Tile::kV + (pg >> 2) * (D * 128) + col * 128;
           const int ch = (pg & 3) * 2;
           *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
           *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
@@ -533,9 +561,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     const bool is_v = (lane & 8) != 0;
     uint32_t n_t = 0;
     bool ok = true;
-    C2Walk walk(p, items);
-    while (walk.more() && ok) {
-      const C2Item m_ = walk.next();
+    while (ok && next()) {
       const int n_pages = (m_.L + kScPg - 1) / kScPg;
       const int* bt = p.block_tables + (long long)m_.b * p.bt_ld;
       auto entry = [&](int j) {                                   // -1: behind the end or outside of the pool
@@ -570,7 +596,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         sc = sc1;
       }
     }
-    if (!ok)
+    if (*abort_flag)
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else if (warp == 12 || warp == 14) {
     // ------------------------------------------------------------------ products of tile x, each tile at its own pace.  The whole warp walks the
@@ -607,10 +633,8 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
     auto skip = [&](uint64_t* bar_free, uint32_t t) {
       if (lane == 0) mbar_arrive(bar_free + (t & 1));
     };
-    C2Walk walk(p, items);
-    for (; walk.more() && ok; ++n_i) {
-      const C2Item nxt = walk.next();
-      const int n = __shfl_sync(0xffffffffu, nxt.n[x], 0), n_kv = __shfl_sync(0xffffffffu, nxt.n_kv, 0);
+    for (; ok && next(); ++n_i) {
+      const int n = __shfl_sync(0xffffffffu, m_.n[x], 0), n_kv = __shfl_sync(0xffffffffu, m_.n_kv, 0);
       ok = wait(q_full, n_i & 1, 0xC22);
       if (!ok) break;
       if (n == 0 && lane == 0) mbar_arrive(q_free);
@@ -652,20 +676,27 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
       }
     }
   } else if (warp == 13) {
-    // ------------------------------------------------------------------ query tiles
+    // ------------------------------------------------------------------ items, two ahead, and their query tiles
     if (lane == 0) {
-      uint32_t n_i = 0;
       bool ok = true;
-      C2Walk walk(p, items);
-      for (; walk.more() && ok; ++n_i) {
-        const C2Item m_ = walk.next();
-        const int row = m_.q_row0 + m_.q0, kvh = m_.kvh;
-        ok = mbar_wait(q_free, (n_i & 1) ^ 1u, abort_flag, p.status, 0xC30);
+      auto publish = [&](int rd) {
+        ok = mbar_wait(&item_free[rd & 1], ((rd >> 1) & 1) ^ 1u, abort_flag, p.status, 0xC31);
+        if (!ok) return;
+        sItem[rd & 1] = c2_item(p, rd, items);
+        mbar_arrive(&item_full[rd & 1]);
+      };
+      publish(0);
+      for (int rd = 0; ok; ++rd) {
+        const C2Item own = sItem[rd & 1];
+        if (own.b < 0) break;
+        publish(rd + 1);
+        ok = ok && mbar_wait(q_free, (rd & 1) ^ 1u, abort_flag, p.status, 0xC30);
         if (!ok) break;
         mbar_expect_tx(q_full, 2u * (uint32_t)(D / 64) * 128u * (uint32_t)(toks * G));
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) tma_load_3d(sQ + x * Tile::kQ + c * kScSub, &tmap_q, q_full, c * 64, kvh * G, row + x * toks);
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_3d(sQ + x * Tile::kQ + c * kScSub, &tmap_q, q_full, c * 64, own.kvh * G, own.q_row0 + own.q0 + x * toks);
       }
       if (!ok)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
@@ -806,23 +837,9 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       // ---- o / l, or this share's o and l
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long at = (long long)(q_row0 + tok) * p.Hq + head, at_part = ((long long)split * p.rows - p.first_row) * p.Hq + at;
-      __nv_bfloat16* out = p.out + (long long)(q_row0 + tok) * p.ldo + head * D;
-      float* part = p.splits > 1 ? p.part_o + at_part * D : nullptr;
-      uint32_t r[2][32];
-      if (n_kv > 0) {
-        tc_fence_after();
-        tmem_ld_32x32b_x32(tO, r[0]);
-#pragma unroll 2
-        for (int c = 0; c < D / 32; ++c) {
-          tmem_ld_wait();
-          if (c + 1 < D / 32) tmem_ld_32x32b_x32(tO + (c + 1) * 32, r[(c + 1) & 1]);
-          if (live) store_outputs(r[c & 1], inv, out + c * 32, part ? part + c * 32 : nullptr);
-        }
-      } else if (live) {                                          // no keys: zeros
-#pragma unroll
-        for (int i = 0; i < 32; ++i) r[0][i] = 0;
-        for (int c = 0; c < D; c += 32) store_outputs(r[0], inv, out + c, part ? part + c : nullptr);
-      }
+      const bool part = p.splits > 1;
+      tc_fence_after();
+      store_outputs<D>(tO, n_kv == 0, inv, !live ? -1 : part ? at_part * D : (long long)(q_row0 + tok) * p.ldo + head * D, p.out, part ? p.part_o : nullptr, [] {});
       if (live) {
         if (part) p.part_ml[at_part] = make_float2(m, l);
         else if (p.ml) p.ml[at] = make_float2(m == -INFINITY ? 0.f : m, inv);
@@ -860,7 +877,7 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll 4
       for (int k = 0; k < kWidePages * D / 128; ++k) {
-        const int i = k * 128 + r, pg = i / D, dim = i % D, sw = dim & 7, ch = pg * 2;
+        const int i = k * 128 + value_piece(r), pg = i / D, dim = i % D, col = output_column(dim), sw = col & 7, ch = pg * 2;
         const int left = L - (page0 + j * kWidePages + pg) * kScPg;       // tokens of the page; the others are cleared
         uint4 v = reinterpret_cast<const uint4*>(sStV + s * Tile::kStage)[i];
         if (left < kScPg) {
@@ -873,7 +890,7 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
         }
         uint4 lo, hi;
         sc_widen16(v, lo, hi);
-        uint8_t* rowp = sV + s * Tile::kV + dim * 128;
+        uint8_t* rowp = sV + s * Tile::kV + col * 128;
         *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
         *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
       }
