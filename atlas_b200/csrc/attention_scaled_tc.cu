@@ -1022,7 +1022,7 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
   float* sOwn = sSum + kScRows;                                    // [128] this CTA's sums
   float* sOther = sOwn + kScRows;                                  // [128] the other CTA's, in the first one
   uint64_t* bars = reinterpret_cast<uint64_t*>(sOther + kScRows);
-  uint64_t* q_full = bars;                                         // [stages] one arrival + the tile's bytes
+  uint64_t* q_full = bars;                                         // [stages] the tile's bytes, its references
   uint64_t* q_empty = q_full + kSwStages;                          // [stages] QK done
   uint64_t* s_full = q_empty + kSwStages;                          // [stages]
   uint64_t* s_free = s_full + kSwStages;                           // [stages] 8 warps
@@ -1042,7 +1042,7 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
   const int n_q = r_hi > r_lo ? (r_hi - r_lo + 2 * toks - 1) / (2 * toks) : 0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSwStages; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); }
+    for (int s = 0; s < kSwStages; ++s) { mbar_init(&q_full[s], 2); mbar_init(&q_empty[s], 1); mbar_init(&s_full[s], 1); mbar_init(&s_free[s], 8); }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -1082,30 +1082,41 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
   const uint32_t tS = *tmem_slot;
 
   if (warp == 0) {
-    // ------------------------------------------------------------------ producer: query rows, their M and 1 / l
+    // ------------------------------------------------------------------ producer: query rows as soon as the last product has read its buffer, and
+    // their M and 1 / l, loaded a tile ahead, when the sums have (both of a tile, loaded then: 118 in place of 104 us for 2 x 3001 rows)
     bool ok = true;
-    for (int j = 0; j < n_q && ok; ++j) {
-      const int s = j % kSwStages, q0 = r_lo + j * 2 * toks;
-      if (lane == 0) ok = mbar_wait(&q_empty[s], ((j / kSwStages) & 1) ^ 1u, abort_flag, p.status, 0xB00) &&
-                          mbar_wait(&s_free[s], ((j / kSwStages) & 1) ^ 1u, abort_flag, p.status, 0xB01);
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      if (!ok) break;
+    float2 x[kScRows / 32];
+    auto references = [&](int j) {
+      const int q0 = r_lo + j * 2 * toks;
 #pragma unroll
-      for (int i = 0; i < kScRows; i += 32) {
-        const int r = i + lane, tok = q0 + r / G;
-        float2 x = make_float2(INFINITY, 0.f);                     // a row that is not there adds 2^-inf * 0
-        if (r < toks * G && tok < q_len) x = p.ml[(long long)(q_row0 + tok) * p.Hq + kvh * G + r % G];
-        sM[s * 2 * kScRows + r] = -x.x;
-        sM[s * 2 * kScRows + kScRows + r] = x.y;
+      for (int i = 0; i < kScRows / 32; ++i) {
+        const int r = i * 32 + lane, tok = q0 + r / G;
+        x[i] = make_float2(INFINITY, 0.f);                         // a row that is not there adds 2^-inf * 0
+        if (r < toks * G && tok < q_len) x[i] = p.ml[(long long)(q_row0 + tok) * p.Hq + kvh * G + r % G];
       }
-      __syncwarp();
+    };
+    if (n_q > 0) references(0);
+    for (int j = 0; j < n_q; ++j) {
+      const int s = j % kSwStages, q0 = r_lo + j * 2 * toks;
+      ok = mbar_wait(&q_empty[s], ((j / kSwStages) & 1) ^ 1u, abort_flag, p.status, 0xB00);
+      if (!__all_sync(0xffffffffu, ok)) break;
       if (lane == 0) {
         mbar_expect_tx(&q_full[s], (uint32_t)(D / 64) * 128u * (uint32_t)(toks * G));
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) tma_load_3d(sQ + s * kQ + c * kScSub, &tmap_q, &q_full[s], c * 64, kvh * G, q_row0 + q0);
       }
+      ok = mbar_wait(&s_free[s], ((j / kSwStages) & 1) ^ 1u, abort_flag, p.status, 0xB01);
+      if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+      for (int i = 0; i < kScRows / 32; ++i) {
+        sM[s * 2 * kScRows + i * 32 + lane] = -x[i].x;
+        sM[s * 2 * kScRows + kScRows + i * 32 + lane] = x[i].y;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[s]);
+      if (j + 1 < n_q) references(j + 1);
     }
-    if (!ok)
+    if (*abort_flag)
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ products: S^T = K Q^T (the whole warp, one elected lane issues)
@@ -1151,7 +1162,7 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
       const int c_lo = max(tok - first, 0) * G, c_hi = (p.window > 0 ? min(tok + p.window - first, there) : there) * G;
       const uint64_t f2 = pair2(f, f);
       uint64_t sum2 = 0;
-#pragma unroll 1
+#pragma unroll 2
       for (int c = half * 64; c < half * 64 + 64; c += 32) {
         uint32_t r[32];
         tmem_ld_32x32b_x32(tS + s * kScRows + t_lane + c, r);

@@ -730,7 +730,7 @@ kv_evict_move_kernel(const MoveParams p) {
         if (pr >= 0) {
           mine[a] = ((1u << end) - 1u) & ~((1u << r) - 1u);
 #pragma unroll
-          for (int i = 0; i < V; ++i) col[a][i] = reinterpret_cast<const uint4*>(c.v + head + pr * step)[lane * V + i];
+          for (int i = 0; i < V; ++i) col[a][i] = reinterpret_cast<const uint4*>(c.v + head + pr * step)[i * 32 + lane];
         }
       }
     }
@@ -776,7 +776,7 @@ kv_evict_move_kernel(const MoveParams p) {
   }
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    reinterpret_cast<uint4*>(p.v + base)[lane * V + i] = make_uint4(word[i][0], word[i][1], word[i][2], word[i][3]);
+    reinterpret_cast<uint4*>(p.v + base)[i * 32 + lane] = make_uint4(word[i][0], word[i][1], word[i][2], word[i][3]);
   if (lane == 0) p.vs[to * c.vs_ld + h * c.vs_h] = pow2i(e);
 }
 
