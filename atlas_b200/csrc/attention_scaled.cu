@@ -431,8 +431,56 @@ ATLAS_DEVICE Pieces pieces_of(const ScaledDecodeParams& p, int item, int lane) {
   return Pieces{(long long)item + w0, np > 0 ? (start + np - 1) / run - w0 + 1 : 0};
 }
 
-// A few pieces a pair: a thread joins four neighbouring output numbers by itself, two global loads deep and without a barrier.  (Blocks that
-// share the factors, four barriers: 20 us for 128 sequences of 8 heads.)
+// Four neighbouring output numbers of a pair and their heads' references and sums, over pieces of it.
+struct Joined {
+  float m[4], l[4], o[4];
+  ATLAS_DEVICE void clear() {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { m[j] = -INFINITY; l[j] = 0.f; o[j] = 0.f; }
+  }
+  // kAtOnce pieces, `step` apart, those before n: all their loads are in flight together
+  template <int kAtOnce>
+  ATLAS_DEVICE void add(const float2* ml, const float* part, const int (&c)[4], int cols, long long piece, int i, int step, int n) {
+    float2 y[kAtOnce][4];
+    float4 x[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[k][j] = make_float2(-INFINITY, 0.f);
+      if (i + k * step < n) {
+        x[k] = *reinterpret_cast<const float4*>(part + (i + k * step) * piece);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[k][j] = ml[(i + k * step) * cols + c[j]];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float top = m[j];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, y[k][j].x);
+      const float ref = top == -INFINITY ? 0.f : top, f0 = fast_exp2(m[j] - ref);
+      l[j] *= f0;
+      o[j] *= f0;
+      m[j] = top;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float f = fast_exp2(y[k][j].x - ref);        // a piece without a visible token: 2^-inf
+        l[j] = fmaf(y[k][j].y, f, l[j]);
+        o[j] = fmaf(j == 0 ? x[k].x : j == 1 ? x[k].y : j == 2 ? x[k].z : x[k].w, f, o[j]);
+      }
+    }
+  }
+};
+ATLAS_DEVICE void store_joined(const ScaledDecodeParams& p, int b, int pair, int c, int d, int D, float m, float l, float o) {
+  const int head = pair % p.tiles * p.cols + c, h = pair / p.tiles;
+  if (head >= p.G) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;              // no token: zeros
+  p.out[(long long)p.query_start_loc[b] * p.ldo + ((long long)h * p.G + head) * D + d] = __float2bfloat16_rn(o * inv);
+  if (p.ml && d == 0) reinterpret_cast<float2*>(p.ml)[((long long)b * p.Hkv + h) * p.G + head] = make_float2(m == -INFINITY ? 0.f : m, inv);
+}
+
+// A few pieces a pair: a thread joins four neighbouring output numbers by itself, without a barrier.
 template <int D>
 __global__ void __launch_bounds__(128)
 scaled_join_kernel(const ScaledDecodeParams p) {
@@ -446,143 +494,56 @@ scaled_join_kernel(const ScaledDecodeParams p) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) c[j] = (e0 + j) % p.cols;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + pc.first * p.cols;
-  const float* src = p.part_o + pc.first * D * p.cols + e0;
-  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 4
-  for (int i = 0; i < pc.n; ++i)
+  const float* part = p.part_o + pc.first * D * p.cols + e0;
+  Joined t;
+  t.clear();
+#pragma unroll 1
+  for (int i = 0; i < pc.n; i += 4) t.add<4>(ml, part, c, p.cols, (long long)D * p.cols, i, 1, pc.n);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], ml[i * p.cols + c[j]].x);
-  float l[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) m[j] = m[j] == -INFINITY ? 0.f : m[j];
-#pragma unroll 4
-  for (int i = 0; i < pc.n; ++i) {
-    const float4 x = *reinterpret_cast<const float4*>(src + (long long)i * D * p.cols);
-    const float xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 y = ml[i * p.cols + c[j]];
-      const float f = fast_exp2(y.x - m[j]);             // a piece without a visible token: 2^-inf
-      l[j] += y.y * f;
-      o[j] = fmaf(xs[j], f, o[j]);
-    }
-  }
-  const long long row = (long long)p.query_start_loc[b] * p.ldo + (long long)(pair / p.tiles) * p.G * D;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int head = (pair % p.tiles) * p.cols + c[j], d = (e0 + j) / p.cols;
-    if (head >= p.G) continue;
-    const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];    // no token: zeros
-    p.out[row + head * D + d] = __float2bfloat16_rn(o[j] * inv);
-    if (p.ml && d == 0) reinterpret_cast<float2*>(p.ml)[((long long)b * p.Hkv + pair / p.tiles) * p.G + head] = make_float2(m[j], inv);
-  }
+  for (int j = 0; j < 4; ++j) store_joined(p, b, pair, c[j], (e0 + j) / p.cols, D, t.m[j], t.l[j], t.o[j]);
 }
 
-// Hundreds of pieces a pair (long sequences, few pairs): a thread owns four neighbouring output numbers and every sixteenth piece, so that
-// their loads overlap (3 x 65531 tokens of 2 heads: 13 us, with four groups of pieces 26 us).
-constexpr int kSmChunk = 256;                            // pieces whose factors are in shared memory at a time
+// Many pieces a pair (long sequences, few pairs): sixteen warps take every sixteenth piece of the same 128 output numbers.
+constexpr int kSdMergeWarps = 16;
 
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kSdMergeWarps * 32)
 scaled_merge_kernel(const ScaledDecodeParams p) {
-  constexpr int kGroups = 16, kQuads = 256 / kGroups;
-  __shared__ float factor[kSmChunk][16];
-  __shared__ float part[16][17];
-  __shared__ float top[16], sum[16];
-  __shared__ float4 quad[256];
+  __shared__ float sm[kSdMergeWarps][128], sl[kSdMergeWarps][128], so[kSdMergeWarps][128];
   chain_trigger();
   chain_wait();
-  const int tid = threadIdx.x, lane = tid & 31;
   const int item = blockIdx.x, hn = p.Hkv * p.tiles, b = item / hn, pair = item % hn;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Pieces pc = pieces_of(p, item, lane);
-  const int pieces = pc.n;
-  const long long piece0 = pc.first;
-  // ---- references and sums of the heads: thread (piece lane, head)
-  const int pl = tid >> 4, hc = tid & 15;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + piece0 * p.cols + hc;
-  float2 x[kSmChunk / 16];
-  float m = -INFINITY;
-  for (int i0 = 0; i0 < pieces; i0 += kSmChunk) {
-    const int n = min(pieces - i0, kSmChunk);
+  const int e0 = blockIdx.y * 128 + 4 * lane;
+  Joined t;
+  t.clear();
+  if (e0 < D * p.cols) {
+    int c[4];
 #pragma unroll
-    for (int k = 0; k < kSmChunk / 16; ++k) {
-      x[k] = make_float2(-INFINITY, 0.f);
-      if (hc < p.cols && pl + 16 * k < n) x[k] = ml[(long long)(i0 + pl + 16 * k) * p.cols];
-    }
-#pragma unroll
-    for (int k = 0; k < kSmChunk / 16; ++k) m = fmaxf(m, x[k].x);
+    for (int j = 0; j < 4; ++j) c[j] = (e0 + j) % p.cols;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + pc.first * p.cols;
+    const float* part = p.part_o + pc.first * D * p.cols + e0;
+#pragma unroll 1
+    for (int i = warp; i < pc.n; i += 4 * kSdMergeWarps) t.add<4>(ml, part, c, p.cols, (long long)D * p.cols, i, kSdMergeWarps, pc.n);
   }
-  part[pl][hc] = m;
+  *reinterpret_cast<float4*>(&sm[warp][4 * lane]) = make_float4(t.m[0], t.m[1], t.m[2], t.m[3]);
+  *reinterpret_cast<float4*>(&sl[warp][4 * lane]) = make_float4(t.l[0], t.l[1], t.l[2], t.l[3]);
+  *reinterpret_cast<float4*>(&so[warp][4 * lane]) = make_float4(t.o[0], t.o[1], t.o[2], t.o[3]);
   __syncthreads();
-  if (tid < 16) {
+  const int e = blockIdx.y * 128 + threadIdx.x;
+  if (threadIdx.x >= 128 || e >= D * p.cols) return;
+  float m = -INFINITY, l = 0.f, o = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, part[i][tid]);
-    top[tid] = m == -INFINITY ? 0.f : m;
+  for (int w = 0; w < kSdMergeWarps; ++w) m = fmaxf(m, sm[w][threadIdx.x]);
+  const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int w = 0; w < kSdMergeWarps; ++w) {
+    const float f = fast_exp2(sm[w][threadIdx.x] - ref);
+    l = fmaf(sl[w][threadIdx.x], f, l);
+    o = fmaf(so[w][threadIdx.x], f, o);
   }
-  __syncthreads();
-  // ---- outputs [channel][head], numbers 4 * quad .. of this block
-  const int per = 4 * kQuads / (2 * p.cols) * (2 * p.cols);     // whole channels, whole quads
-  const int qd = tid % kQuads, grp = tid / kQuads;
-  const int e0 = (int)blockIdx.y * per + 4 * qd;
-  const bool live = 4 * qd < per && e0 < D * p.cols;
-  int c[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c[j] = (e0 + j) % p.cols;
-  const float* src = p.part_o + piece0 * D * p.cols + e0;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  const float ref = top[hc];
-  for (int i0 = 0; i0 < pieces; i0 += kSmChunk) {
-    const int n = min(pieces - i0, kSmChunk);
-#pragma unroll
-    for (int k = 0; k < kSmChunk / 16; ++k) {
-      if (pl + 16 * k >= n) break;
-      if (pieces > kSmChunk && hc < p.cols) x[k] = ml[(long long)(i0 + pl + 16 * k) * p.cols];
-      const float f = fast_exp2(x[k].x - ref);           // a piece without a visible token: 2^-inf
-      factor[pl + 16 * k][hc] = f;
-      l += x[k].y * f;
-    }
-    __syncthreads();
-    if (live)
-#pragma unroll 8
-      for (int i = grp; i < n; i += kGroups) {
-        const float4 o = *reinterpret_cast<const float4*>(src + (long long)(i0 + i) * D * p.cols);
-        acc.x = fmaf(o.x, factor[i][c[0]], acc.x);
-        acc.y = fmaf(o.y, factor[i][c[1]], acc.y);
-        acc.z = fmaf(o.z, factor[i][c[2]], acc.z);
-        acc.w = fmaf(o.w, factor[i][c[3]], acc.w);
-      }
-    __syncthreads();
-  }
-  part[pl][hc] = l;
-  quad[tid] = acc;
-  __syncthreads();
-  if (tid < 16) {
-    l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) l += part[i][tid];
-    const float inv = l == 0.f ? 0.f : 1.f / l;          // no token: zeros
-    sum[tid] = inv;
-    const int head = (pair % p.tiles) * p.cols + tid;
-    if (p.ml && blockIdx.y == 0 && tid < p.cols && head < p.G)
-      reinterpret_cast<float2*>(p.ml)[((long long)b * p.Hkv + pair / p.tiles) * p.G + head] = make_float2(top[tid], inv);
-  }
-  __syncthreads();
-  // ---- rows of a head's channels
-  const int chans = per / p.cols;
-  const long long row = (long long)p.query_start_loc[b] * p.ldo;
-  for (int i = tid; i < per; i += 256) {
-    const int cc = i / chans, dd = i % chans;
-    const int hh = (pair % p.tiles) * p.cols + cc, dg = blockIdx.y * chans + dd;
-    if (hh < p.G && dg < D) {
-      const int e = dd * p.cols + cc;
-      const float* q = reinterpret_cast<const float*>(quad);
-      float o = 0.f;
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) o += q[4 * kQuads * k + e];
-      p.out[row + ((pair / p.tiles) * p.G + hh) * D + dg] = __float2bfloat16_rn(o * sum[cc]);
-    }
-  }
+  store_joined(p, b, pair, e % p.cols, e / p.cols, D, m, l, o);
 }
 
 // weights[b, h, j] += sum over the pair's heads of 2^(s - M) / l, a thread per token.
@@ -614,16 +575,18 @@ using namespace atlas;
 namespace {
 
 template <int D, int NT>
-int decode_launch(ScaledDecodeParams p, int blocks, int items, cudaStream_t st) {
+int decode_launch(ScaledDecodeParams p, int blocks, int items, long long max_len, cudaStream_t st) {
   constexpr int smem = kSdRings;
   p.warps = blocks * kSdWarps<D, NT>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(scaled_decode_kernel<D, NT>), smem) != cudaSuccess) return -20;
   if (launch_chain(scaled_decode_kernel<D, NT>, dim3(blocks), dim3(kSdWarps<D, NT> * 32), smem, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
-  // Up to sixteen pieces a pair on average are joined by single threads.
-  const bool few = 16ll * items >= p.warps;
-  const int chans = 64 / (2 * p.cols) * 2;
-  const cudaError_t e = few ? launch_chain(scaled_join_kernel<D>, dim3(items, (D * p.cols / 4 + 127) / 128), dim3(128), 0, st, p)
-                            : launch_chain(scaled_merge_kernel<D>, dim3(items, (D + chans - 1) / chans), dim3(256), 0, st, p);
+  // Single threads join up to four pieces a pair on average (128 x 1152 tokens of 8 heads, 3 a pair: 65 us with the attention, 89 by blocks), and
+  // up to sixteen if no pair can have hundreds (a warp has two pages or more, and its share of the longest sequence's list): 32 x 4096 ragged
+  // tokens with weights, 9 a pair, 59 us, 62 by blocks; but 3 x 65531 tokens, 197 a pair, 89 us, 42 by blocks.
+  const long long most = min((max_len + 2 * kSdPage - 1) / (2 * kSdPage), (long long)p.warps * p.nd / items + 1) + 1;
+  const bool few = 4ll * items >= p.warps || (16ll * items >= p.warps && most <= 256);
+  const cudaError_t e = few ? launch_chain(scaled_join_kernel<D>, dim3(items, (D * p.cols + 511) / 512), dim3(128), 0, st, p)
+                            : launch_chain(scaled_merge_kernel<D>, dim3(items, (D * p.cols + 127) / 128), dim3(kSdMergeWarps * 32), 0, st, p);
   if (e != cudaSuccess) { cudaGetLastError(); return -20; }
   return 0;
 }
@@ -665,8 +628,8 @@ extern "C" int atlas_attn_scaled_decode(const void* record) {
   cudaStream_t st = (cudaStream_t)r.stream;
   const int blocks = (int)r.blocks, n = (int)items;
   int rc;
-  if (p.G <= 8) rc = D == 64 ? decode_launch<64, 1>(p, blocks, n, st) : D == 128 ? decode_launch<128, 1>(p, blocks, n, st) : decode_launch<256, 1>(p, blocks, n, st);
-  else rc = D == 64 ? decode_launch<64, 2>(p, blocks, n, st) : D == 128 ? decode_launch<128, 2>(p, blocks, n, st) : decode_launch<256, 2>(p, blocks, n, st);
+  if (p.G <= 8) rc = D == 64 ? decode_launch<64, 1>(p, blocks, n, r.max_len, st) : D == 128 ? decode_launch<128, 1>(p, blocks, n, r.max_len, st) : decode_launch<256, 1>(p, blocks, n, r.max_len, st);
+  else rc = D == 64 ? decode_launch<64, 2>(p, blocks, n, r.max_len, st) : D == 128 ? decode_launch<128, 2>(p, blocks, n, r.max_len, st) : decode_launch<256, 2>(p, blocks, n, r.max_len, st);
   if (rc || !r.weights) return rc;
   const long long chunks = (r.max_len + 1023) / 1024;
   if (launch_chain(scaled_weigh_kernel, dim3((unsigned)(r.nd * r.Hkv), (unsigned)(chunks < 1 ? 1 : chunks < 64 ? chunks : 64)), dim3(256),

@@ -1,9 +1,9 @@
 // Chunk attention over the FP8 cache with a power-of-two scale per (page, head), on the 5th-generation tensor cores, and the softmax weight
 // that each cached token got from a chunk's rows.
 //
-// As in attention_scaled.cu the codes are the operands and the scales live in the exponent: s_j = f q . k^_j with f = softmax scale * log2(e) *
-// 2^(row's own power) * key page's scale, p_j = 2^(s_j + ev - M) in f16, o = sum p_j v^_j / sum p_j 2^-ev.  A page covers 16 score columns, so
-// f and ev - M are constants of a multiply-add over them, and a page's largest score is found before they are applied.
+// As in attention_scaled.cu the codes are the operands and the scales live in the exponent: s_j = f q . k^_j with f = softmax scale * log2(e) * key
+// page's scale, p_j = 2^(s_j + ev - M) in f16, o = sum p_j v^_j / sum p_j 2^-ev.  A page covers 16 score columns, so f and ev - M are constants
+// of a multiply-add over them, and a page's largest score is found before they are applied.
 //
 // scaled_chunk2_kernel (heads of 64 and 128), scaled_chunk_wide_kernel (256): tiles of 128 query rows of a key head; the G query heads of a key
 // head are packed into the rows (row = token * G + head), so that a page is fetched and widened once for all of them.  One warp fetches pages
@@ -182,15 +182,19 @@ scaled_chunk_join_kernel(const ScChunkParams p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- two tiles at a time
-// Heads of 64 and 128: two query tiles share every widened key tile, so that one tile's products run under the other one's softmax, and P
-// stays in TMEM.  Persistent, one CTA per SM; items (pair of query tiles, key head) with the most keys first.
+// Heads of 64 and 128: two query tiles share every widened key tile.  Persistent, one CTA per SM; items (pair of query tiles, key head) with the
+// most keys first.
 //   warps 0..3, 4..7   softmax of tile A and of tile B, a thread a row
-//   warp 15            pages by bulk copies, their scales
 //   warps 8..11        keys to bf16, values to f16 (two buffers of each)
-//   warps 12, 14       products of tile A and of tile B; QK_{j+1} behind PV_j, whose P lies where the scores go
-//   warp 13            query tiles by TMA, as they are (bf16: keys are exact in it)
-// Per pair of tiles and 128 keys: products 2048 clocks of the tensor cores, exponentials 2048 of the special-function units, shared memory
-// 1536 for operands and 512 for the widened tiles.
+//   warps 12, 14       products of tile A and of tile B, by halves of a key tile: scores of 64 keys go behind the product that read P out of
+//                      the same columns, so that the softmax finds the next half ready (whole key tiles: 138 in place of 115 us, 8 x 1024 rows)
+//   warp 13            the items, and query tiles by TMA, as they are (bf16: keys are exact in it)
+//   warp 15            pages by bulk copies, their scales
+// Per pair of tiles and 128 keys: products 2048 clocks of the tensor cores, exponentials 2048 of the special-function units, shared memory 3072
+// (2048 for operands, 512 for the widened tiles, 512 for the codes).  Measured 5000: a softmax thread's chain of 2500 for 64 keys, half of it
+// exponentials shared by two warps a scheduler; no unit is busy for more than half of the time (issue slots 43 %).  Rounds of 16 or 32 columns,
+// a part of the exponentials as polynomials, and the tiles half a step apart were slower or no faster.  8 x 1024 rows of 32 heads of 128:
+// 109 us, 630 TFLOP/s; two sequences of 3001 rows: 150.
 constexpr int kC2Threads = 512;
 constexpr int kC2Kv = 128, kC2Pages = 8, kC2Ring = 8;
 
@@ -413,6 +417,12 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   }
   if (warp == 12) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   if (warp == 13 && lane == 0) tma_prefetch_desc(&tmap_q);
+  // rows behind a tile's last whole token are never loaded: zeros (whatever lay there could be NaN, which sends its warp through the rare path)
+  for (int i = threadIdx.x; i < 2 * (D / 64) * (kScRows - toks * G) * 8; i += kC2Threads) {
+    const int rest = kScRows - toks * G, row = toks * G + (i >> 3) % rest, sub = (i >> 3) / rest;
+    *reinterpret_cast<uint4*>(sQ + sub * kScSub + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -716,10 +726,12 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
 // memory once for 64 keys), two buffers of 64 score columns the rest.
 //   warps 0..3     query rows to TMEM, softmax, a thread a row; P goes over its scores
 //   warps 4..7     keys to bf16          warps 8..11   values to f16          (two buffers of each)
-//   warp 12        products: QK_{j+2} behind PV_j, whose P lies where the scores go
+//   warps 14, 12   products: scores (of key tile j + 2 behind PV_j, whose P lies where they go), outputs
 //   warp 13        pages by bulk copies, their scales
 // Per 64 keys: products 512 clocks, exponentials 512, shared memory 1536 (512 for operands, 512 for the widened tiles, 512 for the codes).
-constexpr int kWideThreads = 448, kWideKv = 64, kWidePages = 4, kWideRing = 8;
+// Measured 3000, the softmax thread's chain again.  517 rows of 16 heads behind 4096 tokens: 57 us, 660 TFLOP/s (P through shared memory, two
+// threads a row, one group of widening warps: 115).
+constexpr int kWideThreads = 480, kWideKv = 64, kWidePages = 4, kWideRing = 8;
 
 struct WideTile {
   static constexpr int D = 256;
@@ -790,7 +802,7 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
     const int tok = q0 + row / G, head = kvh * G + row % G;
     const bool live = row < toks * G && tok < q_len;
     const __nv_bfloat16* q = p.q + (long long)(q_row0 + tok) * p.ldq + head * D;
-#pragma unroll 2
+#pragma unroll 4
     for (int c = 0; c < D / 32; ++c) {
       uint32_t v[16];
 #pragma unroll
@@ -898,40 +910,42 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       __syncwarp();
       if (lane == 0) { mbar_arrive(&v_full[s]); mbar_arrive(&stage_free[2 + s]); }
     }
-  } else if (warp == 12) {
-    // ------------------------------------------------------------------ products (the whole warp, one elected lane issues)
-    constexpr uint32_t kIdescS = make_idesc(kScRows, kWideKv, 1u), kIdescO = make_idesc(kScRows, D, 0u);      // bf16 scores, f16 outputs
+  } else if (warp == 12 || warp == 14) {
+    // ------------------------------------------------------------------ products (whole warps, one elected lane issues): warp 14 scores, warp 12
+    // outputs, so that neither waits for the other's queue
     const uint32_t dK = desc_low(sK), dV = desc_low(sV), tQ = tmem + 128, tO = tmem + 256;
-    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, site)); };
-    auto score = [&](int j) -> bool {
-      if (!wait(&k_full[j & 1], (j >> 1) & 1, 0xA20)) return false;
-      tc_fence_after();
-      if (elect_one()) {
+    auto wait = [&](uint64_t* bar, int j, uint32_t site) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar + (j & 1), (j >> 1) & 1, abort_flag, p.status, site)); };
+    if (warp == 14) {
+      constexpr uint32_t kIdesc = make_idesc(kScRows, kWideKv, 1u);         // bf16
+      if (__all_sync(0xffffffffu, mbar_wait(q_ready, 0, abort_flag, p.status, 0xA21)))
+        for (int j = 0; j < n_kv; ++j) {
+          // the product that read P out of these columns is done
+          if (!wait(k_full, j, 0xA20) || (j >= 2 && !wait(pv_done, j - 2, 0xA24))) break;
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          umma_f16_ta(tmem + (j & 1) * kWideKv, tQ + ks * 8, dK + (j & 1) * (Tile::kK >> 4) + (ks >> 2) * (Tile::kSub >> 4) + 2 * (ks & 3), kIdescS,
-                      ks > 0 ? 1u : 0u);
-        umma_commit(&s_full[j & 1]);
-        umma_commit(&k_free[j & 1]);
-      }
-      __syncwarp();
-      return true;
-    };
-    bool ok = wait(q_ready, 0, 0xA21);
-    for (int j = 0; j < min(n_kv, 2) && ok; ++j) ok = score(j);
-    for (int j = 0; j < n_kv && ok; ++j) {
-      ok = wait(&v_full[j & 1], (j >> 1) & 1, 0xA22) && wait(&p_ready[j & 1], (j >> 1) & 1, 0xA23);
-      if (!ok) break;
-      tc_fence_after();
-      if (elect_one()) {
+            for (int ks = 0; ks < D / 16; ++ks)
+              umma_f16_ta(tmem + (j & 1) * kWideKv, tQ + ks * 8, dK + (j & 1) * (Tile::kK >> 4) + (ks >> 2) * (Tile::kSub >> 4) + 2 * (ks & 3), kIdesc,
+                          ks > 0 ? 1u : 0u);
+            umma_commit(&s_full[j & 1]);
+            umma_commit(&k_free[j & 1]);
+          }
+          __syncwarp();
+        }
+    } else {
+      constexpr uint32_t kIdesc = make_idesc(kScRows, D, 0u);               // f16
+      for (int j = 0; j < n_kv; ++j) {
+        if (!wait(v_full, j, 0xA22) || !wait(p_ready, j, 0xA23)) break;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < kWideKv / 16; ++ks)
-          umma_f16_ta(tO, tmem + (j & 1) * kWideKv + ks * 8, dV + (j & 1) * (Tile::kV >> 4) + 2 * ks, kIdescO, (j > 0 || ks > 0) ? 1u : 0u);
-        umma_commit(&pv_done[j & 1]);
-        umma_commit(&v_free[j & 1]);
+          for (int ks = 0; ks < kWideKv / 16; ++ks)
+            umma_f16_ta(tO, tmem + (j & 1) * kWideKv + ks * 8, dV + (j & 1) * (Tile::kV >> 4) + 2 * ks, kIdesc, (j > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(&pv_done[j & 1]);
+          umma_commit(&v_free[j & 1]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      if (j + 2 < n_kv) ok = wait(&pv_done[j & 1], (j >> 1) & 1, 0xA24) && score(j + 2);
     }
   } else {
     // ------------------------------------------------------------------ pages: lanes 0..3 keys, 8..11 values, entries and scales two tiles ahead
@@ -1252,10 +1266,9 @@ int launch_wide(dim3 grid, const ScChunkParams& p, cudaStream_t st) {
 }  // namespace
 
 // Rows of chunk sequences: `tiles` query tiles of 128 / G tokens (heads of 64 and 128: pairs of tiles), each (sequence, first token in its
-// chunk); `ml` (or null) gets
-// every row's reference and 1 / l.  `splits` > 1: part_o [splits][rows][Hq][D] and part_ml
-// [splits][rows][Hq][2] for the rows from first_row on, the chunks'.  With `weights`, tiles of 128 cached tokens follow, each (sequence, first token), whose sums grow by the
-// rows' softmax weights.  Arguments as one record (see kv_scaled.cu).  -1: sizes or alignment outside of what the kernels take.
+// chunk); `ml` (or null) gets every row's reference and 1 / l.  `splits` > 1: part_o [splits][rows][Hq][D] and part_ml [splits][rows][Hq][2]
+// for the rows from first_row on, the chunks'.  With `weights`, tiles of 128 cached tokens follow, each (sequence, first token), whose sums grow
+// by the rows' softmax weights.  Arguments as one record (see kv_scaled.cu).  -1: sizes or alignment outside of what the kernels take.
 struct ChunkRecord {
   const void* q; long long ldq; void* out; long long ldo; const void* k_cache; const void* v_cache;
   const float* ks; long long ks_ld, ks_h; const float* vs; long long vs_ld, vs_h;

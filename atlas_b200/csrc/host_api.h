@@ -269,6 +269,14 @@ int atlas_map_norm_kv_write(const void* q, long long ldq, const void* k, long lo
 int atlas_map_difference(const void* a, const void* gate, long long ldg, void* out, int T, int H, int D, int dv, float lam, float rest, float eps,
                          int f32, void* stream);
 
+// ---- FP8 cache with a scale per (block, head) (kv_scaled.cu, attention_scaled.cu, attention_scaled_tc.cu).  Arguments as one record each, all of
+// its fields eight bytes wide; the records stand beside the functions.
+int atlas_kv_scaled_write(const void* record);
+int atlas_kv_scaled_read(const void* record);
+int atlas_kv_evict(const void* record);
+int atlas_attn_scaled_decode(const void* record);
+int atlas_attn_scaled_chunk(const void* record);
+
 // ---- short convolution (conv1d.cu)
 int atlas_conv1d_bias_silu(const void* x, long long ldx, const void* w, const void* bias, int C, int W, void* state,
                            const int* seq_of_token, const int* qsl, const int* slots, const unsigned char* has, void* y, long long ldy,

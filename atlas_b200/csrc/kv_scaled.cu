@@ -842,7 +842,7 @@ extern "C" int atlas_kv_scaled_write(const void* record) {
   if (r.T <= 0) return 0;
   if (D != 64 && D != 128 && D != 256) return -1;
   const int V = D / 32;
-  if (r.T > 0x7fffffff || r.rotary < 0 || r.rotary > D || r.rotary % 16 || r.num_pages <= 0 || r.num_pages > (1 << 27) || r.Hkv <= 0 || r.Hq < 0)
+  if (r.T > 0x7fffffff || r.rotary < 0 || r.rotary > D || r.rotary % 16 || r.num_pages <= 0 || r.num_pages >= (1 << 27) || r.Hkv <= 0 || r.Hq < 0)
     return -1;
   if (r.ldk % V || r.ldv % V || !aligned(r.k, 2 * V) || !aligned(r.v, 2 * V) || !aligned(r.k_cache, 16) ||
       !aligned(r.v_cache, 16) || !aligned(r.rope, 16))
