@@ -643,7 +643,7 @@ struct MoveParams {
 // once, as a whole, for all tokens that come from it, kAhead pages at a time.  (A warp for two pages, keys and values one after the other: 31
 // instead of 20 us for one sequence's 4096 tokens.)
 template <int D>
-__global__ void __launch_bounds__(128, D == 256 ? 3 : 6)
+__global__ void __launch_bounds__(128, D == 256 ? 3 : 8)
 kv_evict_move_kernel(const MoveParams p) {
   constexpr int V = D / 32;
   constexpr int kAhead = 2;      // four pages ahead leave room for four blocks an SM in place of six: 138 us a call, not 115 (32 x 4096 tokens to 1024)
