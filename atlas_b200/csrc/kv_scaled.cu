@@ -641,12 +641,12 @@ struct MoveParams {
 
 // A warp fills one page of one head's keys or values.  A kept value token's 16-byte columns hold its neighbours too: every source page is read
 // once, as a whole, for all tokens that come from it, kAhead pages at a time.  (A warp for two pages, keys and values one after the other: 31
-// instead of 20 us for one sequence's 4096 tokens.)
+// instead of 20 us for one sequence's 4096 tokens.)  Eight blocks an SM: 1024 of them, that sequence's, run at once (six: 47 us for the call, not 45).
 template <int D>
 __global__ void __launch_bounds__(128, D == 256 ? 3 : 8)
 kv_evict_move_kernel(const MoveParams p) {
   constexpr int V = D / 32;
-  constexpr int kAhead = 2;      // four pages ahead leave room for four blocks an SM in place of six: 138 us a call, not 115 (32 x 4096 tokens to 1024)
+  constexpr int kAhead = 2;      // four pages ahead take the registers of a third of the warps: 138 us a call, not 115 (32 x 4096 tokens to 1024)
   chain_trigger();
   chain_wait();
   const int lane = threadIdx.x & 31;
