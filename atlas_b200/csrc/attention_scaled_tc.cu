@@ -190,8 +190,8 @@ scaled_chunk_join_kernel(const ScChunkParams p) {
 //                      the same columns, so that the softmax finds the next half ready (whole key tiles: 138 in place of 115 us, 8 x 1024 rows)
 //   warp 13            the items, and query tiles by TMA, as they are (bf16: keys are exact in it)
 //   warp 15            pages by bulk copies, their scales
-// Per pair of tiles and 128 keys: products 2048 clocks of the tensor cores, exponentials 2048 of the special-function units, shared memory 3072
-// (2048 for operands, 512 for the widened tiles, 512 for the codes).  Measured 5000: a softmax thread's chain of 2500 for 64 keys, half of it
+// Per pair of tiles and 128 keys: products 2048 clocks of the tensor cores, exponentials 2048 of the special-function units, shared memory 2048
+// for operands, 512 for the widened tiles and 512 for the codes.  Measured 5000: a softmax thread's chain of 2500 for 64 keys, half of it
 // exponentials shared by two warps a scheduler; no unit is busy for more than half of the time (issue slots 43 %).  Rounds of 16 or 32 columns,
 // a part of the exponentials as polynomials, and the tiles half a step apart were slower or no faster.  8 x 1024 rows of 32 heads of 128:
 // 109 us, 630 TFLOP/s; two sequences of 3001 rows: 150.
