@@ -225,7 +225,7 @@ def check_attention(d, hkv, g, lens, rows, window, weigh, smallest=False):
     if smallest:
         # f16 has steps of 2^-24 below 2^-14: a weight p_j = 2^(s_j + ev_j - M) is off by 2^-25 at most however small it is, so the output by
         # 2^-25 sum_j |code_j| / l over the window's tokens.  The token that the reference M comes from has p >= 1, l >= 2^-ev of it, and
-        # 448 * 2^ev < 2 max |v| there (ev is the smallest that fits): n 2^-24 max |v| altogether.
+        # 448 * 2^ev < 2 max |v| there (a block's largest code is above 224): n 2^-24 max |v| altogether.
         bound = bound + window * 2.0 ** -24 * float((v.float().abs().nan_to_num(0.0).amax((1, 3)) * vs).max())
     assert (got.double().cpu() - out).abs().le(bound).all()
     if weigh:
