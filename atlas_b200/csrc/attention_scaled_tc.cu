@@ -1091,7 +1091,7 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
   }
   if (threadIdx.x < kScRows) sSum[threadIdx.x] = 0.f;
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();          // the other CTA runs, too: without rows of its own a CTA stores into it at once
   tc_fence_after();
   const uint32_t tS = *tmem_slot;
 
