@@ -406,6 +406,13 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][k], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
       }
+    } else if (p.scores) {                            // a page outside of the pool is skipped, its tokens get no weight
+      const int c0 = (it % p.tiles) * 8 * NT;
+      for (int j = lane; j < kSdPage * 8 * NT; j += 32) {
+        const int tok = tok0 + j / (8 * NT), c = c0 + j % (8 * NT);
+        if (tok < len && tok < p.width && c < p.score_cols)
+          p.scores[((long long)(it / p.tiles) * p.width + tok) * p.score_cols + c] = -INFINITY;
+      }
     }
     __syncwarp();
     if (i + kStages < n) {

@@ -77,6 +77,18 @@ ATLAS_DEVICE uint32_t h2_to_bf2(uint32_t v) {      // e4m3 numbers: exact in bot
 ATLAS_DEVICE int scale_exponent(float s) { return (int)((__float_as_uint(s) >> 23) & 255u) - 127; }
 ATLAS_DEVICE float exact_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// A page whose table entry lies outside of the pool is skipped: its codes are zeros, which the copying warp puts where the copy would have gone,
+// and its value exponent is -inf, so that no column of it has a weight.
+ATLAS_DEVICE float2 skipped_page() { return make_float2(1.f, -INFINITY); }
+template <int D>
+ATLAS_DEVICE void clear_pages(uint8_t* stage, uint32_t pages) {      // the whole warp; 16 * D bytes a page
+  const int lane = threadIdx.x & 31;
+  for (uint32_t left = pages; left; left &= left - 1)
+    for (int i = lane; i < D; i += 32) reinterpret_cast<uint4*>(stage)[(__ffs(left) - 1) * D + i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
+  __syncwarp();
+}
+
 // Column of TMEM that holds channel `d` of the outputs (rows of the value tiles go there): of 32 channels 8 i + 2 k + e, column 8 k + 2 i + e.
 // A load of 16 lanes x 256 bits gives thread 4 r + i columns 8 k + 2 i and one more of rows r and r + 8: eight channels in a row.
 ATLAS_DEVICE int output_column(int d) { return (d & ~31) | (d & 6) << 2 | (d >> 2 & 6) | (d & 1); }
@@ -324,7 +336,7 @@ ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const floa
       w[q >> 1][(q & 1) * 8 + i / 2] = sc_h2(e.x, e.y);
     }
     const float2 s = unpair2(s2);
-    l = fmaf(s.x + s.y, exact_pow2(-(int)f[q].y), l);
+    l = fmaf(s.x + s.y, exact_pow2((int)fminf(-f[q].y, 127.f)), l);      // a skipped page: 0 times anything
   }
   tmem_st_32x32b_x16(tP, w[0]);
   tmem_st_32x32b_x16(tP + 16, w[1]);
@@ -589,14 +601,17 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         const float sc1 = scale_of(blk1);
         const bool live = (unsigned)blk < (unsigned)p.num_pages;
         const uint32_t pages = __ballot_sync(0xffffffffu, live);
+        const bool skip = lane < 8 && m_.page0 + j * kC2Pages + lane < n_pages && !live;
+        const uint32_t skipped = __ballot_sync(0xffffffffu, skip);
         const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
-        if (lane < 8) sScale[(n_t % kC2Ring) * 8 + lane] = make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
+        if (lane < 8) sScale[(n_t % kC2Ring) * 8 + lane] = skip ? skipped_page() : make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
         __syncwarp();
         const long long at = ((long long)blk * p.Hkv + m_.kvh) * (kScPg * D);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           ok = mbar_wait(&ks_free[w], (n_t & 1) ^ 1u, abort_flag, p.status, 0xC30 + w);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          if (skipped) clear_pages<D>(w ? sStV : sStK, skipped);
           if (lane == 0) mbar_expect_tx(&ks_full[w], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
           __syncwarp();
           if (live && is_v == (w == 1)) sc_bulk((w ? sStV : sStK) + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &ks_full[w]);
@@ -968,6 +983,8 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       const float sc1 = scale_of(blk1);
       const bool live = (unsigned)blk < (unsigned)p.num_pages;
       const uint32_t pages = __ballot_sync(0xffffffffu, live);
+      const bool skip = lane < kWidePages && page0 + j * kWidePages + lane < n_pages && !live;
+      const uint32_t skipped = __ballot_sync(0xffffffffu, skip);
       const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
       const long long at = ((long long)blk * p.Hkv + kvh) * (kScPg * D);
 #pragma unroll
@@ -975,9 +992,11 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
         ok = mbar_wait(&stage_free[2 * w + s], ((j >> 1) & 1) ^ 1u, abort_flag, p.status, 0xA30 + w);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         if (w == 0) {                                             // tile j - kWideRing is done: its keys left this stage long ago
-          if (lane < kWidePages) sScale[(j % kWideRing) * kWidePages + lane] = make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
+          if (lane < kWidePages)
+            sScale[(j % kWideRing) * kWidePages + lane] = skip ? skipped_page() : make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
           __syncwarp();
         }
+        if (skipped) clear_pages<D>((w ? sStV : sStK) + s * Tile::kStage, skipped);
         if (lane == 0) mbar_expect_tx(&stage_full[2 * w + s], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
         __syncwarp();
         if (live && is_v == (w == 1))
@@ -1157,9 +1176,11 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
     const int trow = lane_group * 32 + lane, tok = k0 + trow;
     const uint32_t t_lane = (uint32_t)(lane_group * 32) << 16;
     float f = 0.f;
+    bool skip = true;                                      // a token of a page outside of the pool gets no weight
     if (tok < L) {
       const int blk = p.block_tables[(long long)b * p.bt_ld + tok / kScPg];
-      if (blk >= 0 && blk < p.num_pages) f = p.scale_log2 * p.k_scale[blk * p.ks_ld + kvh * p.ks_h];
+      skip = blk < 0 || blk >= p.num_pages;
+      if (!skip) f = p.scale_log2 * p.k_scale[blk * p.ks_ld + kvh * p.ks_h];
     }
     float total = 0.f;
     bool ok = true;
@@ -1206,6 +1227,7 @@ scaled_chunk_weigh_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScWe
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_free[s]);
     }
+    if (skip) total = 0.f;
     if (half == 1) sSum[trow] = total;
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
     if (half == 0) {

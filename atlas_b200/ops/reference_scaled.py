@@ -46,7 +46,7 @@ def qk_norm_rope_kv_write(q, k, v, positions, rope_cache, rotary_dim, k_cache, v
     t = 0
     while t < len(slots):
         s = slots[t]
-        if s < 0:
+        if s < 0 or s >= k_cache.shape[0] * bs:                                   # padding, or outside of the pool
             t += 1
             continue
         blk, off, n = s // bs, s % bs, 1
@@ -67,9 +67,16 @@ def qk_norm_rope_kv_write(q, k, v, positions, rope_cache, rotary_dim, k_cache, v
 
 
 def values(cache: torch.Tensor, scales: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
-    """fp32 ``[n * block, Hkv, D]`` of the given blocks."""
-    raw = cache.view(torch.uint8)[blocks].view(FP8).float()
-    return (raw * scales[blocks][:, None, :, None]).reshape(-1, *raw.shape[2:])
+    """fp32 ``[n * block, Hkv, D]`` of the given blocks; zeros where one lies outside of the pool."""
+    there = pooled(blocks, cache.shape[0])
+    at = torch.where(there, blocks, torch.zeros_like(blocks))
+    raw = cache.view(torch.uint8)[at].view(FP8).float()
+    x = torch.where(there[:, None, None, None], raw * scales[at][:, None, :, None], torch.zeros((), device=raw.device))
+    return x.reshape(-1, *raw.shape[2:])
+
+
+def pooled(blocks: torch.Tensor, num_blocks: int) -> torch.Tensor:
+    return (blocks >= 0) & (blocks < num_blocks)
 
 
 def kv_read(k_cache, v_cache, block_tables, seq_lens, max_len: int, k_scale, v_scale) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -99,10 +106,11 @@ def paged_attention(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc
         kk, vv = values(k_cache, k_scale, blocks)[:L], values(v_cache, v_scale, blocks)[:L]
         s = torch.einsum("qhgd,khd->hgqk", q[r0:r1].float().view(n, hkv, Hq // hkv, D), kk) * scale
         qpos, kpos = torch.arange(L - n, L, device=q.device)[:, None], torch.arange(L, device=q.device)[None]
-        mask = kpos <= qpos
+        mask = (kpos <= qpos) & pooled(blocks, nb).repeat_interleave(bs)[None, :L]       # a block outside of the pool is skipped
         if sliding_window:
             mask &= kpos > qpos - sliding_window
         p = torch.softmax(s.masked_fill(~mask, float("-inf")), -1)
+        p = torch.where(mask.any(-1)[:, None], p, torch.zeros((), device=q.device))      # a row that sees nothing: zeros
         out[r0:r1] = torch.einsum("hgqk,khd->qhgd", p, vv).reshape(n, Hq, D).to(q.dtype)
         if weights is not None:
             weights[b, :, :L] += p.sum((1, 2))

@@ -102,3 +102,23 @@ def evict64(weights, n, keep, sink, recent):
         return list(range(n))
     mid = sorted(range(sink, n - recent), key=lambda j: (-float(weights[j]) if weights[j] == weights[j] else float("inf"), j))
     return sorted(list(range(sink)) + mid[:keep - sink - recent] + list(range(n - recent, n)))
+
+
+def attention64_over(q, kk, vv, scale, window=0, there=None):
+    """``q [r, hq, d]``, ``kk`` and ``vv [n, hkv, d]`` of one sequence, its last ``r`` tokens the queries'; ``there [n]``: tokens that are not
+    skipped.  Returns (out, sum of p |v|, largest sum of magnitudes of a visible score, weights [hkv, n])."""
+    r, hq, d = q.shape
+    n, hkv, _ = kk.shape
+    qq = q.double().cpu().view(r, hkv, hq // hkv, d)
+    s = torch.einsum("rhgd,nhd->hgrn", qq, kk) * scale
+    size = torch.einsum("rhgd,nhd->hgrn", qq.abs(), kk.abs()) * abs(scale)
+    pos, key = torch.arange(n - r, n)[:, None], torch.arange(n)[None]
+    see = key <= pos
+    if window:
+        see &= key > pos - window
+    if there is not None:
+        see &= there[None]
+    p = torch.softmax(s.masked_fill(~see, float("-inf")), -1).nan_to_num(0.0)
+    back = lambda x: x.permute(2, 0, 1, 3).reshape(r, hq, -1)
+    out, mag = (back(torch.einsum("hgrn,nhd->hgrd", p, x)) for x in (vv, vv.abs()))
+    return out, mag, back(size.masked_fill(~see, 0.0).amax(-1, keepdim=True))[..., 0], p.sum((1, 2))

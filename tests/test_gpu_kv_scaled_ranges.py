@@ -2,9 +2,13 @@
 import pytest
 import torch
 
-from test_gpu_kv_scaled import check_attention
+from atlas_b200 import ops
+from atlas_b200.ops import cuda as K
+from kv_scaled_cases import BS, attention64_over, attention_bound, dequant, make_cache, tables_for
+from test_gpu_kv_scaled import batch_of, check_attention
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
 
 
 # ----------------------------------------------------------------------------- weights of few rows
@@ -17,3 +21,48 @@ pytestmark = pytest.mark.gpu
 def test_weights_where_one_cta_of_a_pair_has_no_rows(d, hkv, g, lens, rows, window):
     for _ in range(3):
         check_attention(d, hkv, g, lens, rows, window, True, smallest=window > 0)
+
+
+# ----------------------------------------------------------------------------- table entries outside of the pool
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("d,hkv,g,lens,rows,window,gone", [
+    (128, 2, 4, [100, 40], [1, 1], 0, [(0, 0), (0, 3), (1, 1)]),
+    (64, 1, 16, [700, 16], [1, 1], 0, [(0, 0), (0, 20), (0, 43), (1, 0)]),
+    (256, 2, 3, [90, 33], [1, 1], 20, [(0, 4), (1, 2)]),
+    (128, 2, 4, [300, 40], [300, 17], 0, [(0, 0), (0, 9), (0, 18), (1, 0), (1, 1), (1, 2)]),
+    (64, 4, 3, [500], [200], 0, [(0, 3), (0, 4), (0, 25)]),
+    (256, 2, 8, [300, 70], [90, 70], 0, [(0, 0), (0, 6), (1, 4)]),
+    (256, 1, 4, [400], [300], 50, [(0, 5), (0, 12)]),
+    (128, 1, 4, [4000], [30], 0, [(0, i) for i in range(0, 250, 3)]),
+    (128, 1, 8, [600, 90], [1, 90], 0, [(0, 30), (1, 0)]),
+])
+def test_blocks_outside_of_the_pool_are_skipped(d, hkv, g, lens, rows, window, gone, weigh):
+    """In every kernel alike: their tokens have no weight, and nothing of what lay in memory before comes in."""
+    gen = torch.Generator().manual_seed(d + sum(lens))
+    tables, nb = tables_for(lens, gen, DEV, extra_cols=1)
+    k, v, ks, vs = make_cache(nb, hkv, d, gen, DEV)
+    kk = [dequant(k, ks, t, n) for t, n in zip(tables, lens)]
+    vv = [dequant(v, vs, t, n) for t, n in zip(tables, lens)]
+    there = [torch.ones(n, dtype=torch.bool) for n in lens]
+    for x, (i, page) in enumerate(gone):
+        tables[i, page] = (-1, nb, -2 ** 31, 2 ** 31 - 1, -7)[x % 5]
+        there[i][page * BS:(page + 1) * BS] = False
+    q = torch.randn(sum(rows), hkv * g, d, generator=gen).to(torch.bfloat16).to(DEV)
+    start = torch.rand(len(lens), hkv, max(lens) + 3, generator=gen)
+    w = start.clone().to(DEV) if weigh else None
+    for _ in range(2):
+        if weigh:
+            w.copy_(start)
+        got = ops.paged_attention(q, k, v, batch_of(lens, rows, tables), d ** -0.5, ks, vs, window or None, weights=w)
+        r0 = 0
+        for i, (n, r) in enumerate(zip(lens, rows)):
+            out, mag, amp, sums = attention64_over(q[r0:r0 + r], kk[i], vv[i], d ** -0.5, window, there[i])
+            assert (got[r0:r0 + r].double().cpu() - out).abs().le(attention_bound(out, mag, amp, d)).all()
+            if weigh:
+                have, want = w[i].double().cpu(), start[i].double()
+                want[:, :n] += sums
+                rel = 4 * (d / 16 + 8) * 2.0 ** -23 * (float(amp.max()) + 2.0) + 2.0 ** -20
+                assert (have[:, :n] - want[:, :n]).abs().le(rel * sums + (r * g / 32 + 8) * 2.0 ** -23 * want[:, :n] + 1e-37).all()
+                assert torch.equal(have[:, n:], want[:, n:])
+            r0 += r
+    assert K.check_status() == 0
