@@ -5,9 +5,9 @@
 //
 //   o = sum_j 2^(s_j) 2^ev v^_j / sum_j 2^(s_j) = sum_j p_j v^_j / sum_j p_j 2^-ev,     p_j = 2^(s_j + ev - M)
 //
-// so both scales ride in the exponent's multiply-add and the codes go to the tensor cores as they are.  M is the running maximum of
-// s_j + ev, that is of what a token can add to the output: p in f16 keeps its 11 bits wherever they matter, however far the pages'
-// scales are apart.  q is brought to 2^14 by a power of two and is exact in f16; the sums are fp32.
+// so both scales ride in the exponent's multiply-add and the codes go to the tensor cores as they are.  M follows the maximum of s_j + ev, that is
+// of what a token can add to the output, over the pages whose ev lie close together, and p is f16; pages whose ev is far from theirs have p as two
+// bf16 terms and hardly move M (tc_util.cuh).  q is brought to 2^14 by a power of two; the sums are fp32.
 //
 // scaled_decode_kernel: bound by the cache's bytes (2 D a token and key head).  The pages of all (sequence, key head) pairs form one list, cut
 // into equal runs, a run per warp: ragged batches and single long sequences fill the GPU alike.  A warp is on its own: it copies its pages
@@ -50,6 +50,12 @@ struct ScaledDecodeParams {
 ATLAS_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+ATLAS_DEVICE void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -101,7 +107,7 @@ ATLAS_DEVICE int run_length(int pages, int warps) { return max((pages + warps - 
 // One entry of the page list.
 struct PageRef {
   int item;            // (sequence * Hkv + key head) * tiles + tile
-  int tok0;            // first token of the page
+  int tok0;            // first token of the page, one more for a far page (tc_util.cuh)
   int block;           // -1: an entry outside of the pool, skipped
   float sk, ev;        // key scale, value exponent
 };
@@ -201,12 +207,18 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
     const int pair = at / np, pg = first + at % np;
     r.item = b * hn + pair;
     r.tok0 = pg * kSdPage;
-    const int block = p.block_tables[(long long)b * p.bt_ld + pg];
+    const int* row = p.block_tables + (long long)b * p.bt_ld;
+    const int block = row[pg], ends[2] = {row[first], row[first + np - 1]};
     if (block >= 0 && block < p.num_pages) {
       const int h = pair / p.tiles;
+      auto value_exponent = [&](int blk) { return scale_exponent(p.v_scale[blk * p.vs_ld + h * p.vs_h]); };
+      const int ev = value_exponent(block);
       r.block = block;
       r.sk = p.k_scale[block * p.ks_ld + h * p.ks_h];
-      r.ev = (float)((int)((__float_as_uint(p.v_scale[block * p.vs_ld + h * p.vs_h]) >> 23) & 255u) - 127);
+      r.ev = (float)ev;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (exponents_apart(ev, value_exponent((unsigned)ends[i] < (unsigned)p.num_pages ? ends[i] : block))) r.tok0 |= 1;
     }
     return r;
   };
@@ -314,7 +326,9 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
       ++cur_chunk;
       nxt = fetch(cur_chunk + 1);
     }
-    const int it = __shfl_sync(0xffffffffu, cur.item, i & 31), tok0 = __shfl_sync(0xffffffffu, cur.tok0, i & 31);
+    const int it = __shfl_sync(0xffffffffu, cur.item, i & 31), tok0_far = __shfl_sync(0xffffffffu, cur.tok0, i & 31);
+    const int tok0 = tok0_far & ~1;
+    const bool far = tok0_far & 1;
     const int block = __shfl_sync(0xffffffffu, cur.block, i & 31);
     const float sk = __shfl_sync(0xffffffffu, cur.sk, i & 31), ev = __shfl_sync(0xffffffffu, cur.ev, i & 31);
     if (it != item) {
@@ -359,7 +373,7 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
           if (tok < lo_tok || tok >= len) vmask &= ~(0xffu << (8 * j));
         }
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[NT][2], pl[NT][2];                  // p of tokens tok_r and tok_r + 2; a far page: the first terms, the second ones
       const float undo = __uint_as_float((uint32_t)(127 - (int)ev) << 23);     // 2^-ev
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -374,15 +388,16 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
         }
         const float s00 = see0 ? fmaf(sc[nt][0], f0, ev) : -INFINITY, s01 = see0 ? fmaf(sc[nt][1], f1, ev) : -INFINITY;
         const float s10 = see1 ? fmaf(sc[nt][2], f0, ev) : -INFINITY, s11 = see1 ? fmaf(sc[nt][3], f1, ev) : -INFINITY;
-        float x0 = fmaxf(s00, s10), x1 = fmaxf(s01, s11);
-        // The reference moves only when a score passes it by 2^8 (p stays inside f16): rarely after the first pages.
-        if (__any_sync(0xffffffffu, x0 > m0[nt] + 8.f || x1 > m1[nt] + 8.f)) {
+        const float slack = far ? kFarSlack : 0.f;
+        float x0 = fmaxf(s00, s10) - slack, x1 = fmaxf(s01, s11) - slack;
+        // The reference moves only when a score passes what set it by 2^8 (p stays inside f16): rarely after the first pages.
+        if (__any_sync(0xffffffffu, x0 > m0[nt] + kMoves || x1 > m1[nt] + kMoves)) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
           }
-          const float n0m = fmaxf(m0[nt], x0), n1m = fmaxf(m1[nt], x1);
+          const float n0m = fmaxf(m0[nt], x0 - kHeadroom), n1m = fmaxf(m1[nt], x1 - kHeadroom);
           const float r0 = m0[nt] == -INFINITY ? 0.f : fast_exp2(m0[nt] - n0m), r1 = m1[nt] == -INFINITY ? 0.f : fast_exp2(m1[nt] - n1m);
           m0[nt] = n0m; m1[nt] = n1m;
           l0[nt] *= r0; l1[nt] *= r1;
@@ -393,18 +408,45 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
         const float p00 = fast_exp2(s00 - r0), p01 = fast_exp2(s01 - r1), p10 = fast_exp2(s10 - r0), p11 = fast_exp2(s11 - r1);
         l0[nt] += (p00 + p10) * undo;
         l1[nt] += (p01 + p11) * undo;
-        pb[nt][0] = transpose8x8(f16x2(p00, p01));
-        pb[nt][1] = transpose8x8(f16x2(p10, p11));
+        if (!far) {
+          pb[nt][0] = transpose8x8(f16x2(p00, p01));
+          pb[nt][1] = transpose8x8(f16x2(p10, p11));
+        } else {
+          uint32_t hi[2], lo[2];
+          two_terms(p00, p01, hi[0], lo[0]);
+          two_terms(p10, p11, hi[1], lo[1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) { pb[nt][j] = transpose8x8(hi[j]); pl[nt][j] = transpose8x8(lo[j]); }
+        }
       }
       // ---- outputs: rows are channels, a lane takes tokens 4t .. 4t + 3 of channels 16 k + g and + 8
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
+      auto values = [&](int k, uint32_t (&f)[4]) {
         const uint32_t x = *reinterpret_cast<const uint32_t*>(vp + (16 * k + g) * kSdPage + 4 * t) & vmask;
         const uint32_t y = *reinterpret_cast<const uint32_t*>(vp + (16 * k + g + 8) * kSdPage + 4 * t) & vmask;
-        const uint32_t f0 = e4m3x2_to_f16x2(x & 0xffffu), f1 = e4m3x2_to_f16x2(y & 0xffffu);
-        const uint32_t f2 = e4m3x2_to_f16x2(x >> 16), f3 = e4m3x2_to_f16x2(y >> 16);
+        f[0] = e4m3x2_to_f16x2(x & 0xffffu); f[1] = e4m3x2_to_f16x2(y & 0xffffu);
+        f[2] = e4m3x2_to_f16x2(x >> 16); f[3] = e4m3x2_to_f16x2(y >> 16);
+      };
+      if (!far) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][k], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
+        for (int k = 0; k < KS; ++k) {
+          uint32_t f[4];
+          values(k, f);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][k], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t f[4];
+          values(k, f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[j] = h2_to_bf2(f[j]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_bf16(acc[nt][k], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
+            mma_bf16(acc[nt][k], f[0], f[1], f[2], f[3], pl[nt][0], pl[nt][1]);
+          }
+        }
       }
     } else if (p.scores) {                            // a page outside of the pool is skipped, its tokens get no weight
       const int c0 = (it % p.tiles) * 8 * NT;

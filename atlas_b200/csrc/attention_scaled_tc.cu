@@ -2,7 +2,7 @@
 // that each cached token got from a chunk's rows.
 //
 // As in attention_scaled.cu the codes are the operands and the scales live in the exponent: s_j = f q . k^_j with f = softmax scale * log2(e) * key
-// page's scale, p_j = 2^(s_j + ev - M) in f16, o = sum p_j v^_j / sum p_j 2^-ev.  A page covers 16 score columns, so f and ev - M are constants
+// page's scale, p_j = 2^(s_j + ev - M) in f16 or, in key tiles with a far page (tc_util.cuh), as two bf16 terms, o = sum p_j v^_j / sum p_j 2^-ev.  A page covers 16 score columns, so f and ev - M are constants
 // of a multiply-add over them, and a page's largest score is found before they are applied.
 //
 // scaled_chunk2_kernel (heads of 64 and 128), scaled_chunk_wide_kernel (256): tiles of 128 query rows of a key head; the G query heads of a key
@@ -13,6 +13,8 @@
 // scaled_chunk_weigh_kernel: a cluster of two CTAs per (128 cached tokens, key head); tiles of the chunk's rows go by, every other one to each.
 // S^T = K Q^T in bf16 (an e4m3 number is one exactly, and Q stays as it is): a TMEM lane is a token, so that the sum over rows and heads is a
 // register's sum, and the two CTAs' sums are added in their order, with no atomics.
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_api.h"
 #include "tc_util.cuh"
@@ -44,6 +46,9 @@ ATLAS_DEVICE void sc_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* 
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+ATLAS_DEVICE void sc_expect(uint64_t* bar, uint32_t bytes) {      // without arriving
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 // The low word of a descriptor (make_smem_desc_sw128) carries the address, which steps along K; the high word is the same for all tiles.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 ATLAS_DEVICE uint32_t desc_low(const void* p) { return ((smem_u32(p) & 0x3FFFFu) >> 4) | (1u << 16); }
@@ -70,11 +75,7 @@ ATLAS_DEVICE void sc_widen16(const uint4 v, uint4& lo, uint4& hi) {
   lo.x = sc_e4m3x2(v.x); lo.y = sc_e4m3x2(v.x >> 16); lo.z = sc_e4m3x2(v.y); lo.w = sc_e4m3x2(v.y >> 16);
   hi.x = sc_e4m3x2(v.z); hi.y = sc_e4m3x2(v.z >> 16); hi.z = sc_e4m3x2(v.w); hi.w = sc_e4m3x2(v.w >> 16);
 }
-ATLAS_DEVICE uint32_t h2_to_bf2(uint32_t v) {      // e4m3 numbers: exact in both
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-  return pack_bf16x2(f.x, f.y);
-}
-ATLAS_DEVICE int scale_exponent(float s) { return (int)((__float_as_uint(s) >> 23) & 255u) - 127; }
+ATLAS_DEVICE uint4 f16_to_bf16(uint4 v) { return make_uint4(h2_to_bf2(v.x), h2_to_bf2(v.y), h2_to_bf2(v.z), h2_to_bf2(v.w)); }
 ATLAS_DEVICE float exact_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // A page whose table entry lies outside of the pool is skipped: its codes are zeros, which the copying warp puts where the copy would have gone,
@@ -208,7 +209,7 @@ scaled_chunk_join_kernel(const ScChunkParams p) {
 // a part of the exponentials as polynomials, and the tiles half a step apart were slower or no faster.  8 x 1024 rows of 32 heads of 128:
 // 109 us, 630 TFLOP/s; two sequences of 3001 rows: 150.
 constexpr int kC2Threads = 512;
-constexpr int kC2Kv = 128, kC2Pages = 8, kC2Ring = 8;
+constexpr int kC2Kv = 128, kC2Pages = 8, kC2Ring = 8, kC2Scales = kC2Pages + 1;
 
 template <int D>
 struct C2Tile {
@@ -216,7 +217,7 @@ struct C2Tile {
   static constexpr int kK = (D / 64) * kScSub;                    // 128 keys
   static constexpr int kV = 2 * D * 128;                          // D channels x 128 tokens
   static constexpr int kStage = kC2Kv * D;                        // the pages of a key tile
-  static constexpr int kSmem = 2 * (kQ + kK + kV) + 2 * kStage + kC2Ring * 64 + 512 + 1024;      // at most 227 KB
+  static constexpr int kSmem = 2 * (kQ + kK + kV) + 2 * kStage + kC2Ring * kC2Scales * 8 + 448 + 1024;      // at most 227 KB
 };
 
 // A from TMEM: a row a lane, two 16-bit numbers a column
@@ -265,12 +266,13 @@ ATLAS_DEVICE float max3_nan(float a, float b, float c) {
   return r;
 }
 // A row's step over 64 score columns (a thread a row): their largest s + ev, then p = 2^(s + ev - m) as f16 over the first half of the columns
-// at tP.  f: (score factor, value exponent) of the four pages; columns [lo, hi) are visible.  The reference m moves only when a score passes
-// it by 2^8 (p stays inside f16), which is rare after a row's first columns; the output, where there is one, then moves with it, after
-// wait_output() has seen the last product that goes to it.  False: that wait ran out.
-template <int D, typename Wait>
-ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const float2 (&f)[4], bool whole, int hi, int lo, bool output, float& m, float& l,
-                               Wait wait_output) {
+// at tP, or, where the key tile has a far page (tc_util.cuh), as two bf16 terms over both halves.  f: (score factor, value exponent) of the four
+// pages; columns [lo, hi) are visible.  The reference m moves only when a score passes what set it by 2^8 (p stays inside f16), which is rare
+// after a row's first columns; the output, where there is one, then moves with it, after wait_output() has seen the last product that goes to
+// it.  False: that wait ran out.
+template <int D, bool kFar, typename Wait>
+ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const float2 (&f)[4], bool whole, int hi, int lo, bool output, float& m,
+                               float& l, Wait wait_output) {
   uint32_t v[2][32];
   tmem_ld_32x32b_x32(tS, v[0]);
   tmem_ld_32x32b_x32(tS + 32, v[1]);
@@ -296,12 +298,12 @@ ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const floa
     a = max3_nan(a, __uint_as_float(u[14]), __uint_as_float(u[15]));
     mx[q] = fmaf(max3_nan(a, z, z), f[q].x, f[q].y);
   }
-  const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-  if (__any_sync(0xffffffffu, !(top <= m + 8.f))) {               // NaN too: the row is NaN from here on
+  const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) - (kFar ? kFarSlack : 0.f);
+  if (__any_sync(0xffffffffu, !(top <= m + kMoves))) {            // NaN too: the row is NaN from here on
     float alpha = 1.f;
-    if (!(top <= m + 8.f)) {
-      alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - top);
-      m = top;
+    if (!(top <= m + kMoves)) {
+      alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - (top - kHeadroom));
+      m = top - kHeadroom;
     }
     l *= alpha;
     if (output) {
@@ -319,9 +321,8 @@ ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const floa
     }
   }
   const float ref = (m == -INFINITY) ? 0.f : m;
-  uint32_t w[2][16];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  // p of page q, two columns at a time: put(column / 2, p, p)
+  auto page = [&](int q, auto put) {
     const uint32_t* u = &v[q >> 1][(q & 1) * 16];
     const float add = f[q].y - ref;
     const uint64_t f2 = pair2(f[q].x, f[q].x), a2 = pair2(add, add);
@@ -333,16 +334,43 @@ ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const floa
       e.x = fast_exp2(e.x);
       e.y = fast_exp2(e.y);
       s2 = add2(s2, pair2(e.x, e.y));
-      w[q >> 1][(q & 1) * 8 + i / 2] = sc_h2(e.x, e.y);
+      put(i / 2, e.x, e.y);
     }
     const float2 s = unpair2(s2);
     l = fmaf(s.x + s.y, exact_pow2((int)fminf(-f[q].y, 127.f)), l);      // a skipped page: 0 times anything
+  };
+  if constexpr (!kFar) {
+    uint32_t w[2][16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) page(q, [&](int i, float a, float b) { w[q >> 1][(q & 1) * 8 + i] = sc_h2(a, b); });
+    tmem_st_32x32b_x16(tP, w[0]);
+    tmem_st_32x32b_x16(tP + 16, w[1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t hi2[16], lo2[16];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) page(2 * k + q, [&](int i, float a, float b) { two_terms(a, b, hi2[q * 8 + i], lo2[q * 8 + i]); });
+      tmem_st_32x32b_x16(tP + 16 * k, hi2);
+      tmem_st_32x32b_x16(tP + 32 + 16 * k, lo2);
+    }
   }
-  tmem_st_32x32b_x16(tP, w[0]);
-  tmem_st_32x32b_x16(tP + 16, w[1]);
   tmem_st_wait();
   return true;
 }
+
+// The value scales (powers of two) of pages that are not far: of the first page of the CTA's keys and the sequence's newest one, 0 where that is
+// not in the pool.
+struct NearScales {
+  float least, most;
+  ATLAS_DEVICE void begin(float first, float last) {
+    if (first == 0.f) first = last;
+    if (last == 0.f) last = first;
+    least = fmaxf(first, last) * exact_pow2(-kFarApart);
+    most = first == 0.f ? INFINITY : fminf(first, last) * exact_pow2(kFarApart);
+  }
+  ATLAS_DEVICE bool far(float scale) const { return scale < least || scale > most; }
+};
 
 struct alignas(16) C2Item {
   int b, kvh, split, L, q_row0, q_len, q0, ctx0, page0;           // b < 0: no more; page0: the first of this share of the keys
@@ -391,8 +419,8 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   uint8_t* sV = sK + 2 * Tile::kK;                                // two buffers: 2 sub-tiles [D channels][64 tokens]
   uint8_t* sStK = sV + 2 * Tile::kV;                              // the pages as they come, keys and values
   uint8_t* sStV = sStK + Tile::kStage;
-  float2* sScale = reinterpret_cast<float2*>(sStV + Tile::kStage);  // [kC2Ring][8] (score factor, value exponent) of a page
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + kC2Ring * 8);
+  float2* sScale = reinterpret_cast<float2*>(sStV + Tile::kStage);  // [kC2Ring][8 pages: (score factor, value exponent); is one far?]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + kC2Ring * kC2Scales);
   uint64_t* q_full = bars;
   uint64_t* q_free = bars + 1;                                    // the item's last QK
   uint64_t* k_full = bars + 2;                                    // [2] 4 warps
@@ -477,7 +505,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         const int kv0 = (m_.page0 + j * kC2Pages) * kScPg;
         const int hi = end - kv0, lo = start - kv0;
         const bool whole = __all_sync(0xffffffffu, hi >= kC2Kv && lo <= 0);
-        const float2* sc = sScale + ((ring + j) % kC2Ring) * 8;
+        const float2* sc = sScale + ((ring + j) % kC2Ring) * kC2Scales;
         // ---- 64 columns at a time; P takes half of the columns that its scores had
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {                               // no further unrolled: the roles' code shares one instruction cache
@@ -487,9 +515,12 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
           float2 f[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) f[q] = sc[c * 4 + q];
-          ok = softmax_step<D>(tS + c * 64, tS + c * 64, tO, f, whole, hi - c * 64, lo - c * 64, j > 0 || c == 1, m, l, [&] {
+          auto output_there = [&] {
             return (bool)__all_sync(0xffffffffu, mbar_wait(c ? &pv_half[x] : &pv_done[x], (n_s - 2 + c) & 1, abort_flag, p.status, 0xC04 + x));
-          });
+          };
+          ok = sc[kC2Pages].x == 0.f
+                   ? softmax_step<D, false>(tS + c * 64, tS + c * 64, tO, f, whole, hi - c * 64, lo - c * 64, j > 0 || c == 1, m, l, output_there)
+                   : softmax_step<D, true>(tS + c * 64, tS + c * 64, tO, f, whole, hi - c * 64, lo - c * 64, j > 0 || c == 1, m, l, output_there);
           if (!ok) break;
           tc_fence_before();
           __syncwarp();
@@ -543,8 +574,8 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
           sc_widen16(reinterpret_cast<const uint4*>(sStK)[trow * (D / 16) + c], lo, hi);
           uint8_t* rowp = sK + s * Tile::kK + (c >> 2) * kScSub + (trow >> 3) * 1024 + tsw * 128;
           const int ch = (c & 3) * 2;
-          *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = make_uint4(h2_to_bf2(lo.x), h2_to_bf2(lo.y), h2_to_bf2(lo.z), h2_to_bf2(lo.w));
-          *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ tsw) << 4)) = make_uint4(h2_to_bf2(hi.x), h2_to_bf2(hi.y), h2_to_bf2(hi.z), h2_to_bf2(hi.w));
+          *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = f16_to_bf16(lo);
+          *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ tsw) << 4)) = f16_to_bf16(hi);
         }
         fence_proxy_async();                                      // the tile for the products, and the pages read before they are copied over
         __syncwarp();
@@ -553,26 +584,31 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         ok = mbar_wait(&ks_full[1], n_t & 1, abort_flag, p.status, 0xC12) &&
              mbar_wait(&v_free[s], ((n_t >> 1) & 1) ^ 1u, abort_flag, p.status, 0xC13);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        auto widen = [&](auto far) {                              // a far page: bf16; the usual loop stays free of that
 #pragma unroll 4
-        for (int k = 0; k < kPer; ++k) {
-          const int i = k * 128 + value_piece(r), pg = i / D, dim = i % D, col = output_column(dim), sw = col & 7;
-          const int left = L - (page0 + j * kC2Pages + pg) * kScPg;      // tokens of the page; the others are cleared
-          uint4 v = reinterpret_cast<const uint4*>(sStV)[i];
-          if (left < kScPg) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+          for (int k = 0; k < kPer; ++k) {
+            const int i = k * 128 + value_piece(r), pg = i / D, dim = i % D, col = output_column(dim), sw = col & 7;
+            const int left = L - (page0 + j * kC2Pages + pg) * kScPg;      // tokens of the page; the others are cleared
+            uint4 v = reinterpret_cast<const uint4*>(sStV)[i];
+            if (left < kScPg) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int there = min(max(left - 4 * q, 0), 4);
-              w[q] = there == 4 ? w[q] : (w[q] & ((1u << (8 * there)) - 1u));
+              for (int q = 0; q < 4; ++q) {
+                const int there = min(max(left - 4 * q, 0), 4);
+                w[q] = there == 4 ? w[q] : (w[q] & ((1u << (8 * there)) - 1u));
+              }
             }
+            uint4 lo, hi;
+            sc_widen16(v, lo, hi);
+            if constexpr (decltype(far)::value) { lo = f16_to_bf16(lo); hi = f16_to_bf16(hi); }
+            uint8_t* rowp = sV + s * Tile::kV + (pg >> 2) * (D * 128) + col * 128;
+            const int ch = (pg & 3) * 2;
+            *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
+            *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
           }
-          uint4 lo, hi;
-          sc_widen16(v, lo, hi);
-          uint8_t* rowp = sV + s * Tile::kV + (pg >> 2) * (D * 128) + col * 128;
-          const int ch = (pg & 3) * 2;
-          *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
-          *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
-        }
+        };
+        if (sScale[n_t % kC2Ring * kC2Scales + kC2Pages].x == 0.f) widen(std::false_type{});
+        else widen(std::true_type{});
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) { mbar_arrive(&v_full[s]); mbar_arrive(&ks_free[1]); }
@@ -594,8 +630,11 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         if ((unsigned)blk >= (unsigned)p.num_pages) return 1.f;
         return is_v ? p.v_scale[blk * p.vs_ld + m_.kvh * p.vs_h] : p.k_scale[blk * p.ks_ld + m_.kvh * p.ks_h];
       };
+      const int newest = n_pages > 0 ? bt[n_pages - 1] : -1;
       int blk = entry(0), blk1 = entry(1);
+      const float last = (unsigned)newest < (unsigned)p.num_pages ? p.v_scale[newest * p.vs_ld + m_.kvh * p.vs_h] : 0.f;
       float sc = scale_of(blk);
+      NearScales near;
       for (int j = 0; j < m_.n_kv; ++j, ++n_t) {
         const int blk2 = entry(j + 2);
         const float sc1 = scale_of(blk1);
@@ -603,18 +642,25 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         const uint32_t pages = __ballot_sync(0xffffffffu, live);
         const bool skip = lane < 8 && m_.page0 + j * kC2Pages + lane < n_pages && !live;
         const uint32_t skipped = __ballot_sync(0xffffffffu, skip);
-        const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
-        if (lane < 8) sScale[(n_t % kC2Ring) * 8 + lane] = skip ? skipped_page() : make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
-        __syncwarp();
         const long long at = ((long long)blk * p.Hkv + m_.kvh) * (kScPg * D);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           ok = mbar_wait(&ks_free[w], (n_t & 1) ^ 1u, abort_flag, p.status, 0xC30 + w);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           if (skipped) clear_pages<D>(w ? sStV : sStK, skipped);
-          if (lane == 0) mbar_expect_tx(&ks_full[w], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
+          if (lane == 0) sc_expect(&ks_full[w], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
           __syncwarp();
           if (live && is_v == (w == 1)) sc_bulk((w ? sStV : sStK) + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &ks_full[w]);
+          if (w == 0) {                                             // under the copies: the scales may not be there yet
+            const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
+            if (j == 0) near.begin(pages >> 8 & 1 ? __shfl_sync(0xffffffffu, sc, 8) : 0.f, last);
+            const bool far = __any_sync(0xffffffffu, live && is_v && near.far(sc));
+            float2* to = sScale + n_t % kC2Ring * kC2Scales;
+            if (lane < 8) to[lane] = skip ? skipped_page() : make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
+            if (lane == 8) to[kC2Pages].x = far;
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&ks_full[w]);
         }
         if (!ok) break;
         blk = blk1; blk1 = blk2;
@@ -626,7 +672,8 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
   } else if (warp == 12 || warp == 14) {
     // ------------------------------------------------------------------ products of tile x, each tile at its own pace.  The whole warp walks the
     // list and one elected lane issues: descriptors stay in uniform registers so (under a lane's branch an MMA took 110 clocks to issue).
-    constexpr uint32_t kIdescS = make_idesc(kScRows, 64, 1u), kIdescO = make_idesc(kScRows, D, 0u);      // bf16 scores, f16 outputs
+    constexpr uint32_t kIdescS = make_idesc(kScRows, 64, 1u);      // bf16 scores
+    constexpr uint32_t kIdescO = make_idesc(kScRows, D, 0u), kIdescFar = make_idesc(kScRows, D, 1u);      // f16 outputs; bf16, of two terms
     const int x = (warp - 12) >> 1;
     const uint32_t dQ = desc_low(sQ + x * Tile::kQ), dK = desc_low(sK), dV = desc_low(sV);
     const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * D;
@@ -677,10 +724,17 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
             ok = wait(&p_ready[2 * x + half], (pvs - half) & 1, 0xC2A);
             if (!ok) break;
             tc_fence_after();
+            const bool far = sScale[n_t % kC2Ring * kC2Scales + kC2Pages].x != 0.f;
             if (elect_one()) {
-              const uint32_t bd = dV + (n_t & 1) * (Tile::kV >> 4) + half * (D * 128 >> 4);
+              const uint32_t tP = tS + half * 64, bd = dV + (n_t & 1) * (Tile::kV >> 4) + half * (D * 128 >> 4);
+              const uint32_t more = j > 0 || half > 0;
+              if (!far) {
 #pragma unroll
-              for (int ks = 0; ks < kC2Kv / 32; ++ks) umma_f16_ta(tO, tS + half * 64 + ks * 8, bd + 2 * ks, kIdescO, (j > 0 || half > 0 || ks > 0) ? 1u : 0u);
+                for (int ks = 0; ks < kC2Kv / 32; ++ks) umma_f16_ta(tO, tP + ks * 8, bd + 2 * ks, kIdescO, ks > 0 ? 1u : more);
+              } else {
+#pragma unroll
+                for (int ks = 0; ks < kC2Kv / 16; ++ks) umma_f16_ta(tO, tP + ks * 8, bd + 2 * (ks % 4), kIdescFar, ks > 0 ? 1u : more);
+              }
               if (half == 0) {
                 umma_commit(&pv_half[x]);
               } else {
@@ -780,6 +834,7 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
   uint64_t* q_ready = bars + 22;                                  // 4 warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  uint32_t* sFar = tmem_slot + 2;                                 // [kWideRing] whether a key tile has a far page
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.G, toks = kScRows / G;
@@ -851,9 +906,9 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = sScale[(j % kWideRing) * kWidePages + i];
       const uint32_t tS = tmem + sb * kWideKv + t_lane;
-      ok = softmax_step<D>(tS, tS, tO, f, whole, hi, lo, j > 0, m, l, [&] {
-        return (bool)__all_sync(0xffffffffu, mbar_wait(&pv_done[sb ^ 1], ((j - 1) >> 1) & 1, abort_flag, p.status, 0xA01));
-      });
+      auto output_there = [&] { return (bool)__all_sync(0xffffffffu, mbar_wait(&pv_done[sb ^ 1], ((j - 1) >> 1) & 1, abort_flag, p.status, 0xA01)); };
+      ok = sFar[j % kWideRing] == 0 ? softmax_step<D, false>(tS, tS, tO, f, whole, hi, lo, j > 0, m, l, output_there)
+                                    : softmax_step<D, true>(tS, tS, tO, f, whole, hi, lo, j > 0, m, l, output_there);
       if (!ok) break;
       tc_fence_before();
       __syncwarp();
@@ -887,8 +942,8 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
         uint4 lo, hi;
         sc_widen16(*reinterpret_cast<const uint4*>(sStK + s * Tile::kStage + trow * D + sub * 64 + (lane & 3) * 16), lo, hi);
         uint8_t* rowp = sK + s * Tile::kK + sub * Tile::kSub + trow * 128;
-        *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = make_uint4(h2_to_bf2(lo.x), h2_to_bf2(lo.y), h2_to_bf2(lo.z), h2_to_bf2(lo.w));
-        *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ tsw) << 4)) = make_uint4(h2_to_bf2(hi.x), h2_to_bf2(hi.y), h2_to_bf2(hi.z), h2_to_bf2(hi.w));
+        *reinterpret_cast<uint4*>(rowp + ((ch ^ tsw) << 4)) = f16_to_bf16(lo);
+        *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ tsw) << 4)) = f16_to_bf16(hi);
       }
       fence_proxy_async();                                        // the tile for the products, and the pages read before they are copied over
       __syncwarp();
@@ -902,25 +957,30 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       const bool ok = mbar_wait(&stage_full[2 + s], (j >> 1) & 1, abort_flag, p.status, 0xA12) &&
                       mbar_wait(&v_free[s], ((j >> 1) & 1) ^ 1u, abort_flag, p.status, 0xA13);
       if (!__all_sync(0xffffffffu, ok)) break;
+      auto widen = [&](auto far) {                                // a far page: bf16; the usual loop stays free of that
 #pragma unroll 4
-      for (int k = 0; k < kWidePages * D / 128; ++k) {
-        const int i = k * 128 + value_piece(r), pg = i / D, dim = i % D, col = output_column(dim), sw = col & 7, ch = pg * 2;
-        const int left = L - (page0 + j * kWidePages + pg) * kScPg;       // tokens of the page; the others are cleared
-        uint4 v = reinterpret_cast<const uint4*>(sStV + s * Tile::kStage)[i];
-        if (left < kScPg) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+        for (int k = 0; k < kWidePages * D / 128; ++k) {
+          const int i = k * 128 + value_piece(r), pg = i / D, dim = i % D, col = output_column(dim), sw = col & 7, ch = pg * 2;
+          const int left = L - (page0 + j * kWidePages + pg) * kScPg;       // tokens of the page; the others are cleared
+          uint4 v = reinterpret_cast<const uint4*>(sStV + s * Tile::kStage)[i];
+          if (left < kScPg) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int there = min(max(left - 4 * q, 0), 4);
-            w[q] = there == 4 ? w[q] : (w[q] & ((1u << (8 * there)) - 1u));
+            for (int q = 0; q < 4; ++q) {
+              const int there = min(max(left - 4 * q, 0), 4);
+              w[q] = there == 4 ? w[q] : (w[q] & ((1u << (8 * there)) - 1u));
+            }
           }
+          uint4 lo, hi;
+          sc_widen16(v, lo, hi);
+          if constexpr (decltype(far)::value) { lo = f16_to_bf16(lo); hi = f16_to_bf16(hi); }
+          uint8_t* rowp = sV + s * Tile::kV + col * 128;
+          *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
+          *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
         }
-        uint4 lo, hi;
-        sc_widen16(v, lo, hi);
-        uint8_t* rowp = sV + s * Tile::kV + col * 128;
-        *reinterpret_cast<uint4*>(rowp + ((ch ^ sw) << 4)) = lo;
-        *reinterpret_cast<uint4*>(rowp + (((ch + 1) ^ sw) << 4)) = hi;
-      }
+      };
+      if (sFar[j % kWideRing] == 0) widen(std::false_type{});
+      else widen(std::true_type{});
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) { mbar_arrive(&v_full[s]); mbar_arrive(&stage_free[2 + s]); }
@@ -948,14 +1008,21 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
           __syncwarp();
         }
     } else {
-      constexpr uint32_t kIdesc = make_idesc(kScRows, D, 0u);               // f16
+      constexpr uint32_t kIdesc = make_idesc(kScRows, D, 0u), kIdescFar = make_idesc(kScRows, D, 1u);      // f16; bf16, of two terms
       for (int j = 0; j < n_kv; ++j) {
         if (!wait(v_full, j, 0xA22) || !wait(p_ready, j, 0xA23)) break;
         tc_fence_after();
+        const bool far = sFar[j % kWideRing] != 0;
         if (elect_one()) {
+          const uint32_t tP = tmem + (j & 1) * kWideKv, bd = dV + (j & 1) * (Tile::kV >> 4);
+          const uint32_t more = j > 0;
+          if (!far) {
 #pragma unroll
-          for (int ks = 0; ks < kWideKv / 16; ++ks)
-            umma_f16_ta(tO, tmem + (j & 1) * kWideKv + ks * 8, dV + (j & 1) * (Tile::kV >> 4) + 2 * ks, kIdesc, (j > 0 || ks > 0) ? 1u : 0u);
+            for (int ks = 0; ks < kWideKv / 16; ++ks) umma_f16_ta(tO, tP + ks * 8, bd + 2 * ks, kIdesc, ks > 0 ? 1u : more);
+          } else {
+#pragma unroll
+            for (int ks = 0; ks < kWideKv / 8; ++ks) umma_f16_ta(tO, tP + ks * 8, bd + 2 * (ks % 4), kIdescFar, ks > 0 ? 1u : more);
+          }
           umma_commit(&pv_done[j & 1]);
           umma_commit(&v_free[j & 1]);
         }
@@ -975,8 +1042,11 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       if ((unsigned)blk >= (unsigned)p.num_pages) return 1.f;
       return is_v ? p.v_scale[blk * p.vs_ld + kvh * p.vs_h] : p.k_scale[blk * p.ks_ld + kvh * p.ks_h];
     };
+    const int newest = n_pages > 0 ? bt[n_pages - 1] : -1;
     int blk = entry(0), blk1 = entry(1);
+    const float last = (unsigned)newest < (unsigned)p.num_pages ? p.v_scale[newest * p.vs_ld + kvh * p.vs_h] : 0.f;
     float sc = scale_of(blk);
+    NearScales near;
     bool ok = true;
     for (int j = 0; j < n_kv; ++j) {
       const int blk2 = entry(j + 2), s = j & 1;
@@ -985,22 +1055,25 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       const uint32_t pages = __ballot_sync(0xffffffffu, live);
       const bool skip = lane < kWidePages && page0 + j * kWidePages + lane < n_pages && !live;
       const uint32_t skipped = __ballot_sync(0xffffffffu, skip);
-      const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
       const long long at = ((long long)blk * p.Hkv + kvh) * (kScPg * D);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         ok = mbar_wait(&stage_free[2 * w + s], ((j >> 1) & 1) ^ 1u, abort_flag, p.status, 0xA30 + w);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        if (w == 0) {                                             // tile j - kWideRing is done: its keys left this stage long ago
-          if (lane < kWidePages)
-            sScale[(j % kWideRing) * kWidePages + lane] = skip ? skipped_page() : make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
-          __syncwarp();
-        }
         if (skipped) clear_pages<D>((w ? sStV : sStK) + s * Tile::kStage, skipped);
-        if (lane == 0) mbar_expect_tx(&stage_full[2 * w + s], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
+        if (lane == 0) sc_expect(&stage_full[2 * w + s], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
         __syncwarp();
         if (live && is_v == (w == 1))
           sc_bulk((w ? sStV : sStK) + s * Tile::kStage + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &stage_full[2 * w + s]);
+        if (w == 0) {                                             // under the copies, as above; tile j - kWideRing is done: its keys left this stage long ago
+          const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
+          if (j == 0) near.begin(pages >> 8 & 1 ? __shfl_sync(0xffffffffu, sc, 8) : 0.f, last);
+          const bool far = __any_sync(0xffffffffu, live && is_v && near.far(sc));
+          if (lane < kWidePages) sScale[(j % kWideRing) * kWidePages + lane] = skip ? skipped_page() : make_float2(p.scale_log2 * sc, (float)scale_exponent(vs));
+          if (lane == 8) sFar[j % kWideRing] = far;
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&stage_full[2 * w + s]);
       }
       if (!ok) break;
       blk = blk1; blk1 = blk2;

@@ -4,7 +4,7 @@ import torch
 
 from atlas_b200 import ops
 from atlas_b200.ops import cuda as K
-from kv_scaled_cases import BS, attention64_over, attention_bound, dequant, make_cache, tables_for
+from kv_scaled_cases import BS, FP8, attention64_over, attention_bound, dequant, make_cache, power_scale, tables_for
 from test_gpu_kv_scaled import batch_of, check_attention
 
 pytestmark = pytest.mark.gpu
@@ -66,3 +66,77 @@ def test_blocks_outside_of_the_pool_are_skipped(d, hkv, g, lens, rows, window, g
                 assert torch.equal(have[:, n:], want[:, n:])
             r0 += r
     assert K.check_status() == 0
+
+
+# ----------------------------------------------------------------------------- values of very different size
+def _check(q, k, v, ks, vs, tables, lens, rows, scale, window=0):
+    got = ops.paged_attention(q, k, v, batch_of(lens, rows, tables), scale, ks, vs, window or None)
+    assert K.check_status() == 0
+    r0 = 0
+    for i, (n, r) in enumerate(zip(lens, rows)):
+        out, mag, amp, _ = attention64_over(q[r0:r0 + r], dequant(k, ks, tables[i], n), dequant(v, vs, tables[i], n), scale, window)
+        assert (got[r0:r0 + r].double().cpu() - out).abs().le(attention_bound(out, mag, amp, q.shape[2])).all()
+        r0 += r
+
+
+def _put(cache, scales, block, values):
+    """A block's values [16, hkv, d], rounded by its own scales."""
+    s = power_scale(values.abs().amax((0, 2)))
+    codes = (values / s[None, :, None]).float().clamp(-448, 448).to(FP8)
+    cache.view(torch.uint8)[block] = codes.view(torch.uint8).to(cache.device)
+    scales[block] = s.float().to(scales.device)
+
+
+LOUD = [  # d, hkv, g, length, rows, window, page of the loud token, its place there
+    (128, 2, 4, 300, 1, 0, 7, 3),
+    (128, 2, 4, 300, 1, 0, 0, 0),
+    (128, 2, 4, 300, 1, 0, 18, 5),                        # the newest page
+    (64, 1, 12, 1000, 1, 0, 30, 15),
+    (256, 1, 8, 700, 1, 0, 20, 9),
+    (128, 1, 4, 200, 1, 100, 6, 2),                       # outside of the window, its neighbours are not
+    (128, 2, 4, 300, 40, 0, 7, 3),
+    (128, 2, 4, 300, 40, 0, 0, 1),
+    (128, 2, 4, 300, 300, 0, 9, 14),                      # behind most rows
+    (128, 2, 4, 300, 200, 0, 18, 11),                     # the newest token of all
+    (64, 2, 3, 400, 150, 0, 12, 0),
+    (64, 2, 3, 400, 150, 60, 16, 7),
+    (256, 2, 8, 300, 40, 0, 3, 8),
+    (256, 1, 4, 500, 300, 0, 20, 2),
+    (256, 1, 4, 2100, 16, 0, 60, 2),
+    (128, 1, 4, 4000, 30, 0, 100, 6),
+]
+
+
+@pytest.mark.parametrize("ratio", [16, 20, 26, 40])
+@pytest.mark.parametrize("weight", ["none", "some"])
+@pytest.mark.parametrize("d,hkv,g,n,r,window,page,place", LOUD)
+def test_a_loud_token_beside_quiet_ones(d, hkv, g, n, r, window, page, place, weight, ratio):
+    """One token's values are 2^ratio times all others'.  It has no weight to speak of, or one of about 2^-ratio, with which it is a good part of
+    the output."""
+    gen = torch.Generator().manual_seed(n + page)
+    tables, nb = tables_for([n], gen, DEV)
+    k, v, ks, vs = make_cache(nb, hkv, d, gen, DEV, spread=1)
+    scale = d ** -0.5
+    k.view(torch.uint8)[..., 0] = 0                        # channel 0 is that token's alone
+    block = int(tables[0, page])
+    keys, values = dequant(k, ks, tables[0, page:page + 1], BS), dequant(v, vs, tables[0, page:page + 1], BS)
+    keys[place, :, 0] = -(150.0 if weight == "none" else ratio) / (4.0 * scale * 1.4427)
+    values[place] *= 2.0 ** ratio
+    _put(k, ks, block, keys)
+    _put(v, vs, block, values)
+    q = torch.randn(r, hkv * g, d, generator=gen) * 0.5
+    q[..., 0] = 4.0
+    _check(q.to(torch.bfloat16).to(DEV), k, v, ks, vs, tables, [n], [r], scale, window)
+
+
+@pytest.mark.parametrize("spread", [12, 28])
+@pytest.mark.parametrize("d,hkv,g,lens,rows,window", [
+    (128, 4, 4, [300, 77, 1200], [1, 1, 1], 0), (64, 2, 16, [500, 31], [1, 1], 40), (256, 2, 5, [260, 700], [1, 1], 0),
+    (128, 2, 4, [300, 129], [300, 40], 0), (64, 4, 3, [513], [200], 100), (256, 2, 8, [530, 70], [17, 70], 0), (128, 1, 8, [3000], [20], 0)])
+def test_scales_all_over_the_place(d, hkv, g, lens, rows, window, spread):
+    gen = torch.Generator().manual_seed(d + spread)
+    tables, nb = tables_for(lens, gen, DEV)
+    k, v, ks, vs = make_cache(nb, hkv, d, gen, DEV, spread=1)
+    vs *= torch.exp2(torch.randint(-spread, spread + 1, (nb, hkv), generator=gen).float()).to(DEV)
+    q = torch.randn(sum(rows), hkv * g, d, generator=gen).to(torch.bfloat16).to(DEV)
+    _check(q, k, v, ks, vs, tables, lens, rows, d ** -0.5, window)
