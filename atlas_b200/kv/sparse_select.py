@@ -116,7 +116,7 @@ def attend_selected(ops_paged_attention, selector: Optional[BlockSelector], laye
         return ops_paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, window)
     sub = dataclasses.replace(batch, block_tables=tab, seq_lens=lens,
                               max_seq_len=min(batch.max_seq_len, selector.budget * selector.bs))
-    for name in ("_attn_tiles", "_mrope"):
+    for name in ("_step_lists", "_mrope"):
         if hasattr(sub, name):
             delattr(sub, name)
     return ops_paged_attention(q, k_cache, v_cache, sub, scale, k_scale, v_scale, window)

@@ -730,17 +730,7 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
             _check(rc, "attn_prefill_tc")
             return out
     if batch.num_seqs > nd:
-        tiles = getattr(batch, "_attn_tiles", None)
-        if tiles is None:
-            ts, tq = [], []
-            for i in range(nd, batch.num_seqs):
-                for q0 in range(0, batch.query_lens_host[i], 16):
-                    ts.append(i)
-                    tq.append(q0)
-            host = torch.tensor([ts, tq], dtype=torch.int32).pin_memory()
-            tiles = (host.to(q.device, non_blocking=True), len(ts))
-            batch._attn_tiles = tiles
-        tdev, n_tiles = tiles
+        tdev, n_tiles = _row_tiles(q, batch, nd)
         _check(lib().atlas_attn_prefill(q.data_ptr(), q.stride(0), out.data_ptr(), Hq * D, k_cache.data_ptr(),
                                         v_cache.data_ptr(), bt.data_ptr(), bt.stride(0), batch.seq_lens.data_ptr(),
                                         batch.query_start_loc.data_ptr(), tdev[0].data_ptr(), tdev[1].data_ptr(),
@@ -801,10 +791,42 @@ def paged_attention_q8(q, k_cache, v_cache, batch, scale, k_scale, v_scale, slid
     return qo, so
 
 
+def _list_place(device):
+    """(stream that an upload is ordered with, whether a graph is being captured)"""
+    return torch._C._cuda_getCurrentRawStream(device.index), torch._C._cuda_isCurrentStreamCapturing()
+
+
+def _upload(rows, device):
+    host = torch.tensor(rows, dtype=torch.int32).pin_memory()
+    return host.to(device, non_blocking=True), host
+
+
+def step_list(batch, kind: str, build, device):
+    """(device tensor [rows, n], n) of what ``build()`` lists of the step's host lengths, int32, kept on the batch for the layers that come.
+
+    One list a stream: an upload is ordered with its own stream only.  A list of other lengths than the batch has by now is made anew.  A graph
+    that is being captured takes a list that is there (the capture began with a device at rest), and what it took stays with the batch."""
+    nd, lens, rows = batch.num_decodes, batch.seq_lens_host, batch.query_lens_host
+    fits = lambda e: e[0] == nd and e[1] == lens and e[2] == rows
+    lists = batch.__dict__.setdefault("_step_lists", {})
+    stream, capturing = _list_place(device)
+    entry = lists.get((kind, device, stream))
+    if entry is None or not fits(entry):
+        entry = None
+        if capturing:
+            entry = next((e for (k, d, _), e in lists.items() if k == kind and d == device and fits(e)), None)
+        if entry is None:
+            listed = build()
+            entry = (nd, list(lens), list(rows), len(listed[0])) + _upload(listed, device)
+            lists[kind, device, stream] = entry
+    if capturing:
+        batch.__dict__.setdefault("_captured_lists", []).append(entry)
+    return entry[4], entry[3]
+
+
 def _tc_tiles(q, batch, nd: int, tok: int):
     """(device tensor [2, n] of (sequence, first chunk token) per query tile of ``tok`` tokens, n, tok), cached on the batch."""
-    tiles = getattr(batch, "_attn_tiles_tc", None)
-    if tiles is None or tiles[2] != tok:
+    def build():
         work = []
         for i in range(nd, batch.num_seqs):
             qlen = batch.query_lens_host[i]
@@ -814,11 +836,16 @@ def _tc_tiles(q, batch, nd: int, tok: int):
         # tiles with the most keys first: a causal tile costs up to 8x another, and blocks are handed to SMs in index
         # order, so the short ones fill the tail of the launch instead of the long ones making it
         work.sort()
-        ts, tq = [w[1] for w in work], [w[2] for w in work]
-        host = torch.tensor([ts, tq], dtype=torch.int32).pin_memory()
-        tiles = (host.to(q.device, non_blocking=True), len(ts), tok)
-        batch._attn_tiles_tc = tiles
-    return tiles
+        return [w[1] for w in work], [w[2] for w in work]
+    return step_list(batch, f"tiles{tok}", build, q.device) + (tok,)
+
+
+def _row_tiles(q, batch, nd: int):
+    """(device tensor [2, n] of (sequence, first chunk token) per tile of 16 query rows, n), cached on the batch."""
+    def build():
+        work = [(i, q0) for i in range(nd, batch.num_seqs) for q0 in range(0, batch.query_lens_host[i], 16)]
+        return [w[0] for w in work], [w[1] for w in work]
+    return step_list(batch, "rows", build, q.device)
 
 
 def _paged_attention_kv16(q, out, k_cache, v_cache, batch, scale, window, d, scales=None, chunk=0, sinks=None, softcap=0.0,
@@ -878,17 +905,7 @@ def _paged_attention_kv16(q, out, k_cache, v_cache, batch, scale, window, d, sca
             _check(rc, "attn_prefill_tc16")
             return out
     if batch.num_seqs > nd:
-        tiles = getattr(batch, "_attn_tiles", None)
-        if tiles is None:
-            ts, tq = [], []
-            for i in range(nd, batch.num_seqs):
-                for q0 in range(0, batch.query_lens_host[i], 16):
-                    ts.append(i)
-                    tq.append(q0)
-            host = torch.tensor([ts, tq], dtype=torch.int32).pin_memory()
-            tiles = (host.to(q.device, non_blocking=True), len(ts))
-            batch._attn_tiles = tiles
-        tdev, n_tiles = tiles
+        tdev, n_tiles = _row_tiles(q, batch, nd)
         if fp4:
             _check(L.atlas_attn_prefill_kv4(q.data_ptr(), q.stride(0), out.data_ptr(), Hq * D, k_cache.data_ptr(), v_cache.data_ptr(),
                                             bt.data_ptr(), bt.stride(0), batch.seq_lens.data_ptr(), batch.query_start_loc.data_ptr(),

@@ -194,17 +194,15 @@ def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights
 
 def _weigh_tiles(batch, nd: int, device):
     """Tiles of 128 cached tokens of the chunk sequences, those with the most rows first: (device [2, n], n)."""
-    tiles = getattr(batch, "_weigh_tiles", None)
-    if tiles is None:
+    def build():
         work = []
         for i in range(nd, batch.num_seqs):
             n, rows = batch.seq_lens_host[i], batch.query_lens_host[i]
             if rows:
                 work += [(-(rows - max(0, k0 - (n - rows))), i, k0) for k0 in range(0, n, 128)]
         work.sort()
-        host = torch.tensor([[w[1] for w in work], [w[2] for w in work]], dtype=torch.int32).pin_memory()
-        tiles = batch._weigh_tiles = (host.to(device, non_blocking=True), len(work))
-    return tiles
+        return [w[1] for w in work], [w[2] for w in work]
+    return K.step_list(batch, "cached", build, device)
 
 
 def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding_window: Optional[int] = None,

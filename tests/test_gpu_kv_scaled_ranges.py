@@ -140,3 +140,69 @@ def test_scales_all_over_the_place(d, hkv, g, lens, rows, window, spread):
     vs *= torch.exp2(torch.randint(-spread, spread + 1, (nb, hkv), generator=gen).float()).to(DEV)
     q = torch.randn(sum(rows), hkv * g, d, generator=gen).to(torch.bfloat16).to(DEV)
     _check(q, k, v, ks, vs, tables, lens, rows, d ** -0.5, window)
+
+
+# ----------------------------------------------------------------------------- one batch on several streams, and with other lengths
+def test_a_batch_is_used_on_a_second_stream_at_once():
+    gen = torch.Generator().manual_seed(21)
+    lens, rows = [900, 500], [900, 300]
+    tables, nb = tables_for(lens, gen, DEV)
+    k, v, ks, vs = make_cache(nb, 4, 128, gen, DEV)
+    q = torch.randn(sum(rows), 16, 128, generator=gen).to(torch.bfloat16).to(DEV)
+
+    def call(batch):
+        w = torch.zeros(2, 4, 900, device=DEV)
+        return ops.paged_attention(q, k, v, batch, 0.09, ks, vs, weights=w), w
+    want = call(batch_of(lens, rows, tables))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        batch, got = batch_of(lens, rows, tables), []
+        torch.cuda.synchronize()
+        for s in streams:                                  # fresh: the first call's lists may still be on their way
+            with torch.cuda.stream(s):
+                got.append(call(batch))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_a_batch_whose_sequences_grew():
+    gen = torch.Generator().manual_seed(22)
+    tables, nb = tables_for([400], gen, DEV)
+    k, v, ks, vs = make_cache(nb, 2, 64, gen, DEV)
+    q = torch.randn(30, 4, 64, generator=gen).to(torch.bfloat16).to(DEV)
+    batch = batch_of([200], [30], tables)
+    for n in (200, 390):
+        batch.seq_lens.fill_(n)
+        batch.seq_lens_host[0] = batch.max_seq_len = n
+        w = torch.zeros(1, 2, 400, device=DEV)
+        got = ops.paged_attention(q, k, v, batch, 0.125, ks, vs, weights=w)
+        out, mag, amp, sums = attention64_over(q, dequant(k, ks, tables[0], n), dequant(v, vs, tables[0], n), 0.125)
+        assert (got.double().cpu() - out).abs().le(attention_bound(out, mag, amp, 64)).all()
+        rel = 4 * 12 * 2.0 ** -23 * (float(amp.max()) + 2.0) + 2.0 ** -20
+        assert (w[0, :, :n].double().cpu() - sums).abs().le(rel * sums + 4 * 2.0 ** -23 * sums).all()
+
+
+def test_prompt_rows_with_weights_in_a_graph():
+    """Captured behind a first call on another stream; the batch then goes on with other lengths while the graph lives."""
+    gen = torch.Generator().manual_seed(23)
+    tables, nb = tables_for([300, 90], gen, DEV, extra_cols=4)
+    k, v, ks, vs = make_cache(nb, 2, 128, gen, DEV)
+    lens, rows = [300, 90], [40, 90]
+    q = torch.randn(130, 8, 128, generator=gen).to(torch.bfloat16).to(DEV)
+    batch = batch_of(lens, rows, tables)
+    w = torch.zeros(2, 2, 320, device=DEV)
+    call = lambda: ops.paged_attention(q, k, v, batch, 0.09, ks, vs, weights=w)
+    want = call().clone(), w.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    batch.seq_lens_host[0] = 290                           # other lists from here on
+    for _ in range(3):
+        w.zero_()
+        call()
+    junk = [torch.full((2, n), 1 << 20, dtype=torch.int32, device=DEV) for n in range(1, 20)]
+    w.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want[0]) and torch.equal(w, want[1]) and len(junk) == 19

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from atlas_b200 import ops
+from atlas_b200.ops import cuda as K, cuda_scaled as CS
 from kv_scaled_cases import BS, attention64_over, attention_bound, dequant, make_cache, tables_for
 from test_kv_scaled_cpu import batch_of
 
@@ -59,3 +60,51 @@ def test_blocks_outside_of_the_pool_are_skipped():
     x = torch.ones(2, 2, 64, dtype=torch.bfloat16)
     ops.qk_norm_rope_kv_write(x, x, x, None, None, 0, k, v, torch.tensor([nb * BS, -3], dtype=torch.int32), ks, vs)
     assert torch.equal(k.view(torch.uint8), old[0]) and torch.equal(ks, old[1])
+
+
+# ----------------------------------------------------------------------------- lists of a step
+class Lists:
+    """``step_list`` with streams, captures and uploads of the test's making."""
+
+    def __init__(self, monkeypatch):
+        self.place, self.uploads = (1, False), 0
+        monkeypatch.setattr(K, "_list_place", lambda device: self.place)
+        monkeypatch.setattr(K, "_upload", self.upload)
+
+    def upload(self, rows, device):
+        self.uploads += 1
+        return torch.tensor(rows, dtype=torch.int32), None
+
+
+def test_lists_of_a_step_follow_its_lengths_and_streams(monkeypatch):
+    lists = Lists(monkeypatch)
+    tables = torch.zeros(3, 40, dtype=torch.int32)
+    b = batch_of([5, 300, 200], [1, 40, 200], tables)
+    keys = lambda: CS._weigh_tiles(b, b.num_decodes, torch.device("cpu"))
+    tiles = lambda tok: K._tc_tiles(tables, b, b.num_decodes, tok)
+    first = keys()
+    assert first[1] == 3 + 2 and keys()[0] is first[0] and lists.uploads == 1
+    assert tiles(32)[1] == 2 + 7 and tiles(64)[1] == 1 + 4 and tiles(32)[1] == 9 and lists.uploads == 3      # of both sizes at once
+    lists.place = (2, False)                                                   # a stream that the upload is not ordered with
+    other = keys()
+    assert other[0] is not first[0] and torch.equal(other[0], first[0]) and lists.uploads == 4
+    lists.place = (1, False)
+    assert keys()[0] is first[0]
+    b.seq_lens_host[1] = 500                                                   # the sequence has grown
+    grown = keys()
+    assert grown[1] == 4 + 2 and sorted(grown[0][1][grown[0][0] == 1].tolist()) == [0, 128, 256, 384]
+    b.query_lens_host[2] = 10
+    assert tiles(32)[1] == 2 + 1
+
+
+def test_what_a_graph_was_captured_with_stays(monkeypatch):
+    lists = Lists(monkeypatch)
+    b = batch_of([300], [40], torch.zeros(1, 40, dtype=torch.int32))
+    keys = lambda: CS._weigh_tiles(b, b.num_decodes, torch.device("cpu"))
+    warm = keys()[0]
+    lists.place = (7, True)
+    assert keys()[0] is warm and lists.uploads == 1                            # nothing uploaded inside the graph
+    lists.place = (1, False)
+    b.seq_lens_host[0] = 301
+    assert keys()[0] is not warm
+    assert any(t is warm for e in b._captured_lists for t in e)
