@@ -488,11 +488,13 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale=1.0, v_scale=1.0,
     joins the scaled score of query ``i`` and key ``j``.
 
     With the tensors of :func:`alloc_kv_scales` as ``k_scale`` and ``v_scale`` the cache is FP8 with a scale per (block, head): plain or
-    windowed attention; a block whose table entry lies outside of the pool is skipped.  ``weights [sequences, Hkv, tokens]`` (fp32, such a cache only): every cached token's softmax weight, summed over
+    windowed attention with a ``scale`` from 2^-60 to 2^60; a block whose table entry lies outside of the pool is skipped.  ``weights [sequences, Hkv, tokens]`` (fp32, such a cache only): every cached token's softmax weight, summed over
     the sequence's rows of this step and the query heads of a key head, is added to it."""
     if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor):
         if chunk or sinks is not None or softcap or distance is not None:
             raise ValueError("a block-scaled cache: no chunked attention, softmax sinks, bounded scores or distance biases")
+        if not 2.0 ** -60 <= scale <= 2.0 ** 60:
+            raise ValueError(f"a block-scaled cache: the softmax scale is positive, from 2^-60 to 2^60, not {scale}")
         if on_gpu(q):
             return scaled_ops().paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding_window, weights)
         return ref_scaled.paged_attention(q, k_cache, v_cache, batch.block_tables, batch.seq_lens, batch.query_start_loc, scale, k_scale, v_scale,

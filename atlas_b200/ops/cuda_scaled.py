@@ -226,6 +226,8 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
     longest = batch.max_seq_len
     if window < 0 or rows < B or starts.shape[0] < B + 1 or not 0 <= nd <= B or T < nd:
         raise K.KernelError("attention: a block table, a length and a start for every sequence, a row for every decode, no negative window")
+    if not 2.0 ** -60 <= scale <= 2.0 ** 60:              # scores are masked, and the largest is taken, before it is applied
+        raise K.KernelError(f"the softmax scale is positive, from 2^-60 to 2^60, not {scale}")
     width, sums = 0, (0, 0, 0)
     if weights is not None:
         if weights.dtype != _F32 or weights.dim() != 3 or weights.shape[:2] != (B, hkv) or weights.get_device() != dev \

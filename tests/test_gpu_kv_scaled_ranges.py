@@ -206,3 +206,16 @@ def test_prompt_rows_with_weights_in_a_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want[0]) and torch.equal(w, want[1]) and len(junk) == 19
+
+
+# ----------------------------------------------------------------------------- softmax scales at their ends
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** -30, 2.0 ** 4])
+@pytest.mark.parametrize("d,lens,rows,window", [(128, [300, 50], [1, 1], 0), (128, [300, 50], [200, 50], 0), (64, [90], [90], 20), (256, [200, 40], [70, 1], 0)])
+def test_softmax_scales_at_their_ends(d, lens, rows, window, scale):
+    gen = torch.Generator().manual_seed(d)
+    tables, nb = tables_for(lens, gen, DEV)
+    k, v, ks, vs = make_cache(nb, 2, d, gen, DEV, spread=1)
+    k.view(torch.uint8)[int(tables[0, 1])] = 0             # keys of nothing: the smallest scale
+    ks[int(tables[0, 1])] = 2.0 ** -60
+    q = torch.randn(sum(rows), 8, d, generator=gen).to(torch.bfloat16).to(DEV)
+    _check(q, k, v, ks, vs, tables, lens, rows, scale, window)

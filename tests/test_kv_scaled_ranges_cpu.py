@@ -8,7 +8,7 @@ import torch
 from atlas_b200 import ops
 from atlas_b200.ops import cuda as K, cuda_scaled as CS
 from kv_scaled_cases import BS, attention64_over, attention_bound, dequant, make_cache, tables_for
-from test_kv_scaled_cpu import batch_of
+from test_kv_scaled_cpu import batch_of, parts
 
 CSRC = pathlib.Path(__file__).resolve().parent.parent / "atlas_b200" / "csrc"
 
@@ -108,3 +108,15 @@ def test_what_a_graph_was_captured_with_stays(monkeypatch):
     b.seq_lens_host[0] = 301
     assert keys()[0] is not warm
     assert any(t is warm for e in b._captured_lists for t in e)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), 2.0 ** -61, 2.0 ** 61])
+def test_softmax_scales_that_are_refused(scale):
+    k, v, ks, vs = parts()
+    for rows in ([1], [3]):
+        b = batch_of([20], rows, torch.zeros(1, 2, dtype=torch.int32))
+        q = torch.ones(rows[0], 4, 64, dtype=torch.bfloat16)
+        with pytest.raises(K.KernelError, match="softmax scale"):
+            CS.paged_attention(q, k, v, b, scale, ks, vs)
+        with pytest.raises(ValueError, match="softmax scale"):
+            ops.paged_attention(q, k, v, b, scale, ks, vs)
