@@ -645,7 +645,7 @@ int decode_launch(ScaledDecodeParams p, int blocks, int items, long long max_len
 // Decode rows of a step: sequence b's row is query_start_loc[b].  Arguments as one record (see kv_scaled.cu).  Workspaces: part_o [pieces][D]
 // [cols] and part_ml [pieces][cols][2] with cols = min(G rounded up to two, 16) and pieces = pairs + 16 blocks, a pair being (sequence, key head,
 // group of 16 query heads).  With `weights`: scores [nd * Hkv][width][G rounded up to two], ml [nd][Hq][2] and the sums
-// [sequence][head][token], `width` tokens each.  -1: sizes or alignment outside of what the kernels take.
+// [sequence][head][token], at least `width` tokens each, of which no sequence has more.  -1: sizes or alignment outside of what the kernels take.
 struct DecodeRecord {
   const void* q; long long ldq; void* out; long long ldo; const void* k_cache; const void* v_cache;
   const float* ks; long long ks_ld, ks_h; const float* vs; long long vs_ld, vs_h;

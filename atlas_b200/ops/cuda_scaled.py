@@ -251,12 +251,14 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
             blocks = max(1, min((pages + LEAST - 1) // LEAST, K._num_sms[index]))
             pieces = items + blocks * WARPS
             n_o, n_ml = pieces * n_cols * d, pieces * n_cols * 2
-            n_s, n_r = (nd * hkv * width * ((g + 1) // 2 * 2), nd * hq * 2) if weights is not None else (0, 0)
+            # the scores go through memory, for as many tokens as there are; a graph's sequences grow up to the width of the sums
+            tokens = width if longest <= 0 or torch._C._cuda_isCurrentStreamCapturing() else min(width, longest)
+            n_s, n_r = (nd * hkv * tokens * ((g + 1) // 2 * 2), nd * hq * 2) if weights is not None else (0, 0)
             work = torch.empty(n_o + n_ml + n_s + n_r, dtype=_F32, device=q.device)       # every part a multiple of 16 bytes or the last
             at = work.data_ptr()
             at_s = at + 4 * (n_o + n_ml)
             _call("atlas_attn_scaled_decode", _DECODE.pack(
-                at_q, ldq, at_out, hq * d, *cache, nd, hq, hkv, d, window, nb, longest, blocks, at, at + 4 * n_o, at_s if n_s else 0, width,
+                at_q, ldq, at_out, hq * d, *cache, nd, hq, hkv, d, window, nb, longest, blocks, at, at + 4 * n_o, at_s if n_s else 0, tokens,
                 at_s + 4 * n_s if n_r else 0, *sums, scale, status, stream), "attn_scaled_decode")
         if B > nd:
             tiles, n, _ = K._tc_tiles(q, batch, nd, 128 // g * (2 if d <= 128 else 1))

@@ -219,3 +219,22 @@ def test_softmax_scales_at_their_ends(d, lens, rows, window, scale):
     ks[int(tables[0, 1])] = 2.0 ** -60
     q = torch.randn(sum(rows), 8, d, generator=gen).to(torch.bfloat16).to(DEV)
     _check(q, k, v, ks, vs, tables, lens, rows, scale, window)
+
+
+# ----------------------------------------------------------------------------- sums much wider than the sequences
+def test_scratch_goes_by_the_sequences_not_by_the_width_of_the_sums():
+    gen = torch.Generator().manual_seed(31)
+    lens = [100, 37, 60, 1]
+    tables, nb = tables_for(lens, gen, DEV)
+    k, v, ks, vs = make_cache(nb, 8, 64, gen, DEV)
+    q = torch.randn(4, 32, 64, generator=gen).to(torch.bfloat16).to(DEV)
+    call = lambda w: ops.paged_attention(q, k, v, batch_of(lens, [1] * 4, tables), 0.125, ks, vs, weights=w)
+    narrow, wide = torch.zeros(4, 8, 100, device=DEV), torch.zeros(4, 8, 1 << 18, device=DEV)
+    want = call(narrow)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = call(wide)
+    # outputs, pieces and the scores of 4 x 8 x 100 x 4 heads: all below 8 MB; by the width the scores alone took 134 MB
+    assert torch.cuda.max_memory_allocated() - before < 8 << 20
+    assert torch.equal(got, want) and torch.equal(wide[..., :100], narrow) and not wide[..., 100:].any()
