@@ -37,7 +37,7 @@ struct ScChunkParams {
   float2* ml;                                     // [rows of the step][Hq] (M, 1 / l) or null
   // Few rows behind many keys: the keys of a query tile go to `splits` CTAs in equal shares, whose parts are joined by scaled_chunk_join_kernel
   int splits, first_row, rows;
-  float* part_o; float2* part_ml;                 // [split][rows][Hq][D] and [split][rows][Hq] (M, l), rows from first_row on
+  float* part_o; float2* part_ml;                 // [split][rows][Hq][D] and [split][rows][Hq] (M, l), rows from first_row on; no output of empty shares
   status_t* status;
 };
 
@@ -178,8 +178,9 @@ scaled_chunk_join_kernel(const ScChunkParams p) {
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float2 x = p.part_ml[s * step + u];
-    const float f = fast_exp2(x.x - ref);                        // a share that the row sees nothing of: 2^-inf
+    const float f = fast_exp2(x.x - ref);
     l += x.y * f;
+    if (x.x == -INFINITY) continue;                              // a share that the row sees nothing of may have no output
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       const float2 y = *reinterpret_cast<const float2*>(p.part_o + (s * step + u) * D + i * 64 + lane * 2);
@@ -539,7 +540,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
       }
-      store_outputs<D>(tO, n == 0, inv, !live ? -1 : part ? at_part * D : (long long)(m_.q_row0 + tok) * p.ldo + head * D, p.out, part ? p.part_o : nullptr, [&] {
+      store_outputs<D>(tO, n == 0, inv, !live || (part && n == 0) ? -1 : part ? at_part * D : (long long)(m_.q_row0 + tok) * p.ldo + head * D, p.out, part ? p.part_o : nullptr, [&] {
         if (n == 0) return;
         tc_fence_before();
         __syncwarp();
@@ -921,7 +922,7 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
       const long long at = (long long)(q_row0 + tok) * p.Hq + head, at_part = ((long long)split * p.rows - p.first_row) * p.Hq + at;
       const bool part = p.splits > 1;
       tc_fence_after();
-      store_outputs<D>(tO, n_kv == 0, inv, !live ? -1 : part ? at_part * D : (long long)(q_row0 + tok) * p.ldo + head * D, p.out, part ? p.part_o : nullptr, [] {});
+      store_outputs<D>(tO, n_kv == 0, inv, !live || (part && n_kv == 0) ? -1 : part ? at_part * D : (long long)(q_row0 + tok) * p.ldo + head * D, p.out, part ? p.part_o : nullptr, [] {});
       if (live) {
         if (part) p.part_ml[at_part] = make_float2(m, l);
         else if (p.ml) p.ml[at] = make_float2(m == -INFINITY ? 0.f : m, inv);

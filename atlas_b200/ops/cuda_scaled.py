@@ -205,6 +205,13 @@ def _weigh_tiles(batch, nd: int, device):
     return K.step_list(batch, "cached", build, device)
 
 
+def key_shares(lens, items: int, window: int, sms: int) -> int:
+    """Shares of the keys of prompt rows' sequences of ``lens`` tokens.  Few query tiles behind many keys: as many as fill the GPU once, at least
+    512 tokens of the longest each."""
+    longest = max(lens, default=0)
+    return max(1, min(sms // items, (min(longest, window + 128) if window else longest) // 512)) if items else 1
+
+
 def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding_window: Optional[int] = None,
                     weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     nb, hkv, d = check_cache(k_cache, v_cache, k_scale, v_scale)
@@ -251,9 +258,11 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
             blocks = max(1, min((pages + LEAST - 1) // LEAST, K._num_sms[index]))
             pieces = items + blocks * WARPS
             n_o, n_ml = pieces * n_cols * d, pieces * n_cols * 2
-            # the scores go through memory, for as many tokens as there are; a graph's sequences grow up to the width of the sums
-            tokens = width if longest <= 0 or torch._C._cuda_isCurrentStreamCapturing() else min(width, longest)
-            n_s, n_r = (nd * hkv * tokens * ((g + 1) // 2 * 2), nd * hq * 2) if weights is not None else (0, 0)
+            n_s = n_r = tokens = 0
+            if weights is not None:
+                # the scores go through memory, for as many tokens as there are; a graph's sequences grow up to the width of the sums
+                tokens = width if longest <= 0 or torch._C._cuda_isCurrentStreamCapturing() else min(width, longest)
+                n_s, n_r = nd * hkv * tokens * ((g + 1) // 2 * 2), nd * hq * 2
             work = torch.empty(n_o + n_ml + n_s + n_r, dtype=_F32, device=q.device)       # every part a multiple of 16 bytes or the last
             at = work.data_ptr()
             at_s = at + 4 * (n_o + n_ml)
@@ -264,8 +273,7 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
             tiles, n, _ = K._tc_tiles(q, batch, nd, 128 // g * (2 if d <= 128 else 1))
             ml = key_tiles = parts = None
             at_keys = n_keys = n_o = 0
-            # few query tiles behind many keys: as many shares of the keys as fill the GPU once, at least four key tiles each
-            splits = max(1, min(K._num_sms[index] // (n * hkv), (min(longest, window + 128) if window else longest) // 512)) if n else 1
+            splits = key_shares(batch.seq_lens_host[nd:], n * hkv, window, K._num_sms[index])
             if splits > 1:
                 n_o = splits * (T - nd) * hq * d
                 parts = torch.empty(n_o + splits * (T - nd) * hq * 2, dtype=_F32, device=q.device)

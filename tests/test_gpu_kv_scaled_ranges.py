@@ -238,3 +238,13 @@ def test_scratch_goes_by_the_sequences_not_by_the_width_of_the_sums():
     # outputs, pieces and the scores of 4 x 8 x 100 x 4 heads: all below 8 MB; by the width the scores alone took 134 MB
     assert torch.cuda.max_memory_allocated() - before < 8 << 20
     assert torch.equal(got, want) and torch.equal(wide[..., :100], narrow) and not wide[..., 100:].any()
+
+
+# ----------------------------------------------------------------------------- shares of the keys, empty ones among them
+@pytest.mark.parametrize("d,hkv,g,lens,rows,window", [
+    (128, 2, 4, [9000, 32], [1, 32], 0), (64, 1, 4, [20000, 3, 700], [1, 3, 20], 0), (256, 2, 4, [8000, 40], [1, 17], 0),
+    (128, 1, 4, [6000, 20, 300], [30, 20, 10], 0), (64, 1, 8, [5000, 9], [16, 9], 1500), (256, 1, 8, [7000, 12], [10, 12], 0)])
+def test_short_prompts_beside_long_sequences(d, hkv, g, lens, rows, window):
+    check_attention(d, hkv, g, lens, rows, window, True, smallest=window > 0)
+    torch.empty(1 << 26, device=DEV).fill_(float("nan"))    # what a workspace may hold
+    check_attention(d, hkv, g, lens, rows, window, True, smallest=window > 0)

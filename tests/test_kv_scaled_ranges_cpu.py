@@ -120,3 +120,35 @@ def test_softmax_scales_that_are_refused(scale):
             CS.paged_attention(q, k, v, b, scale, ks, vs)
         with pytest.raises(ValueError, match="softmax scale"):
             ops.paged_attention(q, k, v, b, scale, ks, vs)
+
+
+def test_shares_of_the_keys_go_by_the_prompts():
+    assert CS.key_shares([], 0, 0, 148) == 1
+    assert CS.key_shares([32], 8, 0, 148) == 1                                 # beside any number of long single tokens
+    assert CS.key_shares([65000, 100], 8, 0, 148) == 18
+    assert CS.key_shares([4096], 8, 0, 148) == 8                               # at least 512 tokens each
+    assert CS.key_shares([65000], 8, 2000, 148) == 4
+    assert CS.key_shares([65000], 200, 0, 148) == 1
+
+
+def test_short_prompts_beside_a_long_single_token_are_not_cut(monkeypatch):
+    """The record of the prompt rows' call, as far as it goes without a GPU."""
+    class Stop(Exception):
+        pass
+    seen = {}
+
+    def call(name, record, what):
+        if name == "atlas_attn_scaled_chunk":
+            seen["splits"] = CS._CHUNK.unpack(record)[27]
+            raise Stop
+    Lists(monkeypatch)
+    monkeypatch.setattr(CS, "_call", call)
+    monkeypatch.setattr(CS, "_place", lambda t: (CS._HERE, 0, 0))
+    monkeypatch.setitem(K._num_sms, 0, 148)
+    monkeypatch.setitem(K._status_ptr, 0, 0)
+    k, v, ks, vs = parts()
+    for lens, rows, want in (([40000, 32], [1, 32], 1), ([40000, 9000], [1, 32], 17)):
+        b = batch_of(lens, rows, torch.zeros(2, 2500, dtype=torch.int32))
+        with pytest.raises(Stop):
+            CS.paged_attention(torch.zeros(33, 4, 64, dtype=torch.bfloat16), k, v, b, 0.125, ks, vs)
+        assert seen["splits"] == want
