@@ -669,7 +669,7 @@ extern "C" int atlas_attn_scaled_decode(const void* record) {
   p.cols = p.G <= 16 ? (p.G + 1) / 2 * 2 : 16;
   // the list's entries and the runs' bounds are 32-bit numbers
   const long long items = r.nd * r.Hkv * p.tiles;
-  if (items * r.bt_cols > 0x3fffffffll || items > 0x7fffffffll || r.bt_cols > (1 << 26) || r.blocks <= 0 || r.blocks > 65535) return -1;
+  if (items * r.bt_cols > 0x3fffffffll || items > 0x7fffffffll || r.bt_cols > (1 << 25) || r.window < 0 || r.window > (1 << 29) || r.blocks <= 0 || r.blocks > 65535) return -1;
   p.window = (int)r.window; p.num_pages = (int)r.num_pages;
   p.scale_log2 = (float)(r.scale * 1.4426950408889634);
   p.part_o = r.part_o; p.part_ml = r.part_ml;

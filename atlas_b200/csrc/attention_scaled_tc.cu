@@ -1381,7 +1381,7 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
   if ((reinterpret_cast<uintptr_t>(r.q) & 15) || r.ldq % 8 || r.ldo % 8 || (reinterpret_cast<uintptr_t>(r.out) & 15)) return -1;
   if ((reinterpret_cast<uintptr_t>(r.k_cache) | reinterpret_cast<uintptr_t>(r.v_cache)) & 15) return -1;
   if (!(r.scale >= 0x1p-60 && r.scale <= 0x1p60)) return -1;      // scores are masked, and the largest is taken, before their factor is applied
-  if (r.bt_cols > (1 << 26) || r.tiles > 0x7fffffffll || r.total_tokens > 0x7fffffffll || (r.weights && !r.ml)) return -1;
+  if (r.bt_cols > (1 << 25) || r.window < 0 || r.window > (1 << 29) || r.tiles > 0x7fffffffll || r.total_tokens > 0x7fffffffll || (r.weights && !r.ml)) return -1;
   if (r.splits < 1 || r.splits > 65535 || (r.splits > 1 && (!r.part_o || !r.part_ml)) || r.first_row < 0 || r.first_row >= r.total_tokens) return -1;
   const int Hq = (int)r.Hq, Hkv = (int)r.Hkv, G = Hq / Hkv;
   CUtensorMap tq;

@@ -231,6 +231,7 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
     window, nd, B = int(sliding_window or 0), batch.num_decodes, lens.shape[0]
     rows, cols = bt.shape
     longest = batch.max_seq_len
+    window = min(window, max(1, cols * BLOCK))              # no sequence is longer: the kernels' sums of positions stay in 32 bits
     if window < 0 or rows < B or starts.shape[0] < B + 1 or not 0 <= nd <= B or T < nd:
         raise K.KernelError("attention: a block table, a length and a start for every sequence, a row for every decode, no negative window")
     if not 2.0 ** -60 <= scale <= 2.0 ** 60:              # scores are masked, and the largest is taken, before it is applied

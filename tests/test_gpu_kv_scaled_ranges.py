@@ -248,3 +248,17 @@ def test_short_prompts_beside_long_sequences(d, hkv, g, lens, rows, window):
     check_attention(d, hkv, g, lens, rows, window, True, smallest=window > 0)
     torch.empty(1 << 26, device=DEV).fill_(float("nan"))    # what a workspace may hold
     check_attention(d, hkv, g, lens, rows, window, True, smallest=window > 0)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 40])
+@pytest.mark.parametrize("d,lens,rows", [(128, [300, 200], [1, 200]), (64, [400], [100]), (256, [150], [90])])
+def test_windows_longer_than_everything(d, lens, rows, window):
+    gen = torch.Generator().manual_seed(d)
+    tables, nb = tables_for(lens, gen, DEV)
+    k, v, ks, vs = make_cache(nb, 2, d, gen, DEV)
+    q = torch.randn(sum(rows), 8, d, generator=gen).to(torch.bfloat16).to(DEV)
+    out = []
+    for w in (None, window):
+        sums = torch.zeros(len(lens), 2, max(lens), device=DEV)
+        out.append((ops.paged_attention(q, k, v, batch_of(lens, rows, tables), d ** -0.5, ks, vs, w, weights=sums), sums))
+    assert all(torch.equal(a, b) for a, b in zip(*out)) and out[0][1].sum() > 0

@@ -131,24 +131,37 @@ def test_shares_of_the_keys_go_by_the_prompts():
     assert CS.key_shares([65000], 200, 0, 148) == 1
 
 
-def test_short_prompts_beside_a_long_single_token_are_not_cut(monkeypatch):
-    """The record of the prompt rows' call, as far as it goes without a GPU."""
-    class Stop(Exception):
-        pass
-    seen = {}
+class Records:
+    """The records of the attention's calls, as far as they go without a GPU."""
 
-    def call(name, record, what):
-        if name == "atlas_attn_scaled_chunk":
-            seen["splits"] = CS._CHUNK.unpack(record)[27]
-            raise Stop
-    Lists(monkeypatch)
-    monkeypatch.setattr(CS, "_call", call)
-    monkeypatch.setattr(CS, "_place", lambda t: (CS._HERE, 0, 0))
-    monkeypatch.setitem(K._num_sms, 0, 148)
-    monkeypatch.setitem(K._status_ptr, 0, 0)
+    def __init__(self, monkeypatch):
+        self.seen = {}
+        Lists(monkeypatch)
+        monkeypatch.setattr(CS, "_call", lambda name, record, what: self.seen.update({name: record}))
+        monkeypatch.setattr(CS, "_place", lambda t: (CS._HERE, 0, 0))
+        monkeypatch.setitem(K._num_sms, 0, 148)
+        monkeypatch.setitem(K._status_ptr, 0, 0)
+
+    def decode(self, field):
+        return CS._DECODE.unpack(self.seen["atlas_attn_scaled_decode"])[field]
+
+    def chunk(self, field):
+        return CS._CHUNK.unpack(self.seen["atlas_attn_scaled_chunk"])[field]
+
+
+def test_short_prompts_beside_a_long_single_token_are_not_cut(monkeypatch):
+    records = Records(monkeypatch)
     k, v, ks, vs = parts()
     for lens, rows, want in (([40000, 32], [1, 32], 1), ([40000, 9000], [1, 32], 17)):
         b = batch_of(lens, rows, torch.zeros(2, 2500, dtype=torch.int32))
-        with pytest.raises(Stop):
-            CS.paged_attention(torch.zeros(33, 4, 64, dtype=torch.bfloat16), k, v, b, 0.125, ks, vs)
-        assert seen["splits"] == want
+        CS.paged_attention(torch.zeros(33, 4, 64, dtype=torch.bfloat16), k, v, b, 0.125, ks, vs)
+        assert records.chunk(27) == want
+
+
+def test_windows_reach_no_further_than_the_tables(monkeypatch):
+    records = Records(monkeypatch)
+    k, v, ks, vs = parts()
+    b = batch_of([30, 20], [1, 7], torch.zeros(2, 2, dtype=torch.int32))
+    for window, want in ((None, 0), (5, 5), (32, 32), (33, 32), (2 ** 31 - 1, 32), (2 ** 40, 32)):
+        CS.paged_attention(torch.zeros(8, 4, 64, dtype=torch.bfloat16), k, v, b, 0.125, ks, vs, window)
+        assert records.decode(21) == records.chunk(24) == want
