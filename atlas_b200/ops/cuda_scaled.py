@@ -75,6 +75,25 @@ def check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale, v_scale) 
     return nb, hkv, d
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether all elements have places of their own (a view that was not interleaved with itself)."""
+    reach = 0
+    for step, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if step <= reach:
+            return False
+        reach += step * (size - 1)
+    return True
+
+
+def _writable(k_cache, v_cache, k_scale, v_scale) -> None:
+    """What a call writes is not written through two places at once."""
+    h2 = 2 * k_cache.shape[2]
+    own = k_scale.stride() == (h2, 2) == v_scale.stride() or (_apart(k_scale) and _apart(v_scale))      # as alloc_kv_scales has them
+    if not own or (k_scale.numel() and k_scale.data_ptr() == v_scale.data_ptr()) \
+            or (k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr()):
+        raise K.KernelError("keys, values and their scales have places of their own (allocate the scales with ops.alloc_kv_scales)")
+
+
 def _ints(t: torch.Tensor, what: str, dev: int, dims: int) -> None:
     if t.dtype != _I32 or t.dim() != dims or t.get_device() != dev or (t.stride(-1) != 1 and t.numel() > 1):
         raise K.KernelError(f"{what}: int32 with {dims} dimension{'s' if dims > 1 else ''} on the cache's device, rows contiguous")
@@ -101,6 +120,7 @@ def alloc_kv_scales(num_blocks: int, hkv: int, device) -> Tuple[torch.Tensor, to
 def qk_norm_rope_kv_write(q, k, v, positions, rope_cache, rotary_dim, k_cache, v_cache, slot_mapping, k_scale, v_scale, q_norm_w=None,
                           k_norm_w=None, eps=1e-6, norm_plus_one=False, norm_dim=0) -> torch.Tensor:
     nb, hkv, d = check_cache(k_cache, v_cache, k_scale, v_scale)
+    _writable(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.get_device()
     for x, what in ((q, "queries"), (k, "keys"), (v, "values")):
         _heads(x, what, dev, d)
@@ -163,6 +183,7 @@ def kv_read(k_cache, v_cache, block_tables, seq_lens, max_len: int, k_scale, v_s
 
 def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep: int, new_tables, sink: int, recent: int):
     nb, hkv, d = check_cache(k_cache, v_cache, k_scale, v_scale)
+    _writable(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.get_device()
     for t, what, n in ((block_tables, "block tables", 2), (new_tables, "new block tables", 2), (seq_lens, "sequence lengths", 1)):
         _ints(t, what, dev, n)
@@ -241,6 +262,8 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
         if weights.dtype != _F32 or weights.dim() != 3 or weights.shape[:2] != (B, hkv) or weights.get_device() != dev \
                 or weights.stride(2) != 1 or weights.shape[2] < longest:
             raise K.KernelError(f"weights are fp32 [{B}, {hkv}, at least {longest}] beside the cache, tokens contiguous")
+        if not (weights.is_contiguous() or _apart(weights)):
+            raise K.KernelError("weights: every sequence and head has sums of its own")
         width = weights.shape[2]
         sums = (weights.data_ptr(), weights.stride(0), weights.stride(1))
     if T == 0 or B == 0:

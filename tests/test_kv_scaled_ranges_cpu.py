@@ -8,7 +8,7 @@ import torch
 from atlas_b200 import ops
 from atlas_b200.ops import cuda as K, cuda_scaled as CS
 from kv_scaled_cases import BS, attention64_over, attention_bound, dequant, make_cache, tables_for
-from test_kv_scaled_cpu import batch_of, parts
+from test_kv_scaled_cpu import attend, batch_of, parts, write
 
 CSRC = pathlib.Path(__file__).resolve().parent.parent / "atlas_b200" / "csrc"
 
@@ -165,3 +165,24 @@ def test_windows_reach_no_further_than_the_tables(monkeypatch):
     for window, want in ((None, 0), (5, 5), (32, 32), (33, 32), (2 ** 31 - 1, 32), (2 ** 40, 32)):
         CS.paged_attention(torch.zeros(8, 4, 64, dtype=torch.bfloat16), k, v, b, 0.125, ks, vs, window)
         assert records.decode(21) == records.chunk(24) == want
+
+
+# ----------------------------------------------------------------------------- refusals
+def test_what_is_written_has_places_of_its_own():
+    k, v, ks, vs = parts()
+    one = torch.ones(1, 1)
+    good = torch.ones(4, 5)[:, ::2][:, :2], torch.ones(2, 4).t()               # strides of their own kind, but apart
+    for scales in ((one.expand(4, 2), vs), (ks, one.expand(4, 2)), (ks, ks), (torch.ones(4, 1).expand(4, 2), vs),
+                   (torch.ones(8).as_strided((4, 2), (1, 1)), vs), (torch.ones(8).as_strided((4, 2), (1, 2)), vs)):
+        with pytest.raises(K.KernelError, match="places of their own"):
+            write(k, v, *scales)
+        with pytest.raises(K.KernelError, match="places of their own"):
+            CS.kv_evict(k, v, *scales, torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(1, 2, 9), 4,
+                        torch.zeros(1, 2, dtype=torch.int32), 0, 0)
+    with pytest.raises(K.KernelError, match="GPU"):                             # past the checks
+        write(k, v, *good)
+    for w in (torch.zeros(1, 2, 32).expand(2, 2, 32), torch.zeros(2, 1, 32).expand(2, 2, 32), torch.zeros(200).as_strided((2, 2, 32), (40, 20, 1))):
+        with pytest.raises(K.KernelError, match="of its own"):
+            attend(k, v, ks, vs, weights=w)
+    with pytest.raises(K.KernelError, match="GPU"):
+        attend(k, v, ks, vs, weights=torch.zeros(2, 3, 40)[:, 1:, 3:])
