@@ -657,7 +657,7 @@ extern "C" int atlas_attn_scaled_decode(const void* record) {
   const DecodeRecord& r = *static_cast<const DecodeRecord*>(record);
   const int D = (int)r.D;
   if (r.nd <= 0) return 0;
-  if ((D != 64 && D != 128 && D != 256) || r.Hkv <= 0 || r.Hq % r.Hkv || r.ldq % 8 || (reinterpret_cast<uintptr_t>(r.q) & 15)) return -1;
+  if ((D != 64 && D != 128 && D != 256) || r.Hkv <= 0 || r.Hq < r.Hkv || r.Hq % r.Hkv || r.Hq / r.Hkv > 128 || r.ldq % 8 || (reinterpret_cast<uintptr_t>(r.q) & 15)) return -1;
   if ((reinterpret_cast<uintptr_t>(r.k_cache) | reinterpret_cast<uintptr_t>(r.v_cache)) & 15) return -1;
   if (!(r.scale >= 0x1p-60 && r.scale <= 0x1p60)) return -1;
   ScaledDecodeParams p;

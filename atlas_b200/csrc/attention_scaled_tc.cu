@@ -1377,7 +1377,7 @@ extern "C" int atlas_attn_scaled_chunk(const void* record) {
   const ChunkRecord& r = *static_cast<const ChunkRecord*>(record);
   const int D = (int)r.D;
   if (r.tiles <= 0) return 0;
-  if ((D != 64 && D != 128 && D != 256) || r.Hkv <= 0 || r.Hkv > 65535 || r.Hq % r.Hkv || r.Hq / r.Hkv > kScRows) return -1;
+  if ((D != 64 && D != 128 && D != 256) || r.Hkv <= 0 || r.Hkv > 65535 || r.Hq < r.Hkv || r.Hq % r.Hkv || r.Hq / r.Hkv > kScRows) return -1;
   if ((reinterpret_cast<uintptr_t>(r.q) & 15) || r.ldq % 8 || r.ldo % 8 || (reinterpret_cast<uintptr_t>(r.out) & 15)) return -1;
   if ((reinterpret_cast<uintptr_t>(r.k_cache) | reinterpret_cast<uintptr_t>(r.v_cache)) & 15) return -1;
   if (!(r.scale >= 0x1p-60 && r.scale <= 0x1p60)) return -1;      // scores are masked, and the largest is taken, before their factor is applied

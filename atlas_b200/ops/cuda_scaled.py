@@ -60,6 +60,8 @@ def check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale, v_scale) 
     if len(shape) != 4:
         raise K.KernelError("a cache has four dimensions: blocks, tokens, heads, channels")
     nb, bs, hkv, d = shape
+    if hkv < 1:
+        raise K.KernelError("a cache has at least one head")
     if k_cache.dtype != _FP8 or v_cache.dtype != _FP8 or v_cache.shape != shape:
         raise K.KernelError("block scales belong to an FP8 (e4m3) cache of keys and values of one size")
     if bs != BLOCK or d not in HEAD_DIMS:
@@ -240,8 +242,8 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
     _heads(q, "queries", dev, d)
     T, hq, _ = q.shape
     g = hq // hkv
-    if hq % hkv or g > 128:
-        raise K.KernelError(f"{hq} query heads over {hkv} key heads: up to 128 for each")
+    if hq % hkv or not 1 <= g <= 128:
+        raise K.KernelError(f"{hq} query heads over {hkv} key heads: 1 to 128 for each")
     ldq, at_q = q.stride(0), q.data_ptr()
     if ldq % 8 or at_q % 16:
         raise K.KernelError("queries start on 16 bytes in every row")

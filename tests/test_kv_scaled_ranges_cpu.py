@@ -1,4 +1,5 @@
 """The block-scaled FP8 cache without a GPU, at the ends of what its calls allow."""
+import ctypes
 import pathlib
 import re
 
@@ -186,3 +187,30 @@ def test_what_is_written_has_places_of_its_own():
             attend(k, v, ks, vs, weights=w)
     with pytest.raises(K.KernelError, match="GPU"):
         attend(k, v, ks, vs, weights=torch.zeros(2, 3, 40)[:, 1:, 3:])
+
+
+def test_no_heads_are_refused():
+    k, v, ks, vs = parts()
+    with pytest.raises(K.KernelError, match="0 query heads"):
+        attend(k, v, ks, vs, q=torch.zeros(2, 0, 64, dtype=torch.bfloat16))
+    for call in (attend, write):
+        with pytest.raises(K.KernelError, match="at least one head"):
+            call(*parts(hkv=0))
+
+
+def test_entry_points_refuse_what_would_divide_by_zero():
+    """Straight at the library: these returns come before anything is launched."""
+    if not pathlib.Path(K.LIB_PATH).exists():
+        pytest.skip("the kernels are not built")
+    lib = K.lib()
+    for name, record, hq in (("atlas_attn_scaled_decode", CS._DECODE, 18), ("atlas_attn_scaled_chunk", CS._CHUNK, 21)):
+        f = getattr(lib, name)
+        f.argtypes = [ctypes.c_char_p]
+        n = len(record.unpack(bytes(record.size)))
+        real = next(i for i, x in enumerate(record.unpack(bytes(record.size))) if isinstance(x, float))
+        for heads in ((0, 1), (1, 2), (129, 1)):
+            a = [0] * n
+            a[real] = 0.125
+            a[17] = a[19] = 1                                                  # one sequence, one tile
+            a[hq], a[hq + 1], a[hq + 2] = heads + (64,)
+            assert f(record.pack(*a)) == -1
