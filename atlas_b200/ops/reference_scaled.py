@@ -128,12 +128,15 @@ def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights
         n = min(L, keep)
         if n <= 0:
             continue
-        w = torch.nan_to_num(weights[b, :, :L], nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
+        w = weights[b, :, :L]
         if L <= keep:
             pos = torch.arange(L, device=dev).expand(hkv, L)
         else:
             room = keep - sink - recent
-            best = torch.sort(w[:, sink:L - recent], dim=1, descending=True, stable=True).indices[:, :room] + sink
+            mid = w[:, sink:L - recent]
+            order = torch.sort(torch.where(mid.isnan(), torch.full_like(mid, float("-inf")), mid), dim=1, descending=True, stable=True).indices
+            last = torch.sort(mid.isnan().gather(1, order).to(torch.uint8), dim=1, stable=True).indices             # NaN below -inf, too
+            best = order.gather(1, last)[:, :room] + sink
             ends = torch.cat([torch.arange(sink, device=dev), torch.arange(L - recent, L, device=dev)]).expand(hkv, -1)
             pos = torch.sort(torch.cat([best, ends], 1), dim=1).values
         kept[b, :, :n] = pos.to(torch.int32)

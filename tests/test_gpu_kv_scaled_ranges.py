@@ -262,3 +262,19 @@ def test_windows_longer_than_everything(d, lens, rows, window):
         sums = torch.zeros(len(lens), 2, max(lens), device=DEV)
         out.append((ops.paged_attention(q, k, v, batch_of(lens, rows, tables), d ** -0.5, ks, vs, w, weights=sums), sums))
     assert all(torch.equal(a, b) for a, b in zip(*out)) and out[0][1].sum() > 0
+
+
+# ----------------------------------------------------------------------------- eviction
+def test_eviction_takes_minus_infinity_before_nan():
+    gen = torch.Generator().manual_seed(6)
+    tables, nb = tables_for([60], gen, DEV)
+    to, spare = tables_for([40], gen, DEV)
+    k, v, ks, vs = make_cache(nb + spare, 2, 64, gen, DEV)
+    w = torch.rand(1, 2, 60, generator=gen)
+    w[..., ::3] = float("nan")
+    w[..., 1::3] = float("-inf")
+    for keep in (10, 30, 40):
+        kept = ops.kv_evict(k, v, ks, vs, tables, torch.tensor([60], dtype=torch.int32, device=DEV), w.to(DEV), keep, to + nb, sink=1, recent=2)[1]
+        for h in range(2):
+            mid = sorted(range(1, 58), key=lambda j: (w[0, h, j] != w[0, h, j], -float(w[0, h, j].nan_to_num(0.0, neginf=-1.0)), j))
+            assert kept[0, h].tolist() == sorted([0, 58, 59] + mid[:keep - 3])

@@ -214,3 +214,18 @@ def test_entry_points_refuse_what_would_divide_by_zero():
             a[17] = a[19] = 1                                                  # one sequence, one tile
             a[hq], a[hq + 1], a[hq + 2] = heads + (64,)
             assert f(record.pack(*a)) == -1
+
+
+def test_eviction_takes_minus_infinity_before_nan():
+    gen = torch.Generator().manual_seed(6)
+    tables, nb = tables_for([60], gen, "cpu")
+    to, spare = tables_for([40], gen, "cpu")
+    k, v, ks, vs = make_cache(nb + spare, 2, 64, gen, "cpu", kernel_layout=False)
+    w = torch.rand(1, 2, 60, generator=gen)
+    w[..., ::3] = float("nan")
+    w[..., 1::3] = float("-inf")
+    for keep in (10, 30, 40):
+        kept = ops.kv_evict(k, v, ks, vs, tables, torch.tensor([60], dtype=torch.int32), w, keep, to + nb, sink=1, recent=2)[1]
+        for h in range(2):
+            mid = sorted(range(1, 58), key=lambda j: (w[0, h, j] != w[0, h, j], -float(w[0, h, j].nan_to_num(0.0, neginf=-1.0)), j))
+            assert kept[0, h].tolist() == sorted([0, 58, 59] + mid[:keep - 3])
