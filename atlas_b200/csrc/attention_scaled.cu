@@ -296,8 +296,8 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
       }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // largest magnitude to [2^13, 2^14): bf16 numbers are exact in f16 then, down to 2^-37 of it
-      const int e = min(max(13 - ((int)(__float_as_uint(amax) >> 23) - 127), -100), 100);
+      // largest magnitude to [2^13, 2^14): bf16 numbers are exact in f16 then down to 2^-30 of it, and off by 2^-38 of it at most below
+      const int e = min(max(13 - ((int)(__float_as_uint(amax) >> 23) - 127), -114), 126);      // both powers are normal fp32 numbers
       const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int i = 0; i < KS; ++i)

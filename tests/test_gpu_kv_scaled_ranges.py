@@ -278,3 +278,17 @@ def test_eviction_takes_minus_infinity_before_nan():
         for h in range(2):
             mid = sorted(range(1, 58), key=lambda j: (w[0, h, j] != w[0, h, j], -float(w[0, h, j].nan_to_num(0.0, neginf=-1.0)), j))
             assert kept[0, h].tolist() == sorted([0, 58, 59] + mid[:keep - 3])
+
+
+# ----------------------------------------------------------------------------- queries at the ends of their type
+@pytest.mark.parametrize("power,scale,key", [(116, 2.0 ** -60, -60), (-120, 2.0 ** 60, 58), (-126, 2.0 ** 60, 60), (90, 2.0 ** -45, -45)])
+@pytest.mark.parametrize("d,lens,rows", [(128, [200, 33], [1, 1]), (64, [70], [1]), (256, [100], [1]), (128, [150], [40]), (256, [150], [40])])
+def test_queries_of_any_size(d, lens, rows, power, scale, key):
+    gen = torch.Generator().manual_seed(d + rows[0])
+    tables, nb = tables_for(lens, gen, DEV)
+    k, v, ks, vs = make_cache(nb, 2, d, gen, DEV, spread=1)
+    for i in range(nb):
+        k.view(torch.uint8)[i] = (torch.randn(BS, 2, d, generator=gen) * 0.5).to(FP8).view(torch.uint8).to(DEV)
+    ks.fill_(2.0 ** key)
+    q = (torch.randn(sum(rows), 8, d, generator=gen) * 2.0 ** power).to(torch.bfloat16).to(DEV)
+    _check(q, k, v, ks, vs, tables, lens, rows, scale)
