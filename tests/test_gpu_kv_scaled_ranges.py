@@ -1,11 +1,13 @@
 """The block-scaled FP8 cache on the GPU, at the ends of what its calls allow."""
+import numpy as np
 import pytest
 import torch
 
 from atlas_b200 import ops
 from atlas_b200.ops import cuda as K
-from kv_scaled_cases import BS, FP8, attention64_over, attention_bound, dequant, make_cache, power_scale, tables_for
+from kv_scaled_cases import BS, FP8, attention64_over, attention_bound, dequant, make_cache, nearest_e4m3, power_scale, tables_for
 from test_gpu_kv_scaled import batch_of, check_attention
+import test_gpu_kv_scaled as base
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -292,3 +294,54 @@ def test_queries_of_any_size(d, lens, rows, power, scale, key):
     ks.fill_(2.0 ** key)
     q = (torch.randn(sum(rows), 8, d, generator=gen) * 2.0 ** power).to(torch.bfloat16).to(DEV)
     _check(q, k, v, ks, vs, tables, lens, rows, scale)
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
+@pytest.mark.parametrize("hkv,lens,keep,sink,recent", [
+    (80, [9000], 50, 2, 3),                                # a block a head, more tokens than its registers hold
+    (5, [9001, 8200, 20] * 6, 20, 0, 1),
+    (40, [18011], 300, 1, 0),                              # two blocks a head
+    (1, [80000], 4096, 16, 512),                           # eight
+])
+def test_evict_of_more_tokens_than_registers_hold(hkv, lens, keep, sink, recent, kind):
+    gen = torch.Generator().manual_seed(keep)
+    tables, nb = tables_for(lens, gen, DEV)
+    to, spare = tables_for([min(n, keep) for n in lens], gen, DEV)
+    k, v, ks, vs = make_cache(nb + spare, hkv, 64, gen, DEV)
+    w = torch.rand(len(lens), hkv, max(lens), generator=gen)
+    if kind == "ties":
+        w = (w * 4).floor() / 4
+    elif kind == "odd":
+        w = torch.where(w < 0.2, torch.full_like(w, float("nan")), torch.where(w < 0.4, torch.full_like(w, float("inf")), w - 0.7))
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    new, kept, out_w = ops.kv_evict(k, v, ks, vs, tables, n, w.to(DEV), keep, to + nb, sink=sink, recent=recent)
+    assert new.tolist() == [min(x, keep) for x in lens]
+    kept, out_w = kept.cpu(), out_w.cpu()
+    heavy = torch.where(w.isnan(), torch.full_like(w, float("-inf")), w).numpy()
+    for i, m in enumerate(lens):
+        for h in range(hkv):
+            pos = np.arange(min(m, keep))
+            if m > keep:
+                mid = np.arange(sink, m - recent)
+                best = mid[np.lexsort((mid, -heavy[i, h, mid]))][:keep - sink - recent]
+                pos = np.sort(np.concatenate([np.arange(sink), best, np.arange(m - recent, m)]))
+            assert kept[i, h, :len(pos)].tolist() == pos.tolist() and (kept[i, h, len(pos):] == -1).all()
+            assert torch.equal(out_w[i, h, :len(pos)].view(torch.int32), w[i, h, torch.from_numpy(pos)].view(torch.int32))
+        was, now = dequant(v, vs, tables[i], m)[:, 0], dequant(v, vs, to[i] + nb, min(m, keep))[:, 0]
+        pages = torch.nn.functional.pad(was[kept[i, 0, :min(m, keep)].long()], (0, 0, 0, -min(m, keep) % BS)).view(-1, BS, 64)
+        scale = power_scale(pages.abs().amax((1, 2)))[:, None, None]
+        assert torch.equal(now, (nearest_e4m3(pages / scale) * scale).view(-1, 64)[:min(m, keep)])
+
+
+# ----------------------------------------------------------------------------- writing steps of thousands of rows
+@pytest.mark.parametrize("d,hkv,g,rot,norm,plus_one,lens,rows", [
+    (64, 3, 2, 32, True, False, [40, 17, 1, 2500, 190], [1, 1, 1, 2100, 187]),         # single rows before prompts that begin inside a page
+    (128, 1, 1, 128, False, False, [2041, 700], [2036, 13]),
+    (256, 5, 1, 64, True, True, [16, 2200], [1, 2187]),
+    (128, 2, 3, 0, False, False, [23] * 100, [21] * 100),                               # every run crosses a block's rows
+    (64, 1, 4, 64, False, False, [7] * 300, [7] * 300),                                 # several runs in a block's rows
+    (128, 9, 1, 16, True, False, [600], [520]), (64, 7, 2, 64, False, False, [2050], [2047]),      # on both sides of the plans' borders
+    (64, 7, 2, 64, False, False, [2050], [2048]), (128, 3, 1, 128, False, False, [515], [512]), (128, 3, 1, 128, False, False, [515], [513]),
+])
+def test_writes_of_many_rows(d, hkv, g, rot, norm, plus_one, lens, rows):
+    base.test_write_sets_and_raises_block_scales(d, hkv, g, rot, norm, plus_one, lens, rows)
