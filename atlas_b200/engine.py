@@ -11,6 +11,7 @@ from __future__ import annotations
 import itertools
 import os
 import time
+import warnings
 from dataclasses import dataclass, field
 from typing import Any, Callable, Dict, Hashable, List, Optional, Sequence as Seq
 
@@ -146,6 +147,9 @@ class LLMEngine:
         if want == "fp8_scaled":
             # a power of two per (block, head), set from what the block holds; where that does not apply, the plain FP8 cache
             self.kv_block_scales = self.model.takes_block_scales(self.cfg.block_size) and not self.cfg.sparse_attention_blocks
+            if not self.kv_block_scales:
+                warnings.warn("kv_cache_dtype fp8_scaled: a layer of this model, the block size or block selection does not take scales by block; "
+                              "the KV cache is plain FP8")
             want = "fp8"
         if want == "bf16":
             return torch.bfloat16           # GPU: the general mma.sync attention kernel on a 16-bit cache

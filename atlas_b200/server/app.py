@@ -486,7 +486,7 @@ def create_app(state: ServerState) -> FastAPI:
         import dataclasses
         return {"model": S.model_name, "engine": dataclasses.asdict(e.cfg), "scheduler": e.snapshot(),
                 "tool_call_parser": S.tool_parser_name, "grammar_backend": S.grammar.backend if S.grammar else None,
-                "kv_cache_dtype": str(e.kv_dtype), "num_kv_blocks": e.pool.num_blocks,
+                "kv_cache_dtype": str(e.kv_dtype), "kv_block_scales": getattr(e, "kv_block_scales", False), "num_kv_blocks": e.pool.num_blocks,
                 "serve_plan": S.args.get("serve_plan"), "trace": TRACER.summary()}
 
     @app.get("/trace")

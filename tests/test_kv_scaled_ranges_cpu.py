@@ -2,13 +2,16 @@
 import ctypes
 import pathlib
 import re
+import warnings
 
 import pytest
 import torch
 
 from atlas_b200 import ops
+from atlas_b200.config import tiny_deepseek, tiny_dense
 from atlas_b200.ops import cuda as K, cuda_scaled as CS
 from kv_scaled_cases import BS, attention64_over, attention_bound, dequant, make_cache, tables_for
+from test_kv_scaled_engine_cpu import engine
 from test_kv_scaled_cpu import attend, batch_of, parts, write
 
 CSRC = pathlib.Path(__file__).resolve().parent.parent / "atlas_b200" / "csrc"
@@ -229,3 +232,16 @@ def test_eviction_takes_minus_infinity_before_nan():
         for h in range(2):
             mid = sorted(range(1, 58), key=lambda j: (w[0, h, j] != w[0, h, j], -float(w[0, h, j].nan_to_num(0.0, neginf=-1.0)), j))
             assert kept[0, h].tolist() == sorted([0, 58, 59] + mid[:keep - 3])
+
+
+# ----------------------------------------------------------------------------- the engine's option
+@pytest.mark.parametrize("make, kw", [(tiny_deepseek, {}), (tiny_dense, {"block_size": 32}), (tiny_dense, {"sparse_attention_blocks": 8})])
+def test_the_engine_says_where_block_scales_do_not_apply(make, kw):
+    with pytest.warns(UserWarning, match="fp8_scaled"):
+        assert not engine(make(), **kw).kv_block_scales
+
+
+def test_the_engine_is_silent_where_they_do():
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert engine().kv_block_scales
