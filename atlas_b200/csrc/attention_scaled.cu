@@ -7,7 +7,7 @@
 //
 // so both scales ride in the exponent's multiply-add and the codes go to the tensor cores as they are.  M follows the maximum of s_j + ev, that is
 // of what a token can add to the output, over the pages whose ev lie close together, and p is f16; pages whose ev is far from theirs have p as two
-// bf16 terms and hardly move M (tc_util.cuh).  q is brought to 2^14 by a power of two; the sums are fp32.
+// bf16 terms and hardly move M (kv_scaled.cuh).  q is brought to 2^14 by a power of two; the sums are fp32.
 //
 // scaled_decode_kernel: bound by the cache's bytes (2 D a token and key head).  The pages of all (sequence, key head) pairs form one list, cut
 // into equal runs, a run per warp: ragged batches and single long sequences fill the GPU alike.  A warp is on its own: it copies its pages
@@ -17,6 +17,7 @@
 // scaled_join_kernel and scaled_merge_kernel join the pieces of a pair.  scaled_weigh_kernel adds 2^(s - M) / l over the pair's heads to the running sums.
 #include "common.cuh"
 #include "host_api.h"
+#include "kv_scaled.cuh"
 #include "tc_util.cuh"
 
 namespace atlas {
@@ -64,20 +65,6 @@ ATLAS_DEVICE uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
-ATLAS_DEVICE uint32_t e4m3x2_to_f16x2(uint32_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(r) : "h"((uint16_t)v));
-  return r;
-}
-ATLAS_DEVICE uint32_t f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-ATLAS_DEVICE void bulk_page(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dst)),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 
 // Pages that the newest token of a sequence of `len` sees, and the first of them.
 ATLAS_DEVICE int seen_pages(int len, int window, int& first) {
@@ -107,7 +94,7 @@ ATLAS_DEVICE int run_length(int pages, int warps) { return max((pages + warps - 
 // One entry of the page list.
 struct PageRef {
   int item;            // (sequence * Hkv + key head) * tiles + tile
-  int tok0;            // first token of the page, one more for a far page (tc_util.cuh)
+  int tok0;            // first token of the page, one more for a far page (kv_scaled.cuh)
   int block;           // -1: an entry outside of the pool, skipped
   float sk, ev;        // key scale, value exponent
 };
@@ -304,7 +291,7 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[2 * i + j]));
-          qf[nt][i][j] = f16x2(f.x * up, f.y * up);
+          qf[nt][i][j] = pack_f16x2(f.x * up, f.y * up);
         }
       const float a = p.scale_log2 * down;
       a0[nt] = __shfl_sync(0xffffffffu, a, 8 * t);            // head 2t is the row g = 2t, lanes 8t ..
@@ -409,8 +396,8 @@ scaled_decode_kernel(const ScaledDecodeParams p) {
         l0[nt] += (p00 + p10) * undo;
         l1[nt] += (p01 + p11) * undo;
         if (!far) {
-          pb[nt][0] = transpose8x8(f16x2(p00, p01));
-          pb[nt][1] = transpose8x8(f16x2(p10, p11));
+          pb[nt][0] = transpose8x8(pack_f16x2(p00, p01));
+          pb[nt][1] = transpose8x8(pack_f16x2(p10, p11));
         } else {
           uint32_t hi[2], lo[2];
           two_terms(p00, p01, hi[0], lo[0]);
@@ -631,7 +618,8 @@ int decode_launch(ScaledDecodeParams p, int blocks, int items, long long max_len
   if (launch_chain(scaled_decode_kernel<D, NT>, dim3(blocks), dim3(kSdWarps<D, NT> * 32), smem, st, p) != cudaSuccess) { cudaGetLastError(); return -20; }
   // Single threads join up to four pieces a pair on average (128 x 1152 tokens of 8 heads, 3 a pair: 65 us with the attention, 89 by blocks), and
   // up to sixteen if no pair can have hundreds (a warp has two pages or more, and its share of the longest sequence's list): 32 x 4096 ragged
-  // tokens with weights, 9 a pair, 59 us, 62 by blocks; but 3 x 65531 tokens, 197 a pair, 89 us, 42 by blocks.
+  // tokens with weights, 9 a pair, 59 us, 62 by blocks; but 3 x 65531 tokens, 197 a pair, 89 us, 42 by blocks.  Both come to the same sums; a
+  // captured step chooses by the length that it was captured for.
   const long long most = min((max_len + 2 * kSdPage - 1) / (2 * kSdPage), (long long)p.warps * p.nd / items + 1) + 1;
   const bool few = 4ll * items >= p.warps || (16ll * items >= p.warps && most <= 256);
   const cudaError_t e = few ? launch_chain(scaled_join_kernel<D>, dim3(items, (D * p.cols + 511) / 512), dim3(128), 0, st, p)

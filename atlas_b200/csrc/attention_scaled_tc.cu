@@ -2,8 +2,9 @@
 // that each cached token got from a chunk's rows.
 //
 // As in attention_scaled.cu the codes are the operands and the scales live in the exponent: s_j = f q . k^_j with f = softmax scale * log2(e) * key
-// page's scale, p_j = 2^(s_j + ev - M) in f16 or, in key tiles with a far page (tc_util.cuh), as two bf16 terms, o = sum p_j v^_j / sum p_j 2^-ev.  A page covers 16 score columns, so f and ev - M are constants
-// of a multiply-add over them, and a page's largest score is found before they are applied.
+// page's scale, p_j = 2^(s_j + ev - M) in f16 or, in key tiles with a far page (kv_scaled.cuh), as two bf16 terms, o = sum p_j v^_j / sum p_j 2^-ev.
+// A page covers 16 score columns, so f and ev - M are constants of a multiply-add over them, and a page's largest score is found before they are
+// applied.
 //
 // scaled_chunk2_kernel (heads of 64 and 128), scaled_chunk_wide_kernel (256): tiles of 128 query rows of a key head; the G query heads of a key
 // head are packed into the rows (row = token * G + head), so that a page is fetched and widened once for all of them.  One warp fetches pages
@@ -17,6 +18,7 @@
 
 #include "common.cuh"
 #include "host_api.h"
+#include "kv_scaled.cuh"
 #include "tc_util.cuh"
 
 namespace atlas {
@@ -41,11 +43,6 @@ struct ScChunkParams {
   status_t* status;
 };
 
-ATLAS_DEVICE void sc_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dst)),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 ATLAS_DEVICE void sc_expect(uint64_t* bar, uint32_t bytes) {      // without arriving
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
@@ -62,21 +59,11 @@ ATLAS_DEVICE void umma_f16_lo(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, u
       "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
-ATLAS_DEVICE uint32_t sc_e4m3x2(uint32_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(r) : "h"((uint16_t)v));
-  return r;
-}
-ATLAS_DEVICE uint32_t sc_h2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 ATLAS_DEVICE void sc_widen16(const uint4 v, uint4& lo, uint4& hi) {
-  lo.x = sc_e4m3x2(v.x); lo.y = sc_e4m3x2(v.x >> 16); lo.z = sc_e4m3x2(v.y); lo.w = sc_e4m3x2(v.y >> 16);
-  hi.x = sc_e4m3x2(v.z); hi.y = sc_e4m3x2(v.z >> 16); hi.z = sc_e4m3x2(v.w); hi.w = sc_e4m3x2(v.w >> 16);
+  lo.x = e4m3x2_to_f16x2(v.x); lo.y = e4m3x2_to_f16x2(v.x >> 16); lo.z = e4m3x2_to_f16x2(v.y); lo.w = e4m3x2_to_f16x2(v.y >> 16);
+  hi.x = e4m3x2_to_f16x2(v.z); hi.y = e4m3x2_to_f16x2(v.z >> 16); hi.z = e4m3x2_to_f16x2(v.w); hi.w = e4m3x2_to_f16x2(v.w >> 16);
 }
 ATLAS_DEVICE uint4 f16_to_bf16(uint4 v) { return make_uint4(h2_to_bf2(v.x), h2_to_bf2(v.y), h2_to_bf2(v.z), h2_to_bf2(v.w)); }
-ATLAS_DEVICE float exact_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // A page whose table entry lies outside of the pool is skipped: its codes are zeros, which the copying warp puts where the copy would have gone,
 // and its value exponent is -inf, so that no column of it has a weight.
@@ -206,9 +193,9 @@ scaled_chunk_join_kernel(const ScChunkParams p) {
 //   warp 15            pages by bulk copies, their scales
 // Per pair of tiles and 128 keys: products 2048 clocks of the tensor cores, exponentials 2048 of the special-function units, shared memory 2048
 // for operands, 512 for the widened tiles and 512 for the codes.  Measured 5000: a softmax thread's chain of 2500 for 64 keys, half of it
-// exponentials shared by two warps a scheduler; no unit is busy for more than half of the time (issue slots 43 %).  Rounds of 16 or 32 columns,
-// a part of the exponentials as polynomials, and the tiles half a step apart were slower or no faster.  8 x 1024 rows of 32 heads of 128:
-// 109 us, 630 TFLOP/s; two sequences of 3001 rows: 150.
+// exponentials shared by two warps a scheduler; no unit is busy for more than half of the time (issue slots 47 %, tensor cores 42 %, special
+// functions 35 %: profiles/kv_scaled_cache.md).  Rounds of 16 or 32 columns, a part of the exponentials as polynomials, and the tiles half a step
+// apart were slower or no faster.  8 x 1024 rows of 32 heads of 128: 114 us, 602 TFLOP/s; two sequences of 3001 rows: 152.
 constexpr int kC2Threads = 512;
 constexpr int kC2Kv = 128, kC2Pages = 8, kC2Ring = 8, kC2Scales = kC2Pages + 1;
 
@@ -267,7 +254,7 @@ ATLAS_DEVICE float max3_nan(float a, float b, float c) {
   return r;
 }
 // A row's step over 64 score columns (a thread a row): their largest s + ev, then p = 2^(s + ev - m) as f16 over the first half of the columns
-// at tP, or, where the key tile has a far page (tc_util.cuh), as two bf16 terms over both halves.  f: (score factor, value exponent) of the four
+// at tP, or, where the key tile has a far page (kv_scaled.cuh), as two bf16 terms over both halves.  f: (score factor, value exponent) of the four
 // pages; columns [lo, hi) are visible.  The reference m moves only when a score passes what set it by 2^8 (p stays inside f16), which is rare
 // after a row's first columns; the output, where there is one, then moves with it, after wait_output() has seen the last product that goes to
 // it.  False: that wait ran out.
@@ -343,7 +330,7 @@ ATLAS_DEVICE bool softmax_step(uint32_t tS, uint32_t tP, uint32_t tO, const floa
   if constexpr (!kFar) {
     uint32_t w[2][16];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) page(q, [&](int i, float a, float b) { w[q >> 1][(q & 1) * 8 + i] = sc_h2(a, b); });
+    for (int q = 0; q < 4; ++q) page(q, [&](int i, float a, float b) { w[q >> 1][(q & 1) * 8 + i] = pack_f16x2(a, b); });
     tmem_st_32x32b_x16(tP, w[0]);
     tmem_st_32x32b_x16(tP + 16, w[1]);
   } else {
@@ -651,7 +638,7 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
           if (skipped) clear_pages<D>(w ? sStV : sStK, skipped);
           if (lane == 0) sc_expect(&ks_full[w], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
           __syncwarp();
-          if (live && is_v == (w == 1)) sc_bulk((w ? sStV : sStK) + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &ks_full[w]);
+          if (live && is_v == (w == 1)) bulk_page((w ? sStV : sStK) + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &ks_full[w]);
           if (w == 0) {                                             // under the copies: the scales may not be there yet
             const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
             if (j == 0) near.begin(pages >> 8 & 1 ? __shfl_sync(0xffffffffu, sc, 8) : 0.f, last);
@@ -799,8 +786,8 @@ scaled_chunk2_kernel(const __grid_constant__ CUtensorMap tmap_q, const ScChunkPa
 //   warps 14, 12   products: scores (of key tile j + 2 behind PV_j, whose P lies where they go), outputs
 //   warp 13        pages by bulk copies, their scales
 // Per 64 keys: products 512 clocks, exponentials 512, shared memory 1536 (512 for operands, 512 for the widened tiles, 512 for the codes).
-// Measured 3000, the softmax thread's chain again.  517 rows of 16 heads behind 4096 tokens: 57 us, 660 TFLOP/s (P through shared memory, two
-// threads a row, one group of widening warps: 115).
+// Measured 2700, the softmax thread's chain again (issue slots 48 %, tensor cores 40 %).  517 rows of 16 heads behind 4096 tokens: 56 us,
+// 655 TFLOP/s (P through shared memory, two threads a row, one group of widening warps: 115).
 constexpr int kWideThreads = 480, kWideKv = 64, kWidePages = 4, kWideRing = 8;
 
 struct WideTile {
@@ -1065,7 +1052,7 @@ scaled_chunk_wide_kernel(const ScChunkParams p) {
         if (lane == 0) sc_expect(&stage_full[2 * w + s], (uint32_t)__popc((pages >> (8 * w)) & 0xFFu) * (kScPg * D));
         __syncwarp();
         if (live && is_v == (w == 1))
-          sc_bulk((w ? sStV : sStK) + s * Tile::kStage + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &stage_full[2 * w + s]);
+          bulk_page((w ? sStV : sStK) + s * Tile::kStage + (lane & 7) * (kScPg * D), (w ? p.v_cache : p.k_cache) + at, kScPg * D, &stage_full[2 * w + s]);
         if (w == 0) {                                             // under the copies, as above; tile j - kWideRing is done: its keys left this stage long ago
           const float vs = __shfl_sync(0xffffffffu, sc, 8 + (lane & 7));
           if (j == 0) near.begin(pages >> 8 & 1 ? __shfl_sync(0xffffffffu, sc, 8) : 0.f, last);

@@ -16,6 +16,7 @@
 // sectors without a transposition.
 #include "common.cuh"
 #include "host_api.h"
+#include "kv_scaled.cuh"
 
 namespace atlas {
 
@@ -27,8 +28,6 @@ ATLAS_DEVICE int block_exponent(float a) {
   const int e = (int)((__float_as_uint(a) + 0x1FFFFFu) >> 23) - 127 - 8;
   return min(max(e, kScLow), kScHigh);
 }
-ATLAS_DEVICE float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }       // e in [-126, 127]
-ATLAS_DEVICE int exponent_of(float s) { return (int)((__float_as_uint(s) >> 23) & 255u) - 127; }
 
 template <int V>
 struct Codes { uint32_t w[(V + 3) / 4]; };            // V consecutive e4m3 codes, V in {2, 4, 8}
@@ -48,9 +47,8 @@ ATLAS_DEVICE void store_codes(uint8_t* p, const Codes<V>& c) {
   else *reinterpret_cast<uint2*>(p) = make_uint2(c.w[0], c.w[1]);
 }
 ATLAS_DEVICE float2 codes2_to_f32(uint32_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"((uint16_t)two));
-  return __half22float2(*reinterpret_cast<__half2*>(&h));
+  const uint32_t h = e4m3x2_to_f16x2(two);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 ATLAS_DEVICE uint32_t f32_to_codes2(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
 template <int V>
@@ -313,10 +311,10 @@ kv_scaled_write_kernel(const ScaledWriteParams p) {
       }
     }
     int ke = block_exponent(amax.x), ve = block_exponent(amax.y);
-    const int ke_old = exponent_of(k_before), ve_old = exponent_of(v_before);
+    const int ke_old = scale_exponent(k_before), ve_old = scale_exponent(v_before);
     if (off > 0) { ke = max(ke, ke_old); ve = max(ve, ve_old); }
     const bool k_raised = off > 0 && ke != ke_old, v_raised = off > 0 && ve != ve_old;
-    const float k_shift = pow2i(max(ke_old - ke, -126)), v_shift = pow2i(max(ve_old - ve, -126));      // used where the scale rose
+    const float k_shift = exact_pow2(max(ke_old - ke, -126)), v_shift = exact_pow2(max(ve_old - ve, -126));      // used where the scale rose
     // a group's tokens: rows of the run, tokens before them (to the new scale, if it rose), tokens behind them (as they were)
     auto store_group = [&](int g) {
       uint8_t* page_k = p.k_cache + base + lane * V;
@@ -328,11 +326,11 @@ kv_scaled_write_kernel(const ScaledWriteParams p) {
       for (int j = 0; j < 4; ++j) {
         const int s = 4 * g + j, r = s - off;
         if (r >= 0 && r < n) {
-          store_codes<V>(page_k + s * D, narrow<V>(x[j], pow2i(-ke)));
+          store_codes<V>(page_k + s * D, narrow<V>(x[j], exact_pow2(-ke)));
           fresh |= 0xFFu << (8 * j);
           float y[V];
           unpack<V>(v_raw[j], y);
-          const Codes<V> c = narrow<V>(y, pow2i(-ve));
+          const Codes<V> c = narrow<V>(y, exact_pow2(-ve));
 #pragma unroll
           for (int i = 0; i < V; ++i) word[i] |= ((c.w[i >> 2] >> (8 * (i & 3))) & 0xFFu) << (8 * j);
         } else if (r < 0) {
@@ -378,8 +376,8 @@ kv_scaled_write_kernel(const ScaledWriteParams p) {
       }
     }
     if (on && lane == 0 && (W == 1 || (warp & 3) == 0)) {
-      if (off == 0 || k_raised) *ks_at = pow2i(ke);
-      if (off == 0 || v_raised) *vs_at = pow2i(ve);
+      if (off == 0 || k_raised) *ks_at = exact_pow2(ke);
+      if (off == 0 || v_raised) *vs_at = exact_pow2(ve);
     }
   }
 }
@@ -641,7 +639,8 @@ struct MoveParams {
 
 // A warp fills one page of one head's keys or values.  A kept value token's 16-byte columns hold its neighbours too: every source page is read
 // once, as a whole, for all tokens that come from it, kAhead pages at a time.  (A warp for two pages, keys and values one after the other: 31
-// instead of 20 us for one sequence's 4096 tokens.)  Eight blocks an SM: 1024 of them, that sequence's, run at once (six: 47 us for the call, not 45).
+// instead of 20 us for one sequence's 4096 tokens.)  Eight blocks an SM: 1024 of them, that sequence's, run at once (six: 47 us for the call, not 45),
+// for which heads of 128 spill 284 bytes a thread.
 template <int D>
 __global__ void __launch_bounds__(128, D == 256 ? 3 : 8)
 kv_evict_move_kernel(const MoveParams p) {
@@ -693,7 +692,7 @@ kv_evict_move_kernel(const MoveParams p) {
       amax = fmaxf(amax, m * __shfl_sync(0xffffffffu, scale, r));
     }
     const int e = block_exponent(warp_max(amax));
-    const float by = scale * pow2i(-e);                     // a power of two: exact
+    const float by = scale * exact_pow2(-e);                     // a power of two: exact
 #pragma unroll
     for (int r = 0; r < kScPage; ++r) {
       const float f = __shfl_sync(0xffffffffu, by, r);
@@ -704,7 +703,7 @@ kv_evict_move_kernel(const MoveParams p) {
       }
       store_codes<V>(p.k + base + r * D + lane * V, codes[r]);
     }
-    if (lane == 0) p.ks[to * c.ks_ld + h * c.ks_h] = pow2i(e);
+    if (lane == 0) p.ks[to * c.ks_ld + h * c.ks_h] = exact_pow2(e);
     return;
   }
   // values: the distinct source pages in order, first token of each marked
@@ -762,7 +761,7 @@ kv_evict_move_kernel(const MoveParams p) {
     amax = fmaxf(amax, fmaxf(m0 * __shfl_sync(0xffffffffu, scale, r), m1 * __shfl_sync(0xffffffffu, scale, r + 1)));
   }
   const int e = block_exponent(warp_max(amax));
-  const float by = scale * pow2i(-e);
+  const float by = scale * exact_pow2(-e);
 #pragma unroll
   for (int r = 0; r < kScPage; r += 2) {
     const float f0 = __shfl_sync(0xffffffffu, by, r), f1 = __shfl_sync(0xffffffffu, by, r + 1);
@@ -777,7 +776,7 @@ kv_evict_move_kernel(const MoveParams p) {
 #pragma unroll
   for (int i = 0; i < V; ++i)
     reinterpret_cast<uint4*>(p.v + base)[i * 32 + lane] = make_uint4(word[i][0], word[i][1], word[i][2], word[i][3]);
-  if (lane == 0) p.vs[to * c.vs_ld + h * c.vs_h] = pow2i(e);
+  if (lane == 0) p.vs[to * c.vs_ld + h * c.vs_h] = exact_pow2(e);
 }
 
 }  // namespace atlas
@@ -857,9 +856,12 @@ extern "C" int atlas_kv_scaled_write(const void* record) {
   p.k_scale = r.s.ks; p.v_scale = r.s.vs; p.ks_ld = r.s.ks_ld; p.vs_ld = r.s.vs_ld; p.ks_h = (int)r.s.ks_h; p.vs_h = (int)r.s.vs_h;
   p.slots = r.slots; p.T = (int)r.T; p.Hq = (int)r.Hq; p.Hkv = (int)r.Hkv; p.rotary = (int)r.rotary; p.num_pages = (int)r.num_pages;
   p.plus_one = (int)r.plus_one; p.norm_dim = r.norm_dim > 0 ? (int)r.norm_dim : D; p.eps = (float)r.eps;
-  // Up to 512 rows: one row a block, a warp per page.  More are prompts: a page gets four warps, and one row in 16 begins a page; blocks of
-  // four or sixteen rows leave fewer blocks empty, but a mixed step's decode rows go through their block one after the other, which a long
-  // prompt beside them hides.
+  // Up to 512 rows: one row a block, a warp per page, the plan of single tokens.  More are prompts: a page gets four warps, and one row in 16
+  // begins a page; blocks of four or sixteen rows leave fewer blocks empty, but a mixed step's decode rows go through their block one after the
+  // other, which a long prompt beside them hides.  The number of rows does not tell prompts from single tokens, and a prompt of 17 to 512 rows
+  // pays for that (us, a warp per page and four):
+  //   heads of 128   prompts of 32, 128, 512 rows 22.6 / 5.1, 22.9 / 5.3, 25.9 / 8.2   32, 128, 512 single tokens 4.6 / 11.3, 4.9 / 11.6, 8.5 / 19.5
+  //   heads of 256   prompts of 32, 128, 512 rows 18.7 / 6.3, 18.9 / 6.3, 20.6 / 8.1   32, 128, 512 single tokens 4.6 / 17.0, 4.8 / 17.3, 9.9 / 26.4
   p.rows_per_block = p.T <= 512 ? 1 : p.T < 2048 ? 4 : 16;
   p.kv_blocks_x = (p.T + p.rows_per_block - 1) / p.rows_per_block;
   p.kv_blocks_y = p.rows_per_block == 1 ? (p.Hkv + 7) / 8 : (p.Hkv + 1) / 2;

@@ -23,29 +23,6 @@ ATLAS_DEVICE void tmem_st_32x32b_x1(uint32_t taddr, uint32_t v) {
 ATLAS_DEVICE void tmem_ld_32x32b_x1(uint32_t taddr, uint32_t& v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(v) : "r"(taddr) : "memory");
 }
-// ---- the block-scaled FP8 cache (kv_scaled.cu): softmax weights whose value scales lie far apart
-//
-// A token joins an output with p_j = 2^(s_j + ev - M), ev its page's value exponent.  A page's exponent is that of its largest token, so s_j + ev
-// says too much of the others: one token 2^20 times as loud as everything else, itself without weight, lifts its fifteen neighbours by 20, and a
-// reference M that followed them would push the p of all other pages out of f16.  Pages whose exponent is more than kFarApart away from that of
-// the first or of the last page of what is attended over are therefore `far`: their p goes to the tensor cores as two bf16 terms (17 bits at any
-// size; e4m3 is exact in bf16), and they move M only where they pass it by kFarSlack more than others.  The other pages' exponents are within
-// 2 * kFarApart of each other, and their p has f16's 11 bits down to 2^-21 of what set M, steps of 2^-31 of it below: M stays kHeadroom below what
-// set it, and moves when a score passes that by 2^8, so that p is below 2^15.  No limit of f16's or fp32's is met: far p below 2^47, sums of
-// p 2^-ev below 2^107 a token.  Exponents of trained caches lie within a few powers, and a far page costs a second product.
-constexpr int kFarApart = 8;
-constexpr float kFarSlack = 32.f, kHeadroom = 7.f, kMoves = 15.f;
-ATLAS_DEVICE int scale_exponent(float s) { return (int)((__float_as_uint(s) >> 23) & 255u) - 127; }
-ATLAS_DEVICE bool exponents_apart(int a, int b) { return abs(a - b) > kFarApart; }
-// the two bf16 terms of a pair of fp32 numbers
-ATLAS_DEVICE void two_terms(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16x2(a, b);
-  lo = pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
-}
-ATLAS_DEVICE uint32_t h2_to_bf2(uint32_t v) {      // e4m3 numbers: exact in both
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-  return pack_bf16x2(f.x, f.y);
-}
 ATLAS_DEVICE void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 ATLAS_DEVICE float fast_exp2(float x) {
   float y;

@@ -807,6 +807,7 @@ def step_list(batch, kind: str, build, device):
     One list a stream: an upload is ordered with its own stream only.  A list of other lengths than the batch has by now is made anew.  A graph
     that is being captured takes a list that is there (the capture began with a device at rest), and what it took stays with the batch."""
     nd, lens, rows = batch.num_decodes, batch.seq_lens_host, batch.query_lens_host
+    lens, rows = (x if type(x) is list else list(x) for x in (lens, rows))
     fits = lambda e: e[0] == nd and e[1] == lens and e[2] == rows
     lists = batch.__dict__.setdefault("_step_lists", {})
     stream, capturing = _list_place(device)
