@@ -31,7 +31,9 @@ ATLAS_DEVICE void bulk_page(void* dst, const void* src, uint32_t bytes, uint64_t
 // size; e4m3 is exact in bf16), and they move M only where they pass it by kFarSlack more than others.  The other pages' exponents are within
 // 2 * kFarApart of each other, and their p has f16's 11 bits down to 2^-21 of what set M, steps of 2^-31 of it below: M stays kHeadroom below what
 // set it, and moves when a score passes that by 2^8, so that p is below 2^15.  No limit of f16's or fp32's is met: far p below 2^47, sums of
-// p 2^-ev below 2^107 a token.  (p itself ends at 2^-126: pages more than 100 powers quieter than others lose small weights.)  Exponents of trained
+// p 2^-ev below 2^107 a token.  (p itself ends at 2^-126: pages more than 100 powers quieter than others lose small weights.)  What is not told apart
+// is loud and quiet tokens of one page: where every page has tokens 2^20 times as loud as those that carry the weight, loud tokens with weights
+// below 2^-31 of the largest are lost.  e4m3 has lost the quiet ones' values by then: it ends 2^18 below a page's largest.  Exponents of trained
 // caches lie within a few powers, and a far page costs a second product.  Where none is, telling costs prompt rows 2 % (8 x 1024 of 32 heads of 128:
 // 114 in place of 112 us; 517 of 16 heads of 256 behind 4096 tokens: 56 and 55) and single tokens nothing.
 constexpr int kFarApart = 8;

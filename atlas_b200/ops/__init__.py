@@ -488,7 +488,9 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale=1.0, v_scale=1.0,
     joins the scaled score of query ``i`` and key ``j``.
 
     With the tensors of :func:`alloc_kv_scales` as ``k_scale`` and ``v_scale`` the cache is FP8 with a scale per (block, head): plain or
-    windowed attention with a ``scale`` from 2^-60 to 2^60; a block whose table entry lies outside of the pool is skipped.  ``weights [sequences, Hkv, tokens]`` (fp32, such a cache only): every cached token's softmax weight, summed over
+    windowed attention with a ``scale`` from 2^-60 to 2^60; a block whose table entry lies outside of the pool is skipped.  Softmax weights meet
+    the values with 11 bits, 17 in blocks whose value scale is far from the others'; the sums are fp32.  ``weights [sequences, Hkv, tokens]``
+    (fp32, such a cache only, sums of its own for every sequence and head): every cached token's softmax weight, summed over
     the sequence's rows of this step and the query heads of a key head, is added to it."""
     if isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor):
         if chunk or sinks is not None or softcap or distance is not None:
@@ -532,8 +534,8 @@ def kv_read(k_cache, v_cache, block_tables, seq_lens, max_len: int, k_scale, v_s
 
 def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep: int, new_tables, sink: int = 0, recent: int = 0):
     """Keep ``keep`` tokens of every sequence and key head of a block-scaled cache: the first ``sink``, the last ``recent`` and, of those
-    between, the ones with the largest ``weights [sequences, Hkv, tokens]`` (ties: the earlier; NaN below everything).  They move, in their
-    order, into the blocks of ``new_tables [sequences, >= keep / 16]``, which no other table holds, and get scales of their own; the old
+    between, the ones with the largest ``weights [sequences, Hkv, tokens]`` (ties: the earlier; NaN below everything).  The weights reach over
+    the longest sequence (on a GPU, where lengths are not read back, only checked mode says where they do not).  The tokens move, in their order, into the blocks of ``new_tables [sequences, >= keep / 16]``, which no other table holds, and get scales of their own; the old
     blocks stay as they are.  Sequences of at most ``keep`` tokens move whole.
 
     Returns the new lengths (int32), the kept positions ``[sequences, Hkv, keep]`` (int32, -1 behind the last) and their weights."""
@@ -541,6 +543,8 @@ def kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights
         return scaled_ops().kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep, new_tables, sink, recent)
     if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError(f"keeping {keep} tokens of which the first {sink} and the last {recent} are fixed")
+    if seq_lens.numel() and int(seq_lens.max()) > weights.shape[2]:
+        raise ValueError(f"weights of {weights.shape[2]} tokens for sequences of up to {int(seq_lens.max())}")
     return ref_scaled.kv_evict(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, weights, keep, new_tables, sink, recent)
 
 

@@ -9,7 +9,7 @@ import torch
 
 from atlas_b200 import ops
 from atlas_b200.config import tiny_deepseek, tiny_dense
-from atlas_b200.ops import cuda as K, cuda_scaled as CS
+from atlas_b200.ops import checked, cuda as K, cuda_scaled as CS
 from kv_scaled_cases import BS, attention64_over, attention_bound, dequant, make_cache, tables_for
 from test_kv_scaled_engine_cpu import engine
 from test_kv_scaled_cpu import attend, batch_of, parts, write
@@ -232,6 +232,16 @@ def test_eviction_takes_minus_infinity_before_nan():
         for h in range(2):
             mid = sorted(range(1, 58), key=lambda j: (w[0, h, j] != w[0, h, j], -float(w[0, h, j].nan_to_num(0.0, neginf=-1.0)), j))
             assert kept[0, h].tolist() == sorted([0, 58, 59] + mid[:keep - 3])
+
+
+def test_eviction_wants_a_weight_for_every_token():
+    k, v, ks, vs = parts()
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.tensor([20], dtype=torch.int32)
+    to = torch.ones(1, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="weights of 19 tokens"):
+        ops.kv_evict(k, v, ks, vs, t, n, torch.zeros(1, 2, 19), 17, to)
+    with pytest.raises(checked.BoundsViolation):
+        checked.evict(t, n, to, 4, 16, 17, 19)
 
 
 # ----------------------------------------------------------------------------- the engine's option
