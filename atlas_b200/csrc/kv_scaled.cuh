@@ -34,8 +34,9 @@ ATLAS_DEVICE void bulk_page(void* dst, const void* src, uint32_t bytes, uint64_t
 // p 2^-ev below 2^107 a token.  (p itself ends at 2^-126: pages more than 100 powers quieter than others lose small weights.)  What is not told apart
 // is loud and quiet tokens of one page: where every page has tokens 2^20 times as loud as those that carry the weight, loud tokens with weights
 // below 2^-31 of the largest are lost.  e4m3 has lost the quiet ones' values by then: it ends 2^18 below a page's largest.  Exponents of trained
-// caches lie within a few powers, and a far page costs a second product.  Where none is, telling costs prompt rows 2 % (8 x 1024 of 32 heads of 128:
-// 114 in place of 112 us; 517 of 16 heads of 256 behind 4096 tokens: 56 and 55) and single tokens nothing.
+// caches lie within a few powers, and a far page costs a second product: were all pages far, 8 x 1024 prompt rows of 32 heads of 128 would take 147 us
+// in place of 116, 517 rows of 16 heads of 256 behind 4096 tokens 70 in place of 57, 128 x 1152 single tokens 64 in place of 57.  Where none is,
+// telling costs prompt rows 2 % (114 in place of 112 us, 56 of 55) and single tokens nothing.
 constexpr int kFarApart = 8;
 constexpr float kFarSlack = 32.f, kHeadroom = 7.f, kMoves = 15.f;
 ATLAS_DEVICE bool exponents_apart(int a, int b) { return abs(a - b) > kFarApart; }

@@ -345,3 +345,23 @@ def test_evict_of_more_tokens_than_registers_hold(hkv, lens, keep, sink, recent,
 ])
 def test_writes_of_many_rows(d, hkv, g, rot, norm, plus_one, lens, rows):
     base.test_write_sets_and_raises_block_scales(d, hkv, g, rot, norm, plus_one, lens, rows)
+
+
+@pytest.mark.parametrize("d,hkv,g,lens,rows,window", [
+    (128, 2, 4, [300, 77], [1, 1], 0), (64, 2, 16, [500], [1], 40), (256, 2, 5, [260], [1], 0),
+    (128, 2, 4, [300, 129], [300, 40], 0), (256, 2, 8, [530, 70], [17, 70], 0), (128, 1, 8, [3000], [20], 0)])
+def test_weights_do_not_depend_on_the_values_scales(d, hkv, g, lens, rows, window):
+    gen = torch.Generator().manual_seed(d)
+    tables, nb = tables_for(lens, gen, DEV)
+    k, v, ks, vs = make_cache(nb, hkv, d, gen, DEV, spread=1)
+    vs *= torch.exp2(torch.randint(-28, 29, (nb, hkv), generator=gen).float()).to(DEV)
+    q = torch.randn(sum(rows), hkv * g, d, generator=gen).to(torch.bfloat16).to(DEV)
+    w = torch.zeros(len(lens), hkv, max(lens), device=DEV)
+    ops.paged_attention(q, k, v, batch_of(lens, rows, tables), d ** -0.5, ks, vs, window or None, weights=w)
+    r0 = 0
+    for i, (n, r) in enumerate(zip(lens, rows)):
+        _, _, amp, sums = attention64_over(q[r0:r0 + r], dequant(k, ks, tables[i], n), dequant(v, vs, tables[i], n), d ** -0.5, window)
+        # scores and sums in fp32: the exponents s + ev - M and s - M are up to 100 larger than the scores
+        rel = 4 * (d / 16 + 8) * 2.0 ** -23 * (float(amp.max()) + 102.0) + 2.0 ** -20 + (r * g / 32 + 8) * 2.0 ** -23
+        assert (w[i, :, :n].double().cpu() - sums).abs().le(rel * sums + 1e-37).all() and not w[i, :, n:].any()
+        r0 += r
