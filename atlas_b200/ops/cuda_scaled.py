@@ -89,10 +89,9 @@ def _apart(t: torch.Tensor) -> bool:
 
 def _writable(k_cache, v_cache, k_scale, v_scale) -> None:
     """What a call writes is not written through two places at once."""
-    h2 = 2 * k_cache.shape[2]
-    own = k_scale.stride() == (h2, 2) == v_scale.stride() or (_apart(k_scale) and _apart(v_scale))      # as alloc_kv_scales has them
-    if not own or (k_scale.numel() and k_scale.data_ptr() == v_scale.data_ptr()) \
-            or (k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr()):
+    st = k_scale.stride()
+    own = st[1] == 2 and st[0] == 2 * k_scale.shape[1] and v_scale.stride() == st or (_apart(k_scale) and _apart(v_scale))      # first: alloc_kv_scales
+    if not own or k_scale.data_ptr() == v_scale.data_ptr() or k_cache.data_ptr() == v_cache.data_ptr():
         raise K.KernelError("keys, values and their scales have places of their own (allocate the scales with ops.alloc_kv_scales)")
 
 
@@ -257,6 +256,8 @@ def paged_attention(q, k_cache, v_cache, batch, scale, k_scale, v_scale, sliding
     window = min(window, max(1, cols * BLOCK))              # no sequence is longer: the kernels' sums of positions stay in 32 bits
     if window < 0 or rows < B or starts.shape[0] < B + 1 or not 0 <= nd <= B or T < nd:
         raise K.KernelError("attention: a block table, a length and a start for every sequence, a row for every decode, no negative window")
+    if B > nd and (len(batch.query_lens_host) < B or len(batch.seq_lens_host) < B or nd + sum(batch.query_lens_host[nd:B]) > T):
+        raise K.KernelError(f"{T} query rows for {nd} single tokens and chunks of {list(batch.query_lens_host[nd:B])}, whose host lengths a batch has")
     if not 2.0 ** -60 <= scale <= 2.0 ** 60:              # scores are masked, and the largest is taken, before it is applied
         raise K.KernelError(f"the softmax scale is positive, from 2^-60 to 2^60, not {scale}")
     width, sums = 0, (0, 0, 0)

@@ -234,6 +234,18 @@ def test_eviction_takes_minus_infinity_before_nan():
             assert kept[0, h].tolist() == sorted([0, 58, 59] + mid[:keep - 3])
 
 
+def test_attention_wants_a_row_for_every_new_token():
+    parts_ = parts()
+    for rows, T in (((1, 5), 5), ((5, 5), 9), ((20, 3), 22)):
+        with pytest.raises(K.KernelError, match="query rows for"):
+            attend(*parts_, rows=rows, q=torch.zeros(T, 4, 64, dtype=torch.bfloat16))
+    k, v, ks, vs = parts_
+    b = batch_of([20, 5], [1, 5], torch.zeros(2, 2, dtype=torch.int32))
+    b.query_lens_host = []
+    with pytest.raises(K.KernelError, match="host lengths"):
+        CS.paged_attention(torch.zeros(6, 4, 64, dtype=torch.bfloat16), k, v, b, 0.1, ks, vs)
+
+
 def test_eviction_wants_a_weight_for_every_token():
     k, v, ks, vs = parts()
     t, n = torch.zeros(1, 2, dtype=torch.int32), torch.tensor([20], dtype=torch.int32)
